@@ -309,6 +309,72 @@ int atlas_pilot_seeds(const int64_t* cnt, const int64_t* sumsq, const float* sel
                       int64_t Kr, int64_t n_total, double c, double z, int grouped, float* top_seed,
                       int64_t* res_seed_key, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Row maps of a batch from its sequences' lengths, on the device. No counterpart in the reference
+ * (its data loader builds the valid rows and token ids on the host, atlas/data.py:99-116).
+ * lengths [B] (int32, or int64 when lengths_i64): rows of each sequence. stride > 0: a padded batch,
+ * sequence b at row b*stride; stride 0: packed end to end. Of each sequence the first `lead` and the
+ * last `trail` positions are left out of slots and tok (special tokens). Writes
+ *   cu     i32 [B + 1]       prefix sums of the lengths
+ *   slots  i64 [rows]        the row of every kept position, in order; -1 behind the last
+ *   tok    i64 [rows]        its token id seq[b]*1024 + (position - lead) (seq NULL: b); -1 behind the last
+ *   blocks i32 [rows/128 + B + 1, 2]  (b, first position) of every 128 positions of every sequence (an
+ *                            empty sequence has one entry), in order; (-1, -1) behind the last
+ *   counts i64 [3]           kept positions, blocks, lengths that did not fit
+ * A length outside [0, stride] (packed: [0, rows]) is cut to it and counted; packed sequences whose sum
+ * is above `rows` are all taken as empty, and counted once more. slots and tok 16-byte aligned.
+ * ws: device bytes >= atlas_seq_maps_ws_bytes(B) (0 up to 1024 sequences).
+ */
+int64_t atlas_seq_maps_ws_bytes(int64_t B);
+int atlas_seq_maps(const void* lengths, int lengths_i64, int64_t B, int64_t rows, int64_t stride, int64_t lead,
+                   int64_t trail, const int64_t* seq, int32_t* cu, int64_t* slots, int64_t* tok, int32_t* blocks,
+                   int64_t* counts, void* ws, int64_t ws_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Attention over the valid rows of a batch (every row of a sequence attends to every row of the same
+ * sequence), and its gradient. No counterpart in the reference (its forward is the model library's).
+ *   S = scale q k^T;  lse = log sum exp S;  out = exp(S - lse) v
+ *   delta = sum_d dout out;  dS = exp(S - lse) (dout v^T - delta);
+ *   dv = exp(S - lse)^T dout;  dk = scale dS^T q;  dq = scale dS k
+ * q, out, dout, dq [outer, H, rows, D]; k, v, dk, dv [outer, Hk, rows, D], H a multiple of Hk: query
+ * head h uses key head h / (H/Hk), whose gradient is the sum over its query heads. D in [1, 64].
+ * strides_host: a HOST array with (outer, head, row) strides in elements for each tensor, in the order
+ * q, k, v, out (attention) or dout, q, k, v, out, dq, dk, dv (attention_grad); unit stride along D.
+ * lse and delta (workspace): f32 [outer, H, rows] contiguous. cu, blocks [cap, 2], counts: as written by
+ * atlas_seq_maps; padded (packed = 0): outer = B, sequence b in the first cu[b+1]-cu[b] rows of outer
+ * index b; packed: outer = 1, its rows are cu[b] .. cu[b+1]-1. Rows of no sequence are not read and
+ * come out as zero. S, the softmax and all sums are fp32; for 16-bit tensors the probabilities and dS
+ * are rounded to that type before they meet v, q, k or dout.
+ */
+int atlas_attention(const void* q, const void* k, const void* v, int dtype, const int64_t* strides_host, int64_t outer,
+                    int64_t rows, int64_t H, int64_t Hk, int64_t D, const int32_t* cu, const int32_t* blocks,
+                    const int64_t* counts, int64_t B, int64_t cap, int packed, double scale, void* out, float* lse,
+                    void* stream);
+int atlas_attention_grad(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse,
+                         int dtype, const int64_t* strides_host, int64_t outer, int64_t rows, int64_t H, int64_t Hk,
+                         int64_t D, const int32_t* cu, const int32_t* blocks, const int64_t* counts, int64_t B,
+                         int64_t cap, int packed, double scale, void* dq, void* dk, void* dv, float* delta, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Log probabilities of given tokens, and their gradient. No counterpart in the reference.
+ * logits [N, V] of `dtype`, row stride ld, unit column stride; tokens i64 [N, J], J <= 64. Per row:
+ *   logprob f32 [N, J] = log softmax(x)[token];  rank i32 [N, J] = 1 + #{v : x_v > x_token}
+ *   entropy f32 [N], lse f32 [N];  top_id i64 / top_logprob f32 [N, top]: the `top` (<= 32, <= V) most
+ *   likely tokens in order, ties to the lowest id.
+ * A token outside [0, V) means "none": log probability 0, rank 0, no gradient. A row of -inf only has
+ * lse and log probabilities -inf, entropy 0 and a zero gradient. NaN counts as the largest value among
+ * the alternatives and makes the row's numbers NaN.
+ * Gradient of sum g_logprob*logprob + sum g_entropy*entropy by the logits (either g may be NULL), from the
+ * forward call's lse and entropy: dlogits [N, V] of `dtype`, row stride ldd. A token given twice in a row
+ * counts twice.
+ */
+int atlas_token_logprobs(const void* logits, int dtype, int64_t N, int64_t V, int64_t ld, const int64_t* tokens, int64_t J,
+                         int64_t top, float* logprob, int32_t* rank, float* entropy, float* lse, int64_t* top_id,
+                         float* top_logprob, void* stream);
+int atlas_token_logprobs_grad(const void* logits, int dtype, int64_t N, int64_t V, int64_t ld, const int64_t* tokens,
+                              int64_t J, const float* lse, const float* entropy, const float* g_logprob,
+                              const float* g_entropy, void* dlogits, int64_t ldd, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -85,7 +85,7 @@ _KERNELS = {"atlas_grouped_merge": 6, "atlas_last_error": 0, "atlas_abi_version"
 LAUNCHES = {"count": 0}
 
 
-_KERNELS.update({"atlas_ctx_rows": 4, "atlas_ctx_annotations": 2})
+_KERNELS.update({"atlas_ctx_rows": 4, "atlas_ctx_annotations": 2, "atlas_attention_grad": 3})
 
 
 def _n_kernels(name: str, args) -> int:
@@ -93,6 +93,8 @@ def _n_kernels(name: str, args) -> int:
         return 3  # row-major count (+ keys in key order), row-major emit, hard columns
     if name == "atlas_admit":  # candidates, plus the bulk-row kernel when there are bulk rows
         return 2 if (args[6] and args[20]) else 1
+    if name == "atlas_seq_maps":  # more than 1024 sequences: a scan, then the outputs
+        return 2 if args[2] > 1024 else 1
     if name.endswith("_bytes") or name.endswith("_i32"):
         return 0
     return _KERNELS.get(name, 1)

@@ -1,0 +1,346 @@
+// Attention over the valid rows and its gradient on CUDA cores: fp32 tensors, and 16-bit ones whose
+// strides or width TMA cannot address (the tensor-core kernels take the others).
+//
+//   S = scale q k^T,  lse = log sum exp S,  out = exp(S - lse) v
+//   delta = sum_d dout out,  P = exp(S - lse),  dS = P (dout v^T - delta)
+//   dv = P^T dout,  dk = scale dS^T q,  dq = scale dS k
+//
+// 64 x 64 tiles, 256 threads, each with 4 rows (ty + 16 i) and 4 columns (tx + 16 j) of a tile of
+// scores; operands lie in shared memory as fp32 rows of DP + 4 words, read as float4 along the head
+// dimension (the 16 tx of a half warp hit distinct banks, the ty broadcast). The running maximum and
+// sum of the softmax stay in registers. The gradient is two kernels, one CTA per key tile (dk, dv; all query
+// heads of its key head, one after the other) and one per query tile (dq): scores are computed twice, but no
+// sum crosses CTAs, so every result is the same from run to run.
+#include "attn.cuh"
+
+namespace atlas {
+namespace {
+
+constexpr int BT = 64;       // rows of a tile
+constexpr int PP = 80;       // row pitch of a tile of scores: the two ty of a warp in different bank halves
+constexpr int kThreads = 256;
+constexpr float kNegInf = -__builtin_inff();
+
+template <int DT>
+__device__ __forceinline__ void put(typename Elem<DT>::T* p, float v);
+template <>
+__device__ __forceinline__ void put<ATLAS_F32>(float* p, float v) { *p = v; }
+template <>
+__device__ __forceinline__ void put<ATLAS_BF16>(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ void put<ATLAS_F16>(__half* p, float v) { *p = __float2half_rn(v); }
+
+// Rows first .. first + 63 of a head into shared memory, zero behind `len` and behind D.
+template <int DT, int DP>
+__device__ __forceinline__ void load_tile(float* dst, const void* src, const Strides& st, int64_t outer, int head, int64_t row0,
+                                          int first, int len, int D, float mul) {
+  using T = typename Elem<DT>::T;
+  const T* p = reinterpret_cast<const T*>(src) + outer * st.outer + head * st.head + row0 * st.row;
+  for (int i = threadIdx.x; i < BT * DP; i += kThreads) {
+    const int r = i / DP, d = i % DP;
+    const bool on = first + r < len && d < D;
+    dst[r * (DP + 4) + d] = on ? Elem<DT>::f(p[(int64_t)(first + r) * st.row + d]) * mul : 0.f;
+  }
+}
+
+// c[i][j] = sum_d a[ty + 16 i][d] b[tx + 16 j][d]
+template <int DP>
+__device__ __forceinline__ void mm_rows(const float* a, const float* b, int ty, int tx, float (&c)[4][4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c[i][j] = 0.f;
+#pragma unroll 4
+  for (int d = 0; d < DP; d += 4) {
+    float4 x[4], y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[i] = *reinterpret_cast<const float4*>(a + (ty + 16 * i) * (DP + 4) + d);
+      y[i] = *reinterpret_cast<const float4*>(b + (tx + 16 * i) * (DP + 4) + d);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        c[i][j] = fmaf(x[i].x, y[j].x, c[i][j]);
+        c[i][j] = fmaf(x[i].y, y[j].y, c[i][j]);
+        c[i][j] = fmaf(x[i].z, y[j].z, c[i][j]);
+        c[i][j] = fmaf(x[i].w, y[j].w, c[i][j]);
+      }
+  }
+}
+
+// acc[i][c] += sum_n p[ty + 16 i][n] v[n][tx C + c]
+template <int DP>
+__device__ __forceinline__ void mm_cols(const float* p, const float* v, int ty, int tx, float (&acc)[4][DP / 16]) {
+  constexpr int C = DP / 16;
+#pragma unroll 4
+  for (int n = 0; n < BT; n += 4) {
+    float4 x[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4*>(p + (ty + 16 * i) * PP + n);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float y[C];
+#pragma unroll
+      for (int c = 0; c < C; ++c) y[c] = v[(n + k) * (DP + 4) + tx * C + c];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float w = k == 0 ? x[i].x : k == 1 ? x[i].y : k == 2 ? x[i].z : x[i].w;
+#pragma unroll
+        for (int c = 0; c < C; ++c) acc[i][c] = fmaf(w, y[c], acc[i][c]);
+      }
+    }
+  }
+}
+
+__device__ __forceinline__ float row_max(float v) {
+#pragma unroll
+  for (int o = 8; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, o));
+  return v;
+}
+__device__ __forceinline__ float row_sum(float v) {
+#pragma unroll
+  for (int o = 8; o; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  return v;
+}
+
+template <int DT>
+__device__ __forceinline__ void zero_rows(void* dst, const Strides& st, int64_t outer, int head, int64_t from, int64_t to, int D) {
+  using T = typename Elem<DT>::T;
+  T* p = reinterpret_cast<T*>(dst) + outer * st.outer + head * st.head;
+  const int64_t n = (to - from) * D;
+  for (int64_t i = threadIdx.x; i < n; i += kThreads) put<DT>(p + (from + i / D) * st.row + i % D, 0.f);
+}
+
+template <int DT, int DP>
+__device__ __forceinline__ void store_tile(void* dst, const Strides& st, int64_t outer, int head, int64_t row0, int first, int len,
+                                           int D, int ty, int tx, const float (&acc)[4][DP / 16], const float (&mul)[4]) {
+  using T = typename Elem<DT>::T;
+  constexpr int C = DP / 16;
+  T* p = reinterpret_cast<T*>(dst) + outer * st.outer + head * st.head + row0 * st.row;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = first + ty + 16 * i;
+    if (r >= len) continue;
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+      if (tx * C + c < D) put<DT>(p + (int64_t)r * st.row + tx * C + c, acc[i][c] * mul[i]);
+  }
+}
+
+// ---------------------------------------------------------------------------------------- forward
+template <int DT, int DP>
+__global__ void __launch_bounds__(kThreads) attn_fwd_simt_kernel(const AttnArgs a) {
+  extern __shared__ float sm[];
+  constexpr int TILE = BT * (DP + 4);
+  float *sq = sm, *sk = sm + TILE, *sv = sm + 2 * TILE, *sp = sm + 3 * TILE;
+  const int head = blockIdx.y, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+  const int64_t bi = blockIdx.x >> 1;
+  const SeqBlock s = seq_block(a, bi);
+  int64_t z0, z1;
+  if (!(blockIdx.x & 1) && idle_rows(a, s, bi, &z0, &z1)) {
+    zero_rows<DT>(a.out, a.so, s.outer, head, z0, z1, a.D);
+    float* l = a.lse + (s.outer * a.H + head) * a.rows;
+    for (int64_t r = z0 + threadIdx.x; r < z1; r += kThreads) l[r] = 0.f;
+  }
+  const int first = s.first + (blockIdx.x & 1) * BT;
+  if (!s.on || first >= s.len) return;
+  const int kh = head / (a.H / a.Hk);
+  load_tile<DT, DP>(sq, a.q, a.sq, s.outer, head, s.row0, first, s.len, a.D, a.scale);
+  float m[4], l[4], acc[4][DP / 16];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    m[i] = kNegInf;
+    l[i] = 0.f;
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) acc[i][c] = 0.f;
+  }
+  for (int n0 = 0; n0 < s.len; n0 += BT) {
+    __syncthreads();
+    load_tile<DT, DP>(sk, a.k, a.sk, s.outer, kh, s.row0, n0, s.len, a.D, 1.f);
+    load_tile<DT, DP>(sv, a.v, a.sv, s.outer, kh, s.row0, n0, s.len, a.D, 1.f);
+    __syncthreads();
+    float c[4][4];
+    mm_rows<DP>(sq, sk, ty, tx, c);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float mx = kNegInf;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (n0 + tx + 16 * j >= s.len) c[i][j] = kNegInf;
+        mx = fmaxf(mx, c[i][j]);
+      }
+      mx = fmaxf(m[i], row_max(mx));
+      const float ref = mx == kNegInf ? 0.f : mx, f = m[i] == kNegInf ? 0.f : expf(m[i] - ref);
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float e = expf(c[i][j] - ref);
+        sum += e;
+        sp[(ty + 16 * i) * PP + tx + 16 * j] = e;
+      }
+      l[i] = l[i] * f + row_sum(sum);
+      m[i] = mx;
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d) acc[i][d] *= f;
+    }
+    __syncwarp();  // a warp's rows of sp are its own
+    mm_cols<DP>(sp, sv, ty, tx, acc);
+  }
+  float inv[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    inv[i] = 1.f / l[i];
+    const int r = first + ty + 16 * i;
+    if (tx == 0 && r < s.len) a.lse[(s.outer * a.H + head) * a.rows + s.row0 + r] = (m[i] == kNegInf ? 0.f : m[i]) + logf(l[i]);
+  }
+  store_tile<DT, DP>(a.out, a.so, s.outer, head, s.row0, first, s.len, a.D, ty, tx, acc, inv);
+}
+
+// --------------------------------------------------------------------------------------- gradient
+// KEYS: this CTA's rows are keys (dk, dv), the loop runs over the queries of every query head of the
+// key head; otherwise its rows are queries (dq) and the loop runs over the keys.
+template <int DT, int DP, bool KEYS>
+__global__ void __launch_bounds__(kThreads) attn_bwd_simt_kernel(const AttnArgs a) {
+  extern __shared__ float sm[];
+  constexpr int TILE = BT * (DP + 4);
+  // rows of this CTA: k and v (KEYS) or q and dout; of the loop: the other two
+  float *s0 = sm, *s1 = sm + TILE, *t0 = sm + 2 * TILE, *t1 = sm + 3 * TILE, *sp = sm + 4 * TILE, *sd = sp + BT * PP,
+        *s_lse = sd + BT * PP, *s_delta = s_lse + BT;
+  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, group = a.H / a.Hk;
+  const int64_t bi = blockIdx.x >> 1;
+  const SeqBlock s = seq_block(a, bi);
+  int64_t z0, z1;
+  if (!(blockIdx.x & 1) && idle_rows(a, s, bi, &z0, &z1)) {
+    if (KEYS) {
+      zero_rows<DT>(a.dk, a.sdk, s.outer, blockIdx.y, z0, z1, a.D);
+      zero_rows<DT>(a.dv, a.sdv, s.outer, blockIdx.y, z0, z1, a.D);
+    } else {
+      zero_rows<DT>(a.dq, a.sdq, s.outer, blockIdx.y, z0, z1, a.D);
+    }
+  }
+  const int first = s.first + (blockIdx.x & 1) * BT;
+  if (!s.on || first >= s.len) return;
+  const int kh = KEYS ? blockIdx.y : blockIdx.y / group;
+  if (KEYS) {
+    load_tile<DT, DP>(s0, a.k, a.sk, s.outer, kh, s.row0, first, s.len, a.D, 1.f);
+    load_tile<DT, DP>(s1, a.v, a.sv, s.outer, kh, s.row0, first, s.len, a.D, 1.f);
+  } else {
+    load_tile<DT, DP>(s0, a.q, a.sq, s.outer, blockIdx.y, s.row0, first, s.len, a.D, 1.f);
+    load_tile<DT, DP>(s1, a.dout, a.sdo, s.outer, blockIdx.y, s.row0, first, s.len, a.D, 1.f);
+  }
+  float g0[4][DP / 16], g1[4][DP / 16];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int c = 0; c < DP / 16; ++c) g0[i][c] = g1[i][c] = 0.f;
+  for (int h = KEYS ? kh * group : (int)blockIdx.y; h < (KEYS ? (kh + 1) * group : (int)blockIdx.y + 1); ++h) {
+    const float* lse = a.lse + (s.outer * a.H + h) * a.rows + s.row0;
+    const float* delta = a.delta + (s.outer * a.H + h) * a.rows + s.row0;
+    for (int n0 = 0; n0 < s.len; n0 += BT) {
+      __syncthreads();
+      if (KEYS) {
+        load_tile<DT, DP>(t0, a.q, a.sq, s.outer, h, s.row0, n0, s.len, a.D, 1.f);
+        load_tile<DT, DP>(t1, a.dout, a.sdo, s.outer, h, s.row0, n0, s.len, a.D, 1.f);
+      } else {
+        load_tile<DT, DP>(t0, a.k, a.sk, s.outer, kh, s.row0, n0, s.len, a.D, 1.f);
+        load_tile<DT, DP>(t1, a.v, a.sv, s.outer, kh, s.row0, n0, s.len, a.D, 1.f);
+      }
+      const int q0 = KEYS ? n0 : first;
+      if (threadIdx.x < BT) {
+        const bool on = q0 + (int)threadIdx.x < s.len;
+        s_lse[threadIdx.x] = on ? lse[q0 + threadIdx.x] : 0.f;
+        s_delta[threadIdx.x] = on ? delta[q0 + threadIdx.x] : 0.f;
+      }
+      __syncthreads();
+      float c[4][4], d[4][4];
+      mm_rows<DP>(s0, t0, ty, tx, c);
+      mm_rows<DP>(s1, t1, ty, tx, d);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int qi = KEYS ? tx + 16 * j : ty + 16 * i;
+          const bool on = first + ty + 16 * i < s.len && n0 + tx + 16 * j < s.len;
+          const float p = on ? expf(c[i][j] * a.scale - s_lse[qi]) : 0.f;
+          sp[(ty + 16 * i) * PP + tx + 16 * j] = p;
+          sd[(ty + 16 * i) * PP + tx + 16 * j] = on ? p * (d[i][j] - s_delta[qi]) : 0.f;
+        }
+      __syncwarp();
+      if (KEYS) mm_cols<DP>(sp, t1, ty, tx, g1);
+      mm_cols<DP>(sd, t0, ty, tx, g0);
+    }
+  }
+  const float sc[4] = {a.scale, a.scale, a.scale, a.scale}, one[4] = {1.f, 1.f, 1.f, 1.f};
+  if (KEYS) {
+    store_tile<DT, DP>(a.dk, a.sdk, s.outer, kh, s.row0, first, s.len, a.D, ty, tx, g0, sc);
+    store_tile<DT, DP>(a.dv, a.sdv, s.outer, kh, s.row0, first, s.len, a.D, ty, tx, g1, one);
+  } else {
+    store_tile<DT, DP>(a.dq, a.sdq, s.outer, blockIdx.y, s.row0, first, s.len, a.D, ty, tx, g0, sc);
+  }
+}
+
+// delta = sum_d dout out, one warp per row of a block and head.
+template <int DT>
+__global__ void __launch_bounds__(kThreads) attn_delta_kernel(const AttnArgs a) {
+  using T = typename Elem<DT>::T;
+  const SeqBlock s = seq_block(a, blockIdx.x);
+  if (!s.on) return;
+  const int head = blockIdx.y, lane = threadIdx.x & 31;
+  const T* o = reinterpret_cast<const T*>(a.o) + s.outer * a.so.outer + head * a.so.head + s.row0 * a.so.row;
+  const T* g = reinterpret_cast<const T*>(a.dout) + s.outer * a.sdo.outer + head * a.sdo.head + s.row0 * a.sdo.row;
+  for (int r = s.first + (threadIdx.x >> 5); r < min(s.len, s.first + kAttnBlock); r += kThreads / 32) {
+    float v = 0.f;
+    for (int d = lane; d < a.D; d += 32)
+      v = fmaf(Elem<DT>::f(o[(int64_t)r * a.so.row + d]), Elem<DT>::f(g[(int64_t)r * a.sdo.row + d]), v);
+#pragma unroll
+    for (int k = 16; k; k >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, k);
+    if (lane == 0) a.delta[(s.outer * a.H + head) * a.rows + s.row0 + r] = v;
+  }
+}
+
+template <typename K>
+int big_smem(K kernel, int bytes) {
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess
+             ? ATLAS_OK
+             : fail(ATLAS_ERR_CUDA, "attention: shared memory attribute");
+}
+
+template <int DT, int DP>
+int fwd(const AttnArgs& a, cudaStream_t st) {
+  const int bytes = (3 * BT * (DP + 4) + BT * PP) * 4;
+  if (int rc = big_smem(attn_fwd_simt_kernel<DT, DP>, bytes)) return rc;
+  attn_fwd_simt_kernel<DT, DP><<<dim3((unsigned)(2 * a.cap), a.H), kThreads, bytes, st>>>(a);
+  return check_launch("attention");
+}
+
+template <int DT, int DP>
+int bwd(const AttnArgs& a, cudaStream_t st) {
+  const int bytes = (4 * BT * (DP + 4) + 2 * BT * PP + 2 * BT) * 4;
+  if (int rc = big_smem(attn_bwd_simt_kernel<DT, DP, true>, bytes)) return rc;
+  if (int rc = big_smem(attn_bwd_simt_kernel<DT, DP, false>, bytes)) return rc;
+  attn_delta_kernel<DT><<<dim3((unsigned)a.cap, a.H), kThreads, 0, st>>>(a);
+  attn_bwd_simt_kernel<DT, DP, true><<<dim3((unsigned)(2 * a.cap), a.Hk), kThreads, bytes, st>>>(a);
+  attn_bwd_simt_kernel<DT, DP, false><<<dim3((unsigned)(2 * a.cap), a.H), kThreads, bytes, st>>>(a);
+  return check_launch("attention_grad");
+}
+
+template <int DT>
+int dispatch(const AttnArgs& a, bool grad, cudaStream_t st) {
+  if (a.D <= 16) return grad ? bwd<DT, 16>(a, st) : fwd<DT, 16>(a, st);
+  if (a.D <= 32) return grad ? bwd<DT, 32>(a, st) : fwd<DT, 32>(a, st);
+  return grad ? bwd<DT, 64>(a, st) : fwd<DT, 64>(a, st);
+}
+
+}  // namespace
+
+int attn_simt(const AttnArgs& a, int dtype, bool grad, cudaStream_t st) {
+  switch (dtype) {
+    case ATLAS_F32: return dispatch<ATLAS_F32>(a, grad, st);
+    case ATLAS_BF16: return dispatch<ATLAS_BF16>(a, grad, st);
+    default: return dispatch<ATLAS_F16>(a, grad, st);
+  }
+}
+
+}  // namespace atlas

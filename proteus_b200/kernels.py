@@ -5,6 +5,10 @@ atlas/core.py:75-104 — backed only by the sm_100a library (no fallback).
 """
 from __future__ import annotations
 
+import contextlib
+import ctypes
+from typing import NamedTuple
+
 import torch
 
 from . import _lib
@@ -206,3 +210,297 @@ def grouped_merge(state_score, state_pay, g, score, pay, K, pay_fill=None):
 def merge_rows(sc, tok, val, osc, otok, oval):
     G, K = sc.shape
     call("atlas_merge_rows", ptr(sc), ptr(tok), ptr(val), ptr(osc), ptr(otok), ptr(oval), G, K, stream_ptr(sc.device))
+
+
+# ----------------------------------------------------------------------------- a model's batches and answers
+def _on(device):
+    """Make `device` current for the launch (the C ABI launches on the current device)."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _same_device(first, **others):
+    for name, t in others.items():
+        if t.device != first.device:
+            raise ValueError(f"{name} is on {t.device}, the first argument on {first.device}")
+
+
+class SeqPlan(NamedTuple):
+    """Which rows of a batch's tensors belong to which sequence, as attention reads it: `cu` int32
+    [B + 1] prefix sums of the lengths, `blocks` int32 [n, 2] and `counts` int64 [3] of seq_maps, and
+    `stride`, the rows of each sequence in a padded batch (0: packed end to end)."""
+    cu: torch.Tensor
+    blocks: torch.Tensor
+    counts: torch.Tensor
+    stride: int
+
+
+class SeqMaps(NamedTuple):
+    """Result of seq_maps (see there)."""
+    cu: torch.Tensor
+    slots: torch.Tensor
+    tok: torch.Tensor
+    blocks: torch.Tensor
+    counts: torch.Tensor
+
+    def plan(self, stride: int) -> SeqPlan:
+        return SeqPlan(self.cu, self.blocks, self.counts, int(stride))
+
+
+def seq_maps(lengths, n_rows: int, *, stride: int = 0, lead: int = 0, trail: int = 0, seq=None) -> SeqMaps:
+    """The row maps of a batch, built on the device from its sequences' lengths without a host read:
+    `lengths` int32 or int64 [B] counts every row of a sequence, special tokens included; the batch's
+    tensors have `n_rows` rows, sequence b at row b*stride (padded, stride > 0) or right behind the one
+    before it (packed, stride 0). `lead` and `trail` positions at a sequence's start and end (<cls>,
+    <eos>) get no slot. Returns SeqMaps:
+
+      cu     int32 [B + 1]                    prefix sums of the lengths
+      slots  int64 [n_rows]                   rows of the kept positions, in order (a batch's valid rows)
+      tok    int64 [n_rows]                   their token ids: pack_tok(seq[b], position - lead); seq None: b
+      blocks int32 [n_rows // 128 + B + 1, 2] (sequence, first position) of every 128 positions
+      counts int64 [3]                        kept positions, blocks, lengths that did not fit
+
+    slots, tok and blocks are -1 behind their last entry. A length outside [0, stride] (packed:
+    [0, n_rows]) is cut and counted in counts[2]; packed sequences that together do not fit are all
+    taken as empty, which counts once more."""
+    require_cuda(lengths, "lengths")
+    if lengths.dim() != 1 or lengths.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"lengths must be int32 or int64 [B], got {lengths.dtype} {list(lengths.shape)}")
+    dev, B = lengths.device, lengths.numel()
+    if n_rows < 1 or stride < 0 or lead < 0 or trail < 0 or stride * B > n_rows:
+        raise ValueError(f"{B} sequences of stride {stride} (lead {lead}, trail {trail}) do not fit {n_rows} rows")
+    if seq is not None:
+        _same_device(lengths, seq=seq)
+        if seq.shape != lengths.shape or seq.dtype != torch.int64:
+            raise TypeError(f"seq must be int64 [{B}], got {seq.dtype} {list(seq.shape)}")
+        seq = seq.contiguous()
+    lengths = lengths.contiguous()
+    i64 = dict(dtype=torch.int64, device=dev)
+    cap = n_rows // 128 + B + 1
+    if B == 0:
+        none = torch.full((n_rows,), -1, **i64)
+        return SeqMaps(torch.zeros(1, dtype=torch.int32, device=dev), none, none.clone(),
+                       torch.full((cap, 2), -1, dtype=torch.int32, device=dev), torch.zeros(3, **i64))
+    cu = torch.empty(B + 1, dtype=torch.int32, device=dev)
+    blocks = torch.empty(cap, 2, dtype=torch.int32, device=dev)
+    slots, tok, counts = torch.empty(n_rows, **i64), torch.empty(n_rows, **i64), torch.empty(3, **i64)
+    need = int(_lib.load().atlas_seq_maps_ws_bytes(B))
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    with _on(dev):
+        call("atlas_seq_maps", ptr(lengths), int(lengths.dtype == torch.int64), B, n_rows, stride, lead, trail, ptr(seq),
+             ptr(cu), ptr(slots), ptr(tok), ptr(blocks), ptr(counts), ptr(ws), need, stream_ptr(dev))
+    return SeqMaps(cu, slots, tok, blocks, counts)
+
+
+def _rows_like(t, heads: int):
+    """An uninitialised [outer, heads, rows, D] tensor whose memory is [outer, rows, heads, D], the
+    layout the next projection reads."""
+    o, _, n, d = t.shape
+    return torch.empty(o, n, heads, d, dtype=t.dtype, device=t.device).transpose(1, 2)
+
+
+def _unit(t):
+    return t if t.stride(-1) == 1 else t.contiguous()
+
+
+def _strides(*ts):
+    s = [x for t in ts for x in t.stride()[:3]]
+    return (ctypes.c_int64 * len(s))(*s)
+
+
+def _check_attention(q, k, v, plan):
+    require_cuda(q, "q")
+    _same_device(q, k=k, v=v, cu=plan.cu, blocks=plan.blocks, counts=plan.counts)
+    if q.dim() != 4 or k.shape != v.shape or k.dim() != 4 or (q.shape[0], q.shape[2], q.shape[3]) != \
+            (k.shape[0], k.shape[2], k.shape[3]):
+        raise ValueError(f"q [outer, H, rows, D], k and v [outer, Hk, rows, D]: got {list(q.shape)}, {list(k.shape)}, {list(v.shape)}")
+    if not q.dtype == k.dtype == v.dtype:
+        raise TypeError(f"q, k and v must have one dtype, got {q.dtype}, {k.dtype}, {v.dtype}")
+    dtype_code(q.dtype)
+    if not 1 <= q.shape[3] <= 64:
+        raise ValueError(f"head dimension {q.shape[3]}: 1 to 64 are supported")
+    if k.shape[1] < 1 or q.shape[1] % k.shape[1]:
+        raise ValueError(f"{q.shape[1]} query heads over {k.shape[1]} key heads: not a multiple")
+    B = plan.cu.numel() - 1
+    if B < 0 or plan.cu.dtype != torch.int32 or plan.blocks.dtype != torch.int32 or plan.counts.dtype != torch.int64 or \
+            plan.blocks.dim() != 2 or plan.blocks.shape[1] != 2 or plan.counts.numel() != 3:
+        raise TypeError("plan: cu int32 [B + 1], blocks int32 [n, 2], counts int64 [3] (seq_maps)")
+    if plan.stride == 0 and q.shape[0] != 1:
+        raise ValueError(f"a packed batch has one outer index, got {q.shape[0]}")
+    if plan.stride and (q.shape[0] != B or q.shape[2] != plan.stride):
+        raise ValueError(f"a padded batch of {B} sequences of stride {plan.stride} against q {list(q.shape)}")
+    if plan.blocks.shape[0] < q.shape[0] * q.shape[2] // 128 + B + 1:
+        raise ValueError(f"plan of {plan.blocks.shape[0]} blocks: too few for {q.shape[0] * q.shape[2]} rows")
+    return B
+
+
+def _attention_forward(q, k, v, plan, scale):
+    B = _check_attention(q, k, v, plan)
+    (o, h, n, d), dev = q.shape, q.device
+    out, lse = _rows_like(q, h), torch.empty(o, h, n, dtype=torch.float32, device=dev)
+    if B == 0 or out.numel() == 0:
+        return out.zero_(), lse.zero_()
+    q, k, v = _unit(q), _unit(k), _unit(v)
+    blocks, counts, cu = plan.blocks.contiguous(), plan.counts.contiguous(), plan.cu.contiguous()
+    s = _strides(q, k, v, out)
+    with _on(dev):
+        call("atlas_attention", ptr(q), ptr(k), ptr(v), dtype_code(q.dtype), ctypes.addressof(s), o, n, h, k.shape[1], d,
+             ptr(cu), ptr(blocks), ptr(counts), B, blocks.shape[0], int(plan.stride == 0), float(scale), ptr(out), ptr(lse),
+             stream_ptr(dev))
+    return out, lse
+
+
+def attention_grad(dout, q, k, v, out, lse, plan: SeqPlan, scale: float | None = None):
+    """(dq, dk, dv) of attention(q, k, v, plan, scale) for the gradient `dout` of its output: the
+    probabilities are computed again from `lse`, the keys' gradients summed over the query heads that
+    share them. No atomics: the same call gives the same bits. Rows of no sequence come out as zero."""
+    B = _check_attention(q, k, v, plan)
+    _same_device(q, dout=dout, out=out, lse=lse)
+    if dout.shape != q.shape or out.shape != q.shape or lse.shape != q.shape[:3]:
+        raise ValueError(f"dout and out must be {list(q.shape)}, lse {list(q.shape[:3])}")
+    if dout.dtype != q.dtype or out.dtype != q.dtype or lse.dtype != torch.float32:
+        raise TypeError(f"dout and out must be {q.dtype}, lse float32")
+    scale = q.shape[3] ** -0.5 if scale is None else scale
+    (o, h, n, d), dev = q.shape, q.device
+    dq, dk, dv = _rows_like(q, h), _rows_like(k, k.shape[1]), _rows_like(v, k.shape[1])
+    if B == 0 or dq.numel() == 0:
+        return dq.zero_(), dk.zero_(), dv.zero_()
+    delta = torch.empty(o, h, n, dtype=torch.float32, device=dev)
+    dout, q, k, v, out, lse = _unit(dout), _unit(q), _unit(k), _unit(v), _unit(out), lse.contiguous()
+    blocks, counts, cu = plan.blocks.contiguous(), plan.counts.contiguous(), plan.cu.contiguous()
+    s = _strides(dout, q, k, v, out, dq, dk, dv)
+    with _on(dev):
+        call("atlas_attention_grad", ptr(dout), ptr(q), ptr(k), ptr(v), ptr(out), ptr(lse), dtype_code(q.dtype), ctypes.addressof(s),
+             o, n, h, k.shape[1], d, ptr(cu), ptr(blocks), ptr(counts), B, blocks.shape[0], int(plan.stride == 0), float(scale),
+             ptr(dq), ptr(dk), ptr(dv), ptr(delta), stream_ptr(dev))
+    return dq, dk, dv
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, cu, blocks, counts, stride, scale):
+        plan = SeqPlan(cu, blocks, counts, stride)
+        out, lse = _attention_forward(q, k, v, plan, scale)
+        ctx.save_for_backward(q, k, v, out, lse, cu, blocks, counts)
+        ctx.stride, ctx.scale = stride, scale
+        ctx.mark_non_differentiable(lse)
+        return out, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, _dlse):
+        q, k, v, out, lse, cu, blocks, counts = ctx.saved_tensors
+        return *attention_grad(dout, q, k, v, out, lse, SeqPlan(cu, blocks, counts, ctx.stride), ctx.scale), *[None] * 5
+
+
+def attention(q, k, v, plan: SeqPlan, scale: float | None = None):
+    """Attention over the valid rows of a batch: every row of a sequence attends to every row of the
+    same sequence. q [outer, H, rows, D] and k, v [outer, Hk, rows, D] (bf16, fp16 or fp32, any strides,
+    D <= 64, query head h reads key head h // (H // Hk)); a padded batch has outer = B and rows =
+    plan.stride, a packed one outer = 1. scale: D ** -0.5 if not given. Returns out (q's shape, memory
+    [outer, rows, H, D]) and the log-sum-exp of the scores, fp32 [outer, H, rows]; both zero in rows of
+    no sequence, whose inputs are never read (they may hold NaN). Differentiable in q, k and v (not
+    through the log-sum-exp)."""
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _Attention.apply(q, k, v, plan.cu, plan.blocks, plan.counts, plan.stride, scale)
+    return _attention_forward(q, k, v, plan, scale)
+
+
+class TokenLogprobs(NamedTuple):
+    """Result of token_logprobs (see there)."""
+    logprob: torch.Tensor
+    rank: torch.Tensor
+    entropy: torch.Tensor
+    lse: torch.Tensor
+    top_id: torch.Tensor
+    top_logprob: torch.Tensor
+
+
+def _check_logits(logits, tokens):
+    require_cuda(logits, "logits")
+    _same_device(logits, tokens=tokens)
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise ValueError(f"logits must be [N, V] with V >= 1, got {list(logits.shape)}")
+    dtype_code(logits.dtype)
+    if tokens.dtype != torch.int64 or tokens.dim() not in (1, 2) or tokens.shape[0] != logits.shape[0]:
+        raise TypeError(f"tokens must be int64 [N] or [N, J], got {tokens.dtype} {list(tokens.shape)}")
+    if tokens.dim() == 2 and tokens.shape[1] > 64:
+        raise ValueError(f"{tokens.shape[1]} tokens a row: at most 64")
+    return 1 if tokens.dim() == 1 else tokens.shape[1]
+
+
+def _row_stride(t):
+    """Row stride for the kernels: of a single row, whatever it says, the row's length."""
+    return max(t.stride(0), t.shape[1]) if t.shape[0] <= 1 else t.stride(0)
+
+
+def _plain_rows(t):
+    """[N, V] with unit column stride and rows that do not overlap (an expanded row is copied out)."""
+    return t if (t.stride(1) == 1 or t.shape[1] == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
+
+
+def _token_logprobs_forward(logits, tokens, top):
+    J = _check_logits(logits, tokens)
+    (N, V), dev = logits.shape, logits.device
+    if not 0 <= top <= min(32, V):
+        raise ValueError(f"top must be in [0, min(32, V)], got {top} for V = {V}")
+    logits, tokens = _plain_rows(logits), tokens.contiguous()
+    f32 = dict(dtype=torch.float32, device=dev)
+    r = TokenLogprobs(torch.empty(tokens.shape, **f32), torch.empty(tokens.shape, dtype=torch.int32, device=dev),
+                      torch.empty(N, **f32), torch.empty(N, **f32), torch.empty(N, top, dtype=torch.int64, device=dev),
+                      torch.empty(N, top, **f32))
+    if N:
+        with _on(dev):
+            call("atlas_token_logprobs", ptr(logits), dtype_code(logits.dtype), N, V, _row_stride(logits), ptr(tokens), J, top,
+                 ptr(r.logprob), ptr(r.rank), ptr(r.entropy), ptr(r.lse), ptr(r.top_id), ptr(r.top_logprob), stream_ptr(dev))
+    return r
+
+
+def token_logprobs_grad(logits, tokens, lse, entropy, g_logprob=None, g_entropy=None):
+    """Gradient by the logits, [N, V] in their dtype, of sum(g_logprob * logprob) + sum(g_entropy *
+    entropy), from token_logprobs' lse and entropy. Either gradient may be None. A token given twice
+    in a row counts twice; one outside [0, V) not at all."""
+    J = _check_logits(logits, tokens)
+    (N, V), dev = logits.shape, logits.device
+    gs = {"lse": (lse, (N,)), "entropy": (entropy, (N,)), "g_logprob": (g_logprob, tuple(tokens.shape)), "g_entropy": (g_entropy, (N,))}
+    for name, (t, shape) in gs.items():
+        if t is None and name.startswith("g_"):
+            continue
+        _same_device(logits, **{name: t})
+        if t.dtype != torch.float32 or tuple(t.shape) != shape:
+            raise TypeError(f"{name} must be float32 {list(shape)}, got {t.dtype} {list(t.shape)}")
+    logits, tokens, lse, entropy = _plain_rows(logits), tokens.contiguous(), lse.contiguous(), entropy.contiguous()
+    g_logprob, g_entropy = (None if g is None else g.contiguous() for g in (g_logprob, g_entropy))
+    dx = torch.empty(N, V, dtype=logits.dtype, device=dev)
+    if N:
+        with _on(dev):
+            call("atlas_token_logprobs_grad", ptr(logits), dtype_code(logits.dtype), N, V, _row_stride(logits), ptr(tokens), J,
+                 ptr(lse), ptr(entropy), ptr(g_logprob), ptr(g_entropy), ptr(dx), V, stream_ptr(dev))
+    return dx
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, top):
+        r = _token_logprobs_forward(logits, tokens, top)
+        ctx.save_for_backward(logits, tokens, r.lse, r.entropy)
+        ctx.mark_non_differentiable(r.rank, r.lse, r.top_id, r.top_logprob)
+        ctx.set_materialize_grads(False)
+        return tuple(r)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_logprob, _rank, g_entropy, *_rest):
+        return token_logprobs_grad(*ctx.saved_tensors, g_logprob, g_entropy), None, None
+
+
+def token_logprobs(logits, tokens, top: int = 0) -> TokenLogprobs:
+    """What a model answers at each row of `logits` [N, V] (bf16, fp16 or fp32; any row stride): for
+    `tokens` int64 [N] or [N, J] (J <= 64) their log probability (fp32) and rank (int32, 1 + how many
+    logits are larger), the row's entropy and log-sum-exp (fp32 [N]), and the `top` (<= 32) most likely
+    tokens (top_id int64, top_logprob fp32 [N, top]; ties to the lowest id). A token outside [0, V)
+    means none: log probability 0, rank 0. A row of -inf only has log probabilities -inf and entropy 0.
+    logprob and entropy are differentiable in the logits."""
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return TokenLogprobs(*_TokenLogprobs.apply(logits, tokens, top))
+    return _token_logprobs_forward(logits, tokens, top)
