@@ -5,6 +5,8 @@
 namespace atlas {
 
 int attn_simt(const AttnArgs& a, int dtype, bool grad, cudaStream_t st);
+bool attn_tc_takes(const AttnArgs& a, int dtype, bool grad);
+int attn_tc(const AttnArgs& a, int dtype, bool grad, cudaStream_t st);
 
 namespace {
 
@@ -41,7 +43,7 @@ extern "C" int atlas_attention(const void* q, const void* k, const void* v, int 
   a.packed = packed; a.scale = (float)scale;
   if (int rc = check(a, dtype, "attention")) return rc;
   ATLAS_REQUIRE(out, "attention: null pointer");
-  return attn_simt(a, dtype, false, (cudaStream_t)stream);
+  return (attn_tc_takes(a, dtype, false) ? attn_tc : attn_simt)(a, dtype, false, (cudaStream_t)stream);
 }
 
 extern "C" int atlas_attention_grad(const void* dout, const void* q, const void* k, const void* v, const void* out,
@@ -61,5 +63,5 @@ extern "C" int atlas_attention_grad(const void* dout, const void* q, const void*
   a.packed = packed; a.scale = (float)scale;
   if (int rc = check(a, dtype, "attention_grad")) return rc;
   ATLAS_REQUIRE(dout && out && dq && dk && dv && delta, "attention_grad: null pointer");
-  return attn_simt(a, dtype, true, (cudaStream_t)stream);
+  return (attn_tc_takes(a, dtype, true) ? attn_tc : attn_simt)(a, dtype, true, (cudaStream_t)stream);
 }

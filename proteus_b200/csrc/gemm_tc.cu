@@ -979,12 +979,14 @@ using namespace atlas;
 
 namespace atlas {
 int filter_device_status(int* v, int reset);  // filter.cu's bounded waits
+int attn_device_status(int* v, int reset);    // attn_tc.cu's
 }
 
 // Status of the bounded waits: the first code recorded by the tensor-core kernels (this file) or,
-// when they recorded none, by the bulk-fed filter (filter.cu); each file keeps its own word.
+// when they recorded none, by the bulk-fed filter (filter.cu) or attention (attn_tc.cu); each file
+// keeps its own word.
 extern "C" int atlas_device_status(int* status_host, int reset) {
-  int v = 0, vf = 0;
+  int v = 0, vf = 0, va = 0;
   if (cudaMemcpyFromSymbol(&v, tc::g_device_status, sizeof(int)) != cudaSuccess)
     return fail(ATLAS_ERR_CUDA, "device_status: read failed");
   if (reset && v) {
@@ -993,7 +995,8 @@ extern "C" int atlas_device_status(int* status_host, int reset) {
       return fail(ATLAS_ERR_CUDA, "device_status: reset failed");
   }
   if (atlas::filter_device_status(&vf, reset) != ATLAS_OK) return fail(ATLAS_ERR_CUDA, "device_status: read failed");
-  if (status_host) *status_host = v ? v : vf;
+  if (atlas::attn_device_status(&va, reset) != ATLAS_OK) return fail(ATLAS_ERR_CUDA, "device_status: read failed");
+  if (status_host) *status_host = v ? v : vf ? vf : va;
   return ATLAS_OK;
 }
 

@@ -11,8 +11,8 @@ namespace tc {
 
 // Device-side status word: kernels record a bounded wait that gave up here instead of hanging.
 // 0 = ok; otherwise the code of the first failing wait. Whole-program compilation gives each
-// translation unit its own copy, so every kernel that waits lives in gemm_tc.cu, which also
-// exports the reader (atlas_device_status).
+// translation unit its own copy: gemm_tc.cu, filter.cu and attn_tc.cu have kernels that wait, and
+// atlas_device_status (gemm_tc.cu) reads all three.
 static __device__ int g_device_status = 0;
 
 constexpr uint32_t kWaitLimit = 1u << 25;  // try_wait polls before giving up (about a second or more)
@@ -113,6 +113,41 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
                : "memory");
 }
 
+// 4-D TMA tile load (own copy), as tma_load_2d.
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, int32_t c0, int32_t c1, int32_t c2, int32_t c3,
+                                            uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar))
+      : "memory");
+}
+
+// Shared-memory writes of this thread become visible to the tensor core's and TMA's reads.
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// D[tmem] (+)= A[tmem] * B[smem desc]: A holds two 16-bit K elements per 32-bit column, row = lane.
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                          uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// 16 registers per thread -> 32 lanes x 16 consecutive 32-bit columns.
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
 // 32 lanes x 32 consecutive 32-bit columns -> 32 registers per thread (thread = lane).
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
@@ -140,7 +175,21 @@ __device__ __forceinline__ uint64_t sdesc_k_sw128(uint32_t addr) {
   return d;
 }
 
-// Instruction descriptors (dense, no negate, K-major A and B).
+// The same tile read with its rows as K (an MN-major operand of 64 elements, 128-byte swizzle): eight
+// rows of 128 bytes are one swizzle atom, the next eight K elements lie 1024 bytes further. One MMA of
+// K = 16 takes 2048 bytes.
+__device__ __forceinline__ uint64_t sdesc_mn_sw128(uint32_t addr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((addr >> 4) & 0x3FFF);       // start address
+  d |= (uint64_t)1 << 16;                      // leading byte offset: next 64 elements of MN (there are none)
+  d |= (uint64_t)(1024 >> 4) << 32;            // stride byte offset: next 8 of K
+  d |= (uint64_t)1 << 46;                      // descriptor version (sm_100)
+  d |= (uint64_t)2 << 61;                      // layout: 128-byte swizzle
+  return d;
+}
+
+// Instruction descriptors (dense, no negate, K-major A and B; kMnB: B is MN-major).
+constexpr uint32_t kMnB = 1u << 16;
 __host__ __device__ constexpr uint32_t idesc_bf16_f32(int M, int N) {
   return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
