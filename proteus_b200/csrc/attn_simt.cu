@@ -300,6 +300,18 @@ __global__ void __launch_bounds__(kThreads) attn_delta_kernel(const AttnArgs a) 
   }
 }
 
+}  // namespace
+
+int attn_delta(const AttnArgs& a, int dtype, cudaStream_t st) {
+  const dim3 grid((unsigned)a.cap, a.H);
+  if (dtype == ATLAS_F32) attn_delta_kernel<ATLAS_F32><<<grid, kThreads, 0, st>>>(a);
+  else if (dtype == ATLAS_BF16) attn_delta_kernel<ATLAS_BF16><<<grid, kThreads, 0, st>>>(a);
+  else attn_delta_kernel<ATLAS_F16><<<grid, kThreads, 0, st>>>(a);
+  return check_launch("attention_grad");
+}
+
+namespace {
+
 template <typename K>
 int big_smem(K kernel, int bytes) {
   return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess
@@ -320,7 +332,7 @@ int bwd(const AttnArgs& a, cudaStream_t st) {
   const int bytes = (4 * BT * (DP + 4) + 2 * BT * PP + 2 * BT) * 4;
   if (int rc = big_smem(attn_bwd_simt_kernel<DT, DP, true>, bytes)) return rc;
   if (int rc = big_smem(attn_bwd_simt_kernel<DT, DP, false>, bytes)) return rc;
-  attn_delta_kernel<DT><<<dim3((unsigned)a.cap, a.H), kThreads, 0, st>>>(a);
+  if (int rc = attn_delta(a, DT, st)) return rc;
   attn_bwd_simt_kernel<DT, DP, true><<<dim3((unsigned)(2 * a.cap), a.Hk), kThreads, bytes, st>>>(a);
   attn_bwd_simt_kernel<DT, DP, false><<<dim3((unsigned)(2 * a.cap), a.H), kThreads, bytes, st>>>(a);
   return check_launch("attention_grad");

@@ -21,6 +21,9 @@
 #include "tc.cuh"
 
 namespace atlas {
+
+int attn_delta(const AttnArgs& a, int dtype, cudaStream_t st);
+
 namespace {
 using namespace tc;
 
@@ -278,9 +281,213 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
   }
 }
 
+// --------------------------------------------------------------------------------------- gradient
+// One launch: CTAs with blockIdx.y < Hk own 128 keys (dk, dv; they loop over the queries of every
+// query head of the key head), the others 128 queries (dq; they loop over the keys). Scores are
+// computed in both, but no sum crosses CTAs. The CTA's two tiles A0, A1 (k, v or q, dout) stay in shared
+// memory, tiles of 64 rows B0, B1 (q, dout or k, v) come in turn:
+//   S = A0 B0^T, dP = A1 B1^T, and with P, dS written over them as 16-bit A operands
+//   keys: dv += P B1, dk += dS B0;  queries: dq += dS B0.
+// Warps 0-7: two threads per row, 32 columns each; warp 8: TMA, and for keys the log-sum-exp and
+// delta of the 64 queries; warp 9: products and TMEM (S, dP, and two sums of 64 columns each).
+constexpr int kBwdThreads = 320;
+constexpr int BN = 64;
+constexpr uint32_t kHalf = BN * 128;
+
+struct BwdSmem {
+  uint8_t a0[kTile], a1[kTile], b0[2][kHalf], b1[2][kHalf];
+  float lse[2][BN], delta[2][BN];  // keys: per loop tile; lse in base 2
+  uint64_t a_full, b_full[2], b_empty[2], s_full, p_full, acc_full;
+  uint32_t tmem;
+};
+
+template <int DT>
+__global__ void __launch_bounds__(kBwdThreads, 2)
+attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
+                   const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mdo, const AttnArgs a, int vec) {
+  extern __shared__ uint8_t raw[];
+  BwdSmem& s = *reinterpret_cast<BwdSmem*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.H / a.Hk;
+  const bool keys = (int)blockIdx.y < a.Hk;
+  const int head = keys ? (int)blockIdx.y : (int)blockIdx.y - a.Hk;  // the CTA's own head
+  const SeqBlock b = seq_block(a, blockIdx.x);
+  int64_t z0, z1;
+  if (idle_rows(a, b, blockIdx.x, &z0, &z1)) {
+    if (keys) {
+      zero_rows16(a.dk, a.sdk, b.outer, head, z0, z1, a.D);
+      zero_rows16(a.dv, a.sdv, b.outer, head, z0, z1, a.D);
+    } else {
+      zero_rows16(a.dq, a.sdq, b.outer, head, z0, z1, a.D);
+    }
+  }
+  if (!b.on || b.first >= b.len) return;
+  const int per = (b.len + BN - 1) / BN;       // loop tiles of one head
+  const int n = keys ? per * group : per;
+  const int live = min(4, (b.len - b.first + 31) / 32);  // lane quarters that have a row
+  if (threadIdx.x == 0) {
+    mbar_init(&s.a_full, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.b_full[i], 33);
+      mbar_init(&s.b_empty[i], 1);
+    }
+    mbar_init(&s.s_full, 1);
+    mbar_init(&s.p_full, live * 64);
+    mbar_init(&s.acc_full, 1);
+    fence_barrier_init();
+  }
+  if (warp == 9) tmem_alloc(&s.tmem, 256);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s.tmem;
+  const int64_t vec0 = b.outer * a.H * a.rows + b.row0;  // lse and delta of query head h: + h rows
+
+  if (warp == 8) {
+    const int r0 = (int)b.row0, o = (int)b.outer, kh = keys ? head : head / group;
+    if (lane == 0) {
+      mbar_arrive_expect_tx(&s.a_full, 2 * kTile);
+      for (int half = 0; half < 2; ++half) {  // boxes of 64 rows
+        tma_load_4d(s.a0 + half * kHalf, keys ? &mk : &mq, 0, r0 + b.first + half * BN, head, o, &s.a_full);
+        tma_load_4d(s.a1 + half * kHalf, keys ? &mv : &mdo, 0, r0 + b.first + half * BN, head, o, &s.a_full);
+      }
+    }
+    for (int i = 0; i < n; ++i) {
+      const int st = i & 1, row = (i % per) * BN, h = keys ? head * group + i / per : kh;
+      if (i >= 2 && !mbar_wait(&s.b_empty[st], ((i >> 1) & 1) ^ 1, 211)) break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&s.b_full[st], 2 * kHalf);
+        tma_load_4d(s.b0[st], keys ? &mq : &mk, 0, r0 + row, h, o, &s.b_full[st]);
+        tma_load_4d(s.b1[st], keys ? &mdo : &mv, 0, r0 + row, h, o, &s.b_full[st]);
+      }
+      if (keys) {
+        for (int j = lane; j < BN; j += 32) {
+          const bool on = row + j < b.len;
+          const int64_t at = vec0 + (int64_t)h * a.rows + row + j;
+          s.lse[st][j] = on ? a.lse[at] * kLog2e : 0.f;
+          s.delta[st][j] = on ? a.delta[at] : 0.f;
+        }
+      }
+      mbar_arrive(&s.b_full[st]);
+    }
+  } else if (warp == 9) {
+    const uint32_t base = DT == ATLAS_BF16 ? idesc_bf16_f32(BM, 0) : idesc_f16_f32(BM, 0);
+    const uint32_t id_sum = base | kMnB | (64u >> 3) << 17;
+    const uint32_t a0 = smem_u32(s.a0), a1 = smem_u32(s.a1);
+    bool ok = mbar_wait(&s.a_full, 0, 212);
+    for (int i = 0; ok && i < n; ++i) {
+      const int st = i & 1, cols = min(BN, b.len - (i % per) * BN), c16 = up16(cols);
+      // S(i) overwrites P(i-1) and dS(i-1): the products that read them must be done
+      if (i && !mbar_wait(&s.b_empty[st ^ 1], ((i - 1) >> 1) & 1, 218)) break;
+      if (!mbar_wait(&s.b_full[st], (i >> 1) & 1, 213)) break;
+      if (cols & 15) {
+        zero_tile_rows(s.b0[st], cols, c16, lane);
+        if (keys) zero_tile_rows(s.b1[st], cols, c16, lane);
+      }
+      tc_fence_after();
+      const uint32_t b0 = smem_u32(s.b0[st]), b1 = smem_u32(s.b1[st]);
+      if (lane == 0) {
+        const uint32_t id = base | (uint32_t)(c16 >> 3) << 17;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) mma_f16(tmem, sdesc_k_sw128(a0 + kk * 32), sdesc_k_sw128(b0 + kk * 32), id, kk > 0);
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) mma_f16(tmem + 64, sdesc_k_sw128(a1 + kk * 32), sdesc_k_sw128(b1 + kk * 32), id, kk > 0);
+        mma_commit(&s.s_full);
+      }
+      __syncwarp();
+      if (!mbar_wait(&s.p_full, i & 1, 214)) break;
+      tc_fence_after();
+      if (lane == 0) {
+        // P and dS are 16-bit over the first half of each thread's own 32 columns of S and dP: the K
+        // elements 0-31 in columns 0-15, 32-63 in columns 32-47
+        for (int kk = 0; kk < c16 / 16; ++kk) {
+          const uint32_t col = (kk >> 1) * 32 + (kk & 1) * 8;
+          if (keys) mma_f16_ts(tmem + 128, tmem + col, sdesc_mn_sw128(b1 + kk * 2048), id_sum, i > 0 || kk > 0);
+          mma_f16_ts(tmem + 192, tmem + 64 + col, sdesc_mn_sw128(b0 + kk * 2048), id_sum, i > 0 || kk > 0);
+        }
+        mma_commit(&s.b_empty[st]);
+        if (i == n - 1) mma_commit(&s.acc_full);
+      }
+      __syncwarp();
+    }
+  } else if ((warp & 3) < live) {
+    const int quarter = warp & 3, half = warp >> 2;  // columns 32 half .. of every loop tile
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+    const int row = b.first + quarter * 32 + lane;
+    const float c = a.scale * kLog2e;
+    float lse = 0.f, delta = 0.f;
+    if (!keys && row < b.len) {
+      lse = a.lse[vec0 + (int64_t)head * a.rows + row] * kLog2e;
+      delta = a.delta[vec0 + (int64_t)head * a.rows + row];
+    }
+    bool ok = true;
+    for (int i = 0; i < n; ++i) {
+      const int st = i & 1, left = min(BN, b.len - (i % per) * BN) - half * 32;  // columns of this thread's part
+      ok = mbar_wait(&s.s_full, i & 1, 215);
+      if (!ok) break;
+      tc_fence_after();
+      if (keys) {  // written by warp 8 before b_full, which the products waited for; seen here by its own wait
+        ok = mbar_wait(&s.b_full[st], (i >> 1) & 1, 216);
+        if (!ok) break;
+      }
+      if (left > 0) {
+        uint32_t x[32], y[32];
+        tmem_ld32(lanes + half * 32, x);
+        tmem_ld32(lanes + 64 + half * 32, y);
+        tmem_ld_wait();
+        uint32_t p[16], d[16];
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+          float w[2], g[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float l = keys ? s.lse[st][half * 32 + j + e] : lse, dl = keys ? s.delta[st][half * 32 + j + e] : delta;
+            w[e] = ex2(fmaf(__uint_as_float(x[j + e]), c, -l));
+            g[e] = w[e] * (__uint_as_float(y[j + e]) - dl);
+            if (j + e >= left) w[e] = g[e] = 0.f;
+          }
+          p[j / 2] = pack2<DT>(w[0], w[1]);
+          d[j / 2] = pack2<DT>(g[0], g[1]);
+        }
+        if (keys) tmem_st16(lanes + half * 32, p);
+        tmem_st16(lanes + 64 + half * 32, d);
+        tmem_st_wait();
+      }
+      tc_fence_before();
+      mbar_arrive(&s.p_full);
+    }
+    if (ok) ok = mbar_wait(&s.acc_full, 0, 217);
+    tc_fence_after();
+    // keys: warps 0-3 write dv, 4-7 dk; queries: warps 4-7 write dq
+    if (ok && (keys || half)) {
+      float acc[64];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t r[32];
+        tmem_ld32(lanes + 128 + half * 64 + h * 32, r);
+        tmem_ld_wait();
+#pragma unroll
+        for (int d = 0; d < 32; ++d) acc[h * 32 + d] = __uint_as_float(r[d]);
+      }
+      if (row < b.len) {
+        void* out = !half ? a.dv : keys ? a.dk : a.dq;
+        const Strides& so = !half ? a.sdv : keys ? a.sdk : a.sdq;
+        uint16_t* dst = reinterpret_cast<uint16_t*>(out) + b.outer * so.outer + head * so.head + (b.row0 + row) * so.row;
+        store_row<DT>(dst, acc, half ? a.scale : 1.f, a.D, vec);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 256);
+  }
+}
+
 // ------------------------------------------------------------------------------------------- host
-// [outer, heads, rows, D] as a 4-D map of boxes of 128 rows x 64 elements; columns from D on read as 0.
-int make_map(CUtensorMap* map, const void* base, int dtype, const Strides& st, int64_t outer, int64_t heads, int64_t rows, int D) {
+// [outer, heads, rows, D] as a 4-D map of boxes of `box_rows` rows x 64 elements; columns from D on read as 0.
+int make_map(CUtensorMap* map, const void* base, int dtype, const Strides& st, int64_t outer, int64_t heads, int64_t rows, int D,
+             int box_rows) {
   using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -297,7 +504,7 @@ int make_map(CUtensorMap* map, const void* base, int dtype, const Strides& st, i
   const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)rows, (cuuint64_t)heads, (cuuint64_t)outer};
   const cuuint64_t strides[3] = {rows > 1 ? (cuuint64_t)st.row * 2 : 128, heads > 1 ? (cuuint64_t)st.head * 2 : 128,
                                  outer > 1 ? (cuuint64_t)st.outer * 2 : 128};
-  const cuuint32_t box[4] = {64, BM, 1, 1}, step[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1}, step[4] = {1, 1, 1, 1};
   const CUresult r = encode(map, dtype == ATLAS_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
                             const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -312,9 +519,9 @@ bool map_ok(const void* p, const Strides& s, int64_t outer, int64_t heads, int64
 template <int DT>
 int fwd(const AttnArgs& a, cudaStream_t st) {
   CUtensorMap mq, mk, mv;
-  if (int rc = make_map(&mq, a.q, DT, a.sq, a.outer, a.H, a.rows, a.D)) return rc;
-  if (int rc = make_map(&mk, a.k, DT, a.sk, a.outer, a.Hk, a.rows, a.D)) return rc;
-  if (int rc = make_map(&mv, a.v, DT, a.sv, a.outer, a.Hk, a.rows, a.D)) return rc;
+  if (int rc = make_map(&mq, a.q, DT, a.sq, a.outer, a.H, a.rows, a.D, BM)) return rc;
+  if (int rc = make_map(&mk, a.k, DT, a.sk, a.outer, a.Hk, a.rows, a.D, BM)) return rc;
+  if (int rc = make_map(&mv, a.v, DT, a.sv, a.outer, a.Hk, a.rows, a.D, BM)) return rc;
   const int bytes = sizeof(FwdSmem) + 1024;
   if (cudaFuncSetAttribute(attn_fwd_tc_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
     return fail(ATLAS_ERR_CUDA, "attention: shared memory attribute");
@@ -323,19 +530,37 @@ int fwd(const AttnArgs& a, cudaStream_t st) {
   return check_launch("attention");
 }
 
+template <int DT>
+int bwd(const AttnArgs& a, cudaStream_t st) {
+  CUtensorMap mq, mk, mv, mdo;
+  if (int rc = make_map(&mq, a.q, DT, a.sq, a.outer, a.H, a.rows, a.D, BN)) return rc;
+  if (int rc = make_map(&mk, a.k, DT, a.sk, a.outer, a.Hk, a.rows, a.D, BN)) return rc;
+  if (int rc = make_map(&mv, a.v, DT, a.sv, a.outer, a.Hk, a.rows, a.D, BN)) return rc;
+  if (int rc = make_map(&mdo, a.dout, DT, a.sdo, a.outer, a.H, a.rows, a.D, BN)) return rc;
+  const int bytes = sizeof(BwdSmem) + 1024;
+  if (cudaFuncSetAttribute(attn_bwd_tc_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+    return fail(ATLAS_ERR_CUDA, "attention_grad: shared memory attribute");
+  const int vec = a.D % 8 == 0 && map_ok(a.dq, a.sdq, a.outer, a.H, a.rows) && map_ok(a.dk, a.sdk, a.outer, a.Hk, a.rows) &&
+                  map_ok(a.dv, a.sdv, a.outer, a.Hk, a.rows);
+  if (int rc = attn_delta(a, DT, st)) return rc;
+  attn_bwd_tc_kernel<DT><<<dim3((unsigned)a.cap, a.Hk + a.H), kBwdThreads, bytes, st>>>(mq, mk, mv, mdo, a, vec);
+  return check_launch("attention_grad");
+}
+
 }  // namespace
 
 // Whether the tensor-core kernels take these tensors: 16-bit, every stride a multiple of 16 bytes (a
 // positive one: an expanded axis has none that TMA accepts), a positive scale (the row maximum is
 // taken before the scale).
 bool attn_tc_takes(const AttnArgs& a, int dtype, bool grad) {
-  if (dtype == ATLAS_F32 || !(a.scale > 0.f) || grad) return false;
+  if (dtype == ATLAS_F32 || !(a.scale > 0.f)) return false;
+  if (grad && (a.H + a.Hk > 65535 || !map_ok(a.dout, a.sdo, a.outer, a.H, a.rows))) return false;
   return map_ok(a.q, a.sq, a.outer, a.H, a.rows) && map_ok(a.k, a.sk, a.outer, a.Hk, a.rows) &&
          map_ok(a.v, a.sv, a.outer, a.Hk, a.rows);
 }
 
 int attn_tc(const AttnArgs& a, int dtype, bool grad, cudaStream_t st) {
-  (void)grad;
+  if (grad) return dtype == ATLAS_BF16 ? bwd<ATLAS_BF16>(a, st) : bwd<ATLAS_F16>(a, st);
   return dtype == ATLAS_BF16 ? fwd<ATLAS_BF16>(a, st) : fwd<ATLAS_F16>(a, st);
 }
 
