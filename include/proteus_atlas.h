@@ -340,7 +340,7 @@ int atlas_seq_maps(const void* lengths, int lengths_i64, int64_t B, int64_t rows
  * head h uses key head h / (H/Hk), whose gradient is the sum over its query heads. D in [1, 64].
  * strides_host: a HOST array with (outer, head, row) strides in elements for each tensor, in the order
  * q, k, v, out (attention) or dout, q, k, v, out, dq, dk, dv (attention_grad); unit stride along D.
- * lse and delta (workspace): f32 [outer, H, rows] contiguous. cu, blocks [cap, 2], counts: as written by
+ * lse: f32 [outer, H, rows] contiguous. ws: device bytes >= atlas_attention_grad_ws_bytes(...). cu, blocks [cap, 2], counts: as written by
  * atlas_seq_maps; padded (packed = 0): outer = B, sequence b in the first cu[b+1]-cu[b] rows of outer
  * index b; packed: outer = 1, its rows are cu[b] .. cu[b+1]-1. Rows of no sequence are not read and
  * come out as zero. S, the softmax and all sums are fp32; for 16-bit tensors the probabilities and dS
@@ -350,10 +350,11 @@ int atlas_attention(const void* q, const void* k, const void* v, int dtype, cons
                     int64_t rows, int64_t H, int64_t Hk, int64_t D, const int32_t* cu, const int32_t* blocks,
                     const int64_t* counts, int64_t B, int64_t cap, int packed, double scale, void* out, float* lse,
                     void* stream);
+int64_t atlas_attention_grad_ws_bytes(int64_t outer, int64_t rows, int64_t H, int64_t Hk, int64_t B);
 int atlas_attention_grad(const void* dout, const void* q, const void* k, const void* v, const void* out, const float* lse,
                          int dtype, const int64_t* strides_host, int64_t outer, int64_t rows, int64_t H, int64_t Hk,
                          int64_t D, const int32_t* cu, const int32_t* blocks, const int64_t* counts, int64_t B,
-                         int64_t cap, int packed, double scale, void* dq, void* dk, void* dv, float* delta, void* stream);
+                         int64_t cap, int packed, double scale, void* dq, void* dk, void* dv, void* ws, int64_t ws_bytes, void* stream);
 
 /* ------------------------------------------------------------------------------------------------
  * Log probabilities of given tokens, and their gradient. No counterpart in the reference.

@@ -46,14 +46,19 @@ extern "C" int atlas_attention(const void* q, const void* k, const void* v, int 
   return (attn_tc_takes(a, dtype, false) ? attn_tc : attn_simt)(a, dtype, false, (cudaStream_t)stream);
 }
 
+extern "C" int64_t atlas_attention_grad_ws_bytes(int64_t outer, int64_t rows, int64_t H, int64_t Hk, int64_t B) {
+  return 4 * (outer * H * rows + B * Hk);
+}
+
 extern "C" int atlas_attention_grad(const void* dout, const void* q, const void* k, const void* v, const void* out,
                                     const float* lse, int dtype, const int64_t* strides_host, int64_t outer, int64_t rows,
                                     int64_t H, int64_t Hk, int64_t D, const int32_t* cu, const int32_t* blocks,
                                     const int64_t* counts, int64_t B, int64_t cap, int packed, double scale, void* dq,
-                                    void* dk, void* dv, float* delta, void* stream) {
+                                    void* dk, void* dv, void* ws, int64_t ws_bytes, void* stream) {
   ATLAS_REQUIRE(strides_host, "attention_grad: null pointer");
   AttnArgs a{};
-  a.dout = dout; a.q = q; a.k = k; a.v = v; a.o = out; a.lse = const_cast<float*>(lse); a.delta = delta;
+  a.dout = dout; a.q = q; a.k = k; a.v = v; a.o = out; a.lse = const_cast<float*>(lse);
+  a.delta = (float*)ws;
   a.dq = dq; a.dk = dk; a.dv = dv;
   a.sdo = at(strides_host, 0); a.sq = at(strides_host, 1); a.sk = at(strides_host, 2); a.sv = at(strides_host, 3);
   a.so = at(strides_host, 4); a.sdq = at(strides_host, 5); a.sdk = at(strides_host, 6); a.sdv = at(strides_host, 7);
@@ -62,6 +67,9 @@ extern "C" int atlas_attention_grad(const void* dout, const void* q, const void*
   a.H = H < 1 || H > 65535 ? 0 : (int)H; a.Hk = Hk < 1 || Hk > 65535 ? 0 : (int)Hk; a.D = D < 1 || D > kAttnMaxDim ? 0 : (int)D;
   a.packed = packed; a.scale = (float)scale;
   if (int rc = check(a, dtype, "attention_grad")) return rc;
-  ATLAS_REQUIRE(dout && out && dq && dk && dv && delta, "attention_grad: null pointer");
+  ATLAS_REQUIRE(dout && out && dq && dk && dv && ws, "attention_grad: null pointer");
+  ATLAS_REQUIRE(ws_bytes >= atlas_attention_grad_ws_bytes(outer, rows, H, Hk, B) && (uintptr_t)ws % 4 == 0,
+                "attention_grad: workspace too small");
+  a.amax = (uint32_t*)ws + outer * H * rows;
   return (attn_tc_takes(a, dtype, true) ? attn_tc : attn_simt)(a, dtype, true, (cudaStream_t)stream);
 }

@@ -19,6 +19,7 @@ struct AttnArgs {
   Strides sq, sk, sv, so, sdo, sdq, sdk, sdv;
   float* lse;    // [outer, H, rows]
   float* delta;  // [outer, H, rows], gradient only
+  uint32_t* amax;  // [B, Hk] bits of the largest |dout|, fp16 gradient on tensor cores only
   const int32_t *cu, *blocks;
   const int64_t* counts;
   int64_t outer, rows, B, cap;

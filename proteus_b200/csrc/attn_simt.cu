@@ -281,32 +281,74 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_simt_kernel(const AttnArgs 
   }
 }
 
-// delta = sum_d dout out, one warp per row of a block and head.
-template <int DT>
+// delta = sum_d dout out of the rows of a block and head, G lanes to a row: 8 lanes with 16-byte loads
+// where rows are aligned for them (VEC), else a warp. For fp16 also the largest |dout| of a sequence and key
+// head (as bits, so that the order of the atomics does not matter).
+template <int DT, bool VEC>
 __global__ void __launch_bounds__(kThreads) attn_delta_kernel(const AttnArgs a) {
   using T = typename Elem<DT>::T;
+  constexpr int E = VEC ? 16 / sizeof(T) : 1;      // elements per load
+  constexpr int G = VEC ? kAttnMaxDim / E : 32;    // lanes per row
+  constexpr int PER = kThreads / G;                // rows at a time
   const SeqBlock s = seq_block(a, blockIdx.x);
   if (!s.on) return;
-  const int head = blockIdx.y, lane = threadIdx.x & 31;
+  const int head = blockIdx.y, sub = threadIdx.x % G;
   const T* o = reinterpret_cast<const T*>(a.o) + s.outer * a.so.outer + head * a.so.head + s.row0 * a.so.row;
   const T* g = reinterpret_cast<const T*>(a.dout) + s.outer * a.sdo.outer + head * a.sdo.head + s.row0 * a.sdo.row;
-  for (int r = s.first + (threadIdx.x >> 5); r < min(s.len, s.first + kAttnBlock); r += kThreads / 32) {
+  float amax = 0.f;
+#pragma unroll 4
+  for (int k = 0; k < kAttnBlock / PER; ++k) {
+    const int r = s.first + k * PER + (int)threadIdx.x / G;
     float v = 0.f;
-    for (int d = lane; d < a.D; d += 32)
-      v = fmaf(Elem<DT>::f(o[(int64_t)r * a.so.row + d]), Elem<DT>::f(g[(int64_t)r * a.sdo.row + d]), v);
+    if (r < s.len)
+      for (int d = sub * E; d < a.D; d += G * E) {
+        T x[E], y[E];
+        if (VEC) {
+          *reinterpret_cast<uint4*>(x) = __ldg(reinterpret_cast<const uint4*>(o + (int64_t)r * a.so.row + d));
+          *reinterpret_cast<uint4*>(y) = __ldg(reinterpret_cast<const uint4*>(g + (int64_t)r * a.sdo.row + d));
+        } else {
+          x[0] = o[(int64_t)r * a.so.row + d];
+          y[0] = g[(int64_t)r * a.sdo.row + d];
+        }
 #pragma unroll
-    for (int k = 16; k; k >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, k);
-    if (lane == 0) a.delta[(s.outer * a.H + head) * a.rows + s.row0 + r] = v;
+        for (int e = 0; e < E; ++e) {
+          const float w = Elem<DT>::f(y[e]);
+          v = fmaf(Elem<DT>::f(x[e]), w, v);
+          if (DT == ATLAS_F16) amax = fabsf(w) > amax || w != w ? fabsf(w) : amax;
+        }
+      }
+#pragma unroll
+    for (int m = G / 2; m; m >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, m);
+    if (sub == 0 && r < s.len) a.delta[(s.outer * a.H + head) * a.rows + s.row0 + r] = v;
+  }
+  if (DT == ATLAS_F16 && a.amax) {
+    const uint32_t u = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(amax));
+    if ((threadIdx.x & 31) == 0) atomicMax(a.amax + (int64_t)s.seq * a.Hk + head / (a.H / a.Hk), u);
   }
 }
 
 }  // namespace
 
-int attn_delta(const AttnArgs& a, int dtype, cudaStream_t st) {
+namespace {
+bool delta_vec(const void* p, const Strides& s, int esize) {
+  const int64_t m = 16 / esize;
+  return (uintptr_t)p % 16 == 0 && s.row % m == 0 && s.head % m == 0 && s.outer % m == 0;
+}
+template <int DT>
+void launch_delta(const AttnArgs& a, cudaStream_t st) {
   const dim3 grid((unsigned)a.cap, a.H);
-  if (dtype == ATLAS_F32) attn_delta_kernel<ATLAS_F32><<<grid, kThreads, 0, st>>>(a);
-  else if (dtype == ATLAS_BF16) attn_delta_kernel<ATLAS_BF16><<<grid, kThreads, 0, st>>>(a);
-  else attn_delta_kernel<ATLAS_F16><<<grid, kThreads, 0, st>>>(a);
+  const int size = DT == ATLAS_F32 ? 4 : 2;
+  if (a.D * size % 16 == 0 && delta_vec(a.o, a.so, size) && delta_vec(a.dout, a.sdo, size))
+    attn_delta_kernel<DT, true><<<grid, kThreads, 0, st>>>(a);
+  else
+    attn_delta_kernel<DT, false><<<grid, kThreads, 0, st>>>(a);
+}
+}  // namespace
+
+int attn_delta(const AttnArgs& a, int dtype, cudaStream_t st) {
+  if (dtype == ATLAS_F32) launch_delta<ATLAS_F32>(a, st);
+  else if (dtype == ATLAS_BF16) launch_delta<ATLAS_BF16>(a, st);
+  else launch_delta<ATLAS_F16>(a, st);
   return check_launch("attention_grad");
 }
 

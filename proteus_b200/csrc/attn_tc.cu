@@ -301,6 +301,14 @@ struct BwdSmem {
   uint32_t tmem;
 };
 
+// dS of fp16 gradients is held in fp16, whose range ends at 6e-8: it is scaled by the power of two that
+// brings the largest |dout| of its sequence and key head to 2^-4, which leaves room for |v| summed over
+// the head dimension up to 2^19, and dk, dq are scaled back in fp32.
+__device__ __forceinline__ float gain_of(uint32_t amax_bits) {
+  const int e = (int)(amax_bits >> 23);
+  return e == 0 || e >= 250 ? 1.f : __uint_as_float((uint32_t)(250 - e) << 23);
+}
+
 template <int DT>
 __global__ void __launch_bounds__(kBwdThreads, 2)
 attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
@@ -414,6 +422,7 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
     const int row = b.first + quarter * 32 + lane;
     const float c = a.scale * kLog2e;
+    const float gain = DT == ATLAS_F16 ? gain_of(a.amax[(int64_t)b.seq * a.Hk + (keys ? head : head / group)]) : 1.f;
     float lse = 0.f, delta = 0.f;
     if (!keys && row < b.len) {
       lse = a.lse[vec0 + (int64_t)head * a.rows + row] * kLog2e;
@@ -442,7 +451,7 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
           for (int e = 0; e < 2; ++e) {
             const float l = keys ? s.lse[st][half * 32 + j + e] : lse, dl = keys ? s.delta[st][half * 32 + j + e] : delta;
             w[e] = ex2(fmaf(__uint_as_float(x[j + e]), c, -l));
-            g[e] = w[e] * (__uint_as_float(y[j + e]) - dl);
+            g[e] = (DT == ATLAS_F16 ? w[e] * gain : w[e]) * (__uint_as_float(y[j + e]) - dl);
             if (j + e >= left) w[e] = g[e] = 0.f;
           }
           p[j / 2] = pack2<DT>(w[0], w[1]);
@@ -472,7 +481,7 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
         void* out = !half ? a.dv : keys ? a.dk : a.dq;
         const Strides& so = !half ? a.sdv : keys ? a.sdk : a.sdq;
         uint16_t* dst = reinterpret_cast<uint16_t*>(out) + b.outer * so.outer + head * so.head + (b.row0 + row) * so.row;
-        store_row<DT>(dst, acc, half ? a.scale : 1.f, a.D, vec);
+        store_row<DT>(dst, acc, half ? a.scale / gain : 1.f, a.D, vec);
       }
     }
   }
@@ -542,6 +551,8 @@ int bwd(const AttnArgs& a, cudaStream_t st) {
     return fail(ATLAS_ERR_CUDA, "attention_grad: shared memory attribute");
   const int vec = a.D % 8 == 0 && map_ok(a.dq, a.sdq, a.outer, a.H, a.rows) && map_ok(a.dk, a.sdk, a.outer, a.Hk, a.rows) &&
                   map_ok(a.dv, a.sdv, a.outer, a.Hk, a.rows);
+  if (DT == ATLAS_F16 && cudaMemsetAsync(a.amax, 0, (size_t)(a.B * a.Hk) * 4, st) != cudaSuccess)
+    return fail(ATLAS_ERR_CUDA, "attention_grad: clearing the workspace failed");
   if (int rc = attn_delta(a, DT, st)) return rc;
   attn_bwd_tc_kernel<DT><<<dim3((unsigned)a.cap, a.Hk + a.H), kBwdThreads, bytes, st>>>(mq, mk, mv, mdo, a, vec);
   return check_launch("attention_grad");

@@ -156,7 +156,11 @@ def _plain(q, k, v, do, where, scale):
             el = es.amax(-1) + U * (n + 8)  # of the log-sum-exp: its terms' and its sum's
             ep = es + el[..., None]         # relative, of a probability
             ref["out"][o, hs, r], ref["lse"][o, hs, r] = out, lse
-            eo = h * A + (ep * P) @ V.abs() + U * n * A
+            # fp16 below its normal range: half its spacing, of P, and of dS at the scale that brings the
+            # largest |dout| to 2^-4 or more
+            fp = 2.0 ** -25 if dt == torch.float16 else 0.0
+            fs = fp * 16 * G.abs().max()
+            eo = h * A + (ep * P + fp) @ V.abs() + U * n * A
             tol["out"][o, hs, r] = eo + h * out.abs()
             tol["lse"][o, hs, r] = el + U * lse.abs()
             dP = G @ V.T
@@ -164,7 +168,7 @@ def _plain(q, k, v, do, where, scale):
             dS = P * (dP - delta)
             # dP: D products; delta from the rounded output; dS rounded once
             ed = (G.abs() * (eo + h * out.abs() + U * D * out.abs())).sum(-1, keepdim=True)
-            eS = ep * dS.abs() + P * (U * D * (G.abs() @ V.abs().T) + ed) + (h + 3 * U) * dS.abs()
+            eS = ep * dS.abs() + P * (U * D * (G.abs() @ V.abs().T) + ed) + (h + 3 * U) * dS.abs() + fs
             ref["dq"][o, hs, r] = dS @ K * scale
             tol["dq"][o, hs, r] = ((eS + U * n * dS.abs()) @ K.abs()) * abs(scale) + h * ref["dq"][o, hs, r].abs()
             N = n * (H // Hk)
@@ -172,7 +176,7 @@ def _plain(q, k, v, do, where, scale):
             ref["dk"][o, j, r] = t(dS, Q) * scale
             tol["dk"][o, j, r] = t(eS + U * N * dS.abs(), Q.abs()) * abs(scale) + h * ref["dk"][o, j, r].abs()
             ref["dv"][o, j, r] = t(P, G)
-            tol["dv"][o, j, r] = t((ep + h + U * N) * P, G.abs()) + h * ref["dv"][o, j, r].abs()
+            tol["dv"][o, j, r] = t((ep + h + U * N) * P + fp, G.abs()) + h * ref["dv"][o, j, r].abs()
     tiny = torch.finfo(dt).tiny if dt != torch.float32 else 0.0
     for name in ("out", "dq", "dk", "dv"):
         tol[name] += tiny
@@ -219,6 +223,29 @@ def test_attention_scale_and_sharp_scores(dtype):
         out, lse = KN.attention(q, k, v, plan, scale)
         dq, dk, dv = KN.attention_grad(do, q, k, v, out, lse, plan, scale)
         _check({"out": out, "lse": lse, "dq": dq, "dk": dk, "dv": dv}, ref, tol)
+
+
+@pytest.mark.parametrize("size", [2.0 ** -12, 1.0, 2.0 ** 5, 2.0 ** 9])
+def test_attention_gradient_of_small_and_large_fp16(size):
+    """Incoming fp16 gradients far from 1: dS would leave fp16's range at its ends; one sequence of
+    gradients 2^6 larger than the others' keeps its own range. (At 2^9 that sequence's own gradients pass
+    65504, fp16's largest: infinite, and no concern of the others.)"""
+    KN = _kn()
+    q, k, v, do, plan, where, _ = _batch([300, 65, 140], True, 4, 2, 64, torch.float16, seed=11)
+    do = do * size
+    do[:, :, 300:365] *= 64
+    ref, tol = _plain(q, k, v, do, where, 0.125)
+    out, lse = KN.attention(q, k, v, plan)
+    dq, dk, dv = KN.attention_grad(do, q, k, v, out, lse, plan)
+    step = 2.0 ** -25  # half the spacing of fp16 below its normal range
+    for name in ("dq", "dk", "dv"):
+        tol[name] += step
+    for o, r in where:
+        if torch.isfinite(do[o, :, r]).all():
+            _check({n: t[o, :, r] for n, t in (("dq", dq), ("dk", dk), ("dv", dv))}, {n: t[o, :, r] for n, t in ref.items()},
+                   {n: t[o, :, r] for n, t in tol.items()})
+        else:
+            assert size == 2.0 ** 9 and r.start == 300
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
