@@ -47,7 +47,7 @@ extern "C" int atlas_attention(const void* q, const void* k, const void* v, int 
 }
 
 extern "C" int64_t atlas_attention_grad_ws_bytes(int64_t outer, int64_t rows, int64_t H, int64_t Hk, int64_t B) {
-  return 4 * (outer * H * rows + B * Hk);
+  return 4 * (2 * H * attn_vec_ld(outer, rows, B) + B * Hk + 1);
 }
 
 extern "C" int atlas_attention_grad(const void* dout, const void* q, const void* k, const void* v, const void* out,
@@ -58,7 +58,6 @@ extern "C" int atlas_attention_grad(const void* dout, const void* q, const void*
   ATLAS_REQUIRE(strides_host, "attention_grad: null pointer");
   AttnArgs a{};
   a.dout = dout; a.q = q; a.k = k; a.v = v; a.o = out; a.lse = const_cast<float*>(lse);
-  a.delta = (float*)ws;
   a.dq = dq; a.dk = dk; a.dv = dv;
   a.sdo = at(strides_host, 0); a.sq = at(strides_host, 1); a.sk = at(strides_host, 2); a.sv = at(strides_host, 3);
   a.so = at(strides_host, 4); a.sdq = at(strides_host, 5); a.sdk = at(strides_host, 6); a.sdv = at(strides_host, 7);
@@ -68,8 +67,16 @@ extern "C" int atlas_attention_grad(const void* dout, const void* q, const void*
   a.packed = packed; a.scale = (float)scale;
   if (int rc = check(a, dtype, "attention_grad")) return rc;
   ATLAS_REQUIRE(dout && out && dq && dk && dv && ws, "attention_grad: null pointer");
-  ATLAS_REQUIRE(ws_bytes >= atlas_attention_grad_ws_bytes(outer, rows, H, Hk, B) && (uintptr_t)ws % 4 == 0,
-                "attention_grad: workspace too small");
-  a.amax = (uint32_t*)ws + outer * H * rows;
-  return (attn_tc_takes(a, dtype, true) ? attn_tc : attn_simt)(a, dtype, true, (cudaStream_t)stream);
+  ATLAS_REQUIRE(ws_bytes >= atlas_attention_grad_ws_bytes(outer, rows, H, Hk, B) && (uintptr_t)ws % 16 == 0,
+                "attention_grad: workspace too small, or not 16-byte aligned");
+  if (!attn_tc_takes(a, dtype, true)) {
+    a.delta = (float*)ws;
+    return attn_simt(a, dtype, true, (cudaStream_t)stream);
+  }
+  a.vec_ld = attn_vec_ld(outer, rows, B);
+  a.lse2 = (float*)ws;
+  a.delta2 = a.lse2 + H * a.vec_ld;
+  a.amax = (uint32_t*)(a.delta2 + H * a.vec_ld);
+  a.counter = a.amax + B * Hk;
+  return attn_tc(a, dtype, true, (cudaStream_t)stream);
 }

@@ -18,8 +18,13 @@ struct AttnArgs {
   void *out, *dq, *dk, *dv;
   Strides sq, sk, sv, so, sdo, sdq, sdk, sdv;
   float* lse;    // [outer, H, rows]
-  float* delta;  // [outer, H, rows], gradient only
-  uint32_t* amax;  // [B, Hk] bits of the largest |dout|, fp16 gradient on tensor cores only
+  // Gradient only. CUDA cores: delta [outer, H, rows]. Tensor cores: for each head the log-sum-exp in
+  // base 2 and delta of all sequences, each from a place that is a multiple of 16 bytes (seq_block's off;
+  // vec_ld values a head), the largest |dout| of a sequence and key head as bits (fp16), and the counter of
+  // work items.
+  float *delta, *lse2, *delta2;
+  int64_t vec_ld;
+  uint32_t *amax, *counter;
   const int32_t *cu, *blocks;
   const int64_t* counts;
   int64_t outer, rows, B, cap;
@@ -32,7 +37,7 @@ struct AttnArgs {
 // table or prefix sums that do not belong to these tensors cannot lead outside them.
 struct SeqBlock {
   int seq, first, len;
-  int64_t row0, outer;
+  int64_t row0, outer, off;
   bool on;     // an entry with a sequence
   bool spare;  // an entry behind the last
 };
@@ -40,9 +45,9 @@ struct SeqBlock {
 __device__ __forceinline__ SeqBlock seq_block(const AttnArgs& a, int64_t i) {
   SeqBlock s{};
   const int64_t n = a.counts[1];
+  const int2 e = reinterpret_cast<const int2*>(a.blocks)[i];  // i < cap: both loads are under way at once
   s.spare = i >= n;
   if (s.spare) return s;
-  const int2 e = reinterpret_cast<const int2*>(a.blocks)[i];
   if (e.x < 0 || e.x >= a.B || e.y < 0) return s;
   const int64_t c0 = a.cu[e.x], c1 = a.cu[e.x + 1];
   s.seq = e.x;
@@ -52,6 +57,8 @@ __device__ __forceinline__ SeqBlock seq_block(const AttnArgs& a, int64_t i) {
   if (s.row0 < 0 || s.row0 > a.rows || s.outer >= a.outer) return s;
   const int64_t len = c1 - c0, room = a.rows - s.row0;
   s.len = (int)(len < 0 ? 0 : len > room ? room : len);
+  if (c0 < 0 || c0 + s.len > a.outer * a.rows) return s;
+  s.off = (c0 + 4 * (int64_t)e.x + 3) & ~(int64_t)3;
   s.on = true;
   return s;
 }
@@ -76,5 +83,9 @@ __device__ __forceinline__ bool idle_rows(const AttnArgs& a, const SeqBlock& s, 
   *to = a.rows;
   return *to > *from;
 }
+
+// Values a head of the padded vectors: every sequence's rows and up to 4 between two, and 128 that a
+// tile may read behind the last.
+inline int64_t attn_vec_ld(int64_t outer, int64_t rows, int64_t B) { return (outer * rows + 4 * B + 128 + 7) / 4 * 4; }
 
 }  // namespace atlas

@@ -109,8 +109,8 @@ template <int DT>
 __device__ __forceinline__ void zero_rows(void* dst, const Strides& st, int64_t outer, int head, int64_t from, int64_t to, int D) {
   using T = typename Elem<DT>::T;
   T* p = reinterpret_cast<T*>(dst) + outer * st.outer + head * st.head;
-  const int64_t n = (to - from) * D;
-  for (int64_t i = threadIdx.x; i < n; i += kThreads) put<DT>(p + (from + i / D) * st.row + i % D, 0.f);
+  for (int64_t r = from + threadIdx.x / 32; r < to; r += kThreads / 32)
+    for (int d = threadIdx.x % 32; d < D; d += 32) put<DT>(p + r * st.row + d, 0.f);
 }
 
 template <int DT, int DP>
@@ -282,8 +282,8 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_simt_kernel(const AttnArgs 
 }
 
 // delta = sum_d dout out of the rows of a block and head, G lanes to a row: 8 lanes with 16-byte loads
-// where rows are aligned for them (VEC), else a warp. For fp16 also the largest |dout| of a sequence and key
-// head (as bits, so that the order of the atomics does not matter).
+// where rows are aligned for them (VEC), else a warp. For the tensor-core kernels also what they need
+// beside it (see AttnArgs); the largest |dout| as bits, so that the order of the atomics does not matter.
 template <int DT, bool VEC>
 __global__ void __launch_bounds__(kThreads) attn_delta_kernel(const AttnArgs a) {
   using T = typename Elem<DT>::T;
@@ -291,8 +291,19 @@ __global__ void __launch_bounds__(kThreads) attn_delta_kernel(const AttnArgs a) 
   constexpr int G = VEC ? kAttnMaxDim / E : 32;    // lanes per row
   constexpr int PER = kThreads / G;                // rows at a time
   const SeqBlock s = seq_block(a, blockIdx.x);
-  if (!s.on) return;
   const int head = blockIdx.y, sub = threadIdx.x % G;
+  if (a.lse2) {  // before the tensor-core kernel: its counter, and the rows that it does not write
+    if (blockIdx.x == 0 && head == 0 && threadIdx.x == 0) *a.counter = 0;
+    int64_t z0, z1;
+    if (idle_rows(a, s, blockIdx.x, &z0, &z1)) {
+      zero_rows<DT>(a.dq, a.sdq, s.outer, head, z0, z1, a.D);
+      if (head < a.Hk) {
+        zero_rows<DT>(a.dk, a.sdk, s.outer, head, z0, z1, a.D);
+        zero_rows<DT>(a.dv, a.sdv, s.outer, head, z0, z1, a.D);
+      }
+    }
+  }
+  if (!s.on) return;
   const T* o = reinterpret_cast<const T*>(a.o) + s.outer * a.so.outer + head * a.so.head + s.row0 * a.so.row;
   const T* g = reinterpret_cast<const T*>(a.dout) + s.outer * a.sdo.outer + head * a.sdo.head + s.row0 * a.sdo.row;
   float amax = 0.f;
@@ -319,9 +330,17 @@ __global__ void __launch_bounds__(kThreads) attn_delta_kernel(const AttnArgs a) 
       }
 #pragma unroll
     for (int m = G / 2; m; m >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, m);
-    if (sub == 0 && r < s.len) a.delta[(s.outer * a.H + head) * a.rows + s.row0 + r] = v;
+    if (sub == 0 && r < s.len) {
+      const int64_t at = (s.outer * a.H + head) * a.rows + s.row0 + r;
+      if (a.lse2) {
+        a.lse2[head * a.vec_ld + s.off + r] = a.lse[at] * 1.4426950408889634f;
+        a.delta2[head * a.vec_ld + s.off + r] = v;
+      } else {
+        a.delta[at] = v;
+      }
+    }
   }
-  if (DT == ATLAS_F16 && a.amax) {
+  if (DT == ATLAS_F16 && a.lse2) {
     const uint32_t u = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(amax));
     if ((threadIdx.x & 31) == 0) atomicMax(a.amax + (int64_t)s.seq * a.Hk + head / (a.H / a.Hk), u);
   }

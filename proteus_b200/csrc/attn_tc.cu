@@ -49,28 +49,21 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 // Zero rows [from, to) of one head (16-bit elements).
 __device__ void zero_rows16(void* dst, const Strides& st, int64_t outer, int head, int64_t from, int64_t to, int D) {
   uint16_t* p = reinterpret_cast<uint16_t*>(dst) + outer * st.outer + head * st.head;
-  const int64_t n = (to - from) * D;
-  for (int64_t i = threadIdx.x; i < n; i += blockDim.x) p[(from + i / D) * st.row + i % D] = 0;
+  for (int64_t r = from + (threadIdx.x >> 5); r < to; r += blockDim.x >> 5)
+    for (int d = threadIdx.x & 31; d < D; d += 32) p[r * st.row + d] = 0;
 }
 
-// One row of 64 accumulators, times `mul`, as D 16-bit elements; `vec`: 16-byte stores are aligned.
-template <int DT>
-__device__ __forceinline__ void store_row(void* dst, const float (&acc)[64], float mul, int D, bool vec) {
+// Up to 32 packed 16-bit elements of a row, of which `n` (or more, or none) exist; `vec`: 16-byte stores
+// are aligned and n a multiple of 8.
+__device__ __forceinline__ void store32(uint16_t* dst, const uint32_t (&w)[16], int n, bool vec) {
   if (vec) {
 #pragma unroll
-    for (int d = 0; d < 64; d += 8)
-      if (d < D) {
-        uint4 w;
-        w.x = pack2<DT>(acc[d] * mul, acc[d + 1] * mul);
-        w.y = pack2<DT>(acc[d + 2] * mul, acc[d + 3] * mul);
-        w.z = pack2<DT>(acc[d + 4] * mul, acc[d + 5] * mul);
-        w.w = pack2<DT>(acc[d + 6] * mul, acc[d + 7] * mul);
-        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(dst) + d) = w;
-      }
+    for (int q = 0; q < 4; ++q)
+      if (q * 8 < n) *reinterpret_cast<uint4*>(dst + q * 8) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
   } else {
 #pragma unroll
-    for (int d = 0; d < 64; ++d)
-      if (d < D) reinterpret_cast<uint16_t*>(dst)[d] = (uint16_t)pack2<DT>(acc[d] * mul, 0.f);
+    for (int e = 0; e < 32; ++e)
+      if (e < n) dst[e] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
   }
 }
 
@@ -154,16 +147,16 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
   } else if (warp == 5) {
     const uint32_t base = DT == ATLAS_BF16 ? idesc_bf16_f32(BM, 0) : idesc_f16_f32(BM, 0);
     const uint32_t id_pv = base | kMnB | (64u >> 3) << 17;
+    const uint64_t qd = sdesc_k_sw128(smem_u32(s.q)), kd = sdesc_k_sw128(smem_u32(s.k[0])), vd = sdesc_mn_sw128(smem_u32(s.v[0]));
     // S(i) = q k(i)^T into buffer i & 1
     auto scores = [&](int i) {
       if (!mbar_wait(&s.k_full[i & 1], (i >> 1) & 1, 203)) return false;
       tc_fence_after();
-      if (lane == 0) {
+      if (elect_one()) {
         const uint32_t id = base | (uint32_t)(up16(min(BM, b.len - i * BM)) >> 3) << 17;
-        const uint32_t q = smem_u32(s.q), k = smem_u32(s.k[i & 1]);
+        const uint64_t k = kd + (i & 1) * (kTile >> 4);
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk)
-          mma_f16(tmem + (i & 1) * 128, sdesc_k_sw128(q + kk * 32), sdesc_k_sw128(k + kk * 32), id, kk > 0);
+        for (int kk = 0; kk < 4; ++kk) mma_f16(tmem + (i & 1) * 128, qd + kk * 2, k + kk * 2, id, kk > 0);
         mma_commit(&s.k_empty[i & 1]);
         mma_commit(&s.s_full[i & 1]);
       }
@@ -178,10 +171,11 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
       if (cols & 15) zero_tile_rows(s.v[bf], cols, up16(cols), lane);
       if (!mbar_wait(&s.p_full[bf], ph, 206)) break;
       tc_fence_after();
-      if (lane == 0) {
-        const uint32_t v = smem_u32(s.v[bf]);
-        for (int kk = 0; kk < up16(cols) / 16; ++kk)
-          mma_f16_ts(tmem + bf * 128 + 64, tmem + bf * 128 + kk * 8, sdesc_mn_sw128(v + kk * 2048), id_pv, kk > 0);
+      if (elect_one()) {
+        const uint64_t v = vd + bf * (kTile >> 4);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          if (kk * 16 < cols) mma_f16_ts(tmem + bf * 128 + 64, tmem + bf * 128 + kk * 8, v + kk * 128, id_pv, kk > 0);
         mma_commit(&s.v_empty[bf]);
         mma_commit(&s.o_full[bf]);
       }
@@ -270,7 +264,14 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
     if (ok && row < b.len) {
       a.lse[(b.outer * a.H + head) * a.rows + b.row0 + row] = ((m == kNegInf ? 0.f : m * c) + log2f(l)) * kLn2;
       uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + b.outer * a.so.outer + head * a.so.head + (b.row0 + row) * a.so.row;
-      store_row<DT>(dst, o, 1.f / l, a.D, vec);
+      const float inv = 1.f / l;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t w[16];
+#pragma unroll
+        for (int d = 0; d < 16; ++d) w[d] = pack2<DT>(o[h * 32 + 2 * d] * inv, o[h * 32 + 2 * d + 1] * inv);
+        store32(dst + h * 32, w, a.D - h * 32, vec);
+      }
     }
   }
   tc_fence_before();
@@ -282,22 +283,37 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
 }
 
 // --------------------------------------------------------------------------------------- gradient
-// One launch: CTAs with blockIdx.y < Hk own 128 keys (dk, dv; they loop over the queries of every
-// query head of the key head), the others 128 queries (dq; they loop over the keys). Scores are
-// computed in both, but no sum crosses CTAs. The CTA's two tiles A0, A1 (k, v or q, dout) stay in shared
-// memory, tiles of 64 rows B0, B1 (q, dout or k, v) come in turn:
-//   S = A0 B0^T, dP = A1 B1^T, and with P, dS written over them as 16-bit A operands
+// Work items: 128 keys of a key head (dk, dv; the loop runs over the queries of every query head that
+// shares it) or 128 queries of a query head (dq; the loop runs over the keys). Scores are computed in
+// both, but no sum crosses items. An item's two tiles A0, A1 (k, v or q, dout) stay in shared memory,
+// tiles of 64 rows B0, B1 (q, dout or k, v) come in turn:
+//   S = A0 B0^T, dP = A1 B1^T, and with the 16-bit P and dS, written over them, as A operands
 //   keys: dv += P B1, dk += dS B0;  queries: dq += dS B0.
-// Warps 0-7: two threads per row, 32 columns each; warp 8: TMA, and for keys the log-sum-exp and
-// delta of the 64 queries; warp 9: products and TMEM (S, dP, and two sums of 64 columns each).
-constexpr int kBwdThreads = 320;
+// One persistent CTA per SM takes items from a counter and runs their tiles as one stream, so that an
+// item's start (look-up, first loads) and end (reading the sums) hide behind its neighbours:
+//   warps 0-15  two groups of eight, each takes every other tile: two threads per row, 32 columns each
+//   warp 16     TMA: items, A tiles (ring of 3), B tiles with the queries' log-sum-exp and delta (ring)
+//   warp 17     scores, up to two tiles ahead of the group that is at work; owns the TMEM
+//   warp 18     sums (products of two small kinds cost their issuing warp 500 clocks a tile each)
+// TMEM: three buffers of S and dP (columns 128 x, 128 x + 64), the sums in 384-447 (dv) and 448-511.
+constexpr int kBwdThreads = 608;
 constexpr int BN = 64;
 constexpr uint32_t kHalf = BN * 128;
+constexpr int kRing = 3;    // items in flight: tile t + 2 may be two items ahead
+constexpr int kStages = 5;  // B tiles in flight
+
+struct BwdItem {
+  int seq, first, len, head, keys, n, row0, outer;  // n: loop tiles; 0 ends the stream
+  int64_t off;                                      // place of the sequence in the padded vectors
+};
 
 struct BwdSmem {
-  uint8_t a0[kTile], a1[kTile], b0[2][kHalf], b1[2][kHalf];
-  float lse[2][BN], delta[2][BN];  // keys: per loop tile; lse in base 2
-  uint64_t a_full, b_full[2], b_empty[2], s_full, p_full, acc_full;
+  uint8_t a0[kRing][kTile], a1[kRing][kTile], b0[kStages][kHalf], b1[kStages][kHalf];
+  float a_lse[kRing][BM], a_delta[kRing][BM];      // queries: of the item's rows
+  float b_lse[kStages][BN], b_delta[kStages][BN];  // keys: of the loop tile's rows
+  BwdItem item[kRing];
+  uint64_t item_full[kRing], item_empty[kRing], a_full[kRing], b_full[kStages], b_empty[kStages], s_full[3], p_full[3],
+      x_done[3], acc_full[kRing], acc_free;
   uint32_t tmem;
 };
 
@@ -309,187 +325,299 @@ __device__ __forceinline__ float gain_of(uint32_t amax_bits) {
   return e == 0 || e >= 250 ? 1.f : __uint_as_float((uint32_t)(250 - e) << 23);
 }
 
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+// P and dS of one thread's 32 columns, over its scores.
+template <int DT, bool KEYS>
+__device__ __forceinline__ void bwd_tile(uint32_t cols, float c, float gain, float lse, float delta, const float* b_lse,
+                                         const float* b_delta, int left) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t x[16], y[16], p[8], d[8];
+    tmem_ld16(cols + h * 16, x);
+    tmem_ld16(cols + 64 + h * 16, y);
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 16; j += 4) {
+      float l4[4] = {lse, lse, lse, lse}, d4[4] = {delta, delta, delta, delta}, w[4], g[4];
+      if (KEYS) {
+        *reinterpret_cast<float4*>(l4) = *reinterpret_cast<const float4*>(b_lse + h * 16 + j);
+        *reinterpret_cast<float4*>(d4) = *reinterpret_cast<const float4*>(b_delta + h * 16 + j);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        w[e] = ex2(fmaf(__uint_as_float(x[j + e]), c, -l4[e]));
+        g[e] = (DT == ATLAS_F16 ? w[e] * gain : w[e]) * (__uint_as_float(y[j + e]) - d4[e]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; e += 2) {
+        p[(j + e) / 2] = pack2<DT>(w[e], w[e + 1]);
+        d[(j + e) / 2] = pack2<DT>(g[e], g[e + 1]);
+      }
+    }
+    if (left < 32) {  // columns behind the end: whatever the scores were, nothing
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int at = h * 16 + 2 * j;
+        const uint32_t keep = at + 1 < left ? 0xFFFFFFFFu : at < left ? 0xFFFFu : 0u;
+        p[j] &= keep;
+        d[j] &= keep;
+      }
+    }
+    if (KEYS) tmem_st8(cols + h * 8, p);
+    tmem_st8(cols + 64 + h * 8, d);
+  }
+  tmem_st_wait();
+}
+
 template <int DT>
-__global__ void __launch_bounds__(kBwdThreads, 2)
+__global__ void __launch_bounds__(kBwdThreads, 1)
 attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                    const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mdo, const AttnArgs a, int vec) {
   extern __shared__ uint8_t raw[];
   BwdSmem& s = *reinterpret_cast<BwdSmem*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.H / a.Hk;
-  const bool keys = (int)blockIdx.y < a.Hk;
-  const int head = keys ? (int)blockIdx.y : (int)blockIdx.y - a.Hk;  // the CTA's own head
-  const SeqBlock b = seq_block(a, blockIdx.x);
-  int64_t z0, z1;
-  if (idle_rows(a, b, blockIdx.x, &z0, &z1)) {
-    if (keys) {
-      zero_rows16(a.dk, a.sdk, b.outer, head, z0, z1, a.D);
-      zero_rows16(a.dv, a.sdv, b.outer, head, z0, z1, a.D);
-    } else {
-      zero_rows16(a.dq, a.sdq, b.outer, head, z0, z1, a.D);
-    }
-  }
-  if (!b.on || b.first >= b.len) return;
-  const int per = (b.len + BN - 1) / BN;       // loop tiles of one head
-  const int n = keys ? per * group : per;
-  const int live = min(4, (b.len - b.first + 31) / 32);  // lane quarters that have a row
   if (threadIdx.x == 0) {
-    mbar_init(&s.a_full, 1);
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&s.b_full[i], 33);
+    for (int i = 0; i < kRing; ++i) {
+      mbar_init(&s.item_full[i], 1);
+      mbar_init(&s.item_empty[i], 18);
+      mbar_init(&s.a_full[i], 1);
+      mbar_init(&s.acc_full[i], 1);
+    }
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&s.b_full[i], 1);
       mbar_init(&s.b_empty[i], 1);
     }
-    mbar_init(&s.s_full, 1);
-    mbar_init(&s.p_full, live * 64);
-    mbar_init(&s.acc_full, 1);
+    for (int i = 0; i < 3; ++i) {
+      mbar_init(&s.s_full[i], 1);
+      mbar_init(&s.p_full[i], 8);
+      mbar_init(&s.x_done[i], 1);
+    }
+    mbar_init(&s.acc_free, 8);
     fence_barrier_init();
   }
-  if (warp == 9) tmem_alloc(&s.tmem, 256);
+  if (warp == 17) tmem_alloc(&s.tmem, 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s.tmem;
-  const int64_t vec0 = b.outer * a.H * a.rows + b.row0;  // lse and delta of query head h: + h rows
 
-  if (warp == 8) {
-    const int r0 = (int)b.row0, o = (int)b.outer, kh = keys ? head : head / group;
+  if (warp == 16) {
     if (lane == 0) {
-      mbar_arrive_expect_tx(&s.a_full, 2 * kTile);
-      for (int half = 0; half < 2; ++half) {  // boxes of 64 rows
-        tma_load_4d(s.a0 + half * kHalf, keys ? &mk : &mq, 0, r0 + b.first + half * BN, head, o, &s.a_full);
-        tma_load_4d(s.a1 + half * kHalf, keys ? &mv : &mdo, 0, r0 + b.first + half * BN, head, o, &s.a_full);
-      }
-    }
-    for (int i = 0; i < n; ++i) {
-      const int st = i & 1, row = (i % per) * BN, h = keys ? head * group + i / per : kh;
-      if (i >= 2 && !mbar_wait(&s.b_empty[st], ((i >> 1) & 1) ^ 1, 211)) break;
-      if (lane == 0) {
-        mbar_arrive_expect_tx(&s.b_full[st], 2 * kHalf);
-        tma_load_4d(s.b0[st], keys ? &mq : &mk, 0, r0 + row, h, o, &s.b_full[st]);
-        tma_load_4d(s.b1[st], keys ? &mdo : &mv, 0, r0 + row, h, o, &s.b_full[st]);
-      }
-      if (keys) {
-        for (int j = lane; j < BN; j += 32) {
-          const bool on = row + j < b.len;
-          const int64_t at = vec0 + (int64_t)h * a.rows + row + j;
-          s.lse[st][j] = on ? a.lse[at] * kLog2e : 0.f;
-          s.delta[st][j] = on ? a.delta[at] : 0.f;
+      const int total = (int)a.cap * (a.Hk + a.H);
+      int next = (int)atomicAdd(a.counter, 1u), k = 0, t = 0;
+      while (true) {
+        BwdItem it{};
+        while (next < total) {  // keys first: theirs are the longest items
+          const int y = next / (int)a.cap, x = next - y * (int)a.cap;
+          const SeqBlock b = seq_block(a, x);
+          next = (int)atomicAdd(a.counter, 1u);
+          if (!b.on || b.first >= b.len) continue;
+          it.keys = y < a.Hk;
+          it.head = it.keys ? y : y - a.Hk;
+          it.seq = b.seq; it.first = b.first; it.len = b.len; it.row0 = (int)b.row0; it.outer = (int)b.outer; it.off = b.off;
+          it.n = (b.len + BN - 1) / BN * (it.keys ? group : 1);
+          break;
         }
-      }
-      mbar_arrive(&s.b_full[st]);
-    }
-  } else if (warp == 9) {
-    const uint32_t base = DT == ATLAS_BF16 ? idesc_bf16_f32(BM, 0) : idesc_f16_f32(BM, 0);
-    const uint32_t id_sum = base | kMnB | (64u >> 3) << 17;
-    const uint32_t a0 = smem_u32(s.a0), a1 = smem_u32(s.a1);
-    bool ok = mbar_wait(&s.a_full, 0, 212);
-    for (int i = 0; ok && i < n; ++i) {
-      const int st = i & 1, cols = min(BN, b.len - (i % per) * BN), c16 = up16(cols);
-      // S(i) overwrites P(i-1) and dS(i-1): the products that read them must be done
-      if (i && !mbar_wait(&s.b_empty[st ^ 1], ((i - 1) >> 1) & 1, 218)) break;
-      if (!mbar_wait(&s.b_full[st], (i >> 1) & 1, 213)) break;
-      if (cols & 15) {
-        zero_tile_rows(s.b0[st], cols, c16, lane);
-        if (keys) zero_tile_rows(s.b1[st], cols, c16, lane);
-      }
-      tc_fence_after();
-      const uint32_t b0 = smem_u32(s.b0[st]), b1 = smem_u32(s.b1[st]);
-      if (lane == 0) {
-        const uint32_t id = base | (uint32_t)(c16 >> 3) << 17;
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) mma_f16(tmem, sdesc_k_sw128(a0 + kk * 32), sdesc_k_sw128(b0 + kk * 32), id, kk > 0);
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) mma_f16(tmem + 64, sdesc_k_sw128(a1 + kk * 32), sdesc_k_sw128(b1 + kk * 32), id, kk > 0);
-        mma_commit(&s.s_full);
-      }
-      __syncwarp();
-      if (!mbar_wait(&s.p_full, i & 1, 214)) break;
-      tc_fence_after();
-      if (lane == 0) {
-        // P and dS are 16-bit over the first half of each thread's own 32 columns of S and dP: the K
-        // elements 0-31 in columns 0-15, 32-63 in columns 32-47
-        for (int kk = 0; kk < c16 / 16; ++kk) {
-          const uint32_t col = (kk >> 1) * 32 + (kk & 1) * 8;
-          if (keys) mma_f16_ts(tmem + 128, tmem + col, sdesc_mn_sw128(b1 + kk * 2048), id_sum, i > 0 || kk > 0);
-          mma_f16_ts(tmem + 192, tmem + 64 + col, sdesc_mn_sw128(b0 + kk * 2048), id_sum, i > 0 || kk > 0);
+        const int r = k % kRing;
+        if (k >= kRing && !mbar_wait(&s.item_empty[r], ((k / kRing) & 1) ^ 1, 211)) break;
+        s.item[r] = it;
+        mbar_arrive(&s.item_full[r]);
+        if (!it.n) break;
+        const bool keys = it.keys;
+        const int kh = it.head / group;
+        const float *lse2 = a.lse2 + it.off, *delta2 = a.delta2 + it.off;
+        mbar_arrive_expect_tx(&s.a_full[r], 2 * kTile + (keys ? 0 : 2 * BM * 4));
+        for (int half = 0; half < 2; ++half) {  // boxes of 64 rows
+          tma_load_4d(s.a0[r] + half * kHalf, keys ? &mk : &mq, 0, it.row0 + it.first + half * BN, it.head, it.outer, &s.a_full[r]);
+          tma_load_4d(s.a1[r] + half * kHalf, keys ? &mv : &mdo, 0, it.row0 + it.first + half * BN, it.head, it.outer, &s.a_full[r]);
         }
-        mma_commit(&s.b_empty[st]);
-        if (i == n - 1) mma_commit(&s.acc_full);
-      }
-      __syncwarp();
-    }
-  } else if ((warp & 3) < live) {
-    const int quarter = warp & 3, half = warp >> 2;  // columns 32 half .. of every loop tile
-    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
-    const int row = b.first + quarter * 32 + lane;
-    const float c = a.scale * kLog2e;
-    const float gain = DT == ATLAS_F16 ? gain_of(a.amax[(int64_t)b.seq * a.Hk + (keys ? head : head / group)]) : 1.f;
-    float lse = 0.f, delta = 0.f;
-    if (!keys && row < b.len) {
-      lse = a.lse[vec0 + (int64_t)head * a.rows + row] * kLog2e;
-      delta = a.delta[vec0 + (int64_t)head * a.rows + row];
-    }
-    bool ok = true;
-    for (int i = 0; i < n; ++i) {
-      const int st = i & 1, left = min(BN, b.len - (i % per) * BN) - half * 32;  // columns of this thread's part
-      ok = mbar_wait(&s.s_full, i & 1, 215);
-      if (!ok) break;
-      tc_fence_after();
-      if (keys) {  // written by warp 8 before b_full, which the products waited for; seen here by its own wait
-        ok = mbar_wait(&s.b_full[st], (i >> 1) & 1, 216);
-        if (!ok) break;
-      }
-      if (left > 0) {
-        uint32_t x[32], y[32];
-        tmem_ld32(lanes + half * 32, x);
-        tmem_ld32(lanes + 64 + half * 32, y);
-        tmem_ld_wait();
-        uint32_t p[16], d[16];
-#pragma unroll
-        for (int j = 0; j < 32; j += 2) {
-          float w[2], g[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float l = keys ? s.lse[st][half * 32 + j + e] : lse, dl = keys ? s.delta[st][half * 32 + j + e] : delta;
-            w[e] = ex2(fmaf(__uint_as_float(x[j + e]), c, -l));
-            g[e] = (DT == ATLAS_F16 ? w[e] * gain : w[e]) * (__uint_as_float(y[j + e]) - dl);
-            if (j + e >= left) w[e] = g[e] = 0.f;
+        if (!keys) {
+          bulk_load(s.a_lse[r], lse2 + it.head * a.vec_ld + it.first, BM * 4, &s.a_full[r]);
+          bulk_load(s.a_delta[r], delta2 + it.head * a.vec_ld + it.first, BM * 4, &s.a_full[r]);
+        }
+        int row = 0, h = keys ? it.head * group : kh;
+        bool ok = true;
+        for (int i = 0; i < it.n; ++i, ++t) {
+          const int st = t % kStages;
+          ok = t < kStages || mbar_wait(&s.b_empty[st], ((t / kStages) & 1) ^ 1, 212);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&s.b_full[st], 2 * kHalf + (keys ? 2 * BN * 4 : 0));
+          tma_load_4d(s.b0[st], keys ? &mq : &mk, 0, it.row0 + row, h, it.outer, &s.b_full[st]);
+          tma_load_4d(s.b1[st], keys ? &mdo : &mv, 0, it.row0 + row, h, it.outer, &s.b_full[st]);
+          if (keys) {
+            bulk_load(s.b_lse[st], lse2 + h * a.vec_ld + row, BN * 4, &s.b_full[st]);
+            bulk_load(s.b_delta[st], delta2 + h * a.vec_ld + row, BN * 4, &s.b_full[st]);
           }
-          p[j / 2] = pack2<DT>(w[0], w[1]);
-          d[j / 2] = pack2<DT>(g[0], g[1]);
+          row += BN;
+          if (row >= it.len) {
+            row = 0;
+            ++h;
+          }
         }
-        if (keys) tmem_st16(lanes + half * 32, p);
-        tmem_st16(lanes + 64 + half * 32, d);
-        tmem_st_wait();
+        if (!ok) break;
+        ++k;
       }
-      tc_fence_before();
-      mbar_arrive(&s.p_full);
     }
-    if (ok) ok = mbar_wait(&s.acc_full, 0, 217);
-    tc_fence_after();
-    // keys: warps 0-3 write dv, 4-7 dk; queries: warps 4-7 write dq
-    if (ok && (keys || half)) {
-      float acc[64];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t r[32];
-        tmem_ld32(lanes + 128 + half * 64 + h * 32, r);
-        tmem_ld_wait();
-#pragma unroll
-        for (int d = 0; d < 32; ++d) acc[h * 32 + d] = __uint_as_float(r[d]);
+  } else if (warp == 17) {
+    const uint32_t base = DT == ATLAS_BF16 ? idesc_bf16_f32(BM, 0) : idesc_f16_f32(BM, 0);
+    bool ok = true;
+    for (int k = 0, t = 0; ok; ++k) {
+      const int r = k % kRing;
+      if (!mbar_wait(&s.item_full[r], (k / kRing) & 1, 213)) break;
+      const int n = s.item[r].n, len = s.item[r].len, keys = s.item[r].keys;
+      if (!n || !mbar_wait(&s.a_full[r], (k / kRing) & 1, 214)) break;
+      const uint32_t ar0 = desc_lo(smem_u32(s.a0[r])), ar1 = desc_lo(smem_u32(s.a1[r]));
+      for (int i = 0, row = 0; i < n; ++i, ++t) {
+        const int x = t % 3, st = t % kStages, cols = min(BN, len - row), c16 = up16(cols);
+        ok = (t < 3 || mbar_wait(&s.x_done[x], ((t / 3) & 1) ^ 1, 216)) && mbar_wait(&s.b_full[st], (t / kStages) & 1, 215);
+        if (!ok) break;
+        if (cols & 15) {
+          zero_tile_rows(s.b0[st], cols, c16, lane);
+          if (keys) zero_tile_rows(s.b1[st], cols, c16, lane);
+        }
+        tc_fence_after();
+        const uint32_t br0 = desc_lo(smem_u32(s.b0[st])), br1 = desc_lo(smem_u32(s.b1[st])), at = tmem + x * 128;
+        const uint32_t id = base | (uint32_t)(c16 >> 3) << 17;
+        if (elect_one()) {
+          mma_f16_lo<false>(at, ar0, br0, id);
+          mma_f16_lo<true>(at, ar0 + 2, br0 + 2, id);
+          mma_f16_lo<true>(at, ar0 + 4, br0 + 4, id);
+          mma_f16_lo<true>(at, ar0 + 6, br0 + 6, id);
+          mma_f16_lo<false>(at + 64, ar1, br1, id);
+          mma_f16_lo<true>(at + 64, ar1 + 2, br1 + 2, id);
+          mma_f16_lo<true>(at + 64, ar1 + 4, br1 + 4, id);
+          mma_f16_lo<true>(at + 64, ar1 + 6, br1 + 6, id);
+          mma_commit(&s.s_full[x]);
+          if (i == n - 1) mma_commit(&s.item_empty[r]);
+        }
+        __syncwarp();
+        row += BN;
+        if (row >= len) row = 0;
       }
-      if (row < b.len) {
-        void* out = !half ? a.dv : keys ? a.dk : a.dq;
-        const Strides& so = !half ? a.sdv : keys ? a.sdk : a.sdq;
-        uint16_t* dst = reinterpret_cast<uint16_t*>(out) + b.outer * so.outer + head * so.head + (b.row0 + row) * so.row;
-        store_row<DT>(dst, acc, half ? a.scale / gain : 1.f, a.D, vec);
+    }
+  } else if (warp == 18) {
+    const uint32_t base = DT == ATLAS_BF16 ? idesc_bf16_f32(BM, 64) : idesc_f16_f32(BM, 64), id = base | kMnB;
+    bool ok = true;
+    for (int k = 0, t = 0; ok; ++k) {
+      const int r = k % kRing;
+      if (!mbar_wait(&s.item_full[r], (k / kRing) & 1, 224)) break;
+      const int n = s.item[r].n, len = s.item[r].len, keys = s.item[r].keys;
+      if (!n || (k && !mbar_wait(&s.acc_free, (k - 1) & 1, 217))) break;
+      for (int i = 0, row = 0; i < n; ++i, ++t) {
+        const int x = t % 3, st = t % kStages, cols = min(BN, len - row);
+        ok = mbar_wait(&s.p_full[x], (t / 3) & 1, 218);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t br0 = desc_lo(smem_u32(s.b0[st])), br1 = desc_lo(smem_u32(s.b1[st])), at = tmem + x * 128;
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            if (kk * 16 < cols) {
+              // K elements 0-31 of P and dS are in the columns 0-15 of S and dP, 32-63 in 32-47
+              const uint32_t col = (kk >> 1) * 32 + (kk & 1) * 8;
+              if (keys) mma_f16_ts_lo(tmem + 384, at + col, br1 + kk * 128, id, i > 0 || kk > 0);
+              mma_f16_ts_lo(tmem + 448, at + 64 + col, br0 + kk * 128, id, i > 0 || kk > 0);
+            }
+          mma_commit(&s.x_done[x]);
+          mma_commit(&s.b_empty[st]);
+          if (i == n - 1) {
+            mma_commit(&s.acc_full[r]);
+            mma_commit(&s.item_empty[r]);
+          }
+        }
+        __syncwarp();
+        row += BN;
+        if (row >= len) row = 0;
       }
+    }
+  } else {
+    const int g = warp >> 3, quarter = warp & 3, half = (warp >> 2) & 1;
+    const int own = quarter * 32 + lane;
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+    const float c = a.scale * kLog2e;
+    bool ok = true;
+    for (int k = 0, t = 0; ok; ++k) {
+      const int r = k % kRing;
+      ok = mbar_wait(&s.item_full[r], (k / kRing) & 1, 219);
+      if (!ok) break;
+      const BwdItem it = s.item[r];
+      if (!it.n) break;
+      const bool live = it.first + quarter * 32 < it.len, keys = it.keys;
+      float lse = 0.f, delta = 0.f, gain = 1.f;
+      if (DT == ATLAS_F16) gain = gain_of(__ldg(a.amax + (int64_t)it.seq * a.Hk + (keys ? it.head : it.head / group)));
+      if (!keys) {
+        ok = mbar_wait(&s.a_full[r], (k / kRing) & 1, 220);
+        if (!ok) break;
+        lse = s.a_lse[r][own];
+        delta = s.a_delta[r][own];
+      }
+      int left = it.len - half * 32;  // columns of this thread's part from here to the end of the head
+      for (int i = 0; i < it.n; ++i, ++t, left -= BN) {
+        if (left + half * 32 <= 0) left = it.len - half * 32;
+        if ((t & 1) != g) continue;
+        const int x = t % 3, st = t % kStages;
+        ok = mbar_wait(&s.s_full[x], (t / 3) & 1, 221) && (!keys || mbar_wait(&s.b_full[st], (t / kStages) & 1, 222));
+        if (!ok) break;
+        tc_fence_after();
+        if (live && left > 0) {
+          const uint32_t at = lanes + x * 128 + half * 32;
+          if (keys) bwd_tile<DT, true>(at, c, gain, 0.f, 0.f, s.b_lse[st] + half * 32, s.b_delta[st] + half * 32, left);
+          else bwd_tile<DT, false>(at, c, gain, lse, delta, nullptr, nullptr, left);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.p_full[x]);
+      }
+      if (!ok) break;
+      if (((t - 1) & 1) == g) {  // this group had the last tile: it reads the sums
+        // one barrier per item in flight: a group may be here for an item of one tile while the sums of
+        // the item before are still to come, and a single barrier's parity would then say too much
+        ok = mbar_wait(&s.acc_full[r], (k / kRing) & 1, 223);
+        if (!ok) break;
+        tc_fence_after();
+        const int row = it.first + own;
+        const float mul = keys && !half ? 1.f : a.scale / gain;
+        uint32_t w[2][16];  // queries: each half writes 32 columns of dq
+        if (live) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (keys || h == 0) {
+              uint32_t v[32];
+              tmem_ld32(lanes + (keys ? (half ? 448 : 384) + h * 32 : 448 + half * 32), v);
+              tmem_ld_wait();
+#pragma unroll
+              for (int d = 0; d < 16; ++d) w[h][d] = pack2<DT>(__uint_as_float(v[2 * d]) * mul, __uint_as_float(v[2 * d + 1]) * mul);
+            }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.acc_free);
+        if (row < it.len) {
+          const Strides& so = !keys ? a.sdq : half ? a.sdk : a.sdv;
+          uint16_t* dst = reinterpret_cast<uint16_t*>(!keys ? a.dq : half ? a.dk : a.dv) + it.outer * so.outer + it.head * so.head +
+                          ((int64_t)it.row0 + row) * so.row;
+          if (keys) {
+            store32(dst, w[0], a.D, vec);
+            store32(dst + 32, w[1], a.D - 32, vec);
+          } else {
+            store32(dst + half * 32, w[0], a.D - half * 32, vec);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.item_empty[r]);
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == 17) {
     tc_fence_after();
-    tmem_dealloc(tmem, 256);
+    tmem_dealloc(tmem, 512);
   }
 }
 
@@ -554,7 +682,8 @@ int bwd(const AttnArgs& a, cudaStream_t st) {
   if (DT == ATLAS_F16 && cudaMemsetAsync(a.amax, 0, (size_t)(a.B * a.Hk) * 4, st) != cudaSuccess)
     return fail(ATLAS_ERR_CUDA, "attention_grad: clearing the workspace failed");
   if (int rc = attn_delta(a, DT, st)) return rc;
-  attn_bwd_tc_kernel<DT><<<dim3((unsigned)a.cap, a.Hk + a.H), kBwdThreads, bytes, st>>>(mq, mk, mv, mdo, a, vec);
+  const int64_t items = a.cap * (a.Hk + a.H);
+  attn_bwd_tc_kernel<DT><<<(unsigned)(items < num_sms() ? items : num_sms()), kBwdThreads, bytes, st>>>(mq, mk, mv, mdo, a, vec);
   return check_launch("attention_grad");
 }
 
@@ -565,7 +694,7 @@ int bwd(const AttnArgs& a, cudaStream_t st) {
 // taken before the scale).
 bool attn_tc_takes(const AttnArgs& a, int dtype, bool grad) {
   if (dtype == ATLAS_F32 || !(a.scale > 0.f)) return false;
-  if (grad && (a.H + a.Hk > 65535 || !map_ok(a.dout, a.sdo, a.outer, a.H, a.rows))) return false;
+  if (grad && (a.cap * (a.H + a.Hk) >= (1LL << 31) || !map_ok(a.dout, a.sdo, a.outer, a.H, a.rows))) return false;
   return map_ok(a.q, a.sq, a.outer, a.H, a.rows) && map_ok(a.k, a.sk, a.outer, a.Hk, a.rows) &&
          map_ok(a.v, a.sv, a.outer, a.Hk, a.rows);
 }

@@ -364,14 +364,14 @@ def attention_grad(dout, q, k, v, out, lse, plan: SeqPlan, scale: float | None =
     dq, dk, dv = _rows_like(q, h), _rows_like(k, k.shape[1]), _rows_like(v, k.shape[1])
     if B == 0 or dq.numel() == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
-    ws = torch.empty(o * h * n + B * k.shape[1], dtype=torch.float32, device=dev)  # atlas_attention_grad_ws_bytes
+    ws = torch.empty(int(_lib.load().atlas_attention_grad_ws_bytes(o, n, h, k.shape[1], B)), dtype=torch.uint8, device=dev)
     dout, q, k, v, out, lse = _unit(dout), _unit(q), _unit(k), _unit(v), _unit(out), lse.contiguous()
     blocks, counts, cu = plan.blocks.contiguous(), plan.counts.contiguous(), plan.cu.contiguous()
     s = _strides(dout, q, k, v, out, dq, dk, dv)
     with _on(dev):
         call("atlas_attention_grad", ptr(dout), ptr(q), ptr(k), ptr(v), ptr(out), ptr(lse), dtype_code(q.dtype), ctypes.addressof(s),
              o, n, h, k.shape[1], d, ptr(cu), ptr(blocks), ptr(counts), B, blocks.shape[0], int(plan.stride == 0), float(scale),
-             ptr(dq), ptr(dk), ptr(dv), ptr(ws), ws.numel() * 4, stream_ptr(dev))
+             ptr(dq), ptr(dk), ptr(dv), ptr(ws), ws.numel(), stream_ptr(dev))
     return dq, dk, dv
 
 
