@@ -18,8 +18,8 @@ struct AttnArgs {
   void *out, *dq, *dk, *dv;
   Strides sq, sk, sv, so, sdo, sdq, sdk, sdv;
   float* lse;    // [outer, H, rows]
-  // Gradient only. CUDA cores: delta [outer, H, rows]. Tensor cores: for each head the log-sum-exp in
-  // base 2 and delta of all sequences, each from a place that is a multiple of 16 bytes (seq_block's off;
+  // Gradient only. CUDA cores: delta [outer, H, rows]. Tensor cores: for each head, negated, the
+  // log-sum-exp in base 2 and delta of all sequences, each from a place that is a multiple of 16 bytes (seq_block's off;
   // vec_ld values a head), the largest |dout| of a sequence and key head as bits (fp16), and the counter of
   // work items.
   float *delta, *lse2, *delta2;

@@ -333,8 +333,8 @@ __global__ void __launch_bounds__(kThreads) attn_delta_kernel(const AttnArgs a) 
     if (sub == 0 && r < s.len) {
       const int64_t at = (s.outer * a.H + head) * a.rows + s.row0 + r;
       if (a.lse2) {
-        a.lse2[head * a.vec_ld + s.off + r] = a.lse[at] * 1.4426950408889634f;
-        a.delta2[head * a.vec_ld + s.off + r] = v;
+        a.lse2[head * a.vec_ld + s.off + r] = a.lse[at] * -1.4426950408889634f;
+        a.delta2[head * a.vec_ld + s.off + r] = -v;
       } else {
         a.delta[at] = v;
       }

@@ -38,6 +38,35 @@ __device__ __forceinline__ float ex2(float v) {
   return r;
 }
 
+// Two fp32 values as one operand of the packed fp32 instructions.
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pair(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(f32x2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ void load_pairs(f32x2 (&v)[2], const float* p) {
+  const ulonglong2 w = *reinterpret_cast<const ulonglong2*>(p);
+  v[0] = w.x;
+  v[1] = w.y;
+}
+
 template <int DT>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   uint32_t r;
@@ -291,12 +320,14 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
 //   keys: dv += P B1, dk += dS B0;  queries: dq += dS B0.
 // One persistent CTA per SM takes items from a counter and runs their tiles as one stream, so that an
 // item's start (look-up, first loads) and end (reading the sums) hide behind its neighbours:
-//   warps 0-15  two groups of eight, each takes every other tile: two threads per row, 32 columns each
+//   warps 0-11  three groups of four, each takes every third tile: one thread per row
+//   warps 12-15 read an item's sums and write them out, while the groups are at the next item
 //   warp 16     TMA: items, A tiles (ring of 3), B tiles with the queries' log-sum-exp and delta (ring)
-//   warp 17     scores, up to two tiles ahead of the group that is at work; owns the TMEM
+//   warp 17     scores; owns the TMEM
 //   warp 18     sums (products of two small kinds cost their issuing warp 500 clocks a tile each)
 // TMEM: three buffers of S and dP (columns 128 x, 128 x + 64), the sums in 384-447 (dv) and 448-511.
 constexpr int kBwdThreads = 608;
+constexpr int kGroups = 3;
 constexpr int BN = 64;
 constexpr uint32_t kHalf = BN * 128;
 constexpr int kRing = 3;    // items in flight: tile t + 2 may be two items ahead
@@ -331,46 +362,66 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
-// P and dS of one thread's 32 columns, over its scores.
+// P and dS of 16 columns of a row from their scores x and dP y, as packed pairs. lse and delta come
+// negated, in pairs (two fp32 operations an instruction); `left` columns are before the end.
 template <int DT, bool KEYS>
-__device__ __forceinline__ void bwd_tile(uint32_t cols, float c, float gain, float lse, float delta, const float* b_lse,
-                                         const float* b_delta, int left) {
+__device__ __forceinline__ void bwd_part(const uint32_t (&x)[16], const uint32_t (&y)[16], f32x2 c2, f32x2 gain2, f32x2 nl, f32x2 nd,
+                                         const float* b_lse, const float* b_delta, int left, uint32_t to_p, uint32_t to_d) {
+  uint32_t p[8], d[8];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    uint32_t x[16], y[16], p[8], d[8];
-    tmem_ld16(cols + h * 16, x);
-    tmem_ld16(cols + 64 + h * 16, y);
-    tmem_ld_wait();
-#pragma unroll
-    for (int j = 0; j < 16; j += 4) {
-      float l4[4] = {lse, lse, lse, lse}, d4[4] = {delta, delta, delta, delta}, w[4], g[4];
-      if (KEYS) {
-        *reinterpret_cast<float4*>(l4) = *reinterpret_cast<const float4*>(b_lse + h * 16 + j);
-        *reinterpret_cast<float4*>(d4) = *reinterpret_cast<const float4*>(b_delta + h * 16 + j);
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        w[e] = ex2(fmaf(__uint_as_float(x[j + e]), c, -l4[e]));
-        g[e] = (DT == ATLAS_F16 ? w[e] * gain : w[e]) * (__uint_as_float(y[j + e]) - d4[e]);
-      }
-#pragma unroll
-      for (int e = 0; e < 4; e += 2) {
-        p[(j + e) / 2] = pack2<DT>(w[e], w[e + 1]);
-        d[(j + e) / 2] = pack2<DT>(g[e], g[e + 1]);
-      }
+  for (int j = 0; j < 16; j += 4) {
+    f32x2 l[2] = {nl, nl}, e[2] = {nd, nd};
+    if (KEYS) {
+      load_pairs(l, b_lse + j);
+      load_pairs(e, b_delta + j);
     }
-    if (left < 32) {  // columns behind the end: whatever the scores were, nothing
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int at = h * 16 + 2 * j;
-        const uint32_t keep = at + 1 < left ? 0xFFFFFFFFu : at < left ? 0xFFFFu : 0u;
-        p[j] &= keep;
-        d[j] &= keep;
-      }
+    for (int k = 0; k < 2; ++k) {
+      const int o = j + 2 * k;
+      float w0, w1, g0, g1;
+      unpair(fma2(pair(__uint_as_float(x[o]), __uint_as_float(x[o + 1])), c2, l[k]), w0, w1);
+      w0 = ex2(w0);
+      w1 = ex2(w1);
+      f32x2 g = add2(pair(__uint_as_float(y[o]), __uint_as_float(y[o + 1])), e[k]);
+      if (DT == ATLAS_F16) g = mul2(g, gain2);
+      unpair(mul2(g, pair(w0, w1)), g0, g1);
+      p[j / 2 + k] = pack2<DT>(w0, w1);
+      d[j / 2 + k] = pack2<DT>(g0, g1);
     }
-    if (KEYS) tmem_st8(cols + h * 8, p);
-    tmem_st8(cols + 64 + h * 8, d);
   }
+  if (left < 16) {  // columns behind the end: whatever the scores were, nothing
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t keep = 2 * j + 1 < left ? 0xFFFFFFFFu : 2 * j < left ? 0xFFFFu : 0u;
+      p[j] &= keep;
+      d[j] &= keep;
+    }
+  }
+  if (KEYS) tmem_st8(to_p, p);
+  tmem_st8(to_d, d);
+}
+
+// One row of a tile: P over the first 32 columns of its scores, dS over the first 32 of dP. The next 16
+// columns are under way from TMEM while 16 are computed; what is written lies over columns already read.
+template <int DT, bool KEYS>
+__device__ __forceinline__ void bwd_tile(uint32_t at, float c, float gain, float nlse, float ndelta, const float* b_lse,
+                                         const float* b_delta, int left) {
+  const f32x2 c2 = pair(c, c), gain2 = pair(gain, gain), nl = pair(nlse, nlse), nd = pair(ndelta, ndelta);
+  uint32_t x[2][16], y[2][16];
+  tmem_ld16(at, x[0]);
+  tmem_ld16(at + 64, y[0]);
+#pragma unroll
+  for (int h = 0; h < 4; ++h) {
+    if (h * 16 >= left) break;
+    tmem_ld_wait();
+    if (h < 3) {
+      tmem_ld16(at + h * 16 + 16, x[(h + 1) & 1]);
+      tmem_ld16(at + 64 + h * 16 + 16, y[(h + 1) & 1]);
+    }
+    bwd_part<DT, KEYS>(x[h & 1], y[h & 1], c2, gain2, nl, nd, b_lse + h * 16, b_delta + h * 16, left - h * 16, at + h * 8,
+                       at + 64 + h * 8);
+  }
+  tmem_ld_wait();
   tmem_st_wait();
 }
 
@@ -384,7 +435,7 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
   if (threadIdx.x == 0) {
     for (int i = 0; i < kRing; ++i) {
       mbar_init(&s.item_full[i], 1);
-      mbar_init(&s.item_empty[i], 18);
+      mbar_init(&s.item_empty[i], 4 * kGroups + 6);
       mbar_init(&s.a_full[i], 1);
       mbar_init(&s.acc_full[i], 1);
     }
@@ -394,10 +445,10 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
     }
     for (int i = 0; i < 3; ++i) {
       mbar_init(&s.s_full[i], 1);
-      mbar_init(&s.p_full[i], 8);
+      mbar_init(&s.p_full[i], 4);
       mbar_init(&s.x_done[i], 1);
     }
-    mbar_init(&s.acc_free, 8);
+    mbar_init(&s.acc_free, 4);
     fence_barrier_init();
   }
   if (warp == 17) tmem_alloc(&s.tmem, 512);
@@ -518,10 +569,8 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
             if (kk * 16 < cols) {
-              // K elements 0-31 of P and dS are in the columns 0-15 of S and dP, 32-63 in 32-47
-              const uint32_t col = (kk >> 1) * 32 + (kk & 1) * 8;
-              if (keys) mma_f16_ts_lo(tmem + 384, at + col, br1 + kk * 128, id, i > 0 || kk > 0);
-              mma_f16_ts_lo(tmem + 448, at + 64 + col, br0 + kk * 128, id, i > 0 || kk > 0);
+              if (keys) mma_f16_ts_lo(tmem + 384, at + kk * 8, br1 + kk * 128, id, i > 0 || kk > 0);
+              mma_f16_ts_lo(tmem + 448, at + 64 + kk * 8, br0 + kk * 128, id, i > 0 || kk > 0);
             }
           mma_commit(&s.x_done[x]);
           mma_commit(&s.b_empty[st]);
@@ -535,8 +584,46 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
         if (row >= len) row = 0;
       }
     }
+  } else if (warp >= 4 * kGroups) {
+    const int quarter = warp & 3;
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+    for (int k = 0;; ++k) {
+      const int r = k % kRing;
+      if (!mbar_wait(&s.item_full[r], (k / kRing) & 1, 225)) break;
+      const BwdItem& it = s.item[r];
+      if (!it.n || !mbar_wait(&s.acc_full[r], (k / kRing) & 1, 223)) break;
+      tc_fence_after();
+      const int row = it.first + quarter * 32 + lane;
+      if (it.first + quarter * 32 < it.len) {
+        const bool keys = it.keys;
+        float mul = a.scale;
+        if (DT == ATLAS_F16) mul /= gain_of(__ldg(a.amax + (int64_t)it.seq * a.Hk + (keys ? it.head : it.head / group)));
+#pragma unroll
+        for (int h = 0; h < 4; ++h)
+          if (keys || h >= 2) {  // dv (keys), then dk or dq
+            uint32_t v[32], w[16];
+            tmem_ld32(lanes + 384 + h * 32, v);
+            tmem_ld_wait();
+            const float f = h < 2 ? 1.f : mul;
+#pragma unroll
+            for (int d = 0; d < 16; ++d) w[d] = pack2<DT>(__uint_as_float(v[2 * d]) * f, __uint_as_float(v[2 * d + 1]) * f);
+            if (row < it.len) {
+              const Strides& so = h < 2 ? a.sdv : keys ? a.sdk : a.sdq;
+              uint16_t* dst = reinterpret_cast<uint16_t*>(h < 2 ? a.dv : keys ? a.dk : a.dq) + it.outer * so.outer +
+                              it.head * so.head + ((int64_t)it.row0 + row) * so.row + (h & 1) * 32;
+              store32(dst, w, a.D - (h & 1) * 32, vec);
+            }
+          }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&s.acc_free);
+        mbar_arrive(&s.item_empty[r]);
+      }
+    }
   } else {
-    const int g = warp >> 3, quarter = warp & 3, half = (warp >> 2) & 1;
+    const int g = warp >> 2, quarter = warp & 3;
     const int own = quarter * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
     const float c = a.scale * kLog2e;
@@ -556,17 +643,17 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
         lse = s.a_lse[r][own];
         delta = s.a_delta[r][own];
       }
-      int left = it.len - half * 32;  // columns of this thread's part from here to the end of the head
+      int left = it.len;  // columns from here to the end of the head
       for (int i = 0; i < it.n; ++i, ++t, left -= BN) {
-        if (left + half * 32 <= 0) left = it.len - half * 32;
-        if ((t & 1) != g) continue;
+        if (left <= 0) left = it.len;
+        if (t % kGroups != g) continue;
         const int x = t % 3, st = t % kStages;
         ok = mbar_wait(&s.s_full[x], (t / 3) & 1, 221) && (!keys || mbar_wait(&s.b_full[st], (t / kStages) & 1, 222));
         if (!ok) break;
         tc_fence_after();
-        if (live && left > 0) {
-          const uint32_t at = lanes + x * 128 + half * 32;
-          if (keys) bwd_tile<DT, true>(at, c, gain, 0.f, 0.f, s.b_lse[st] + half * 32, s.b_delta[st] + half * 32, left);
+        if (live) {
+          const uint32_t at = lanes + x * 128;
+          if (keys) bwd_tile<DT, true>(at, c, gain, 0.f, 0.f, s.b_lse[st], s.b_delta[st], left);
           else bwd_tile<DT, false>(at, c, gain, lse, delta, nullptr, nullptr, left);
         }
         tc_fence_before();
@@ -574,41 +661,6 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
         if (lane == 0) mbar_arrive(&s.p_full[x]);
       }
       if (!ok) break;
-      if (((t - 1) & 1) == g) {  // this group had the last tile: it reads the sums
-        // one barrier per item in flight: a group may be here for an item of one tile while the sums of
-        // the item before are still to come, and a single barrier's parity would then say too much
-        ok = mbar_wait(&s.acc_full[r], (k / kRing) & 1, 223);
-        if (!ok) break;
-        tc_fence_after();
-        const int row = it.first + own;
-        const float mul = keys && !half ? 1.f : a.scale / gain;
-        uint32_t w[2][16];  // queries: each half writes 32 columns of dq
-        if (live) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            if (keys || h == 0) {
-              uint32_t v[32];
-              tmem_ld32(lanes + (keys ? (half ? 448 : 384) + h * 32 : 448 + half * 32), v);
-              tmem_ld_wait();
-#pragma unroll
-              for (int d = 0; d < 16; ++d) w[h][d] = pack2<DT>(__uint_as_float(v[2 * d]) * mul, __uint_as_float(v[2 * d + 1]) * mul);
-            }
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s.acc_free);
-        if (row < it.len) {
-          const Strides& so = !keys ? a.sdq : half ? a.sdk : a.sdv;
-          uint16_t* dst = reinterpret_cast<uint16_t*>(!keys ? a.dq : half ? a.dk : a.dv) + it.outer * so.outer + it.head * so.head +
-                          ((int64_t)it.row0 + row) * so.row;
-          if (keys) {
-            store32(dst, w[0], a.D, vec);
-            store32(dst + 32, w[1], a.D - 32, vec);
-          } else {
-            store32(dst + half * 32, w[0], a.D - half * 32, vec);
-          }
-        }
-      }
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.item_empty[r]);
     }
