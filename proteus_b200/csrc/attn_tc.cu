@@ -179,7 +179,7 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
     const uint64_t qd = sdesc_k_sw128(smem_u32(s.q)), kd = sdesc_k_sw128(smem_u32(s.k[0])), vd = sdesc_mn_sw128(smem_u32(s.v[0]));
     // S(i) = q k(i)^T into buffer i & 1
     auto scores = [&](int i) {
-      if (!mbar_wait(&s.k_full[i & 1], (i >> 1) & 1, 203)) return false;
+      if (!mbar_spin(&s.k_full[i & 1], (i >> 1) & 1, 203)) return false;
       tc_fence_after();
       if (elect_one()) {
         const uint32_t id = base | (uint32_t)(up16(min(BM, b.len - i * BM)) >> 3) << 17;
@@ -196,9 +196,9 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
     for (int i = 0; ok && i < n; ++i) {
       const int bf = i & 1, cols = min(BM, b.len - i * BM);
       const uint32_t ph = (i >> 1) & 1;
-      if (!mbar_wait(&s.v_full[bf], ph, 205)) break;
+      if (!mbar_spin(&s.v_full[bf], ph, 205)) break;
       if (cols & 15) zero_tile_rows(s.v[bf], cols, up16(cols), lane);
-      if (!mbar_wait(&s.p_full[bf], ph, 206)) break;
+      if (!mbar_spin(&s.p_full[bf], ph, 206)) break;
       tc_fence_after();
       if (elect_one()) {
         const uint64_t v = vd + bf * (kTile >> 4);
@@ -209,7 +209,7 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
         mma_commit(&s.o_full[bf]);
       }
       __syncwarp();
-      if (i + 2 < n) ok = mbar_wait(&s.s_free[bf], ph, 207) && scores(i + 2);
+      if (i + 2 < n) ok = mbar_spin(&s.s_free[bf], ph, 207) && scores(i + 2);
     }
   } else if (warp < live) {
     const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
@@ -218,7 +218,7 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
 #pragma unroll
     for (int d = 0; d < 64; ++d) o[d] = 0.f;
     auto take_o = [&](int i) {  // o <- o fold + P(i) v
-      if (!mbar_wait(&s.o_full[i & 1], (i >> 1) & 1, 208)) return false;
+      if (!mbar_wait_soon(&s.o_full[i & 1], (i >> 1) & 1, 208)) return false;
       tc_fence_after();
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -236,7 +236,7 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
     for (int i = 0; i < n; ++i) {
       const int cols = min(BM, b.len - i * BM);
       const uint32_t buf = lanes + (i & 1) * 128;
-      ok = mbar_wait(&s.s_full[i & 1], (i >> 1) & 1, 209);
+      ok = mbar_wait_soon(&s.s_full[i & 1], (i >> 1) & 1, 209);
       if (!ok) break;
       tc_fence_after();
       float mx = kNegInf;
@@ -323,15 +323,16 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
 //   warps 0-11  three groups of four, each takes every third tile: one thread per row
 //   warps 12-15 read an item's sums and write them out, while the groups are at the next item
 //   warp 16     TMA: items, A tiles (ring of 3), B tiles with the queries' log-sum-exp and delta (ring)
-//   warp 17     scores; owns the TMEM
-//   warp 18     sums (products of two small kinds cost their issuing warp 500 clocks a tile each)
+//   warp 17     S; owns the TMEM
+//   warp 18     dP
+//   warp 19     sums (products of two small kinds cost their issuing warp 500 clocks a tile each)
 // TMEM: three buffers of S and dP (columns 128 x, 128 x + 64), the sums in 384-447 (dv) and 448-511.
-constexpr int kBwdThreads = 608;
+constexpr int kBwdThreads = 640;
 constexpr int kGroups = 3;
 constexpr int BN = 64;
 constexpr uint32_t kHalf = BN * 128;
-constexpr int kRing = 3;    // items in flight: tile t + 2 may be two items ahead
-constexpr int kStages = 5;  // B tiles in flight
+constexpr int kRing = 2;    // items in flight: tile t + 2 may be two items ahead
+constexpr int kStages = 9;  // B tiles in flight
 
 struct BwdItem {
   int seq, first, len, head, keys, n, row0, outer;  // n: loop tiles; 0 ends the stream
@@ -435,7 +436,7 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
   if (threadIdx.x == 0) {
     for (int i = 0; i < kRing; ++i) {
       mbar_init(&s.item_full[i], 1);
-      mbar_init(&s.item_empty[i], 4 * kGroups + 6);
+      mbar_init(&s.item_empty[i], 4 * kGroups + 7);
       mbar_init(&s.a_full[i], 1);
       mbar_init(&s.acc_full[i], 1);
     }
@@ -444,7 +445,7 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
       mbar_init(&s.b_empty[i], 1);
     }
     for (int i = 0; i < 3; ++i) {
-      mbar_init(&s.s_full[i], 1);
+      mbar_init(&s.s_full[i], 2);
       mbar_init(&s.p_full[i], 4);
       mbar_init(&s.x_done[i], 1);
     }
@@ -458,7 +459,7 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
   const uint32_t tmem = s.tmem;
 
   if (warp == 16) {
-    if (lane == 0) {
+    if (elect_one()) {
       const int total = (int)a.cap * (a.Hk + a.H);
       int next = (int)atomicAdd(a.counter, 1u), k = 0, t = 0;
       while (true) {
@@ -475,7 +476,7 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
           break;
         }
         const int r = k % kRing;
-        if (k >= kRing && !mbar_wait(&s.item_empty[r], ((k / kRing) & 1) ^ 1, 211)) break;
+        if (k >= kRing && !mbar_wait_soon(&s.item_empty[r], ((k / kRing) & 1) ^ 1, 211)) break;
         s.item[r] = it;
         mbar_arrive(&s.item_full[r]);
         if (!it.n) break;
@@ -495,7 +496,7 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
         bool ok = true;
         for (int i = 0; i < it.n; ++i, ++t) {
           const int st = t % kStages;
-          ok = t < kStages || mbar_wait(&s.b_empty[st], ((t / kStages) & 1) ^ 1, 212);
+          ok = t < kStages || mbar_wait_soon(&s.b_empty[st], ((t / kStages) & 1) ^ 1, 212);
           if (!ok) break;
           mbar_arrive_expect_tx(&s.b_full[st], 2 * kHalf + (keys ? 2 * BN * 4 : 0));
           tma_load_4d(s.b0[st], keys ? &mq : &mk, 0, it.row0 + row, h, it.outer, &s.b_full[st]);
@@ -514,35 +515,35 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
         ++k;
       }
     }
-  } else if (warp == 17) {
+  } else if (warp == 17 || warp == 18) {
+    // Warp 17: S, warp 18: dP. While the tensor core reads its operands, everything else that touches shared
+    // memory takes about 300 clocks, a wait that is over as well: one warp with both could not keep up.
+    const bool dp = warp == 18;
     const uint32_t base = DT == ATLAS_BF16 ? idesc_bf16_f32(BM, 0) : idesc_f16_f32(BM, 0);
     bool ok = true;
     for (int k = 0, t = 0; ok; ++k) {
       const int r = k % kRing;
-      if (!mbar_wait(&s.item_full[r], (k / kRing) & 1, 213)) break;
+      if (!mbar_spin(&s.item_full[r], (k / kRing) & 1, 213)) break;
       const int n = s.item[r].n, len = s.item[r].len, keys = s.item[r].keys;
-      if (!n || !mbar_wait(&s.a_full[r], (k / kRing) & 1, 214)) break;
-      const uint32_t ar0 = desc_lo(smem_u32(s.a0[r])), ar1 = desc_lo(smem_u32(s.a1[r]));
+      if (!n || !mbar_spin(&s.a_full[r], (k / kRing) & 1, 214)) break;
+      const uint32_t ar = desc_lo(smem_u32(dp ? s.a1[r] : s.a0[r]));
       for (int i = 0, row = 0; i < n; ++i, ++t) {
         const int x = t % 3, st = t % kStages, cols = min(BN, len - row), c16 = up16(cols);
-        ok = (t < 3 || mbar_wait(&s.x_done[x], ((t / 3) & 1) ^ 1, 216)) && mbar_wait(&s.b_full[st], (t / kStages) & 1, 215);
+        uint8_t* tile = dp ? s.b1[st] : s.b0[st];
+        ok = mbar_spin(&s.b_full[st], (t / kStages) & 1, 215);
         if (!ok) break;
-        if (cols & 15) {
-          zero_tile_rows(s.b0[st], cols, c16, lane);
-          if (keys) zero_tile_rows(s.b1[st], cols, c16, lane);
-        }
+        // rows behind the end: summed over in dk or dq (queries of S, keys) and in dv (dout, for keys)
+        if ((cols & 15) && (keys || !dp)) zero_tile_rows(tile, cols, c16, lane);
+        ok = t < 3 || mbar_spin(&s.x_done[x], ((t / 3) & 1) ^ 1, 216);
+        if (!ok) break;
         tc_fence_after();
-        const uint32_t br0 = desc_lo(smem_u32(s.b0[st])), br1 = desc_lo(smem_u32(s.b1[st])), at = tmem + x * 128;
+        const uint32_t br = desc_lo(smem_u32(tile)), at = tmem + x * 128 + (dp ? 64 : 0);
         const uint32_t id = base | (uint32_t)(c16 >> 3) << 17;
         if (elect_one()) {
-          mma_f16_lo<false>(at, ar0, br0, id);
-          mma_f16_lo<true>(at, ar0 + 2, br0 + 2, id);
-          mma_f16_lo<true>(at, ar0 + 4, br0 + 4, id);
-          mma_f16_lo<true>(at, ar0 + 6, br0 + 6, id);
-          mma_f16_lo<false>(at + 64, ar1, br1, id);
-          mma_f16_lo<true>(at + 64, ar1 + 2, br1 + 2, id);
-          mma_f16_lo<true>(at + 64, ar1 + 4, br1 + 4, id);
-          mma_f16_lo<true>(at + 64, ar1 + 6, br1 + 6, id);
+          mma_f16_lo<false>(at, ar, br, id);
+          mma_f16_lo<true>(at, ar + 2, br + 2, id);
+          mma_f16_lo<true>(at, ar + 4, br + 4, id);
+          mma_f16_lo<true>(at, ar + 6, br + 6, id);
           mma_commit(&s.s_full[x]);
           if (i == n - 1) mma_commit(&s.item_empty[r]);
         }
@@ -551,17 +552,17 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
         if (row >= len) row = 0;
       }
     }
-  } else if (warp == 18) {
+  } else if (warp == 19) {
     const uint32_t base = DT == ATLAS_BF16 ? idesc_bf16_f32(BM, 64) : idesc_f16_f32(BM, 64), id = base | kMnB;
     bool ok = true;
     for (int k = 0, t = 0; ok; ++k) {
       const int r = k % kRing;
-      if (!mbar_wait(&s.item_full[r], (k / kRing) & 1, 224)) break;
+      if (!mbar_spin(&s.item_full[r], (k / kRing) & 1, 224)) break;
       const int n = s.item[r].n, len = s.item[r].len, keys = s.item[r].keys;
-      if (!n || (k && !mbar_wait(&s.acc_free, (k - 1) & 1, 217))) break;
+      if (!n || (k && !mbar_spin(&s.acc_free, (k - 1) & 1, 217))) break;
       for (int i = 0, row = 0; i < n; ++i, ++t) {
         const int x = t % 3, st = t % kStages, cols = min(BN, len - row);
-        ok = mbar_wait(&s.p_full[x], (t / 3) & 1, 218);
+        ok = mbar_spin(&s.p_full[x], (t / 3) & 1, 218);
         if (!ok) break;
         tc_fence_after();
         const uint32_t br0 = desc_lo(smem_u32(s.b0[st])), br1 = desc_lo(smem_u32(s.b1[st])), at = tmem + x * 128;
@@ -589,9 +590,9 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
     for (int k = 0;; ++k) {
       const int r = k % kRing;
-      if (!mbar_wait(&s.item_full[r], (k / kRing) & 1, 225)) break;
+      if (!mbar_wait_soon(&s.item_full[r], (k / kRing) & 1, 225)) break;
       const BwdItem& it = s.item[r];
-      if (!it.n || !mbar_wait(&s.acc_full[r], (k / kRing) & 1, 223)) break;
+      if (!it.n || !mbar_wait_soon(&s.acc_full[r], (k / kRing) & 1, 223)) break;
       tc_fence_after();
       const int row = it.first + quarter * 32 + lane;
       if (it.first + quarter * 32 < it.len) {
@@ -630,7 +631,7 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
     bool ok = true;
     for (int k = 0, t = 0; ok; ++k) {
       const int r = k % kRing;
-      ok = mbar_wait(&s.item_full[r], (k / kRing) & 1, 219);
+      ok = mbar_wait_soon(&s.item_full[r], (k / kRing) & 1, 219);
       if (!ok) break;
       const BwdItem it = s.item[r];
       if (!it.n) break;
@@ -638,7 +639,7 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
       float lse = 0.f, delta = 0.f, gain = 1.f;
       if (DT == ATLAS_F16) gain = gain_of(__ldg(a.amax + (int64_t)it.seq * a.Hk + (keys ? it.head : it.head / group)));
       if (!keys) {
-        ok = mbar_wait(&s.a_full[r], (k / kRing) & 1, 220);
+        ok = mbar_wait_soon(&s.a_full[r], (k / kRing) & 1, 220);
         if (!ok) break;
         lse = s.a_lse[r][own];
         delta = s.a_delta[r][own];
@@ -648,7 +649,7 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
         if (left <= 0) left = it.len;
         if (t % kGroups != g) continue;
         const int x = t % 3, st = t % kStages;
-        ok = mbar_wait(&s.s_full[x], (t / 3) & 1, 221) && (!keys || mbar_wait(&s.b_full[st], (t / kStages) & 1, 222));
+        ok = mbar_wait_soon(&s.s_full[x], (t / 3) & 1, 221) && (!keys || mbar_wait_soon(&s.b_full[st], (t / kStages) & 1, 222));
         if (!ok) break;
         tc_fence_after();
         if (live) {

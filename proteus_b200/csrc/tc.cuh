@@ -57,6 +57,31 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int co
   return false;
 }
 
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// The same wait for chains of short steps. try_wait takes 140 clocks on a phase that has completed already,
+// test_wait 45 (measured): look once before settling down to wait, or, for the few warps that feed
+// the tensor core, do nothing else but look.
+__device__ __forceinline__ bool mbar_wait_soon(uint64_t* bar, uint32_t parity, int code) {
+  return mbar_test(bar, parity) || mbar_wait(bar, parity, code);
+}
+__device__ __forceinline__ bool mbar_spin(uint64_t* bar, uint32_t parity, int code) {
+  for (uint32_t i = 0; i < kWaitLimit; ++i)
+    if (mbar_test(bar, parity)) return true;
+  atomicCAS(&g_device_status, 0, code);
+  return false;
+}
+
 // 2-D TMA tile load into shared memory, completion counted on `bar`; each CTA loads its own copy.
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int32_t c0, int32_t c1, uint64_t* bar) {
   asm volatile(
