@@ -88,16 +88,22 @@ LAUNCHES = {"count": 0}
 _KERNELS.update({"atlas_ctx_rows": 4, "atlas_ctx_annotations": 2, "atlas_attention_grad": 3})
 
 
+def _count_admit(args):  # candidates, plus the bulk-row kernel when there are bulk rows
+    return 2 if (args[6] and args[20]) else 1
+
+
+def _count_maps(args):  # more than 1024 sequences: totals, a scan, then the outputs
+    return 3 if args[2] > 1024 else 1
+
+
+_KERNELS.update({"atlas_dense_select": 3,  # row-major count (+ keys in key order), row-major emit, hard columns
+                 "atlas_admit": _count_admit, "atlas_seq_maps": _count_maps})
+_KERNELS.update({n: 0 for n in SIGNATURES if n.endswith("_bytes") or n.endswith("_i32")})
+
+
 def _n_kernels(name: str, args) -> int:
-    if name == "atlas_dense_select":
-        return 3  # row-major count (+ keys in key order), row-major emit, hard columns
-    if name == "atlas_admit":  # candidates, plus the bulk-row kernel when there are bulk rows
-        return 2 if (args[6] and args[20]) else 1
-    if name == "atlas_seq_maps":  # more than 1024 sequences: a scan, then the outputs
-        return 2 if args[2] > 1024 else 1
-    if name.endswith("_bytes") or name.endswith("_i32"):
-        return 0
-    return _KERNELS.get(name, 1)
+    n = _KERNELS.get(name, 1)
+    return n if isinstance(n, int) else n(args)
 
 
 def call(name: str, *args):
@@ -119,7 +125,19 @@ def ptr(t):
 
 
 def stream_ptr(device=None):
-    return torch.cuda.current_stream(device).cuda_stream
+    """Handle of the current stream of `device` (a torch.device; None: the current device)."""
+    index = device.index if isinstance(device, torch.device) else None
+    if index is None:
+        return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(index)  # the handle alone: 0.1 us instead of 2
+
+
+def launch(device, name: str, *args):
+    """call(name, *args, stream) with `device` current: the C ABI launches on the current device."""
+    if torch.cuda.current_device() == device.index:
+        return call(name, *args, torch._C._cuda_getCurrentRawStream(device.index))
+    with torch.cuda.device(device):
+        return call(name, *args, torch._C._cuda_getCurrentRawStream(device.index))
 
 
 def dtype_code(dt: torch.dtype) -> int:

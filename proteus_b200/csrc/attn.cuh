@@ -84,6 +84,19 @@ __device__ __forceinline__ bool idle_rows(const AttnArgs& a, const SeqBlock& s, 
   return *to > *from;
 }
 
+// Sets a kernel's dynamic shared memory once per device (each launch of a short sequence would otherwise pay
+// for it on the host).
+template <typename K>
+inline int attn_smem_once(K kernel, int bytes, bool (&done)[64]) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && done[dev]) return ATLAS_OK;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+    return fail(ATLAS_ERR_CUDA, "attention: shared memory attribute");
+  if (dev >= 0 && dev < 64) done[dev] = true;
+  return ATLAS_OK;
+}
+
 // Values a head of the padded vectors: every sequence's rows and up to 4 between two, and 128 that a
 // tile may read behind the last.
 inline int64_t attn_vec_ld(int64_t outer, int64_t rows, int64_t B) { return (outer * rows + 4 * B + 128 + 7) / 4 * 4; }

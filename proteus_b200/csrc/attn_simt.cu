@@ -373,17 +373,11 @@ int attn_delta(const AttnArgs& a, int dtype, cudaStream_t st) {
 
 namespace {
 
-template <typename K>
-int big_smem(K kernel, int bytes) {
-  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess
-             ? ATLAS_OK
-             : fail(ATLAS_ERR_CUDA, "attention: shared memory attribute");
-}
-
 template <int DT, int DP>
 int fwd(const AttnArgs& a, cudaStream_t st) {
   const int bytes = (3 * BT * (DP + 4) + BT * PP) * 4;
-  if (int rc = big_smem(attn_fwd_simt_kernel<DT, DP>, bytes)) return rc;
+  static bool done[64] = {};
+  if (int rc = attn_smem_once(attn_fwd_simt_kernel<DT, DP>, bytes, done)) return rc;
   attn_fwd_simt_kernel<DT, DP><<<dim3((unsigned)(2 * a.cap), a.H), kThreads, bytes, st>>>(a);
   return check_launch("attention");
 }
@@ -391,8 +385,9 @@ int fwd(const AttnArgs& a, cudaStream_t st) {
 template <int DT, int DP>
 int bwd(const AttnArgs& a, cudaStream_t st) {
   const int bytes = (4 * BT * (DP + 4) + 2 * BT * PP + 2 * BT) * 4;
-  if (int rc = big_smem(attn_bwd_simt_kernel<DT, DP, true>, bytes)) return rc;
-  if (int rc = big_smem(attn_bwd_simt_kernel<DT, DP, false>, bytes)) return rc;
+  static bool done[2][64] = {};
+  if (int rc = attn_smem_once(attn_bwd_simt_kernel<DT, DP, true>, bytes, done[0])) return rc;
+  if (int rc = attn_smem_once(attn_bwd_simt_kernel<DT, DP, false>, bytes, done[1])) return rc;
   if (int rc = attn_delta(a, DT, st)) return rc;
   attn_bwd_simt_kernel<DT, DP, true><<<dim3((unsigned)(2 * a.cap), a.Hk), kThreads, bytes, st>>>(a);
   attn_bwd_simt_kernel<DT, DP, false><<<dim3((unsigned)(2 * a.cap), a.H), kThreads, bytes, st>>>(a);

@@ -713,8 +713,8 @@ int fwd(const AttnArgs& a, cudaStream_t st) {
   if (int rc = make_map(&mk, a.k, DT, a.sk, a.outer, a.Hk, a.rows, a.D, BM)) return rc;
   if (int rc = make_map(&mv, a.v, DT, a.sv, a.outer, a.Hk, a.rows, a.D, BM)) return rc;
   const int bytes = sizeof(FwdSmem) + 1024;
-  if (cudaFuncSetAttribute(attn_fwd_tc_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
-    return fail(ATLAS_ERR_CUDA, "attention: shared memory attribute");
+  static bool done[64] = {};
+  if (int rc = attn_smem_once(attn_fwd_tc_kernel<DT>, bytes, done)) return rc;
   const int vec = a.D % 8 == 0 && map_ok(a.out, a.so, a.outer, a.H, a.rows);
   attn_fwd_tc_kernel<DT><<<dim3((unsigned)a.cap, a.H), kFwdThreads, bytes, st>>>(mq, mk, mv, a, vec);
   return check_launch("attention");
@@ -728,8 +728,8 @@ int bwd(const AttnArgs& a, cudaStream_t st) {
   if (int rc = make_map(&mv, a.v, DT, a.sv, a.outer, a.Hk, a.rows, a.D, BN)) return rc;
   if (int rc = make_map(&mdo, a.dout, DT, a.sdo, a.outer, a.H, a.rows, a.D, BN)) return rc;
   const int bytes = sizeof(BwdSmem) + 1024;
-  if (cudaFuncSetAttribute(attn_bwd_tc_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
-    return fail(ATLAS_ERR_CUDA, "attention_grad: shared memory attribute");
+  static bool done[64] = {};
+  if (int rc = attn_smem_once(attn_bwd_tc_kernel<DT>, bytes, done)) return rc;
   const int vec = a.D % 8 == 0 && map_ok(a.dq, a.sdq, a.outer, a.H, a.rows) && map_ok(a.dk, a.sdk, a.outer, a.Hk, a.rows) &&
                   map_ok(a.dv, a.sdv, a.outer, a.Hk, a.rows);
   if (DT == ATLAS_F16 && cudaMemsetAsync(a.amax, 0, (size_t)(a.B * a.Hk) * 4, st) != cudaSuccess)

@@ -8,7 +8,9 @@
 // the outputs, not the sequences, are what the CTAs share out (one long sequence is as even as many
 // short ones), each thread writes two rows with one 16-byte store per array, and up to 1024
 // sequences every CTA scans the lengths again for itself in shared memory (4 KB from L2) instead of
-// waiting for a scan kernel. Above that a first launch writes the prefix sums to the workspace.
+// waiting for a scan kernel. Above that two launches of one CTA per 1024 sequences (totals, then prefix sums)
+// write to the workspace what the last one searches; its CTAs have long runs of outputs, so that the search
+// for a run's first and last sequence, 16 dependent reads for 65536, is paid twice a CTA and not a thread.
 #include "common.cuh"
 
 namespace atlas {
@@ -18,6 +20,7 @@ constexpr int kTile = 128;        // rows of a block
 constexpr int kScan = 1024;       // sequences one CTA scans
 constexpr int kThreads = 512;
 constexpr int kRowsPerCta = 2 * kThreads;
+constexpr int kStage = 1024;      // sequences whose prefix sums a CTA keeps in shared memory
 
 struct MapArgs {
   const void* len;
@@ -29,7 +32,9 @@ struct MapArgs {
   int32_t* blocks;
   int64_t cap;
   int64_t* counts;
-  int32_t *kept_end, *blk_end;  // inclusive prefix sums [B] (the two-launch path)
+  // More than 1024 sequences: totals of each 1024, and inclusive prefix sums [B].
+  int64_t* total;
+  int32_t *kept_end, *blk_end;
 };
 
 __device__ __forceinline__ int64_t raw_len(const MapArgs& a, int64_t b) {
@@ -56,14 +61,12 @@ __device__ __forceinline__ int64_t warp_sum64(int64_t v) {
 
 // Sum over the block (every thread gets it); `red` holds one slot per warp.
 __device__ int64_t block_sum64(int64_t v, int64_t* red) {
-  const int w = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   v = warp_sum64(v);
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[w] = v;
+  if (lane == 0) red[w] = v;
   __syncthreads();
-  int64_t s = 0;
-  for (int i = 0; i < (int)blockDim.x / 32; ++i) s += red[i];
-  return s;
+  return warp_sum64(lane < (int)blockDim.x / 32 ? red[lane] : 0);
 }
 
 // Inclusive scan over the block of one int per thread plus `base`; `red` holds one slot per warp.
@@ -91,22 +94,78 @@ __device__ __forceinline__ int upper(const int32_t* end, int lo, int hi, int i) 
   return lo;
 }
 
-// The outputs of this CTA, from the inclusive prefix sums of kept positions and blocks.
+// The same by a warp: 32 probes a step, so that 65536 sequences take 4 dependent reads and not 16.
+__device__ __forceinline__ int upper_warp(const int32_t* end, int lo, int hi, int i) {
+  const int lane = threadIdx.x & 31;
+  while (lo < hi) {
+    const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+    // probes at the last element of each of 32 parts
+    const int probe = at + step - 1 < hi ? at + step - 1 : hi - 1;
+    const uint32_t above = __ballot_sync(0xFFFFFFFFu, at >= hi || end[probe] > i);
+    const int part = __ffs(above) - 1;  // the first part whose last element is above i
+    if (above == 0) return hi;
+    const int from = lo + part * step;
+    if (from >= hi) return hi;
+    if (step == 1) return from;
+    lo = from;
+    hi = from + step < hi ? from + step : hi;
+  }
+  return lo;
+}
+
+// The outputs of this CTA, an even share of each kind, from the inclusive prefix sums of kept positions and
+// blocks. NARROW: those are in global memory, and four warps first look for the sequences of the share's
+// first and last outputs.
+template <bool NARROW>
 __device__ void fill(const MapArgs& a, const int32_t* kept_end, const int32_t* blk_end, const int32_t* cu) {
+  __shared__ int s_range[4];
+  __shared__ int32_t s_end[NARROW ? kStage : 1], s_first[NARROW ? kStage : 1];
   const int B = (int)a.B;
   const int total = kept_end[B - 1], nblk = blk_end[B - 1];
-  const int64_t i0 = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * 2;
-  if (i0 < a.rows) {
+  const int64_t rper = (a.rows + 2 * gridDim.x - 1) / (2 * gridDim.x) * 2, row0 = blockIdx.x * rper;
+  const int64_t row1 = row0 + rper < a.rows ? row0 + rper : a.rows;
+  const int64_t bper = (a.cap + gridDim.x - 1) / gridDim.x, blk0 = blockIdx.x * bper;
+  const int64_t blk1 = blk0 + bper < a.cap ? blk0 + bper : a.cap;
+  int lo = 0, hi = B, blo = 0, bhi = B;
+  if (NARROW) {
+    const int w = threadIdx.x >> 5;
+    if (w < 4) {
+      const bool last = w & 1, rows = w < 2;
+      const int n = rows ? total : nblk;
+      int64_t i = rows ? (last ? row1 - 1 : row0) : (last ? blk1 - 1 : blk0);
+      if (i > n - 1) i = n - 1;
+      const int at = n ? upper_warp(rows ? kept_end : blk_end, 0, B, (int)(i < 0 ? 0 : i)) : 0;
+      if ((threadIdx.x & 31) == 0) s_range[w] = at;
+    }
+    __syncthreads();
+    lo = s_range[0];
+    hi = s_range[1] + 1;
+    blo = s_range[2];
+    bhi = s_range[3] + 1;
+    if (hi - lo <= kStage) {  // the share's part of the prefix sums in shared memory, indexed from lo
+      for (int i = threadIdx.x; i < hi - lo; i += kThreads) {
+        s_end[i] = kept_end[lo + i];
+        s_first[i] = lo + i ? kept_end[lo + i - 1] : 0;
+      }
+      __syncthreads();
+    }
+  }
+  const bool staged = NARROW && hi - lo <= kStage;
+  for (int64_t i0 = row0 + threadIdx.x * 2; i0 < row1; i0 += 2 * kThreads) {
     int64_t s[2], t[2];
-    int b = i0 < total ? upper(kept_end, 0, B, (int)i0) : B;
+    int b = i0 >= total ? B : staged ? lo + upper(s_end, 0, hi - lo, (int)i0) : upper(kept_end, lo, hi, (int)i0);
     for (int e = 0; e < 2; ++e) {
       const int64_t i = i0 + e;
       if (i >= total) {
         s[e] = t[e] = -1;
         continue;
       }
-      if (kept_end[b] <= i) b = upper(kept_end, b + 1, B, (int)i);
-      const int64_t p = i - (b ? kept_end[b - 1] : 0);
+      if (staged) {
+        if (s_end[b - lo] <= i) b = lo + upper(s_end, b + 1 - lo, hi - lo, (int)i);
+      } else if (kept_end[b] <= i) {
+        b = upper(kept_end, b + 1, hi, (int)i);
+      }
+      const int64_t p = i - (staged ? s_first[b - lo] : b ? kept_end[b - 1] : 0);
       s[e] = (a.stride ? b * a.stride : (int64_t)cu[b]) + a.lead + p;
       t[e] = (a.seq ? a.seq[b] : (int64_t)b) * 1024 + p;  // core.pack_tok
     }
@@ -118,10 +177,10 @@ __device__ void fill(const MapArgs& a, const int32_t* kept_end, const int32_t* b
       a.tok[i0] = t[0];
     }
   }
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < a.cap; i += (int64_t)gridDim.x * kThreads) {
+  for (int64_t i = blk0 + threadIdx.x; i < blk1; i += kThreads) {
     int2 e = make_int2(-1, -1);
     if (i < nblk) {
-      const int b = upper(blk_end, 0, B, (int)i);
+      const int b = upper(blk_end, blo, bhi, (int)i);
       e = make_int2(b, ((int)i - (b ? blk_end[b - 1] : 0)) * kTile);
     }
     reinterpret_cast<int2*>(a.blocks)[i] = e;
@@ -168,37 +227,49 @@ __global__ void __launch_bounds__(kThreads) maps_small_kernel(const MapArgs a) {
     }
   }
   __syncthreads();
-  fill(a, s_kept, s_blk, s_cu);
+  fill<false>(a, s_kept, s_blk, s_cu);
 }
 
-// Two launches, the first: CTA c adds up the lengths of all sequences (for the fit) and of those
-// before its 1024, then scans its own.
+// Three launches, the first: rows, kept positions, blocks and misfits of each 1024 sequences.
+__global__ void __launch_bounds__(kScan) maps_total_kernel(const MapArgs a) {
+  __shared__ int64_t red64[kScan / 32];
+  const int64_t b = (int64_t)blockIdx.x * kScan + threadIdx.x;
+  int bad = 0;
+  const int n = b < a.B ? cut_len(a, b, &bad) : 0;
+  const int64_t t[4] = {block_sum64(n, red64), block_sum64(b < a.B ? kept_of(a, n) : 0, red64),
+                        block_sum64(b < a.B ? blocks_of(n) : 0, red64), block_sum64(bad, red64)};
+  if (threadIdx.x < 4) a.total[blockIdx.x * 4 + threadIdx.x] = t[threadIdx.x];
+}
+
+// The second: the totals before a CTA's own sequences, and the scan of those.
 __global__ void __launch_bounds__(kScan) maps_scan_kernel(const MapArgs a) {
   __shared__ int64_t red64[kScan / 32];
   __shared__ int red[kScan / 32];
-  const int64_t first = (int64_t)blockIdx.x * kScan;
-  int64_t all = 0, pc = 0, pk = 0, pt = 0;
-  int bad = 0;
-#pragma unroll 4
-  for (int64_t b = threadIdx.x; b < a.B; b += kScan) {
-    const int n = cut_len(a, b, &bad);
-    all += n;
-    if (b < first) {
-      pc += n;
-      pk += kept_of(a, n);
-      pt += blocks_of(n);
+  int64_t all = 0, nbad = 0, pc = 0, pk = 0, pt = 0;
+  for (int64_t c = threadIdx.x; c < gridDim.x; c += kScan) {
+    const int64_t* t = a.total + c * 4;
+    all += t[0];
+    nbad += t[3];
+    if (c < blockIdx.x) {
+      pc += t[0];
+      pk += t[1];
+      pt += t[2];
     }
   }
   all = block_sum64(all, red64);
-  const bool fits = all <= a.rows;
-  const int64_t b = first + threadIdx.x;
-  const bool on = b < a.B;
+  nbad = block_sum64(nbad, red64);
+  pc = block_sum64(pc, red64);
+  pk = block_sum64(pk, red64);
+  pt = block_sum64(pt, red64);
+  const int64_t first = (int64_t)blockIdx.x * kScan, b = first + threadIdx.x;
+  const bool on = b < a.B, fits = all <= a.rows;
+  if (!fits) {  // no map at all: every sequence empty, which still has one block
+    pc = pk = 0;
+    pt = first;
+    nbad += 1;
+  }
   int ignore = 0;
   const int n = on && fits ? cut_len(a, b, &ignore) : 0;
-  pc = fits ? block_sum64(pc, red64) : 0;
-  pk = fits ? block_sum64(pk, red64) : 0;
-  pt = fits ? block_sum64(pt, red64) : first;  // an empty sequence still has one block
-  const int64_t nbad = block_sum64(bad, red64) + !fits;
   const int ec = block_scan(n, (int)pc, red);
   const int ek = block_scan(on ? kept_of(a, n) : 0, (int)pk, red);
   const int et = block_scan(on ? blocks_of(n) : 0, (int)pt, red);
@@ -214,14 +285,18 @@ __global__ void __launch_bounds__(kScan) maps_scan_kernel(const MapArgs a) {
   }
 }
 
-__global__ void __launch_bounds__(kThreads) maps_fill_kernel(const MapArgs a) { fill(a, a.kept_end, a.blk_end, a.cu); }
+__global__ void __launch_bounds__(kThreads) maps_fill_kernel(const MapArgs a) {
+  fill<true>(a, a.kept_end, a.blk_end, a.cu);
+}
 
 }  // namespace
 }  // namespace atlas
 
 using namespace atlas;
 
-extern "C" int64_t atlas_seq_maps_ws_bytes(int64_t B) { return B > kScan ? 8 * B : 0; }
+extern "C" int64_t atlas_seq_maps_ws_bytes(int64_t B) {
+  return B > kScan ? 8 * B + 32 * ((B + kScan - 1) / kScan) : 0;
+}
 
 extern "C" int atlas_seq_maps(const void* lengths, int lengths_i64, int64_t B, int64_t rows, int64_t stride, int64_t lead,
                               int64_t trail, const int64_t* seq, int32_t* cu, int64_t* slots, int64_t* tok,
@@ -236,14 +311,21 @@ extern "C" int atlas_seq_maps(const void* lengths, int lengths_i64, int64_t B, i
   ATLAS_REQUIRE(((uintptr_t)slots | (uintptr_t)tok) % 16 == 0 && (uintptr_t)blocks % 8 == 0,
                 "seq_maps: slots and tok must be 16-byte aligned, blocks 8-byte aligned");
   ATLAS_REQUIRE(ws_bytes >= atlas_seq_maps_ws_bytes(B) && (ws || B <= kScan), "seq_maps: workspace too small");
+  ATLAS_REQUIRE((uintptr_t)ws % 8 == 0, "seq_maps: the workspace must be 8-byte aligned");
   MapArgs a{lengths, lengths_i64, B, rows, stride, lead, trail, seq, cu, slots, tok, blocks, rows / kTile + B + 1, counts,
-            (int32_t*)ws, (int32_t*)ws + B};
+            (int64_t*)ws, nullptr, nullptr};
   cudaStream_t st = (cudaStream_t)stream;
-  const unsigned grid = (unsigned)((rows + kRowsPerCta - 1) / kRowsPerCta);
+  // 1024 outputs a CTA while there are few, else an even share of a grid that is resident at once
+  const int64_t want = (rows + kRowsPerCta - 1) / kRowsPerCta, most = 4 * num_sms();
+  const unsigned grid = (unsigned)(want < most ? want : most);
   if (B <= kScan) {
     maps_small_kernel<<<grid, kThreads, 0, st>>>(a);
   } else {
-    maps_scan_kernel<<<(unsigned)((B + kScan - 1) / kScan), kScan, 0, st>>>(a);
+    const unsigned parts = (unsigned)((B + kScan - 1) / kScan);
+    a.kept_end = (int32_t*)(a.total + 4 * parts);
+    a.blk_end = a.kept_end + B;
+    maps_total_kernel<<<parts, kScan, 0, st>>>(a);
+    maps_scan_kernel<<<parts, kScan, 0, st>>>(a);
     maps_fill_kernel<<<grid, kThreads, 0, st>>>(a);
   }
   return check_launch("seq_maps");

@@ -5,14 +5,13 @@ atlas/core.py:75-104 — backed only by the sm_100a library (no fallback).
 """
 from __future__ import annotations
 
-import contextlib
-import ctypes
+import struct
 from typing import NamedTuple
 
 import torch
 
 from . import _lib
-from ._lib import call, dtype_code, ptr, require_cuda, stream_ptr
+from ._lib import call, dtype_code, launch, ptr, require_cuda, stream_ptr
 
 I64_MIN = torch.iinfo(torch.int64).min
 
@@ -213,11 +212,6 @@ def merge_rows(sc, tok, val, osc, otok, oval):
 
 
 # ----------------------------------------------------------------------------- a model's batches and answers
-def _on(device):
-    """Make `device` current for the launch (the C ABI launches on the current device)."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-
-
 def _same_device(first, **others):
     for name, t in others.items():
         if t.device != first.device:
@@ -263,31 +257,33 @@ def seq_maps(lengths, n_rows: int, *, stride: int = 0, lead: int = 0, trail: int
     [0, n_rows]) is cut and counted in counts[2]; packed sequences that together do not fit are all
     taken as empty, which counts once more."""
     require_cuda(lengths, "lengths")
-    if lengths.dim() != 1 or lengths.dtype not in (torch.int32, torch.int64):
-        raise TypeError(f"lengths must be int32 or int64 [B], got {lengths.dtype} {list(lengths.shape)}")
-    dev, B = lengths.device, lengths.numel()
+    dt, dev = lengths.dtype, lengths.device
+    if lengths.dim() != 1 or dt not in (torch.int32, torch.int64):
+        raise TypeError(f"lengths must be int32 or int64 [B], got {dt} {list(lengths.shape)}")
+    B = lengths.shape[0]
     if n_rows < 1 or stride < 0 or lead < 0 or trail < 0 or stride * B > n_rows:
         raise ValueError(f"{B} sequences of stride {stride} (lead {lead}, trail {trail}) do not fit {n_rows} rows")
     if seq is not None:
-        _same_device(lengths, seq=seq)
+        if seq.device != dev:
+            _same_device(lengths, seq=seq)
         if seq.shape != lengths.shape or seq.dtype != torch.int64:
             raise TypeError(f"seq must be int64 [{B}], got {seq.dtype} {list(seq.shape)}")
         seq = seq.contiguous()
     lengths = lengths.contiguous()
-    i64 = dict(dtype=torch.int64, device=dev)
     cap = n_rows // 128 + B + 1
     if B == 0:
-        none = torch.full((n_rows,), -1, **i64)
+        none = torch.full((n_rows,), -1, dtype=torch.int64, device=dev)
         return SeqMaps(torch.zeros(1, dtype=torch.int32, device=dev), none, none.clone(),
-                       torch.full((cap, 2), -1, dtype=torch.int32, device=dev), torch.zeros(3, **i64))
+                       torch.full((cap, 2), -1, dtype=torch.int32, device=dev), torch.zeros(3, dtype=torch.int64, device=dev))
     cu = torch.empty(B + 1, dtype=torch.int32, device=dev)
-    blocks = torch.empty(cap, 2, dtype=torch.int32, device=dev)
-    slots, tok, counts = torch.empty(n_rows, **i64), torch.empty(n_rows, **i64), torch.empty(3, **i64)
-    need = int(_lib.load().atlas_seq_maps_ws_bytes(B))
+    blocks = torch.empty((cap, 2), dtype=torch.int32, device=dev)
+    slots = torch.empty(n_rows, dtype=torch.int64, device=dev)
+    tok = torch.empty(n_rows, dtype=torch.int64, device=dev)
+    counts = torch.empty(3, dtype=torch.int64, device=dev)
+    need = _lib.load().atlas_seq_maps_ws_bytes(B)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    with _on(dev):
-        call("atlas_seq_maps", ptr(lengths), int(lengths.dtype == torch.int64), B, n_rows, stride, lead, trail, ptr(seq),
-             ptr(cu), ptr(slots), ptr(tok), ptr(blocks), ptr(counts), ptr(ws), need, stream_ptr(dev))
+    launch(dev, "atlas_seq_maps", lengths.data_ptr(), int(dt == torch.int64), B, n_rows, stride, lead, trail, ptr(seq),
+           cu.data_ptr(), slots.data_ptr(), tok.data_ptr(), blocks.data_ptr(), counts.data_ptr(), ptr(ws), need)
     return SeqMaps(cu, slots, tok, blocks, counts)
 
 
@@ -303,49 +299,50 @@ def _unit(t):
 
 
 def _strides(*ts):
-    s = [x for t in ts for x in t.stride()[:3]]
-    return (ctypes.c_int64 * len(s))(*s)
+    """The (outer, head, row) strides of the tensors as the host array the C ABI takes."""
+    return struct.pack(f"{3 * len(ts)}q", *[x for t in ts for x in t.stride()[:3]])
 
 
 def _check_attention(q, k, v, plan):
+    """Shapes (outer, H, rows, D), key heads and batch of an attention call, or an error that names what is wrong."""
     require_cuda(q, "q")
-    _same_device(q, k=k, v=v, cu=plan.cu, blocks=plan.blocks, counts=plan.counts)
-    if q.dim() != 4 or k.shape != v.shape or k.dim() != 4 or (q.shape[0], q.shape[2], q.shape[3]) != \
-            (k.shape[0], k.shape[2], k.shape[3]):
-        raise ValueError(f"q [outer, H, rows, D], k and v [outer, Hk, rows, D]: got {list(q.shape)}, {list(k.shape)}, {list(v.shape)}")
+    cu, blocks, counts, stride = plan
+    dev = q.device
+    if not (k.device == dev and v.device == dev and cu.device == dev and blocks.device == dev and counts.device == dev):
+        _same_device(q, k=k, v=v, cu=cu, blocks=blocks, counts=counts)
+    qs, ks = q.shape, k.shape
+    if len(qs) != 4 or len(ks) != 4 or ks != v.shape or qs[0] != ks[0] or qs[2:] != ks[2:]:
+        raise ValueError(f"q [outer, H, rows, D], k and v [outer, Hk, rows, D]: got {list(qs)}, {list(ks)}, {list(v.shape)}")
     if not q.dtype == k.dtype == v.dtype:
         raise TypeError(f"q, k and v must have one dtype, got {q.dtype}, {k.dtype}, {v.dtype}")
-    dtype_code(q.dtype)
-    if not 1 <= q.shape[3] <= 64:
-        raise ValueError(f"head dimension {q.shape[3]}: 1 to 64 are supported")
-    if k.shape[1] < 1 or q.shape[1] % k.shape[1]:
-        raise ValueError(f"{q.shape[1]} query heads over {k.shape[1]} key heads: not a multiple")
-    B = plan.cu.numel() - 1
-    if B < 0 or plan.cu.dtype != torch.int32 or plan.blocks.dtype != torch.int32 or plan.counts.dtype != torch.int64 or \
-            plan.blocks.dim() != 2 or plan.blocks.shape[1] != 2 or plan.counts.numel() != 3:
+    (o, h, n, d), hk, B, bs = qs, ks[1], cu.shape[0] - 1, blocks.shape
+    if not 1 <= d <= 64:
+        raise ValueError(f"head dimension {d}: 1 to 64 are supported")
+    if hk < 1 or h % hk:
+        raise ValueError(f"{h} query heads over {hk} key heads: not a multiple")
+    if B < 0 or cu.dtype != torch.int32 or blocks.dtype != torch.int32 or counts.dtype != torch.int64 or len(bs) != 2 or \
+            bs[1] != 2 or counts.shape != (3,):
         raise TypeError("plan: cu int32 [B + 1], blocks int32 [n, 2], counts int64 [3] (seq_maps)")
-    if plan.stride == 0 and q.shape[0] != 1:
-        raise ValueError(f"a packed batch has one outer index, got {q.shape[0]}")
-    if plan.stride and (q.shape[0] != B or q.shape[2] != plan.stride):
-        raise ValueError(f"a padded batch of {B} sequences of stride {plan.stride} against q {list(q.shape)}")
-    if plan.blocks.shape[0] < q.shape[0] * q.shape[2] // 128 + B + 1:
-        raise ValueError(f"plan of {plan.blocks.shape[0]} blocks: too few for {q.shape[0] * q.shape[2]} rows")
-    return B
+    if stride == 0 and o != 1:
+        raise ValueError(f"a packed batch has one outer index, got {o}")
+    if stride and (o != B or n != stride):
+        raise ValueError(f"a padded batch of {B} sequences of stride {stride} against q {list(qs)}")
+    if bs[0] < o * n // 128 + B + 1:
+        raise ValueError(f"plan of {bs[0]} blocks: too few for {o * n} rows")
+    return o, h, n, d, hk, B
 
 
 def _attention_forward(q, k, v, plan, scale):
-    B = _check_attention(q, k, v, plan)
-    (o, h, n, d), dev = q.shape, q.device
+    o, h, n, d, hk, B = _check_attention(q, k, v, plan)
+    dev = q.device
     out, lse = _rows_like(q, h), torch.empty(o, h, n, dtype=torch.float32, device=dev)
     if B == 0 or out.numel() == 0:
         return out.zero_(), lse.zero_()
     q, k, v = _unit(q), _unit(k), _unit(v)
-    blocks, counts, cu = plan.blocks.contiguous(), plan.counts.contiguous(), plan.cu.contiguous()
-    s = _strides(q, k, v, out)
-    with _on(dev):
-        call("atlas_attention", ptr(q), ptr(k), ptr(v), dtype_code(q.dtype), ctypes.addressof(s), o, n, h, k.shape[1], d,
-             ptr(cu), ptr(blocks), ptr(counts), B, blocks.shape[0], int(plan.stride == 0), float(scale), ptr(out), ptr(lse),
-             stream_ptr(dev))
+    cu, blocks, counts = plan.cu.contiguous(), plan.blocks.contiguous(), plan.counts.contiguous()
+    launch(dev, "atlas_attention", q.data_ptr(), k.data_ptr(), v.data_ptr(), dtype_code(q.dtype), _strides(q, k, v, out), o, n, h, hk,
+           d, cu.data_ptr(), blocks.data_ptr(), counts.data_ptr(), B, blocks.shape[0], int(plan.stride == 0), scale, out.data_ptr(),
+           lse.data_ptr())
     return out, lse
 
 
@@ -353,25 +350,25 @@ def attention_grad(dout, q, k, v, out, lse, plan: SeqPlan, scale: float | None =
     """(dq, dk, dv) of attention(q, k, v, plan, scale) for the gradient `dout` of its output: the
     probabilities are computed again from `lse`, the keys' gradients summed over the query heads that
     share them. No atomics: the same call gives the same bits. Rows of no sequence come out as zero."""
-    B = _check_attention(q, k, v, plan)
-    _same_device(q, dout=dout, out=out, lse=lse)
+    o, h, n, d, hk, B = _check_attention(q, k, v, plan)
+    dev = q.device
+    if not (dout.device == dev and out.device == dev and lse.device == dev):
+        _same_device(q, dout=dout, out=out, lse=lse)
     if dout.shape != q.shape or out.shape != q.shape or lse.shape != q.shape[:3]:
         raise ValueError(f"dout and out must be {list(q.shape)}, lse {list(q.shape[:3])}")
     if dout.dtype != q.dtype or out.dtype != q.dtype or lse.dtype != torch.float32:
         raise TypeError(f"dout and out must be {q.dtype}, lse float32")
-    scale = q.shape[3] ** -0.5 if scale is None else scale
-    (o, h, n, d), dev = q.shape, q.device
-    dq, dk, dv = _rows_like(q, h), _rows_like(k, k.shape[1]), _rows_like(v, k.shape[1])
+    scale = d ** -0.5 if scale is None else float(scale)
+    dq, dk, dv = _rows_like(q, h), _rows_like(k, hk), _rows_like(v, hk)
     if B == 0 or dq.numel() == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
-    ws = torch.empty(int(_lib.load().atlas_attention_grad_ws_bytes(o, n, h, k.shape[1], B)), dtype=torch.uint8, device=dev)
+    ws = torch.empty(int(_lib.load().atlas_attention_grad_ws_bytes(o, n, h, hk, B)), dtype=torch.uint8, device=dev)
     dout, q, k, v, out, lse = _unit(dout), _unit(q), _unit(k), _unit(v), _unit(out), lse.contiguous()
-    blocks, counts, cu = plan.blocks.contiguous(), plan.counts.contiguous(), plan.cu.contiguous()
-    s = _strides(dout, q, k, v, out, dq, dk, dv)
-    with _on(dev):
-        call("atlas_attention_grad", ptr(dout), ptr(q), ptr(k), ptr(v), ptr(out), ptr(lse), dtype_code(q.dtype), ctypes.addressof(s),
-             o, n, h, k.shape[1], d, ptr(cu), ptr(blocks), ptr(counts), B, blocks.shape[0], int(plan.stride == 0), float(scale),
-             ptr(dq), ptr(dk), ptr(dv), ptr(ws), ws.numel(), stream_ptr(dev))
+    cu, blocks, counts = plan.cu.contiguous(), plan.blocks.contiguous(), plan.counts.contiguous()
+    launch(dev, "atlas_attention_grad", dout.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(),
+           dtype_code(q.dtype), _strides(dout, q, k, v, out, dq, dk, dv), o, n, h, hk, d, cu.data_ptr(), blocks.data_ptr(),
+           counts.data_ptr(), B, blocks.shape[0], int(plan.stride == 0), scale, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+           ws.data_ptr(), ws.shape[0])
     return dq, dk, dv
 
 
@@ -417,65 +414,70 @@ class TokenLogprobs(NamedTuple):
 
 
 def _check_logits(logits, tokens):
+    """N, V and the tokens of a row, or an error that names what is wrong."""
     require_cuda(logits, "logits")
-    _same_device(logits, tokens=tokens)
-    if logits.dim() != 2 or logits.shape[1] < 1:
-        raise ValueError(f"logits must be [N, V] with V >= 1, got {list(logits.shape)}")
-    dtype_code(logits.dtype)
-    if tokens.dtype != torch.int64 or tokens.dim() not in (1, 2) or tokens.shape[0] != logits.shape[0]:
-        raise TypeError(f"tokens must be int64 [N] or [N, J], got {tokens.dtype} {list(tokens.shape)}")
-    if tokens.dim() == 2 and tokens.shape[1] > 64:
-        raise ValueError(f"{tokens.shape[1]} tokens a row: at most 64")
-    return 1 if tokens.dim() == 1 else tokens.shape[1]
+    if tokens.device != logits.device:
+        _same_device(logits, tokens=tokens)
+    shape, given = logits.shape, tokens.shape
+    if len(shape) != 2 or shape[1] < 1:
+        raise ValueError(f"logits must be [N, V] with V >= 1, got {list(shape)}")
+    if tokens.dtype != torch.int64 or not 1 <= len(given) <= 2 or given[0] != shape[0]:
+        raise TypeError(f"tokens must be int64 [N] or [N, J], got {tokens.dtype} {list(given)}")
+    J = given[1] if len(given) == 2 else 1
+    if J > 64:
+        raise ValueError(f"{J} tokens a row: at most 64")
+    return *shape, J
 
 
-def _row_stride(t):
-    """Row stride for the kernels: of a single row, whatever it says, the row's length."""
-    return max(t.stride(0), t.shape[1]) if t.shape[0] <= 1 else t.stride(0)
-
-
-def _plain_rows(t):
-    """[N, V] with unit column stride and rows that do not overlap (an expanded row is copied out)."""
-    return t if (t.stride(1) == 1 or t.shape[1] == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]) else t.contiguous()
+def _plain_rows(t, N, V):
+    """t [N, V] with unit column stride and rows that do not overlap (an expanded row is copied out), and its
+    row stride (of a single row, whatever that says, the row's length)."""
+    s0, s1 = t.stride()
+    if (s1 == 1 or V == 1) and (N <= 1 or s0 >= V):
+        return t, max(s0, V)
+    return t.contiguous(), V
 
 
 def _token_logprobs_forward(logits, tokens, top):
-    J = _check_logits(logits, tokens)
-    (N, V), dev = logits.shape, logits.device
+    N, V, J = _check_logits(logits, tokens)
+    dt, dev = dtype_code(logits.dtype), logits.device
     if not 0 <= top <= min(32, V):
         raise ValueError(f"top must be in [0, min(32, V)], got {top} for V = {V}")
-    logits, tokens = _plain_rows(logits), tokens.contiguous()
-    f32 = dict(dtype=torch.float32, device=dev)
-    r = TokenLogprobs(torch.empty(tokens.shape, **f32), torch.empty(tokens.shape, dtype=torch.int32, device=dev),
-                      torch.empty(N, **f32), torch.empty(N, **f32), torch.empty(N, top, dtype=torch.int64, device=dev),
-                      torch.empty(N, top, **f32))
+    (logits, ld), tokens = _plain_rows(logits, N, V), tokens.contiguous()
+    rank = torch.empty(tokens.shape, dtype=torch.int32, device=dev)
+    top_id = torch.empty((N, top), dtype=torch.int64, device=dev)
+    logprob, entropy, lse, top_logprob = torch.empty(N * (J + 2 + top), dtype=torch.float32, device=dev).split((N * J, N, N, N * top))
+    logprob, top_logprob = logprob.view(tokens.shape), top_logprob.view(N, top)
     if N:
-        with _on(dev):
-            call("atlas_token_logprobs", ptr(logits), dtype_code(logits.dtype), N, V, _row_stride(logits), ptr(tokens), J, top,
-                 ptr(r.logprob), ptr(r.rank), ptr(r.entropy), ptr(r.lse), ptr(r.top_id), ptr(r.top_logprob), stream_ptr(dev))
-    return r
+        launch(dev, "atlas_token_logprobs", logits.data_ptr(), dt, N, V, ld, tokens.data_ptr(), J, top, logprob.data_ptr(),
+               rank.data_ptr(), entropy.data_ptr(), lse.data_ptr(), top_id.data_ptr(), top_logprob.data_ptr())
+    return TokenLogprobs(logprob, rank, entropy, lse, top_id, top_logprob)
+
+
+def _row_vector(logits, name, t, shape):
+    if t.device != logits.device:
+        _same_device(logits, **{name: t})
+    if t.dtype != torch.float32 or t.shape != shape:
+        raise TypeError(f"{name} must be float32 {list(shape)}, got {t.dtype} {list(t.shape)}")
+    return t.contiguous()
 
 
 def token_logprobs_grad(logits, tokens, lse, entropy, g_logprob=None, g_entropy=None):
     """Gradient by the logits, [N, V] in their dtype, of sum(g_logprob * logprob) + sum(g_entropy *
     entropy), from token_logprobs' lse and entropy. Either gradient may be None. A token given twice
     in a row counts twice; one outside [0, V) not at all."""
-    J = _check_logits(logits, tokens)
-    (N, V), dev = logits.shape, logits.device
-    gs = {"lse": (lse, (N,)), "entropy": (entropy, (N,)), "g_logprob": (g_logprob, tuple(tokens.shape)), "g_entropy": (g_entropy, (N,))}
-    for name, (t, shape) in gs.items():
-        if t is None and name.startswith("g_"):
-            continue
-        _same_device(logits, **{name: t})
-        if t.dtype != torch.float32 or tuple(t.shape) != shape:
-            raise TypeError(f"{name} must be float32 {list(shape)}, got {t.dtype} {list(t.shape)}")
-    logits, tokens, lse, entropy = _plain_rows(logits), tokens.contiguous(), lse.contiguous(), entropy.contiguous()
-    g_logprob, g_entropy = (None if g is None else g.contiguous() for g in (g_logprob, g_entropy))
-    dx = torch.empty(N, V, dtype=logits.dtype, device=dev)
+    N, V, J = _check_logits(logits, tokens)
+    dt, dev = dtype_code(logits.dtype), logits.device
+    lse, entropy = _row_vector(logits, "lse", lse, (N,)), _row_vector(logits, "entropy", entropy, (N,))
+    if g_logprob is not None:
+        g_logprob = _row_vector(logits, "g_logprob", g_logprob, tokens.shape)
+    if g_entropy is not None:
+        g_entropy = _row_vector(logits, "g_entropy", g_entropy, (N,))
+    (logits, ld), tokens = _plain_rows(logits, N, V), tokens.contiguous()
+    dx = torch.empty((N, V), dtype=logits.dtype, device=dev)
     if N:
-        with _on(dev):
-            call("atlas_token_logprobs_grad", ptr(logits), dtype_code(logits.dtype), N, V, _row_stride(logits), ptr(tokens), J,
-                 ptr(lse), ptr(entropy), ptr(g_logprob), ptr(g_entropy), ptr(dx), V, stream_ptr(dev))
+        launch(dev, "atlas_token_logprobs_grad", logits.data_ptr(), dt, N, V, ld, tokens.data_ptr(), J, lse.data_ptr(),
+               entropy.data_ptr(), ptr(g_logprob), ptr(g_entropy), dx.data_ptr(), V)
     return dx
 
 
