@@ -47,6 +47,30 @@ __device__ __forceinline__ float ex2(float v) {
   return r;
 }
 
+// Two fp32 values as one operand of the packed fp32 instructions.
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 pair(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(f32x2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // Order of the alternatives as an unsigned integer: -0 as +0, NaN above all, never 0.
 __device__ __forceinline__ uint32_t order_key(float v) {
   if (v != v) return 0xFFFFFFFFu;
@@ -195,7 +219,10 @@ __global__ void __launch_bounds__(256) logprobs_short_kernel(const LpArgs a) {
 // streams its part with 16-byte loads. Alternatives: each warp keeps its 32 best so far as 64-bit
 // keys (order << 32 | ~index), sorted over the lanes; what beats the n-th of them is collected in
 // shared memory, and every 32 of those are sorted (bitonic) and merged into the list.
-constexpr int kLongThreads = 512, kLongWarps = kLongThreads / 32;
+// Threads of a CTA: 128 where rows fill the GPU (4095 x 50003 bf16: 98 us, 256 threads 104, 512 144: a row's
+// start and end overlap with other rows), 512 where a cluster shares one row (65537 bf16: 14 us, 128 20).
+constexpr int long_threads(int CL) { return CL == 1 ? 128 : 512; }
+constexpr int kLongUnroll = 2;
 
 __device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int o) { return __shfl_xor_sync(kFull, v, o); }
 
@@ -240,6 +267,12 @@ struct TopList {
     buf = b;
     n = n_;
   }
+  // The n-th largest of the lanes' own largest values: n entries at least are as large.
+  __device__ __forceinline__ void seed(float mx, int lane) {
+    const uint64_t v = warp_sort_desc((uint64_t)order_key(mx) << 32, lane);
+    bar = __shfl_sync(kFull, v, n - 1) - 1;
+    bar_hi = (uint32_t)((bar + 1) >> 32);
+  }
   __device__ __noinline__ void flush(int lane) {
     __syncwarp();
     const uint64_t v = lane < held ? buf[lane] : 0;
@@ -248,8 +281,11 @@ struct TopList {
     buf[lane] = rest;
     held = max(0, held - 32);
     list = merge_lists(list, warp_sort_desc(v, lane), lane);
-    bar = __shfl_sync(kFull, list, n - 1);
-    bar_hi = (uint32_t)(bar >> 32);
+    const uint64_t nth = __shfl_sync(kFull, list, n - 1);
+    if (nth > bar) {
+      bar = nth;
+      bar_hi = (uint32_t)(bar >> 32);
+    }
     __syncwarp();
   }
   __device__ __forceinline__ void offer(uint64_t key, int lane) {
@@ -264,47 +300,113 @@ struct TopList {
 
 __device__ __forceinline__ uint64_t full_key(uint32_t k, uint32_t id) { return ((uint64_t)k << 32) | (uint32_t)~id; }
 
+// 16 bytes of a row as the kernels look at them: the largest, and how many are above a given value. For
+// 16-bit types both two values at a time (max passes over a NaN, a comparison with one is false).
+template <int DT>
+struct Vec {
+  using T = typename Elem<DT>::T;
+  static constexpr int N = 16 / sizeof(T);
+  uint4 raw;
+  __device__ __forceinline__ float at(int i) const { return Elem<DT>::f(reinterpret_cast<const T*>(&raw)[i]); }
+  __device__ __forceinline__ float top() const {
+    if constexpr (DT == ATLAS_F32) {
+      return fmaxf(fmaxf(at(0), at(1)), fmaxf(at(2), at(3)));
+    } else if constexpr (DT == ATLAS_BF16) {
+      const auto* w = reinterpret_cast<const __nv_bfloat162*>(&raw);
+      const __nv_bfloat162 m = __hmax2(__hmax2(w[0], w[1]), __hmax2(w[2], w[3]));
+      return fmaxf(__low2float(m), __high2float(m));
+    } else {
+      const auto* w = reinterpret_cast<const __half2*>(&raw);
+      const __half2 m = __hmax2(__hmax2(w[0], w[1]), __hmax2(w[2], w[3]));
+      return fmaxf(__low2float(m), __high2float(m));
+    }
+  }
+  // x: a value of the row's type
+  __device__ __forceinline__ int above(float x) const {
+    if constexpr (DT == ATLAS_F32) {
+      return (at(0) > x) + (at(1) > x) + (at(2) > x) + (at(3) > x);
+    } else if constexpr (DT == ATLAS_BF16) {
+      const auto* w = reinterpret_cast<const __nv_bfloat162*>(&raw);
+      const __nv_bfloat162 b = __float2bfloat162_rn(x);
+      const __nv_bfloat162 n = __hadd2(__hadd2(__hgt2(w[0], b), __hgt2(w[1], b)), __hadd2(__hgt2(w[2], b), __hgt2(w[3], b)));
+      return (int)(__low2float(n) + __high2float(n));
+    } else {
+      const auto* w = reinterpret_cast<const __half2*>(&raw);
+      const __half2 b = __float2half2_rn(x);
+      const __half2 n = __hadd2(__hadd2(__hgt2(w[0], b), __hgt2(w[1], b)), __hadd2(__hgt2(w[2], b), __hgt2(w[3], b)));
+      return (int)(__low2float(n) + __high2float(n));
+    }
+  }
+  __device__ static __forceinline__ uint4 lowest() {  // -inf throughout
+    const uint32_t u = DT == ATLAS_F32 ? 0xFF800000u : DT == ATLAS_BF16 ? 0xFF80FF80u : 0xFC00FC00u;
+    return make_uint4(u, u, u, u);
+  }
+};
+
 template <int G>
 struct Given {
   float x[G];
   int c[G];
 };
 
-// One slice of the row: `n` (<= VEC) values at columns v.. of this lane.
-template <int G, int VEC, bool STATS>
-__device__ __forceinline__ void take(const float (&x)[VEC], int n, uint32_t v, int lane, Stat& s, Given<G>& g, TopList& top,
-                                     bool want_top) {
+// The columns v .. of one vector of this lane (`on`: there is one; the others are all -inf).
+template <int DT, int G, bool STATS, bool TOP>
+__device__ __forceinline__ void take(const Vec<DT>& q, bool on, uint32_t v, int lane, Stat& s, Given<G>& g, TopList& top) {
+  constexpr int N = Vec<DT>::N;
   if (STATS) {
-    float mx = kNegInf;
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) mx = fmaxf(mx, x[i]);
-    if (want_top) {
-      // NaN sorts first: fmaxf passes over it, so it is looked for apart
+    const float mx = q.top();
+    if (TOP) {
+      if (top.bar == 0) top.seed(on ? mx : kNegInf, lane);
+      // NaN sorts first: the maximum passes over it, so it is looked for apart
       bool any = false;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) any |= x[i] != x[i];
-      any |= n > 0 && order_key(mx) >= top.bar_hi;
+      for (int i = 0; i < N; ++i) any |= q.at(i) != q.at(i);
+      any |= on && order_key(mx) >= top.bar_hi;
       if (__any_sync(kFull, any)) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) top.offer(i < n ? full_key(order_key(x[i]), v + i) : 0, lane);
+        for (int i = 0; i < N; ++i) top.offer(on ? full_key(order_key(q.at(i)), v + i) : 0, lane);
       }
     }
     if (mx > s.M) raise_to(s, mx);
     const float ref = ref_of(s.M);
+    const f32x2 nref = pair(-ref, -ref), l2 = pair(kLog2e, kLog2e);
+    f32x2 z = 0, t = 0;
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) add_term(s, x[i], ref);
+    for (int i = 0; i < N; i += 2) {
+      float d0, d1, e0, e1;
+      const f32x2 d = add2(pair(q.at(i), q.at(i + 1)), nref);
+      unpair(mul2(d, l2), e0, e1);
+      unpair(d, d0, d1);
+      const f32x2 e = pair(ex2(e0), ex2(e1));
+      z = add2(z, e);
+      t = fma2(e, pair(fmaxf(d0, -1000.f), fmaxf(d1, -1000.f)), t);  // d = -inf: its term is 0
+    }
+    float z0, z1, t0, t1;
+    unpair(z, z0, z1);
+    unpair(t, t0, t1);
+    s.Z += z0 + z1;
+    s.T += t0 + t1;
   }
 #pragma unroll
-  for (int k = 0; k < G; ++k)
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) g.c[k] += x[i] > g.x[k];
+  for (int k = 0; k < G; ++k) g.c[k] += q.above(g.x[k]);
 }
 
-template <int DT, int G, bool STATS>
-__device__ __forceinline__ void stream_row(const typename Elem<DT>::T* xr, int c0, int c1, Stat& s, Given<G>& g, TopList& top,
-                                           bool want_top) {
+// One single column for each lane of a warp.
+template <int G, bool STATS, bool TOP>
+__device__ __forceinline__ void take_one(float x, bool on, uint32_t v, int lane, Stat& s, Given<G>& g, TopList& top) {
+  if (STATS) {
+    if (TOP) top.offer(on ? full_key(order_key(x), v) : 0, lane);
+    if (x > s.M) raise_to(s, x);
+    add_term(s, x, ref_of(s.M));
+  }
+#pragma unroll
+  for (int k = 0; k < G; ++k) g.c[k] += x > g.x[k];
+}
+
+template <int DT, int G, int NT, bool STATS, bool TOP>
+__device__ __forceinline__ void stream_row(const typename Elem<DT>::T* xr, int c0, int c1, Stat& s, Given<G>& g, TopList& top) {
   using T = typename Elem<DT>::T;
-  constexpr int VEC = 16 / sizeof(T), U = 4;
+  constexpr int VEC = 16 / sizeof(T), U = kLongUnroll;
   const int lane = threadIdx.x & 31;
   // columns up to the first 16-byte boundary and behind the last: one each for the lanes of warp 0
   const int mis = (int)((reinterpret_cast<uintptr_t>(xr + c0) & 15) / sizeof(T));
@@ -314,41 +416,49 @@ __device__ __forceinline__ void stream_row(const typename Elem<DT>::T* xr, int c
   if (threadIdx.x < 32) {
     const int v = lane < head ? c0 + lane : t0 + lane - head;
     const bool on = v < c1;
-    float x[1] = {on ? Elem<DT>::f(xr[v]) : kNegInf};
-    take<G, 1, STATS>(x, on, v, lane, s, g, top, want_top);
+    take_one<G, STATS, TOP>(on ? Elem<DT>::f(xr[v]) : kNegInf, on, v, lane, s, g, top);
   }
+  // U vectors of a thread are under way while the U before them are worked on
   const uint4* xv = reinterpret_cast<const uint4*>(xr + b0);
-  for (int i0 = 0; i0 < nvec; i0 += U * kLongThreads) {
-    uint4 raw[U];
+  Vec<DT> q[2][U];
+  auto fetch = [&](int i0, Vec<DT>(&r)[U]) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * kLongThreads + (int)threadIdx.x;
-      if (i < nvec) raw[u] = __ldg(xv + i);
+      const int i = i0 + u * NT + (int)threadIdx.x;
+      r[u].raw = i < nvec ? __ldg(xv + i) : Vec<DT>::lowest();
     }
+  };
+  auto work = [&](int i0, const Vec<DT>(&r)[U]) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * kLongThreads + (int)threadIdx.x;
-      if (i0 + u * kLongThreads + (int)(threadIdx.x & ~31u) >= nvec) break;  // the whole warp is behind the end
-      float x[VEC];
-      const T* e = reinterpret_cast<const T*>(&raw[u]);
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) x[k] = i < nvec ? Elem<DT>::f(e[k]) : kNegInf;
-      take<G, VEC, STATS>(x, i < nvec ? VEC : 0, b0 + i * VEC, lane, s, g, top, want_top);
+      const int i = i0 + u * NT + (int)threadIdx.x;
+      if (i0 + u * NT + (int)(threadIdx.x & ~31u) >= nvec) break;  // the whole warp is behind the end
+      take<DT, G, STATS, TOP>(r[u], i < nvec, b0 + i * VEC, lane, s, g, top);
     }
+  };
+  constexpr int STEP = U * NT;
+  fetch(0, q[0]);
+  for (int i0 = 0; i0 < nvec; i0 += 2 * STEP) {
+    fetch(i0 + STEP, q[1]);
+    work(i0, q[0]);
+    fetch(i0 + 2 * STEP, q[0]);
+    work(i0 + STEP, q[1]);
   }
 }
 
+template <int NT>
 struct LongSmem {
-  uint64_t buf[kLongWarps][64];
+  uint64_t buf[NT / 32][64];
   uint64_t list[32];
-  Stat warp[kLongWarps], cta;
+  Stat warp[NT / 32], cta;
   int cnt[kMaxGiven];
 };
 
-template <int DT, int G, int CL>
-__global__ void __launch_bounds__(kLongThreads) logprobs_long_kernel(const LpArgs a) {
+template <int DT, int G, int CL, bool TOP>
+__global__ void __launch_bounds__(long_threads(CL)) logprobs_long_kernel(const LpArgs a) {
   using T = typename Elem<DT>::T;
-  __shared__ LongSmem sm;
+  constexpr int NT = long_threads(CL), NW = NT / 32;
+  __shared__ LongSmem<NT> sm;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t row = blockIdx.x / CL;
   const int part = blockIdx.x % CL;
@@ -368,8 +478,8 @@ __global__ void __launch_bounds__(kLongThreads) logprobs_long_kernel(const LpArg
       g.x[k] = t >= 0 && t < V ? Elem<DT>::f(xr[t]) : -kNegInf;
       g.c[k] = 0;
     }
-    if (j0 == 0) stream_row<DT, G, true>(xr, c0, c1, s, g, top, a.top > 0);
-    else stream_row<DT, G, false>(xr, c0, c1, s, g, top, false);
+    if (j0 == 0) stream_row<DT, G, NT, true, TOP>(xr, c0, c1, s, g, top);
+    else stream_row<DT, G, NT, false, false>(xr, c0, c1, s, g, top);
 #pragma unroll
     for (int k = 0; k < G; ++k) {
       const int c = __reduce_add_sync(kFull, g.c[k]);
@@ -378,29 +488,36 @@ __global__ void __launch_bounds__(kLongThreads) logprobs_long_kernel(const LpArg
   }
   s = warp_join(s);
   if (lane == 0) sm.warp[w] = s;
-  if (a.top) {
+  if (TOP) {
     while (top.held > 0) top.flush(lane);
     sm.buf[w][lane] = top.list;
   }
   __syncthreads();
-  for (int o = kLongWarps / 2; a.top && o; o >>= 1) {
+  for (int o = NW / 2; TOP && o; o >>= 1) {
     if (w < o) sm.buf[w][lane] = merge_lists(sm.buf[w][lane], sm.buf[w + o][lane], lane);
     __syncthreads();
   }
   if (w == 0) {
-    s = lane < kLongWarps ? sm.warp[lane] : Stat{kNegInf, 0.f, 0.f};
+    s = lane < NW ? sm.warp[lane] : Stat{kNegInf, 0.f, 0.f};
     s = warp_join(s);
     if (lane == 0) sm.cta = s;
-    sm.list[lane] = a.top ? sm.buf[0][lane] : 0;
+    sm.list[lane] = TOP ? sm.buf[0][lane] : 0;
   }
   cg::cluster_group cl = cg::this_cluster();
   if (CL > 1) cl.sync();
+  if (CL > 1 && TOP && part == 0) {  // the parts' lists, merged by a tree of warps
+    if (w < CL) sm.buf[w][lane] = cl.map_shared_rank(&sm, w < CL ? w : 0)->list[lane];
+    __syncthreads();
+    for (int o = CL / 2; o; o >>= 1) {
+      if (w < o) sm.buf[w][lane] = merge_lists(sm.buf[w][lane], sm.buf[w + o][lane], lane);
+      __syncthreads();
+    }
+  }
   if (part == 0 && w == 0) {
-    uint64_t list = sm.list[lane];
+    const uint64_t list = CL > 1 ? sm.buf[0][lane] : sm.list[lane];
     if (CL > 1) {
       s = lane < CL ? cl.map_shared_rank(&sm, lane < CL ? lane : 0)->cta : Stat{kNegInf, 0.f, 0.f};
       s = warp_join(s);
-      for (int r = 1; a.top && r < CL; ++r) list = merge_lists(list, cl.map_shared_rank(&sm, r)->list[lane], lane);
     }
     float lz, lse, ent;
     finish(s, &lz, &lse, &ent);
@@ -419,7 +536,7 @@ __global__ void __launch_bounds__(kLongThreads) logprobs_long_kernel(const LpArg
       a.logprob[row * a.J + j] = on ? logprob_of(Elem<DT>::f(xr[t]), s, lz, lse) : 0.f;
       a.rank[row * a.J + j] = on ? c : 0;
     }
-    if (lane < a.top) {
+    if (TOP && lane < a.top) {
       a.top_id[row * a.top + lane] = (int64_t)(uint32_t)~(uint32_t)list;
       a.top_logprob[row * a.top + lane] = logprob_of(key_value((uint32_t)(list >> 32)), s, lz, lse);
     }
@@ -568,14 +685,31 @@ __global__ void __launch_bounds__(kGradThreads) logprobs_grad_long_kernel(const 
     const int nvec = (c1 - c0 - head) / VEC, b0 = c0 + head, t0 = b0 + nvec * VEC;
     for (int v = c0 + threadIdx.x; v < b0; v += kGradThreads) put<DT>(dr + v, grad_of(r, Elem<DT>::f(xr[v])));
     for (int v = t0 + threadIdx.x; v < c1; v += kGradThreads) put<DT>(dr + v, grad_of(r, Elem<DT>::f(xr[v])));
-#pragma unroll 4
-    for (int i = threadIdx.x; i < nvec; i += kGradThreads) {
-      uint4 raw = __ldg(reinterpret_cast<const uint4*>(xr + b0) + i), out;
-      const T* e = reinterpret_cast<const T*>(&raw);
-      T* o = reinterpret_cast<T*>(&out);
+    const f32x2 nm = pair(-r.m, -r.m), nlz = pair(-r.lz, -r.lz), l2 = pair(kLog2e, kLog2e), ga = pair(r.a, r.a), gb = pair(-r.b, -r.b);
+    constexpr int U = 4;
+    for (int i0 = threadIdx.x; i0 < nvec; i0 += U * kGradThreads) {
+      uint4 raw[U];
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) put<DT>(o + k, grad_of(r, Elem<DT>::f(e[k])));
-      reinterpret_cast<uint4*>(dr + b0)[i] = out;
+      for (int u = 0; u < U; ++u)
+        if (i0 + u * kGradThreads < nvec) raw[u] = __ldcs(reinterpret_cast<const uint4*>(xr + b0) + i0 + u * kGradThreads);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (i0 + u * kGradThreads >= nvec) break;
+        const T* e = reinterpret_cast<const T*>(&raw[u]);
+        uint4 out;
+        T* o = reinterpret_cast<T*>(&out);
+#pragma unroll
+        for (int k = 0; k < VEC; k += 2) {
+          float y0, y1, p0, p1;
+          const f32x2 y = add2(add2(pair(Elem<DT>::f(e[k]), Elem<DT>::f(e[k + 1])), nm), nlz);
+          unpair(mul2(y, l2), p0, p1);
+          unpair(y, y0, y1);
+          unpair(mul2(pair(ex2(p0), ex2(p1)), fma2(gb, pair(fmaxf(y0, -1000.f), fmaxf(y1, -1000.f)), ga)), p0, p1);
+          put<DT>(o + k, r.none ? 0.f : p0);
+          put<DT>(o + k + 1, r.none ? 0.f : p1);
+        }
+        __stcs(reinterpret_cast<uint4*>(dr + b0) + i0 + u * kGradThreads, out);
+      }
     }
     __syncthreads();
     if (threadIdx.x < J) {
@@ -590,6 +724,12 @@ __global__ void __launch_bounds__(kGradThreads) logprobs_grad_long_kernel(const 
       if (first) put<DT>(dr + t, grad_of(r, Elem<DT>::f(xr[t])) + g);
     }
   }
+}
+
+template <int DT, int CL, bool TOP>
+void launch_long(const cudaLaunchConfig_t& cfg, const LpArgs& a) {
+  if (a.J <= 1) cudaLaunchKernelEx(&cfg, logprobs_long_kernel<DT, 1, CL, TOP>, a);
+  else cudaLaunchKernelEx(&cfg, logprobs_long_kernel<DT, 8, CL, TOP>, a);
 }
 
 template <int DT>
@@ -607,17 +747,12 @@ int launch_fwd(const LpArgs& a, cudaStream_t st) {
     at[0].val.clusterDim.x = 8;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.gridDim = dim3((unsigned)(split ? a.N * 8 : a.N));
-    cfg.blockDim = dim3(kLongThreads);
+    cfg.blockDim = dim3(long_threads(split ? 8 : 1));
     cfg.stream = st;
     cfg.attrs = at;
     cfg.numAttrs = split ? 1 : 0;
-    if (split) {
-      if (a.J <= 1) cudaLaunchKernelEx(&cfg, logprobs_long_kernel<DT, 1, 8>, a);
-      else cudaLaunchKernelEx(&cfg, logprobs_long_kernel<DT, 8, 8>, a);
-    } else {
-      if (a.J <= 1) cudaLaunchKernelEx(&cfg, logprobs_long_kernel<DT, 1, 1>, a);
-      else cudaLaunchKernelEx(&cfg, logprobs_long_kernel<DT, 8, 1>, a);
-    }
+    if (split) a.top ? launch_long<DT, 8, true>(cfg, a) : launch_long<DT, 8, false>(cfg, a);
+    else a.top ? launch_long<DT, 1, true>(cfg, a) : launch_long<DT, 1, false>(cfg, a);
   }
   return check_launch("token_logprobs");
 }

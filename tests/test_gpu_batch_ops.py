@@ -544,7 +544,14 @@ def test_token_logprobs_strides_and_autograd(V):
     plain = base[:, 3:V + 3].contiguous()
     want = KN.token_logprobs(plain, tokens, top=4)
     for x in (base[:, 3:V + 3], plain.t().contiguous().t()):
-        assert all(torch.equal(a, b) for a, b in zip(KN.token_logprobs(x, tokens, top=4), want))
+        # 16-byte loads start at a boundary of memory: another start adds the same terms in another order, and
+        # each order is within the bound of the 64-bit value
+        got = KN.token_logprobs(x, tokens, top=4)
+        lp, rank, ent, lse, ids, tl, te, ts = _scores(plain, tokens, 4)
+        _close(got.logprob, lp, tl)
+        _close(got.entropy, ent, te)
+        _close(got.lse, lse, ts)
+        assert torch.equal(got.rank, want.rank) and torch.equal(got.top_id, ids) and torch.equal(want.top_id, ids)
     e = plain[:1].expand(6, V)
     assert torch.equal(KN.token_logprobs(e, tokens).lse, want.lse[:1].expand(6))
     x = plain.clone().requires_grad_()
