@@ -6,6 +6,10 @@ pre-GELU FFN activation [B, L, d_ff], handed to the sink flattened to [B*L, d_ff
 the live activation, consumed by the sink's kernels on the current stream before the forward
 moves on.
 
+Attention: PyTorch's (sdpa), or with `attn="rows"` this library's kernels over the valid rows of the
+batch (kernels.attention): they plan nothing per batch shape, read no padding, and are differentiable,
+for gradients of an answer by the units. `lm_head` and `readout` give the model's answers at chosen rows.
+
 Weights: this build has no network, so `load` builds the architecture from its published
 configuration with a seeded random init (the reference's `control="random"`), unless a local
 HuggingFace checkpoint directory is given.
@@ -15,6 +19,8 @@ from __future__ import annotations
 import os
 
 import torch
+
+from . import kernels as KN
 
 # name -> (layers, d_model, d_ff, heads)
 ARCH = {
@@ -53,8 +59,11 @@ def esm_config(name: str):
                      attention_probs_dropout_prob=0.0)
 
 
-def load(name: str, control: str = "none", dtype=torch.bfloat16, device="cpu", seed: int = 0):
-    """Returns (model, tokenizer-like vocab, info) as the reference's load() (esm.py:21-49)."""
+def load(name: str, control: str = "none", dtype=torch.bfloat16, device="cpu", seed: int = 0, attn: str = "sdpa"):
+    """Returns (model, tokenizer-like vocab, info) as the reference's load() (esm.py:21-49). attn: "sdpa",
+    or "rows" for attention by this library's kernels (attach_attention)."""
+    if attn not in ("sdpa", "rows"):
+        raise ValueError(f"unknown attention {attn!r} (sdpa, rows)")
     from transformers import EsmModel
     local = name if os.path.isdir(str(name)) else None
     if local:
@@ -79,6 +88,8 @@ def load(name: str, control: str = "none", dtype=torch.bfloat16, device="cpu", s
     elif control not in ("none", "random"):
         raise ValueError(control)
     model = model.to(device=device, dtype=dtype).eval()
+    if attn == "rows":
+        attach_attention(model)
     info = {"hf": arch, "control": control if local else "random",
             "attn": getattr(model.config, "_attn_implementation", "eager"),
             "n_layers": model.config.num_hidden_layers, "d_model": model.config.hidden_size,
@@ -98,6 +109,79 @@ def attach(model, sink):
             sink(i, out.reshape(-1, out.shape[-1]))
         handles.append(mod.register_forward_hook(hook))
     return handles
+
+
+class _RowsPlan:
+    """The plan of the forward that is under way, shared by a model's attention modules."""
+    plan = None
+
+
+def _rows_attention(module, query, key, value, attention_mask, scaling=None, dropout=0.0, **kw):
+    """transformers' attention interface over kernels.attention: [B, H, L, D] in, [B, L, H, D] out."""
+    if dropout or kw.get("is_causal"):
+        raise ValueError("attention over the valid rows has neither dropout nor a causal mask")
+    out, _ = KN.attention(query, key, value, module.atlas_plan.plan, scaling)
+    return out.transpose(1, 2), None
+
+
+def batch_plan(attention_mask: torch.Tensor) -> "KN.SeqPlan":
+    """The plan of a padded batch from its [B, L] mask, whose rows must be ones followed by zeros."""
+    B, L = attention_mask.shape
+    return KN.seq_maps(attention_mask.sum(1, dtype=torch.int64), B * L, stride=L).plan(L)
+
+
+def attach_attention(model, check: bool = True):
+    """Let every attention layer of `model` run kernels.attention over the valid rows of its batch; returns
+    the hook handle (model.set_attn_implementation puts another attention back). The batch's attention_mask
+    has to be ones followed by zeros, as Batch's are; `check` looks at it, which waits for the device once a
+    forward, so a loop that builds its masks so itself turns it off. Rows of padding come out of attention
+    as zeros."""
+    from transformers import AttentionInterface, AttentionMaskInterface
+    AttentionInterface.register("atlas_rows", _rows_attention)
+    AttentionMaskInterface.register("atlas_rows", lambda *a, **k: None)  # the plan says which rows are valid
+    holder = _RowsPlan()
+    for layer in model.encoder.layer:
+        layer.attention.self.atlas_plan = holder
+
+    def hook(_module, args, kwargs):
+        x = args[0] if args else kwargs.get("input_ids")
+        if x is None:
+            x = kwargs["inputs_embeds"]
+        mask = args[1] if len(args) > 1 else kwargs.get("attention_mask")
+        if mask is None:
+            mask = torch.ones(x.shape[:2], dtype=torch.int64, device=x.device)
+        if check and bool((mask[:, 1:] > mask[:, :-1]).any()):
+            raise ValueError("attention over the valid rows: attention_mask must be ones followed by zeros in every row")
+        holder.plan = batch_plan(mask)
+
+    model.set_attn_implementation("atlas_rows")
+    return model.register_forward_pre_hook(hook, with_kwargs=True)
+
+
+def lm_head(model, name: str | None = None, seed: int = 0):
+    """The language-model head of an EsmModel (hidden states -> logits over its alphabet), in its dtype and on
+    its device: of a local HuggingFace checkpoint directory `name`, else of the architecture with a seeded
+    random init; its projection is the model's own embedding matrix."""
+    import copy
+    from transformers import EsmForMaskedLM
+    w = model.get_input_embeddings().weight
+    if name is not None and os.path.isdir(str(name)):
+        head = EsmForMaskedLM.from_pretrained(name).lm_head
+    else:
+        cfg = copy.deepcopy(model.config)
+        cfg.num_hidden_layers = 1
+        cfg._attn_implementation = "eager"
+        torch.manual_seed(seed)
+        with torch.device(w.device):
+            head = EsmForMaskedLM(cfg).lm_head
+        head.decoder.weight = w
+    return head.to(device=w.device, dtype=w.dtype).eval()
+
+
+def readout(hidden: torch.Tensor, head, rows: torch.Tensor, tokens: torch.Tensor, top: int = 0) -> "KN.TokenLogprobs":
+    """What the model answers at `rows` (int64, of the flattened [B*L] positions) of its last hidden states
+    [B, L, d]: kernels.token_logprobs of the head's logits there, for `tokens` ([N] or [N, J] ids)."""
+    return KN.token_logprobs(head(hidden.reshape(-1, hidden.shape[-1]).index_select(0, rows)), tokens, top=top)
 
 
 def flops_per_batch(info: dict, n_rows: int, Lmax: int) -> float:

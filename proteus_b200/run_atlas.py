@@ -6,7 +6,7 @@
 Outputs in --out (as the reference, run_atlas.py:3-8): ckpt/ckpt_<batch>.pt (atomic, last 2 kept),
 batches.jsonl (one record per batch; its GPU times come from CUDA events read a few batches later,
 so the loop never drains the GPU to time a batch), run.json (summary), atlas.pt (final result +
-sha256 digests of the exact fields). With several ranks each rank checkpoints its own shard under ckpt/rank<r>/ and
+sha256 digests of the exact fields); with --readout N readout/<batch>.pt. With several ranks each rank checkpoints its own shard under ckpt/rank<r>/ and
 the shard states are combined exactly (proteus_b200.dist.merge_states) before rank 0 writes atlas.pt.
 
 --data accepts the reference's Swiss-Prot .pt format or `synthetic:<n_seq>[:<seed>]` (C4-like
@@ -29,7 +29,8 @@ import torch
 
 from .core import Atlas, AtlasConfig
 from .data import SwissProt, shuffled_order, synthetic_dataset
-from .esm import attach, flops_per_batch, load
+from .esm import attach, attach_attention, flops_per_batch, lm_head, load, readout
+from .kernels import seq_maps
 from .pilot import pilot_pass
 
 
@@ -112,6 +113,36 @@ class CheckpointWriter:
             raise e
 
 
+class ReadoutWriter:
+    """What the model answered, one file per batch of the plan. `put` starts the copies to pinned host memory;
+    `drain(keep)` writes the batches whose copies are done, all but the newest `keep` at the latest, so that
+    the loop does not wait for the device. Written again, a batch's file has the same contents (a resumed run
+    repeats the batches after its checkpoint)."""
+
+    def __init__(self, d: Path):
+        self.d = d
+        d.mkdir(parents=True, exist_ok=True)
+        self._pending = []
+
+    def put(self, batch: int, tok: torch.Tensor, r):
+        small = {"tok": tok, "logprob": r.logprob, "rank": r.rank, "entropy": r.entropy, "top_id": r.top_id.to(torch.int16),
+                 "top_logprob": r.top_logprob}
+        host = {k: torch.empty(v.shape, dtype=v.dtype, pin_memory=True).copy_(v, non_blocking=True) for k, v in small.items()}
+        done = torch.cuda.Event()
+        done.record()
+        self._pending.append((batch, host, done))
+
+    def drain(self, keep: int):
+        while self._pending:
+            batch, host, done = self._pending[0]
+            if len(self._pending) > keep:
+                done.synchronize()
+            elif not done.query():
+                return
+            self._pending.pop(0)
+            atomic_save(host, self.d / f"{batch}.pt")
+
+
 def load_latest_ckpt(d: Path):
     """(path, checkpoint dict) of the newest readable checkpoint in d, or (None, None). A newest file
     that cannot be read (truncated by a kill during a copy, or damaged) is reported and skipped in
@@ -172,6 +203,11 @@ def parser():
     ap.add_argument("--deadline", type=float, default=0.0)
     ap.add_argument("--host-ctx", action="store_true",
                     help="build batch contexts with the host make_ctx (as the reference) instead of on the device")
+    ap.add_argument("--attn", default="sdpa", choices=["sdpa", "rows"],
+                    help="the forward's attention: PyTorch's, or this library's kernels over the valid rows")
+    ap.add_argument("--readout", type=int, default=-1, metavar="N",
+                    help="also write what the model answers at every residue (log probability and rank of the "
+                         "residue, entropy, the N most likely tokens) to readout/<batch>.pt")
     return ap
 
 
@@ -182,6 +218,8 @@ def _args_key(a) -> dict:
     key = {k: getattr(a, k) for k in keep}
     if getattr(a, "control_seed", None) is not None:
         key["control_seed"] = a.control_seed
+    if getattr(a, "attn", "sdpa") != "sdpa":  # rounds differently: not to be resumed with the other
+        key["attn"] = a.attn
     return key
 
 
@@ -320,6 +358,10 @@ def main(argv=None):
         order = order[: a.max_seqs]
     ctl_seed = a.seed if a.control_seed is None else a.control_seed
     model, tok, info = load(a.model, a.control, dtype=dtype, device=dev, seed=ctl_seed)
+    if a.attn == "rows":
+        attach_attention(model, check=False)  # make_batch's masks are ones followed by zeros
+        info["attn"] = "atlas_rows"
+    head = lm_head(model, a.model, seed=ctl_seed) if a.readout >= 0 else None
     info["control_seed"] = ctl_seed
     vocab = tok.get_vocab()
     L, D = info["n_layers"], info["d_ff"]
@@ -376,6 +418,7 @@ def main(argv=None):
     ckpt_s, batch_s, last_ckpt_s = 0.0, 0.0, None
 
     writer = CheckpointWriter(ck_dir, keep=2)
+    answers = ReadoutWriter(out / "readout") if head is not None else None
 
     def save_ckpt(next_batch):
         """Snapshot now, write in the background; the time on the batch loop's path is the host copy
@@ -480,13 +523,15 @@ def main(argv=None):
                     ctx = atlas.make_ctx_device(b.n_rows, b.valid_rows, b.tok, b.ann)
                 n_before = atlas.n_seen
                 atlas.begin_batch(ctx)
-                model(input_ids=ids, attention_mask=am)
+                states = model(input_ids=ids, attention_mask=am).last_hidden_state
                 redo = atlas.end_batch()
                 assert redo == []
                 gram_flushed = bi % a.gram_flush_every == a.gram_flush_every - 1
                 if gram_flushed:
                     atlas.flush_gram()
                 eb = ev()
+                if head is not None:
+                    answers.put(bi * world + rank, ctx.tok, readout(states, head, ctx.valid_rows, ids.view(-1)[ctx.valid_rows], a.readout))
                 if prof is not None:
                     sync(dev)
                     prof.__exit__(None, None, None)
@@ -507,6 +552,8 @@ def main(argv=None):
                 rec["ckpt_s"] = last_ckpt_s
                 pending.append([rec, e0, ea, eb, fe])
                 drain(lag)
+                if head is not None:
+                    answers.drain(lag)
                 item = next(src_iter, None)
                 if a.deadline and item is not None and \
                         time.time() > a.deadline - 2 * (batch_s + max(ckpt_s, 30.0)):
@@ -541,7 +588,12 @@ def main(argv=None):
         b.attention_mask = b.attention_mask.pin_memory()
         if a.host_ctx:
             return b, atlas.make_ctx(b.n_rows, b.valid_rows, b.tok, b.ann, device="cpu")
-        return b, atlas.make_ctx_device(b.n_rows, b.valid_rows.pin_memory(), b.tok.pin_memory(),
+        # the valid rows and token ids from the lengths, on the device (they are 16 bytes a residue to copy)
+        n_v, Lmax = b.valid_rows.numel(), b.input_ids.shape[1]
+        with torch.cuda.device(dev), torch.cuda.stream(side):
+            lengths, seq = (t.pin_memory().to(dev, non_blocking=True) for t in (b.attention_mask.sum(1), b.seq_idx))
+            maps = seq_maps(lengths, b.n_rows, stride=Lmax, lead=1, trail=1, seq=seq)
+        return b, atlas.make_ctx_device(b.n_rows, maps.slots[:n_v], maps.tok[:n_v],
                                         b.ann.pin_memory() if b.ann is not None else None, stream=side)
 
     with torch.no_grad():
@@ -556,6 +608,8 @@ def main(argv=None):
         finally:
             if prefetch is not None:
                 prefetch.close()
+            if answers is not None:
+                answers.drain(0)
     if code is not None:
         finish_process_group()
         return
