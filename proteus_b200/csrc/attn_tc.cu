@@ -107,18 +107,73 @@ __device__ __forceinline__ void zero_tile_rows(uint8_t* tile, int from, int to, 
 __device__ __forceinline__ int up16(int n) { return (n + 15) & ~15; }
 
 // ---------------------------------------------------------------------------------------- forward
-// Warps 0-3: softmax, one thread per query; warp 4: TMA; warp 5: products and TMEM.
-// TMEM: two buffers of 128 columns. S(i) fills buffer i & 1, P(i) overwrites its columns 0-63 as 16-bit,
-// P(i) v lands in its columns 64-127. The softmax warps fold P(i-1) v into registers between the
-// maximum of S(i) and its exponentials: the product has had that long to finish, and S(i+1)
-// can be computed during the exponentials.
+// Warps 0-3: softmax, one thread per query; warp 4: TMA; warp 5: products and TMEM. Key tiles of 96 rows.
+// TMEM: two buffers of scores (columns 0-95, 96-191), P(i) over the first half of S(i), the output in
+// 192-255, where all products accumulate.
+//
+// The reference that exponents are taken from is the maximum of a row's FIRST tile, not a running one: any
+// reference gives the same quotient, and fp32 sums and bf16 probabilities have range for 2^64 above it. So a
+// tile costs one pass (no maximum, no rescaling): a packed multiply-add, an exponential, a packed sum and half a
+// conversion a score. The tile's sum tells when the reference was too low (2^64; fp16 P: 2^15), or when there is
+// none yet (all scores so far -inf); the warp then takes the tile's maximum, rescales the output in TMEM and
+// does the tile again, whose scores are still there, since P is held in registers until it is accepted.
 constexpr int kFwdThreads = 192;
+constexpr int KT = 96;
+constexpr uint32_t kKeyTile = KT * 128;
 
 struct FwdSmem {
-  uint8_t q[kTile], k[2][kTile], v[2][kTile];
-  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], s_free[2];
+  uint8_t q[kTile], k[2][kKeyTile], v[2][kKeyTile];
+  uint64_t q_full, k_full[2], k_empty[2], v_full[2], s_full[2], p_full[2], o_done[2];
   uint32_t tmem;
 };
+
+// Probabilities of a row's tile against `ref` (negated) into p, their sum returned; `cols` of 96 are before the end.
+template <int DT>
+__device__ __forceinline__ float fwd_tile(uint32_t buf, float c, float nref, int cols, uint32_t (&p)[KT / 2]) {
+  const f32x2 c2 = pair(c, c), r2 = pair(nref, nref);
+  uint32_t x[2][32];
+  f32x2 sum[2] = {0, 0};
+  tmem_ld32(buf, x[0]);
+#pragma unroll
+  for (int h = 0; h < 3; ++h) {
+    if (h * 32 >= cols) break;
+    tmem_ld_wait();
+    if (h < 2) tmem_ld32(buf + h * 32 + 32, x[(h + 1) & 1]);
+    uint32_t(&y)[32] = x[h & 1];
+    if (h * 32 + 32 > cols) {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (h * 32 + j >= cols) y[j] = 0xFF800000u;  // -inf
+    }
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+      float a, b;
+      unpair(fma2(pair(__uint_as_float(y[j]), __uint_as_float(y[j + 1])), c2, r2), a, b);
+      a = ex2(a);
+      b = ex2(b);
+      sum[(j >> 1) & 1] = add2(sum[(j >> 1) & 1], pair(a, b));
+      p[h * 16 + j / 2] = pack2<DT>(a, b);
+    }
+  }
+  tmem_ld_wait();
+  float a, b;
+  unpair(add2(sum[0], sum[1]), a, b);
+  return a + b;
+}
+
+__device__ __forceinline__ float fwd_max(uint32_t buf, int cols) {
+  float mx = kNegInf;
+#pragma unroll
+  for (int h = 0; h < 3; ++h) {
+    if (h * 32 >= cols) break;
+    uint32_t x[32];
+    tmem_ld32(buf + h * 32, x);
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 32; ++j) mx = fmaxf(mx, h * 32 + j < cols ? __uint_as_float(x[j]) : kNegInf);
+  }
+  return mx;
+}
 
 template <int DT>
 __global__ void __launch_bounds__(kFwdThreads, 2)
@@ -135,7 +190,7 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
     for (int64_t r = z0 + threadIdx.x; r < z1; r += kFwdThreads) l[r] = 0.f;
   }
   if (!b.on || b.first >= b.len) return;
-  const int kh = head / (a.H / a.Hk), n = (b.len + BM - 1) / BM;
+  const int kh = head / (a.H / a.Hk), n = (b.len + KT - 1) / KT;
   const int live = min(4, (b.len - b.first + 31) / 32);  // softmax warps that have a row
   if (threadIdx.x == 0) {
     mbar_init(&s.q_full, 1);
@@ -143,11 +198,9 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
       mbar_init(&s.k_full[i], 1);
       mbar_init(&s.k_empty[i], 1);
       mbar_init(&s.v_full[i], 1);
-      mbar_init(&s.v_empty[i], 1);
       mbar_init(&s.s_full[i], 1);
-      mbar_init(&s.o_full[i], 1);
-      mbar_init(&s.p_full[i], live * 32);
-      mbar_init(&s.s_free[i], live * 32);
+      mbar_init(&s.o_done[i], 1);
+      mbar_init(&s.p_full[i], live);
     }
     fence_barrier_init();
   }
@@ -158,7 +211,7 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
   const uint32_t tmem = s.tmem;
 
   if (warp == 4) {
-    if (lane == 0) {
+    if (elect_one()) {
       const int r0 = (int)b.row0, o = (int)b.outer;
       mbar_arrive_expect_tx(&s.q_full, kTile);
       tma_load_4d(s.q, &mq, 0, r0 + b.first, head, o, &s.q_full);
@@ -166,140 +219,121 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
         const int st = i & 1;
         const uint32_t ph = ((i >> 1) & 1) ^ 1;
         if (i >= 2 && !mbar_wait(&s.k_empty[st], ph, 201)) break;
-        mbar_arrive_expect_tx(&s.k_full[st], kTile);
-        tma_load_4d(s.k[st], &mk, 0, r0 + i * BM, kh, o, &s.k_full[st]);
-        if (i >= 2 && !mbar_wait(&s.v_empty[st], ph, 202)) break;
-        mbar_arrive_expect_tx(&s.v_full[st], kTile);
-        tma_load_4d(s.v[st], &mv, 0, r0 + i * BM, kh, o, &s.v_full[st]);
+        mbar_arrive_expect_tx(&s.k_full[st], kKeyTile);
+        tma_load_4d(s.k[st], &mk, 0, r0 + i * KT, kh, o, &s.k_full[st]);
+        if (i >= 2 && !mbar_wait(&s.o_done[st], ph, 202)) break;
+        mbar_arrive_expect_tx(&s.v_full[st], kKeyTile);
+        tma_load_4d(s.v[st], &mv, 0, r0 + i * KT, kh, o, &s.v_full[st]);
       }
     }
   } else if (warp == 5) {
     const uint32_t base = DT == ATLAS_BF16 ? idesc_bf16_f32(BM, 0) : idesc_f16_f32(BM, 0);
     const uint32_t id_pv = base | kMnB | (64u >> 3) << 17;
-    const uint64_t qd = sdesc_k_sw128(smem_u32(s.q)), kd = sdesc_k_sw128(smem_u32(s.k[0])), vd = sdesc_mn_sw128(smem_u32(s.v[0]));
+    const uint32_t qd = desc_lo(smem_u32(s.q)), kd = desc_lo(smem_u32(s.k[0])), vd = desc_lo(smem_u32(s.v[0]));
     // S(i) = q k(i)^T into buffer i & 1
     auto scores = [&](int i) {
       if (!mbar_spin(&s.k_full[i & 1], (i >> 1) & 1, 203)) return false;
       tc_fence_after();
+      const uint32_t id = base | (uint32_t)(up16(min(KT, b.len - i * KT)) >> 3) << 17;
+      const uint32_t k = kd + (i & 1) * (kKeyTile >> 4), at = tmem + (i & 1) * KT;
       if (elect_one()) {
-        const uint32_t id = base | (uint32_t)(up16(min(BM, b.len - i * BM)) >> 3) << 17;
-        const uint64_t k = kd + (i & 1) * (kTile >> 4);
-#pragma unroll
-        for (int kk = 0; kk < 4; ++kk) mma_f16(tmem + (i & 1) * 128, qd + kk * 2, k + kk * 2, id, kk > 0);
+        mma_f16_lo<false>(at, qd, k, id);
+        mma_f16_lo<true>(at, qd + 2, k + 2, id);
+        mma_f16_lo<true>(at, qd + 4, k + 4, id);
+        mma_f16_lo<true>(at, qd + 6, k + 6, id);
         mma_commit(&s.k_empty[i & 1]);
         mma_commit(&s.s_full[i & 1]);
       }
       __syncwarp();
       return true;
     };
-    bool ok = mbar_wait(&s.q_full, 0, 204) && scores(0) && (n < 2 || scores(1));
+    bool ok = mbar_spin(&s.q_full, 0, 204) && scores(0) && (n < 2 || scores(1));
     for (int i = 0; ok && i < n; ++i) {
-      const int bf = i & 1, cols = min(BM, b.len - i * BM);
+      const int bf = i & 1, cols = min(KT, b.len - i * KT);
       const uint32_t ph = (i >> 1) & 1;
       if (!mbar_spin(&s.v_full[bf], ph, 205)) break;
       if (cols & 15) zero_tile_rows(s.v[bf], cols, up16(cols), lane);
       if (!mbar_spin(&s.p_full[bf], ph, 206)) break;
       tc_fence_after();
+      const uint32_t v = vd + bf * (kKeyTile >> 4), at = tmem + bf * KT;
       if (elect_one()) {
-        const uint64_t v = vd + bf * (kTile >> 4);
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-          if (kk * 16 < cols) mma_f16_ts(tmem + bf * 128 + 64, tmem + bf * 128 + kk * 8, v + kk * 128, id_pv, kk > 0);
-        mma_commit(&s.v_empty[bf]);
-        mma_commit(&s.o_full[bf]);
+        for (int kk = 0; kk < KT / 16; ++kk)
+          if (kk * 16 < cols) mma_f16_ts_lo(tmem + 192, at + kk * 8, v + kk * 128, id_pv, i > 0 || kk > 0);
+        mma_commit(&s.o_done[bf]);
       }
       __syncwarp();
-      if (i + 2 < n) ok = mbar_spin(&s.s_free[bf], ph, 207) && scores(i + 2);
+      // S(i+2) overwrites P(i): the product that reads it must be done
+      if (i + 2 < n) ok = mbar_spin(&s.o_done[bf], ph, 207) && scores(i + 2);
     }
   } else if (warp < live) {
     const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
-    const float c = a.scale * kLog2e;
-    float o[64], m = kNegInf, l = 0.f, fold = 1.f;
-#pragma unroll
-    for (int d = 0; d < 64; ++d) o[d] = 0.f;
-    auto take_o = [&](int i) {  // o <- o fold + P(i) v
-      if (!mbar_wait_soon(&s.o_full[i & 1], (i >> 1) & 1, 208)) return false;
-      tc_fence_after();
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t r[32];
-        tmem_ld32(lanes + (i & 1) * 128 + 64 + h * 32, r);
-        tmem_ld_wait();
-#pragma unroll
-        for (int d = 0; d < 32; ++d) o[h * 32 + d] = fmaf(o[h * 32 + d], fold, __uint_as_float(r[d]));
-      }
-      tc_fence_before();
-      mbar_arrive(&s.s_free[i & 1]);
-      return true;
-    };
+    const float c = a.scale * kLog2e, limit = DT == ATLAS_BF16 ? 0x1p64f : 0x1p15f;
+    float ref = kNegInf, l = 0.f;  // ref: in base 2, -inf while there is none
     bool ok = true;
     for (int i = 0; i < n; ++i) {
-      const int cols = min(BM, b.len - i * BM);
-      const uint32_t buf = lanes + (i & 1) * 128;
-      ok = mbar_wait_soon(&s.s_full[i & 1], (i >> 1) & 1, 209);
+      const int bf = i & 1, cols = min(KT, b.len - i * KT);
+      const uint32_t buf = lanes + bf * KT;
+      ok = mbar_wait_soon(&s.s_full[bf], (i >> 1) & 1, 209);
       if (!ok) break;
       tc_fence_after();
-      float mx = kNegInf;
-#pragma unroll
-      for (int h = 0; h < 4; ++h)
-        if (h * 32 < cols) {
-          uint32_t r[32];
-          tmem_ld32(buf + h * 32, r);
-          tmem_ld_wait();
-          if (h * 32 + 32 <= cols) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) mx = fmaxf(mx, __uint_as_float(r[j]));
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) mx = fmaxf(mx, h * 32 + j < cols ? __uint_as_float(r[j]) : kNegInf);
-          }
-        }
-      mx = fmaxf(m, mx);
-      const float ref = mx == kNegInf ? 0.f : mx * c;
-      const float f = m == kNegInf ? 0.f : ex2(fmaf(m, c, -ref));
+      if (i == 0) ref = fwd_max(buf, cols) * c;
+      uint32_t p[KT / 2];
+      float sum = fwd_tile<DT>(buf, c, ref == kNegInf ? 0.f : -ref, cols, p);
       if (i > 0) {
-        ok = take_o(i - 1);
-        if (!ok) break;
-      }
-      fold = f;
-      m = mx;
-      float sum = 0.f;
+        const bool bad = ref == kNegInf || !(sum <= limit);
+        if (__any_sync(0xFFFFFFFFu, bad)) {
+          const float mx = fwd_max(buf, cols) * c;
+          const float to = bad ? fmaxf(ref, mx) : ref;
+          const float f = ref == to || ref == kNegInf ? 1.f : ex2(ref - to);
+          // the sums up to here are complete, and P(i) has not been handed over
+          ok = mbar_wait_soon(&s.o_done[bf ^ 1], ((i - 1) >> 1) & 1, 208);
+          if (!ok) break;
+          tc_fence_after();
 #pragma unroll
-      for (int h = 0; h < 4; ++h)
-        if (h * 32 < cols) {
-          uint32_t r[32], p[16];
-          tmem_ld32(buf + h * 32, r);
-          tmem_ld_wait();
-          if (h * 32 + 32 > cols) {
+          for (int h = 0; h < 4; ++h) {
+            uint32_t o[16];
+            tmem_ld16(lanes + 192 + h * 16, o);
+            tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (h * 32 + j >= cols) r[j] = 0xFF800000u;  // -inf
+            for (int d = 0; d < 16; ++d) o[d] = __float_as_uint(__uint_as_float(o[d]) * f);
+            tmem_st16(lanes + 192 + h * 16, o);
           }
-#pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            const float x = ex2(fmaf(__uint_as_float(r[j]), c, -ref)), y = ex2(fmaf(__uint_as_float(r[j + 1]), c, -ref));
-            sum += x + y;
-            p[j / 2] = pack2<DT>(x, y);
-          }
-          tmem_st16(buf + h * 16, p);
+          ref = to;
+          l *= f;
+          sum = fwd_tile<DT>(buf, c, ref == kNegInf ? 0.f : -ref, cols, p);
         }
-      l = fmaf(l, f, sum);
+      }
+      l += sum;
+#pragma unroll
+      for (int h = 0; h < 3; ++h)
+        if (h * 32 < cols) {
+          uint32_t w[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) w[j] = p[h * 16 + j];
+          tmem_st16(buf + h * 16, w);
+        }
       tmem_st_wait();
       tc_fence_before();
-      mbar_arrive(&s.p_full[i & 1]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.p_full[bf]);
     }
-    if (ok) ok = take_o(n - 1);
+    if (ok) ok = mbar_wait_soon(&s.o_done[(n - 1) & 1], ((n - 1) >> 1) & 1, 210);
+    tc_fence_after();
     const int row = b.first + warp * 32 + lane;
-    if (ok && row < b.len) {
-      a.lse[(b.outer * a.H + head) * a.rows + b.row0 + row] = ((m == kNegInf ? 0.f : m * c) + log2f(l)) * kLn2;
-      uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + b.outer * a.so.outer + head * a.so.head + (b.row0 + row) * a.so.row;
+    if (ok) {
       const float inv = 1.f / l;
+      uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + b.outer * a.so.outer + head * a.so.head + (b.row0 + row) * a.so.row;
+      if (row < b.len)
+        a.lse[(b.outer * a.H + head) * a.rows + b.row0 + row] = ((ref == kNegInf ? 0.f : ref) + log2f(l)) * kLn2;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        uint32_t w[16];
+        uint32_t o[32], w[16];
+        tmem_ld32(lanes + 192 + h * 32, o);
+        tmem_ld_wait();
 #pragma unroll
-        for (int d = 0; d < 16; ++d) w[d] = pack2<DT>(o[h * 32 + 2 * d] * inv, o[h * 32 + 2 * d + 1] * inv);
-        store32(dst + h * 32, w, a.D - h * 32, vec);
+        for (int d = 0; d < 16; ++d) w[d] = pack2<DT>(__uint_as_float(o[2 * d]) * inv, __uint_as_float(o[2 * d + 1]) * inv);
+        if (row < b.len) store32(dst + h * 32, w, a.D - h * 32, vec);
       }
     }
   }
@@ -710,8 +744,8 @@ template <int DT>
 int fwd(const AttnArgs& a, cudaStream_t st) {
   CUtensorMap mq, mk, mv;
   if (int rc = make_map(&mq, a.q, DT, a.sq, a.outer, a.H, a.rows, a.D, BM)) return rc;
-  if (int rc = make_map(&mk, a.k, DT, a.sk, a.outer, a.Hk, a.rows, a.D, BM)) return rc;
-  if (int rc = make_map(&mv, a.v, DT, a.sv, a.outer, a.Hk, a.rows, a.D, BM)) return rc;
+  if (int rc = make_map(&mk, a.k, DT, a.sk, a.outer, a.Hk, a.rows, a.D, KT)) return rc;
+  if (int rc = make_map(&mv, a.v, DT, a.sv, a.outer, a.Hk, a.rows, a.D, KT)) return rc;
   const int bytes = sizeof(FwdSmem) + 1024;
   static bool done[64] = {};
   if (int rc = attn_smem_once(attn_fwd_tc_kernel<DT>, bytes, done)) return rc;
