@@ -75,13 +75,6 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return r;
 }
 
-// Zero rows [from, to) of one head (16-bit elements).
-__device__ void zero_rows16(void* dst, const Strides& st, int64_t outer, int head, int64_t from, int64_t to, int D) {
-  uint16_t* p = reinterpret_cast<uint16_t*>(dst) + outer * st.outer + head * st.head;
-  for (int64_t r = from + (threadIdx.x >> 5); r < to; r += blockDim.x >> 5)
-    for (int d = threadIdx.x & 31; d < D; d += 32) p[r * st.row + d] = 0;
-}
-
 // Up to 32 packed 16-bit elements of a row, of which `n` (or more, or none) exist; `vec`: 16-byte stores
 // are aligned and n a multiple of 8.
 __device__ __forceinline__ void store32(uint16_t* dst, const uint32_t (&w)[16], int n, bool vec) {
@@ -107,9 +100,14 @@ __device__ __forceinline__ void zero_tile_rows(uint8_t* tile, int from, int to, 
 __device__ __forceinline__ int up16(int n) { return (n + 15) & ~15; }
 
 // ---------------------------------------------------------------------------------------- forward
-// Warps 0-3: softmax, one thread per query; warp 4: TMA; warp 5: products and TMEM. Key tiles of 96 rows.
-// TMEM: two buffers of scores (columns 0-95, 96-191), P(i) over the first half of S(i), the output in
-// 192-255, where all products accumulate.
+// Work items of 128 queries of a head, key tiles of 96 rows. Two CTAs per SM run items as a stream of tiles: a
+// CTA that has loaded its last item takes over one that was not launched yet (cluster launch control), so that
+// an item's look-up, first loads and first scores hide behind the item before.
+//   warps 0-3  softmax, one thread per query
+//   warp 4     TMA, items, and zeros in rows of no sequence
+//   warp 5     scores; TMEM: two buffers of scores (columns 0-95, 96-191), P(t) over the first half of S(t), the
+//              output in 192-255, where an item's products accumulate
+//   warp 6     products with v
 //
 // The reference that exponents are taken from is the maximum of a row's FIRST tile, not a running one: any
 // reference gives the same quotient, and fp32 sums and bf16 probabilities have range for 2^64 above it. So a
@@ -117,33 +115,53 @@ __device__ __forceinline__ int up16(int n) { return (n + 15) & ~15; }
 // conversion a score. The tile's sum tells when the reference was too low (2^64; fp16 P: 2^15), or when there is
 // none yet (all scores so far -inf); the warp then takes the tile's maximum, rescales the output in TMEM and
 // does the tile again, whose scores are still there, since P is held in registers until it is accepted.
-constexpr int kFwdThreads = 192;
+//
+// The last tile of a sequence of several ends at the sequence's end and starts inside the tile before: its
+// columns `lo` .. are new, the ones below count as -inf, and no row behind the end is read.
+constexpr int kFwdThreads = 224;
 constexpr int KT = 96;
+constexpr int kFwdStages = 3;
 constexpr uint32_t kKeyTile = KT * 128;
 
+struct FwdItem {
+  int first, len, head, n, row0, outer;  // n: key tiles; 0 ends the stream
+};
+
 struct FwdSmem {
-  uint8_t q[kTile], k[2][kKeyTile], v[2][kKeyTile];
-  uint64_t q_full, k_full[2], k_empty[2], v_full[2], s_full[2], p_full[2], o_done[2];
+  uint8_t q[2][kTile], k[kFwdStages][kKeyTile], v[kFwdStages][kKeyTile];
+  uint4 stage[4][32 * 4];  // each softmax warp: 32 columns of its 32 rows on their way out
+  FwdItem item[2];
+  uint4 answer;
+  uint64_t item_full[2], item_empty[2], q_full[2], k_full[kFwdStages], k_empty[kFwdStages], v_full[kFwdStages],
+      v_empty[kFwdStages], s_full[2], p_full[2], o_done[2], taken;
   uint32_t tmem;
 };
 
-// Probabilities of a row's tile against `ref` (negated) into p, their sum returned; `cols` of 96 are before the end.
+// Key tile i of n over `len` rows: its first row, and its columns lo .. hi - 1 that count.
+__device__ __forceinline__ int key_tile(int i, int n, int len, int& lo, int& hi) {
+  const int from = i == n - 1 && n > 1 ? len - KT : i * KT;
+  lo = i * KT - from;
+  hi = min(KT, len - from);
+  return from;
+}
+
+// Probabilities of a row's tile against `ref` (negated) into p, their sum returned.
 template <int DT>
-__device__ __forceinline__ float fwd_tile(uint32_t buf, float c, float nref, int cols, uint32_t (&p)[KT / 2]) {
+__device__ __forceinline__ float fwd_tile(uint32_t buf, float c, float nref, int lo, int hi, uint32_t (&p)[KT / 2]) {
   const f32x2 c2 = pair(c, c), r2 = pair(nref, nref);
   uint32_t x[2][32];
   f32x2 sum[2] = {0, 0};
   tmem_ld32(buf, x[0]);
 #pragma unroll
   for (int h = 0; h < 3; ++h) {
-    if (h * 32 >= cols) break;
     tmem_ld_wait();
     if (h < 2) tmem_ld32(buf + h * 32 + 32, x[(h + 1) & 1]);
+    if (h * 32 >= hi || h * 32 + 32 <= lo) continue;
     uint32_t(&y)[32] = x[h & 1];
-    if (h * 32 + 32 > cols) {
+    if (h * 32 + 32 > hi || h * 32 < lo) {
 #pragma unroll
       for (int j = 0; j < 32; ++j)
-        if (h * 32 + j >= cols) y[j] = 0xFF800000u;  // -inf
+        if (h * 32 + j >= hi || h * 32 + j < lo) y[j] = 0xFF800000u;  // -inf
     }
 #pragma unroll
     for (int j = 0; j < 32; j += 2) {
@@ -155,22 +173,22 @@ __device__ __forceinline__ float fwd_tile(uint32_t buf, float c, float nref, int
       p[h * 16 + j / 2] = pack2<DT>(a, b);
     }
   }
-  tmem_ld_wait();
   float a, b;
   unpair(add2(sum[0], sum[1]), a, b);
   return a + b;
 }
 
-__device__ __forceinline__ float fwd_max(uint32_t buf, int cols) {
+__device__ __forceinline__ float fwd_max(uint32_t buf, int lo, int hi) {
   float mx = kNegInf;
 #pragma unroll
   for (int h = 0; h < 3; ++h) {
-    if (h * 32 >= cols) break;
+    if (h * 32 >= hi || h * 32 + 32 <= lo) continue;
     uint32_t x[32];
     tmem_ld32(buf + h * 32, x);
     tmem_ld_wait();
 #pragma unroll
-    for (int j = 0; j < 32; ++j) mx = fmaxf(mx, h * 32 + j < cols ? __uint_as_float(x[j]) : kNegInf);
+    for (int j = 0; j < 32; ++j)
+      mx = fmaxf(mx, h * 32 + j < hi && h * 32 + j >= lo ? __uint_as_float(x[j]) : kNegInf);
   }
   return mx;
 }
@@ -179,29 +197,25 @@ template <int DT>
 __global__ void __launch_bounds__(kFwdThreads, 2)
 attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                    const __grid_constant__ CUtensorMap mv, const AttnArgs a, int vec) {
-  extern __shared__ uint8_t raw[];
-  FwdSmem& s = *reinterpret_cast<FwdSmem*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  const int head = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const SeqBlock b = seq_block(a, blockIdx.x);
-  int64_t z0, z1;
-  if (idle_rows(a, b, blockIdx.x, &z0, &z1)) {
-    zero_rows16(a.out, a.so, b.outer, head, z0, z1, a.D);
-    float* l = a.lse + (b.outer * a.H + head) * a.rows;
-    for (int64_t r = z0 + threadIdx.x; r < z1; r += kFwdThreads) l[r] = 0.f;
-  }
-  if (!b.on || b.first >= b.len) return;
-  const int kh = head / (a.H / a.Hk), n = (b.len + KT - 1) / KT;
-  const int live = min(4, (b.len - b.first + 31) / 32);  // softmax warps that have a row
+  extern __shared__ __align__(1024) uint8_t raw[];
+  FwdSmem& s = *reinterpret_cast<FwdSmem*>(raw);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    mbar_init(&s.q_full, 1);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.item_full[i], 1);
+      mbar_init(&s.item_empty[i], 4);
+      mbar_init(&s.q_full[i], 1);
+      mbar_init(&s.s_full[i], 1);
+      mbar_init(&s.p_full[i], 4);
+      mbar_init(&s.o_done[i], 1);
+    }
+    for (int i = 0; i < kFwdStages; ++i) {
       mbar_init(&s.k_full[i], 1);
       mbar_init(&s.k_empty[i], 1);
       mbar_init(&s.v_full[i], 1);
-      mbar_init(&s.s_full[i], 1);
-      mbar_init(&s.o_done[i], 1);
-      mbar_init(&s.p_full[i], live);
+      mbar_init(&s.v_empty[i], 1);
     }
+    mbar_init(&s.taken, 1);
     fence_barrier_init();
   }
   if (warp == 5) tmem_alloc(&s.tmem, 256);
@@ -211,130 +225,235 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
   const uint32_t tmem = s.tmem;
 
   if (warp == 4) {
-    if (elect_one()) {
-      const int r0 = (int)b.row0, o = (int)b.outer;
-      mbar_arrive_expect_tx(&s.q_full, kTile);
-      tma_load_4d(s.q, &mq, 0, r0 + b.first, head, o, &s.q_full);
-      for (int i = 0; i < n; ++i) {
-        const int st = i & 1;
-        const uint32_t ph = ((i >> 1) & 1) ^ 1;
-        if (i >= 2 && !mbar_wait(&s.k_empty[st], ph, 201)) break;
-        mbar_arrive_expect_tx(&s.k_full[st], kKeyTile);
-        tma_load_4d(s.k[st], &mk, 0, r0 + i * KT, kh, o, &s.k_full[st]);
-        if (i >= 2 && !mbar_wait(&s.o_done[st], ph, 202)) break;
-        mbar_arrive_expect_tx(&s.v_full[st], kKeyTile);
-        tma_load_4d(s.v[st], &mv, 0, r0 + i * KT, kh, o, &s.v_full[st]);
+    int x = blockIdx.x, head = blockIdx.y, k = 0, t = 0;
+    uint32_t asked = 0;
+    bool more = true, ok = true;
+    while (ok) {
+      if (more && elect_one()) {  // the next item is on its way while this one is loaded
+        mbar_arrive_expect_tx(&s.taken, 16);
+        take_cta_async(&s.answer, &s.taken);
       }
+      __syncwarp();
+      const SeqBlock b = more ? seq_block(a, x) : SeqBlock{};
+      int64_t z0, z1;
+      if (more && idle_rows(a, b, x, &z0, &z1)) {
+        uint16_t* o = reinterpret_cast<uint16_t*>(a.out) + b.outer * a.so.outer + head * a.so.head;
+        float* l = a.lse + (b.outer * a.H + head) * a.rows;
+        for (int64_t r = z0; r < z1; ++r)
+          for (int d = lane; d < a.D; d += 32) o[r * a.so.row + d] = 0;
+        for (int64_t r = z0 + lane; r < z1; r += 32) l[r] = 0.f;
+      }
+      if (!more || (b.on && b.first < b.len)) {
+        const int r = k & 1, n = more ? (b.len + KT - 1) / KT : 0;
+        ok = k < 2 || mbar_wait(&s.item_empty[r], ((k >> 1) & 1) ^ 1, 200);
+        if (!ok) break;
+        if (elect_one()) {
+          s.item[r] = FwdItem{b.first, b.len, head, n, (int)b.row0, (int)b.outer};
+          mbar_arrive(&s.item_full[r]);
+        }
+        __syncwarp();
+        if (!more) break;
+        const int r0 = (int)b.row0, o = (int)b.outer, kh = head / (a.H / a.Hk);
+        if (elect_one()) {
+          mbar_arrive_expect_tx(&s.q_full[r], kTile);
+          tma_load_4d(s.q[r], &mq, 0, r0 + b.first, head, o, &s.q_full[r]);
+        }
+        __syncwarp();
+        for (int i = 0; i < n; ++i, ++t) {
+          const int st = t % kFwdStages;
+          const uint32_t ph = ((t / kFwdStages) & 1) ^ 1;
+          int lo, hi;
+          const int row = r0 + key_tile(i, n, b.len, lo, hi);
+          ok = t < kFwdStages || (mbar_wait_soon(&s.k_empty[st], ph, 201) && mbar_wait_soon(&s.v_empty[st], ph, 202));
+          if (!ok) break;
+          if (elect_one()) {
+            mbar_arrive_expect_tx(&s.k_full[st], kKeyTile);
+            tma_load_4d(s.k[st], &mk, 0, row, kh, o, &s.k_full[st]);
+            mbar_arrive_expect_tx(&s.v_full[st], kKeyTile);
+            tma_load_4d(s.v[st], &mv, 0, row, kh, o, &s.v_full[st]);
+          }
+          __syncwarp();
+        }
+        if (!ok) break;
+        ++k;
+      }
+      ok = mbar_wait_soon(&s.taken, asked & 1, 199);
+      ++asked;
+      if (!ok) break;
+      more = taken_cta(&s.answer, x, head);
+      // the answer is read before the next one may overwrite it (generic reads, asynchronous write)
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
     }
   } else if (warp == 5) {
     const uint32_t base = DT == ATLAS_BF16 ? idesc_bf16_f32(BM, 0) : idesc_f16_f32(BM, 0);
-    const uint32_t id_pv = base | kMnB | (64u >> 3) << 17;
-    const uint32_t qd = desc_lo(smem_u32(s.q)), kd = desc_lo(smem_u32(s.k[0])), vd = desc_lo(smem_u32(s.v[0]));
-    // S(i) = q k(i)^T into buffer i & 1
-    auto scores = [&](int i) {
-      if (!mbar_spin(&s.k_full[i & 1], (i >> 1) & 1, 203)) return false;
-      tc_fence_after();
-      const uint32_t id = base | (uint32_t)(up16(min(KT, b.len - i * KT)) >> 3) << 17;
-      const uint32_t k = kd + (i & 1) * (kKeyTile >> 4), at = tmem + (i & 1) * KT;
-      if (elect_one()) {
-        mma_f16_lo<false>(at, qd, k, id);
-        mma_f16_lo<true>(at, qd + 2, k + 2, id);
-        mma_f16_lo<true>(at, qd + 4, k + 4, id);
-        mma_f16_lo<true>(at, qd + 6, k + 6, id);
-        mma_commit(&s.k_empty[i & 1]);
-        mma_commit(&s.s_full[i & 1]);
+    const uint32_t qd = desc_lo(smem_u32(s.q[0])), kd = desc_lo(smem_u32(s.k[0]));
+    bool ok = true;
+    for (int k = 0, t = 0; ok; ++k) {
+      const int r = k & 1;
+      if (!mbar_wait_soon(&s.item_full[r], (k >> 1) & 1, 211)) break;
+      const int n = s.item[r].n, len = s.item[r].len;
+      if (!n || !mbar_wait_soon(&s.q_full[r], (k >> 1) & 1, 204)) break;
+      for (int i = 0; i < n; ++i, ++t) {  // S(t) = q k^T into buffer t & 1
+        const int st = t % kFwdStages, bf = t & 1;
+        ok = mbar_wait_soon(&s.k_full[st], (t / kFwdStages) & 1, 203) &&
+             // it overwrites P(t-2): the product that reads it must be done
+             (t < 2 || mbar_wait_soon(&s.o_done[bf], ((t >> 1) & 1) ^ 1, 207));
+        if (!ok) break;
+        tc_fence_after();
+        int lo, hi;
+        key_tile(i, n, len, lo, hi);
+        const uint32_t id = base | (uint32_t)(up16(hi) >> 3) << 17;
+        const uint32_t q = qd + r * (kTile >> 4), kk = kd + st * (kKeyTile >> 4), at = tmem + bf * KT;
+        if (elect_one()) {
+          mma_f16_lo<false>(at, q, kk, id);
+          mma_f16_lo<true>(at, q + 2, kk + 2, id);
+          mma_f16_lo<true>(at, q + 4, kk + 4, id);
+          mma_f16_lo<true>(at, q + 6, kk + 6, id);
+          mma_commit(&s.k_empty[st]);
+          mma_commit(&s.s_full[bf]);
+        }
+        __syncwarp();
       }
-      __syncwarp();
-      return true;
-    };
-    bool ok = mbar_spin(&s.q_full, 0, 204) && scores(0) && (n < 2 || scores(1));
-    for (int i = 0; ok && i < n; ++i) {
-      const int bf = i & 1, cols = min(KT, b.len - i * KT);
-      const uint32_t ph = (i >> 1) & 1;
-      if (!mbar_spin(&s.v_full[bf], ph, 205)) break;
-      if (cols & 15) zero_tile_rows(s.v[bf], cols, up16(cols), lane);
-      if (!mbar_spin(&s.p_full[bf], ph, 206)) break;
-      tc_fence_after();
-      const uint32_t v = vd + bf * (kKeyTile >> 4), at = tmem + bf * KT;
-      if (elect_one()) {
-#pragma unroll
-        for (int kk = 0; kk < KT / 16; ++kk)
-          if (kk * 16 < cols) mma_f16_ts_lo(tmem + 192, at + kk * 8, v + kk * 128, id_pv, i > 0 || kk > 0);
-        mma_commit(&s.o_done[bf]);
-      }
-      __syncwarp();
-      // S(i+2) overwrites P(i): the product that reads it must be done
-      if (i + 2 < n) ok = mbar_spin(&s.o_done[bf], ph, 207) && scores(i + 2);
     }
-  } else if (warp < live) {
+  } else if (warp == 6) {
+    const uint32_t id = (DT == ATLAS_BF16 ? idesc_bf16_f32(BM, 64) : idesc_f16_f32(BM, 64)) | kMnB;
+    const uint32_t vd = desc_lo(smem_u32(s.v[0]));
+    bool ok = true;
+    for (int k = 0, t = 0; ok; ++k) {
+      if (!mbar_wait_soon(&s.item_full[k & 1], (k >> 1) & 1, 213)) break;
+      const int n = s.item[k & 1].n, len = s.item[k & 1].len;
+      if (!n) break;
+      for (int i = 0; i < n; ++i, ++t) {
+        const int st = t % kFwdStages, bf = t & 1;
+        int lo, hi;
+        key_tile(i, n, len, lo, hi);
+        ok = mbar_wait_soon(&s.v_full[st], (t / kFwdStages) & 1, 205);
+        if (!ok) break;
+        if (hi & 15) zero_tile_rows(s.v[st], hi, up16(hi), lane);  // a sequence of one short tile: rows behind its end
+        // P(t) of an item's first tile comes after its warps have read the last item's output
+        ok = mbar_wait_soon(&s.p_full[bf], (t >> 1) & 1, 206);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t v = vd + st * (kKeyTile >> 4), at = tmem + bf * KT;
+        if (elect_one()) {
+          uint32_t acc = i > 0;
+#pragma unroll
+          for (int kk = 0; kk < KT / 16; ++kk)
+            if (kk * 16 < hi && kk * 16 + 16 > lo) {
+              mma_f16_ts_lo(tmem + 192, at + kk * 8, v + kk * 128, id, acc);
+              acc = 1;
+            }
+          mma_commit(&s.o_done[bf]);
+          mma_commit(&s.v_empty[st]);
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp < 4) {
     const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
     const float c = a.scale * kLog2e, limit = DT == ATLAS_BF16 ? 0x1p64f : 0x1p15f;
-    float ref = kNegInf, l = 0.f;  // ref: in base 2, -inf while there is none
     bool ok = true;
-    for (int i = 0; i < n; ++i) {
-      const int bf = i & 1, cols = min(KT, b.len - i * KT);
-      const uint32_t buf = lanes + bf * KT;
-      ok = mbar_wait_soon(&s.s_full[bf], (i >> 1) & 1, 209);
+    for (int k = 0, t = 0; ok; ++k) {
+      const int r = k & 1;
+      ok = mbar_wait_soon(&s.item_full[r], (k >> 1) & 1, 212);
       if (!ok) break;
-      tc_fence_after();
-      if (i == 0) ref = fwd_max(buf, cols) * c;
-      uint32_t p[KT / 2];
-      float sum = fwd_tile<DT>(buf, c, ref == kNegInf ? 0.f : -ref, cols, p);
-      if (i > 0) {
-        const bool bad = ref == kNegInf || !(sum <= limit);
-        if (__any_sync(0xFFFFFFFFu, bad)) {
-          const float mx = fwd_max(buf, cols) * c;
-          const float to = bad ? fmaxf(ref, mx) : ref;
-          const float f = ref == to || ref == kNegInf ? 1.f : ex2(ref - to);
-          // the sums up to here are complete, and P(i) has not been handed over
-          ok = mbar_wait_soon(&s.o_done[bf ^ 1], ((i - 1) >> 1) & 1, 208);
-          if (!ok) break;
-          tc_fence_after();
+      const FwdItem it = s.item[r];
+      if (!it.n) break;
+      const bool live = it.first + warp * 32 < it.len;
+      float ref = kNegInf, l = 0.f;  // ref: in base 2, -inf while there is none
+      for (int i = 0; i < it.n; ++i, ++t) {
+        const int bf = t & 1;
+        const uint32_t buf = lanes + bf * KT;
+        int lo, hi;
+        key_tile(i, it.n, it.len, lo, hi);
+        ok = mbar_wait_soon(&s.s_full[bf], (t >> 1) & 1, 209);
+        if (!ok) break;
+        tc_fence_after();
+        if (live) {
+          if (i == 0) ref = fwd_max(buf, lo, hi) * c;
+          uint32_t p[KT / 2];
+          float sum = fwd_tile<DT>(buf, c, ref == kNegInf ? 0.f : -ref, lo, hi, p);
+          if (i > 0) {
+            const bool bad = ref == kNegInf || !(sum <= limit);
+            if (__any_sync(0xFFFFFFFFu, bad)) {
+              const float mx = fwd_max(buf, lo, hi) * c;
+              const float to = bad ? fmaxf(ref, mx) : ref;
+              const float f = ref == to || ref == kNegInf ? 1.f : ex2(ref - to);
+              // the products up to here are complete, and P(t) has not been handed over
+              ok = mbar_wait_soon(&s.o_done[bf ^ 1], ((t - 1) >> 1) & 1, 208);
+              if (!ok) break;
+              tc_fence_after();
 #pragma unroll
-          for (int h = 0; h < 4; ++h) {
-            uint32_t o[16];
-            tmem_ld16(lanes + 192 + h * 16, o);
-            tmem_ld_wait();
+              for (int h = 0; h < 4; ++h) {
+                uint32_t o[16];
+                tmem_ld16(lanes + 192 + h * 16, o);
+                tmem_ld_wait();
 #pragma unroll
-            for (int d = 0; d < 16; ++d) o[d] = __float_as_uint(__uint_as_float(o[d]) * f);
-            tmem_st16(lanes + 192 + h * 16, o);
+                for (int d = 0; d < 16; ++d) o[d] = __float_as_uint(__uint_as_float(o[d]) * f);
+                tmem_st16(lanes + 192 + h * 16, o);
+              }
+              ref = to;
+              l *= f;
+              sum = fwd_tile<DT>(buf, c, ref == kNegInf ? 0.f : -ref, lo, hi, p);
+            }
           }
-          ref = to;
-          l *= f;
-          sum = fwd_tile<DT>(buf, c, ref == kNegInf ? 0.f : -ref, cols, p);
+          l += sum;
+#pragma unroll
+          for (int h = 0; h < 3; ++h)
+            if (h * 32 < hi && h * 32 + 32 > lo) {
+              uint32_t w[16];
+#pragma unroll
+              for (int j = 0; j < 16; ++j) w[j] = p[h * 16 + j];
+              tmem_st16(buf + h * 16, w);
+            }
+          tmem_st_wait();
         }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.p_full[bf]);
       }
-      l += sum;
+      if (!ok) break;
+      if (live) {
+        ok = mbar_wait_soon(&s.o_done[(t - 1) & 1], ((t - 1) >> 1) & 1, 210);
+        if (!ok) break;
+        tc_fence_after();
+        const int row0 = it.first + warp * 32;  // the warp's first row
+        const float inv = 1.f / l;
+        const int64_t to = (int64_t)it.row0 + row0;
+        uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + it.outer * a.so.outer + it.head * a.so.head + to * a.so.row;
+        if (row0 + lane < it.len)
+          a.lse[((int64_t)it.outer * a.H + it.head) * a.rows + to + lane] = ((ref == kNegInf ? 0.f : ref) + log2f(l)) * kLn2;
 #pragma unroll
-      for (int h = 0; h < 3; ++h)
-        if (h * 32 < cols) {
-          uint32_t w[16];
+        for (int h = 0; h < 2; ++h) {
+          uint32_t o[32], w[16];
+          tmem_ld32(lanes + 192 + h * 32, o);
+          tmem_ld_wait();
 #pragma unroll
-          for (int j = 0; j < 16; ++j) w[j] = p[h * 16 + j];
-          tmem_st16(buf + h * 16, w);
+          for (int d = 0; d < 16; ++d) w[d] = pack2<DT>(__uint_as_float(o[2 * d]) * inv, __uint_as_float(o[2 * d + 1]) * inv);
+          if (vec) {
+            // through shared memory (16-byte pieces of row x swapped by x / 2, free of bank conflicts both ways), so
+            // that four lanes write 64 contiguous bytes of a row and an instruction covers 8 rows and not 32
+            uint4* st = s.stage[warp];
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              st[lane * 4 + (q ^ ((lane >> 1) & 3))] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+            __syncwarp();
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const int x = q * 8 + (lane >> 2), d = (lane & 3) * 8 + h * 32;
+              const uint4 y = st[x * 4 + ((lane & 3) ^ ((x >> 1) & 3))];
+              if (row0 + x < it.len && d < a.D) *reinterpret_cast<uint4*>(dst + x * a.so.row + d) = y;
+            }
+            __syncwarp();
+          } else if (row0 + lane < it.len) {
+            store32(dst + lane * a.so.row + h * 32, w, a.D - h * 32, false);
+          }
         }
-      tmem_st_wait();
-      tc_fence_before();
+        tc_fence_before();
+      }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&s.p_full[bf]);
-    }
-    if (ok) ok = mbar_wait_soon(&s.o_done[(n - 1) & 1], ((n - 1) >> 1) & 1, 210);
-    tc_fence_after();
-    const int row = b.first + warp * 32 + lane;
-    if (ok) {
-      const float inv = 1.f / l;
-      uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + b.outer * a.so.outer + head * a.so.head + (b.row0 + row) * a.so.row;
-      if (row < b.len)
-        a.lse[(b.outer * a.H + head) * a.rows + b.row0 + row] = ((ref == kNegInf ? 0.f : ref) + log2f(l)) * kLn2;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t o[32], w[16];
-        tmem_ld32(lanes + 192 + h * 32, o);
-        tmem_ld_wait();
-#pragma unroll
-        for (int d = 0; d < 16; ++d) w[d] = pack2<DT>(__uint_as_float(o[2 * d]) * inv, __uint_as_float(o[2 * d + 1]) * inv);
-        if (row < b.len) store32(dst + h * 32, w, a.D - h * 32, vec);
-      }
+      if (lane == 0) mbar_arrive(&s.item_empty[r]);
     }
   }
   tc_fence_before();
@@ -464,8 +583,8 @@ template <int DT>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
                    const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mdo, const AttnArgs a, int vec) {
-  extern __shared__ uint8_t raw[];
-  BwdSmem& s = *reinterpret_cast<BwdSmem*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t raw[];
+  BwdSmem& s = *reinterpret_cast<BwdSmem*>(raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.H / a.Hk;
   if (threadIdx.x == 0) {
     for (int i = 0; i < kRing; ++i) {
@@ -557,18 +676,18 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
     bool ok = true;
     for (int k = 0, t = 0; ok; ++k) {
       const int r = k % kRing;
-      if (!mbar_spin(&s.item_full[r], (k / kRing) & 1, 213)) break;
+      if (!mbar_wait_soon(&s.item_full[r], (k / kRing) & 1, 213)) break;
       const int n = s.item[r].n, len = s.item[r].len, keys = s.item[r].keys;
-      if (!n || !mbar_spin(&s.a_full[r], (k / kRing) & 1, 214)) break;
+      if (!n || !mbar_wait_soon(&s.a_full[r], (k / kRing) & 1, 214)) break;
       const uint32_t ar = desc_lo(smem_u32(dp ? s.a1[r] : s.a0[r]));
       for (int i = 0, row = 0; i < n; ++i, ++t) {
         const int x = t % 3, st = t % kStages, cols = min(BN, len - row), c16 = up16(cols);
         uint8_t* tile = dp ? s.b1[st] : s.b0[st];
-        ok = mbar_spin(&s.b_full[st], (t / kStages) & 1, 215);
+        ok = mbar_wait_soon(&s.b_full[st], (t / kStages) & 1, 215);
         if (!ok) break;
         // rows behind the end: summed over in dk or dq (queries of S, keys) and in dv (dout, for keys)
         if ((cols & 15) && (keys || !dp)) zero_tile_rows(tile, cols, c16, lane);
-        ok = t < 3 || mbar_spin(&s.x_done[x], ((t / 3) & 1) ^ 1, 216);
+        ok = t < 3 || mbar_wait_soon(&s.x_done[x], ((t / 3) & 1) ^ 1, 216);
         if (!ok) break;
         tc_fence_after();
         const uint32_t br = desc_lo(smem_u32(tile)), at = tmem + x * 128 + (dp ? 64 : 0);
@@ -591,12 +710,12 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
     bool ok = true;
     for (int k = 0, t = 0; ok; ++k) {
       const int r = k % kRing;
-      if (!mbar_spin(&s.item_full[r], (k / kRing) & 1, 224)) break;
+      if (!mbar_wait_soon(&s.item_full[r], (k / kRing) & 1, 224)) break;
       const int n = s.item[r].n, len = s.item[r].len, keys = s.item[r].keys;
-      if (!n || (k && !mbar_spin(&s.acc_free, (k - 1) & 1, 217))) break;
+      if (!n || (k && !mbar_wait_soon(&s.acc_free, (k - 1) & 1, 217))) break;
       for (int i = 0, row = 0; i < n; ++i, ++t) {
         const int x = t % 3, st = t % kStages, cols = min(BN, len - row);
-        ok = mbar_spin(&s.p_full[x], (t / 3) & 1, 218);
+        ok = mbar_wait_soon(&s.p_full[x], (t / 3) & 1, 218);
         if (!ok) break;
         tc_fence_after();
         const uint32_t br0 = desc_lo(smem_u32(s.b0[st])), br1 = desc_lo(smem_u32(s.b1[st])), at = tmem + x * 128;
@@ -746,7 +865,7 @@ int fwd(const AttnArgs& a, cudaStream_t st) {
   if (int rc = make_map(&mq, a.q, DT, a.sq, a.outer, a.H, a.rows, a.D, BM)) return rc;
   if (int rc = make_map(&mk, a.k, DT, a.sk, a.outer, a.Hk, a.rows, a.D, KT)) return rc;
   if (int rc = make_map(&mv, a.v, DT, a.sv, a.outer, a.Hk, a.rows, a.D, KT)) return rc;
-  const int bytes = sizeof(FwdSmem) + 1024;
+  const int bytes = sizeof(FwdSmem);
   static bool done[64] = {};
   if (int rc = attn_smem_once(attn_fwd_tc_kernel<DT>, bytes, done)) return rc;
   const int vec = a.D % 8 == 0 && map_ok(a.out, a.so, a.outer, a.H, a.rows);
@@ -761,7 +880,7 @@ int bwd(const AttnArgs& a, cudaStream_t st) {
   if (int rc = make_map(&mk, a.k, DT, a.sk, a.outer, a.Hk, a.rows, a.D, BN)) return rc;
   if (int rc = make_map(&mv, a.v, DT, a.sv, a.outer, a.Hk, a.rows, a.D, BN)) return rc;
   if (int rc = make_map(&mdo, a.dout, DT, a.sdo, a.outer, a.H, a.rows, a.D, BN)) return rc;
-  const int bytes = sizeof(BwdSmem) + 1024;
+  const int bytes = sizeof(BwdSmem);
   static bool done[64] = {};
   if (int rc = attn_smem_once(attn_bwd_tc_kernel<DT>, bytes, done)) return rc;
   const int vec = a.D % 8 == 0 && map_ok(a.dq, a.sdq, a.outer, a.H, a.rows) && map_ok(a.dk, a.sdk, a.outer, a.Hk, a.rows) &&

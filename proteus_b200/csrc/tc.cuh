@@ -276,6 +276,33 @@ __host__ __device__ constexpr uint32_t idesc_s8_s32(int M, int N) {
   return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
+// ---------------------------------------------------------------- cluster launch control
+// A running CTA takes over one that has not been launched yet: the request's answer (16 bytes) lands in shared
+// memory and completes `bar`'s transaction count. No further request may follow an answer of "none left".
+__device__ __forceinline__ void take_cta_async(uint4* answer, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   smem_u32(answer)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ bool taken_cta(const uint4* answer, int& x, int& y) {
+  uint32_t ok, cx, cy;
+  asm volatile(
+      "{\n\t.reg .b128 h;\n\t.reg .pred p;\n\t"
+      "ld.shared.b128 h, [%3];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "mov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::y.b32.b128 %2, h;\n\t}"
+      : "=r"(ok), "=r"(cx), "=r"(cy)
+      : "r"(smem_u32(answer))
+      : "memory");
+  x = (int)cx;
+  y = (int)cy;
+  return ok != 0;
+}
+
 // ---------------------------------------------------------------- CTA pairs (cta_group::2)
 // A cluster of two CTAs on the two SMs of a TPC shares one MMA: the even CTA issues
 // tcgen05.mma.cta_group::2, whose A and B operands are the same shared-memory offsets in both CTAs
