@@ -7,8 +7,10 @@
 //
 // 64 x 64 tiles, 256 threads, each with 4 rows (ty + 16 i) and 4 columns (tx + 16 j) of a tile of
 // scores; operands lie in shared memory as fp32 rows of DP + 4 words, read as float4 along the head
-// dimension (the 16 tx of a half warp hit distinct banks, the ty broadcast). The running maximum and
-// sum of the softmax stay in registers. The gradient is two kernels, one CTA per key tile (dk, dv; all query
+// dimension (the 16 tx of a half warp hit distinct banks, the ty broadcast). The next tile's rows are in
+// registers on their way while this one is worked on. Scores are in base 2 (the queries carry scale log2 e). The
+// exponents' reference is the maximum of a row's first tile; fp32 has range for 2^64 above it, and only a sum
+// beyond that (or no reference yet: scores of -inf so far) raises it and rescales. The gradient is two kernels, one CTA per key tile (dk, dv; all query
 // heads of its key head, one after the other) and one per query tile (dq): scores are computed twice, but no
 // sum crosses CTAs, so every result is the same from run to run.
 #include "attn.cuh"
@@ -30,18 +32,48 @@ __device__ __forceinline__ void put<ATLAS_BF16>(__nv_bfloat16* p, float v) { *p 
 template <>
 __device__ __forceinline__ void put<ATLAS_F16>(__half* p, float v) { *p = __float2half_rn(v); }
 
-// Rows first .. first + 63 of a head into shared memory, zero behind `len` and behind D.
-template <int DT, int DP>
-__device__ __forceinline__ void load_tile(float* dst, const void* src, const Strides& st, int64_t outer, int head, int64_t row0,
-                                          int first, int len, int D, float mul) {
-  using T = typename Elem<DT>::T;
-  const T* p = reinterpret_cast<const T*>(src) + outer * st.outer + head * st.head + row0 * st.row;
-  for (int i = threadIdx.x; i < BT * DP; i += kThreads) {
-    const int r = i / DP, d = i % DP;
-    const bool on = first + r < len && d < D;
-    dst[r * (DP + 4) + d] = on ? Elem<DT>::f(p[(int64_t)(first + r) * st.row + d]) * mul : 0.f;
-  }
+__device__ __forceinline__ float ex2(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
 }
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+// Rows first .. first + 63 of a head, four columns at a time: from memory into registers (zero behind `len` and
+// behind D), and from there into shared memory. `vec`: fp32 rows that 16-byte loads may read.
+template <int DT, int DP>
+struct Tile {
+  float4 r[DP / 16];
+  __device__ __forceinline__ void fetch(const void* src, const Strides& st, int64_t outer, int head, int64_t row0, int first,
+                                        int len, int D, bool vec) {
+    using T = typename Elem<DT>::T;
+    const T* p = reinterpret_cast<const T*>(src) + outer * st.outer + head * st.head + row0 * st.row;
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k) {
+      const int i = threadIdx.x + k * kThreads, x = first + i / (DP / 4), d = i % (DP / 4) * 4;
+      r[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (x < len && d < D) {
+        const T* q = p + (int64_t)x * st.row + d;
+        if (DT == ATLAS_F32 && vec) {
+          r[k] = __ldg(reinterpret_cast<const float4*>(q));
+        } else {
+          r[k].x = Elem<DT>::f(q[0]);
+          if (d + 1 < D) r[k].y = Elem<DT>::f(q[1]);
+          if (d + 2 < D) r[k].z = Elem<DT>::f(q[2]);
+          if (d + 3 < D) r[k].w = Elem<DT>::f(q[3]);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void put(float* dst, float mul) const {
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k) {
+      const int i = threadIdx.x + k * kThreads;
+      *reinterpret_cast<float4*>(dst + i / (DP / 4) * (DP + 4) + i % (DP / 4) * 4) =
+          make_float4(r[k].x * mul, r[k].y * mul, r[k].z * mul, r[k].w * mul);
+    }
+  }
+};
 
 // c[i][j] = sum_d a[ty + 16 i][d] b[tx + 16 j][d]
 template <int DP>
@@ -109,8 +141,8 @@ template <int DT>
 __device__ __forceinline__ void zero_rows(void* dst, const Strides& st, int64_t outer, int head, int64_t from, int64_t to, int D) {
   using T = typename Elem<DT>::T;
   T* p = reinterpret_cast<T*>(dst) + outer * st.outer + head * st.head;
-  for (int64_t r = from + threadIdx.x / 32; r < to; r += kThreads / 32)
-    for (int d = threadIdx.x % 32; d < D; d += 32) put<DT>(p + r * st.row + d, 0.f);
+  for (int64_t r = from + threadIdx.x / 16; r < to; r += kThreads / 16)
+    for (int d = threadIdx.x % 16; d < D; d += 16) put<DT>(p + r * st.row + d, 0.f);
 }
 
 template <int DT, int DP>
@@ -131,7 +163,7 @@ __device__ __forceinline__ void store_tile(void* dst, const Strides& st, int64_t
 
 // ---------------------------------------------------------------------------------------- forward
 template <int DT, int DP>
-__global__ void __launch_bounds__(kThreads) attn_fwd_simt_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(kThreads, DP == 64 ? 2 : 3) attn_fwd_simt_kernel(const AttnArgs a, int vec) {
   extern __shared__ float sm[];
   constexpr int TILE = BT * (DP + 4);
   float *sq = sm, *sk = sm + TILE, *sv = sm + 2 * TILE, *sp = sm + 3 * TILE;
@@ -147,7 +179,11 @@ __global__ void __launch_bounds__(kThreads) attn_fwd_simt_kernel(const AttnArgs 
   const int first = s.first + (blockIdx.x & 1) * BT;
   if (!s.on || first >= s.len) return;
   const int kh = head / (a.H / a.Hk);
-  load_tile<DT, DP>(sq, a.q, a.sq, s.outer, head, s.row0, first, s.len, a.D, a.scale);
+  Tile<DT, DP> tk, tv;
+  tk.fetch(a.q, a.sq, s.outer, head, s.row0, first, s.len, a.D, vec);
+  tk.put(sq, a.scale * kLog2e);
+  tk.fetch(a.k, a.sk, s.outer, kh, s.row0, 0, s.len, a.D, vec);
+  tv.fetch(a.v, a.sv, s.outer, kh, s.row0, 0, s.len, a.D, vec);
   float m[4], l[4], acc[4][DP / 16];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -158,32 +194,54 @@ __global__ void __launch_bounds__(kThreads) attn_fwd_simt_kernel(const AttnArgs 
   }
   for (int n0 = 0; n0 < s.len; n0 += BT) {
     __syncthreads();
-    load_tile<DT, DP>(sk, a.k, a.sk, s.outer, kh, s.row0, n0, s.len, a.D, 1.f);
-    load_tile<DT, DP>(sv, a.v, a.sv, s.outer, kh, s.row0, n0, s.len, a.D, 1.f);
+    tk.put(sk, 1.f);
+    tv.put(sv, 1.f);
     __syncthreads();
+    if (n0 + BT < s.len) {
+      tk.fetch(a.k, a.sk, s.outer, kh, s.row0, n0 + BT, s.len, a.D, vec);
+      tv.fetch(a.v, a.sv, s.outer, kh, s.row0, n0 + BT, s.len, a.D, vec);
+    }
     float c[4][4];
     mm_rows<DP>(sq, sk, ty, tx, c);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float mx = kNegInf;
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < 4; ++j)
         if (n0 + tx + 16 * j >= s.len) c[i][j] = kNegInf;
-        mx = fmaxf(mx, c[i][j]);
-      }
-      mx = fmaxf(m[i], row_max(mx));
-      const float ref = mx == kNegInf ? 0.f : mx, f = m[i] == kNegInf ? 0.f : expf(m[i] - ref);
-      float sum = 0.f;
+    auto highest = [&](int i) { return row_max(fmaxf(fmaxf(c[i][0], c[i][1]), fmaxf(c[i][2], c[i][3]))); };
+    if (n0 == 0) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float e = expf(c[i][j] - ref);
-        sum += e;
-        sp[(ty + 16 * i) * PP + tx + 16 * j] = e;
-      }
-      l[i] = l[i] * f + row_sum(sum);
-      m[i] = mx;
+      for (int i = 0; i < 4; ++i) m[i] = highest(i);
+    }
+    float e[4][4], sum[4];
+    bool bad = false;
+    auto powers = [&] {
 #pragma unroll
-      for (int d = 0; d < DP / 16; ++d) acc[i][d] *= f;
+      for (int i = 0; i < 4; ++i) {
+        const float ref = m[i] == kNegInf ? 0.f : m[i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) e[i][j] = ex2(c[i][j] - ref);
+        sum[i] = (e[i][0] + e[i][1]) + (e[i][2] + e[i][3]);
+        bad |= m[i] == kNegInf || !(sum[i] <= 0x1p64f);
+      }
+    };
+    powers();
+    if (n0 > 0 && __any_sync(0xFFFFFFFFu, bad)) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float to = fmaxf(m[i], highest(i)), f = m[i] == to || m[i] == kNegInf ? 1.f : ex2(m[i] - to);
+        m[i] = to;
+        l[i] *= f;
+#pragma unroll
+        for (int d = 0; d < DP / 16; ++d) acc[i][d] *= f;
+      }
+      powers();
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      l[i] += sum[i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sp[(ty + 16 * i) * PP + tx + 16 * j] = e[i][j];
     }
     __syncwarp();  // a warp's rows of sp are its own
     mm_cols<DP>(sp, sv, ty, tx, acc);
@@ -191,9 +249,10 @@ __global__ void __launch_bounds__(kThreads) attn_fwd_simt_kernel(const AttnArgs 
   float inv[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
+    l[i] = row_sum(l[i]);
     inv[i] = 1.f / l[i];
     const int r = first + ty + 16 * i;
-    if (tx == 0 && r < s.len) a.lse[(s.outer * a.H + head) * a.rows + s.row0 + r] = (m[i] == kNegInf ? 0.f : m[i]) + logf(l[i]);
+    if (tx == 0 && r < s.len) a.lse[(s.outer * a.H + head) * a.rows + s.row0 + r] = ((m[i] == kNegInf ? 0.f : m[i]) + log2f(l[i])) * kLn2;
   }
   store_tile<DT, DP>(a.out, a.so, s.outer, head, s.row0, first, s.len, a.D, ty, tx, acc, inv);
 }
@@ -202,7 +261,7 @@ __global__ void __launch_bounds__(kThreads) attn_fwd_simt_kernel(const AttnArgs 
 // KEYS: this CTA's rows are keys (dk, dv), the loop runs over the queries of every query head of the
 // key head; otherwise its rows are queries (dq) and the loop runs over the keys.
 template <int DT, int DP, bool KEYS>
-__global__ void __launch_bounds__(kThreads) attn_bwd_simt_kernel(const AttnArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) attn_bwd_simt_kernel(const AttnArgs a, int vec) {
   extern __shared__ float sm[];
   constexpr int TILE = BT * (DP + 4);
   // rows of this CTA: k and v (KEYS) or q and dout; of the loop: the other two
@@ -223,13 +282,17 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_simt_kernel(const AttnArgs 
   const int first = s.first + (blockIdx.x & 1) * BT;
   if (!s.on || first >= s.len) return;
   const int kh = KEYS ? blockIdx.y : blockIdx.y / group;
-  if (KEYS) {
-    load_tile<DT, DP>(s0, a.k, a.sk, s.outer, kh, s.row0, first, s.len, a.D, 1.f);
-    load_tile<DT, DP>(s1, a.v, a.sv, s.outer, kh, s.row0, first, s.len, a.D, 1.f);
-  } else {
-    load_tile<DT, DP>(s0, a.q, a.sq, s.outer, blockIdx.y, s.row0, first, s.len, a.D, 1.f);
-    load_tile<DT, DP>(s1, a.dout, a.sdo, s.outer, blockIdx.y, s.row0, first, s.len, a.D, 1.f);
-  }
+  // the queries' scores in base 2: the factor goes to the tile of queries or keys that stays
+  Tile<DT, DP> ta, tb;
+  ta.fetch(KEYS ? a.k : a.q, KEYS ? a.sk : a.sq, s.outer, blockIdx.y, s.row0, first, s.len, a.D, vec);
+  tb.fetch(KEYS ? a.v : a.dout, KEYS ? a.sv : a.sdo, s.outer, blockIdx.y, s.row0, first, s.len, a.D, vec);
+  ta.put(s0, a.scale * kLog2e);
+  tb.put(s1, 1.f);
+  auto fetch = [&](int h, int n0) {
+    ta.fetch(KEYS ? a.q : a.k, KEYS ? a.sq : a.sk, s.outer, KEYS ? h : kh, s.row0, n0, s.len, a.D, vec);
+    tb.fetch(KEYS ? a.dout : a.v, KEYS ? a.sdo : a.sv, s.outer, KEYS ? h : kh, s.row0, n0, s.len, a.D, vec);
+  };
+  fetch(kh * group, 0);
   float g0[4][DP / 16], g1[4][DP / 16];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -240,20 +303,17 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_simt_kernel(const AttnArgs 
     const float* delta = a.delta + (s.outer * a.H + h) * a.rows + s.row0;
     for (int n0 = 0; n0 < s.len; n0 += BT) {
       __syncthreads();
-      if (KEYS) {
-        load_tile<DT, DP>(t0, a.q, a.sq, s.outer, h, s.row0, n0, s.len, a.D, 1.f);
-        load_tile<DT, DP>(t1, a.dout, a.sdo, s.outer, h, s.row0, n0, s.len, a.D, 1.f);
-      } else {
-        load_tile<DT, DP>(t0, a.k, a.sk, s.outer, kh, s.row0, n0, s.len, a.D, 1.f);
-        load_tile<DT, DP>(t1, a.v, a.sv, s.outer, kh, s.row0, n0, s.len, a.D, 1.f);
-      }
+      ta.put(t0, 1.f);
+      tb.put(t1, 1.f);
       const int q0 = KEYS ? n0 : first;
       if (threadIdx.x < BT) {
         const bool on = q0 + (int)threadIdx.x < s.len;
-        s_lse[threadIdx.x] = on ? lse[q0 + threadIdx.x] : 0.f;
+        s_lse[threadIdx.x] = on ? lse[q0 + threadIdx.x] * kLog2e : 0.f;
         s_delta[threadIdx.x] = on ? delta[q0 + threadIdx.x] : 0.f;
       }
       __syncthreads();
+      if (n0 + BT < s.len) fetch(h, n0 + BT);
+      else if (KEYS && h + 1 < (kh + 1) * group) fetch(h + 1, 0);
       float c[4][4], d[4][4];
       mm_rows<DP>(s0, t0, ty, tx, c);
       mm_rows<DP>(s1, t1, ty, tx, d);
@@ -263,7 +323,7 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_simt_kernel(const AttnArgs 
         for (int j = 0; j < 4; ++j) {
           const int qi = KEYS ? tx + 16 * j : ty + 16 * i;
           const bool on = first + ty + 16 * i < s.len && n0 + tx + 16 * j < s.len;
-          const float p = on ? expf(c[i][j] * a.scale - s_lse[qi]) : 0.f;
+          const float p = on ? ex2(c[i][j] - s_lse[qi]) : 0.f;
           sp[(ty + 16 * i) * PP + tx + 16 * j] = p;
           sd[(ty + 16 * i) * PP + tx + 16 * j] = on ? p * (d[i][j] - s_delta[qi]) : 0.f;
         }
@@ -349,15 +409,20 @@ __global__ void __launch_bounds__(kThreads) attn_delta_kernel(const AttnArgs a) 
 }  // namespace
 
 namespace {
-bool delta_vec(const void* p, const Strides& s, int esize) {
+bool rows_of_16(const void* p, const Strides& s, int esize) {
   const int64_t m = 16 / esize;
   return (uintptr_t)p % 16 == 0 && s.row % m == 0 && s.head % m == 0 && s.outer % m == 0;
+}
+// Whether every row that the kernels load is made of whole 16-byte pieces (fp32).
+int vec_rows(const AttnArgs& a, int dtype, bool grad) {
+  return dtype == ATLAS_F32 && a.D % 4 == 0 && rows_of_16(a.q, a.sq, 4) && rows_of_16(a.k, a.sk, 4) && rows_of_16(a.v, a.sv, 4) &&
+         (!grad || rows_of_16(a.dout, a.sdo, 4));
 }
 template <int DT>
 void launch_delta(const AttnArgs& a, cudaStream_t st) {
   const dim3 grid((unsigned)a.cap, a.H);
   const int size = DT == ATLAS_F32 ? 4 : 2;
-  if (a.D * size % 16 == 0 && delta_vec(a.o, a.so, size) && delta_vec(a.dout, a.sdo, size))
+  if (a.D * size % 16 == 0 && rows_of_16(a.o, a.so, size) && rows_of_16(a.dout, a.sdo, size))
     attn_delta_kernel<DT, true><<<grid, kThreads, 0, st>>>(a);
   else
     attn_delta_kernel<DT, false><<<grid, kThreads, 0, st>>>(a);
@@ -378,7 +443,7 @@ int fwd(const AttnArgs& a, cudaStream_t st) {
   const int bytes = (3 * BT * (DP + 4) + BT * PP) * 4;
   static bool done[64] = {};
   if (int rc = attn_smem_once(attn_fwd_simt_kernel<DT, DP>, bytes, done)) return rc;
-  attn_fwd_simt_kernel<DT, DP><<<dim3((unsigned)(2 * a.cap), a.H), kThreads, bytes, st>>>(a);
+  attn_fwd_simt_kernel<DT, DP><<<dim3((unsigned)(2 * a.cap), a.H), kThreads, bytes, st>>>(a, vec_rows(a, DT, false));
   return check_launch("attention");
 }
 
@@ -389,8 +454,9 @@ int bwd(const AttnArgs& a, cudaStream_t st) {
   if (int rc = attn_smem_once(attn_bwd_simt_kernel<DT, DP, true>, bytes, done[0])) return rc;
   if (int rc = attn_smem_once(attn_bwd_simt_kernel<DT, DP, false>, bytes, done[1])) return rc;
   if (int rc = attn_delta(a, DT, st)) return rc;
-  attn_bwd_simt_kernel<DT, DP, true><<<dim3((unsigned)(2 * a.cap), a.Hk), kThreads, bytes, st>>>(a);
-  attn_bwd_simt_kernel<DT, DP, false><<<dim3((unsigned)(2 * a.cap), a.H), kThreads, bytes, st>>>(a);
+  const int vec = vec_rows(a, DT, true);
+  attn_bwd_simt_kernel<DT, DP, true><<<dim3((unsigned)(2 * a.cap), a.Hk), kThreads, bytes, st>>>(a, vec);
+  attn_bwd_simt_kernel<DT, DP, false><<<dim3((unsigned)(2 * a.cap), a.H), kThreads, bytes, st>>>(a, vec);
   return check_launch("attention_grad");
 }
 
