@@ -67,6 +67,12 @@ __device__ __forceinline__ void load_pairs(f32x2 (&v)[2], const float* p) {
   v[1] = w.y;
 }
 
+// Moves registers between warpgroups (see the kernels' shares).
+template <int N>
+__device__ __forceinline__ void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
 template <int DT>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   uint32_t r;
@@ -103,22 +109,24 @@ __device__ __forceinline__ int up16(int n) { return (n + 15) & ~15; }
 // Work items of 128 queries of a head, key tiles of 96 rows. Two CTAs per SM run items as a stream of tiles: a
 // CTA that has loaded its last item takes over one that was not launched yet (cluster launch control), so that
 // an item's look-up, first loads and first scores hide behind the item before.
-//   warps 0-3  softmax, one thread per query
-//   warp 4     TMA, items, and zeros in rows of no sequence
-//   warp 5     scores; TMEM: two buffers of scores (columns 0-95, 96-191), P(t) over the first half of S(t), the
-//              output in 192-255, where an item's products accumulate
-//   warp 6     products with v
+//   warps 0-3   softmax, one thread per query
+//   warps 4-7   read an item's output, divide and write it, while the softmax is at the next item
+//   warp 8      TMA, items, and zeros in rows of no sequence
+//   warp 9      scores; TMEM: two buffers of scores (columns 0-95, 96-191), P(t) over the first half of S(t), the
+//               output in 192-255, where an item's products accumulate
+//   warp 10     products with v
+// Registers are moved from the other eight warps to the softmax's: 384 x 80 = 128 (152 + 48 + 40).
 //
-// The reference that exponents are taken from is the maximum of a row's FIRST tile, not a running one: any
+// The reference that exponents are taken from is the maximum of a row's FIRST 32 scores, not a running one: any
 // reference gives the same quotient, and fp32 sums and bf16 probabilities have range for 2^64 above it. So a
 // tile costs one pass (no maximum, no rescaling): a packed multiply-add, an exponential, a packed sum and half a
 // conversion a score. The tile's sum tells when the reference was too low (2^64; fp16 P: 2^15), or when there is
-// none yet (all scores so far -inf); the warp then takes the tile's maximum, rescales the output in TMEM and
+// none yet (those scores all -inf); the warp then takes the tile's maximum, rescales the output in TMEM and
 // does the tile again, whose scores are still there, since P is held in registers until it is accepted.
 //
 // The last tile of a sequence of several ends at the sequence's end and starts inside the tile before: its
 // columns `lo` .. are new, the ones below count as -inf, and no row behind the end is read.
-constexpr int kFwdThreads = 224;
+constexpr int kFwdThreads = 384;
 constexpr int KT = 96;
 constexpr int kFwdStages = 3;
 constexpr uint32_t kKeyTile = KT * 128;
@@ -129,10 +137,11 @@ struct FwdItem {
 
 struct FwdSmem {
   uint8_t q[2][kTile], k[kFwdStages][kKeyTile], v[kFwdStages][kKeyTile];
-  uint4 stage[4][32 * 4];  // each softmax warp: 32 columns of its 32 rows on their way out
+  uint4 stage[4][32 * 2];  // each writing warp: 16 columns of its 32 rows on their way out
+  float2 stat[2][BM];      // sum and reference of an item's rows
   FwdItem item[2];
   uint4 answer;
-  uint64_t item_full[2], item_empty[2], q_full[2], k_full[kFwdStages], k_empty[kFwdStages], v_full[kFwdStages],
+  uint64_t stat_full[2], o_free, item_full[2], item_empty[2], q_full[2], k_full[kFwdStages], k_empty[kFwdStages], v_full[kFwdStages],
       v_empty[kFwdStages], s_full[2], p_full[2], o_done[2], taken;
   uint32_t tmem;
 };
@@ -158,11 +167,6 @@ __device__ __forceinline__ float fwd_tile(uint32_t buf, float c, float nref, int
     if (h < 2) tmem_ld32(buf + h * 32 + 32, x[(h + 1) & 1]);
     if (h * 32 >= hi || h * 32 + 32 <= lo) continue;
     uint32_t(&y)[32] = x[h & 1];
-    if (h * 32 + 32 > hi || h * 32 < lo) {
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (h * 32 + j >= hi || h * 32 + j < lo) y[j] = 0xFF800000u;  // -inf
-    }
 #pragma unroll
     for (int j = 0; j < 32; j += 2) {
       float a, b;
@@ -178,17 +182,32 @@ __device__ __forceinline__ float fwd_tile(uint32_t buf, float c, float nref, int
   return a + b;
 }
 
-__device__ __forceinline__ float fwd_max(uint32_t buf, int lo, int hi) {
-  float mx = kNegInf;
-#pragma unroll
-  for (int h = 0; h < 3; ++h) {
-    if (h * 32 >= hi || h * 32 + 32 <= lo) continue;
-    uint32_t x[32];
-    tmem_ld32(buf + h * 32, x);
+// Columns outside lo .. hi - 1 of a row's tile become -inf, in TMEM.
+__device__ __noinline__ void fwd_mask(uint32_t buf, int lo, int hi) {
+#pragma unroll 1
+  for (int h = 0; h < KT; h += 16) {
+    if (h >= lo && h + 16 <= hi) continue;
+    uint32_t x[16];
+    tmem_ld16(buf + h, x);
     tmem_ld_wait();
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-      mx = fmaxf(mx, h * 32 + j < hi && h * 32 + j >= lo ? __uint_as_float(x[j]) : kNegInf);
+    for (int j = 0; j < 16; ++j)
+      if (h + j < lo || h + j >= hi) x[j] = 0xFF800000u;
+    tmem_st16(buf + h, x);
+  }
+  tmem_st_wait();
+}
+
+// The largest of `n` (a multiple of 16) columns.
+__device__ __noinline__ float fwd_max(uint32_t buf, int n) {
+  float mx = kNegInf;
+#pragma unroll 1
+  for (int h = 0; h < n; h += 16) {
+    uint32_t x[16];
+    tmem_ld16(buf + h, x);
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) mx = fmaxf(mx, __uint_as_float(x[j]));
   }
   return mx;
 }
@@ -201,14 +220,17 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
   FwdSmem& s = *reinterpret_cast<FwdSmem*>(raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
+#pragma unroll 1
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.item_full[i], 1);
-      mbar_init(&s.item_empty[i], 4);
+      mbar_init(&s.item_empty[i], 8);
+      mbar_init(&s.stat_full[i], 4);
       mbar_init(&s.q_full[i], 1);
       mbar_init(&s.s_full[i], 1);
       mbar_init(&s.p_full[i], 4);
       mbar_init(&s.o_done[i], 1);
     }
+#pragma unroll 1
     for (int i = 0; i < kFwdStages; ++i) {
       mbar_init(&s.k_full[i], 1);
       mbar_init(&s.k_empty[i], 1);
@@ -216,15 +238,17 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
       mbar_init(&s.v_empty[i], 1);
     }
     mbar_init(&s.taken, 1);
+    mbar_init(&s.o_free, 4);
     fence_barrier_init();
   }
-  if (warp == 5) tmem_alloc(&s.tmem, 256);
+  if (warp == 9) tmem_alloc(&s.tmem, 256);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s.tmem;
 
-  if (warp == 4) {
+  if (warp == 8) {
+    regs_dec<40>();
     int x = blockIdx.x, head = blockIdx.y, k = 0, t = 0;
     uint32_t asked = 0;
     bool more = true, ok = true;
@@ -239,8 +263,10 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
       if (more && idle_rows(a, b, x, &z0, &z1)) {
         uint16_t* o = reinterpret_cast<uint16_t*>(a.out) + b.outer * a.so.outer + head * a.so.head;
         float* l = a.lse + (b.outer * a.H + head) * a.rows;
+#pragma unroll 1
         for (int64_t r = z0; r < z1; ++r)
           for (int d = lane; d < a.D; d += 32) o[r * a.so.row + d] = 0;
+#pragma unroll 1
         for (int64_t r = z0 + lane; r < z1; r += 32) l[r] = 0.f;
       }
       if (!more || (b.on && b.first < b.len)) {
@@ -259,6 +285,7 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
           tma_load_4d(s.q[r], &mq, 0, r0 + b.first, head, o, &s.q_full[r]);
         }
         __syncwarp();
+#pragma unroll 1
         for (int i = 0; i < n; ++i, ++t) {
           const int st = t % kFwdStages;
           const uint32_t ph = ((t / kFwdStages) & 1) ^ 1;
@@ -285,15 +312,18 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
     }
-  } else if (warp == 5) {
+  } else if (warp == 9) {
+    regs_dec<40>();
     const uint32_t base = DT == ATLAS_BF16 ? idesc_bf16_f32(BM, 0) : idesc_f16_f32(BM, 0);
     const uint32_t qd = desc_lo(smem_u32(s.q[0])), kd = desc_lo(smem_u32(s.k[0]));
     bool ok = true;
+#pragma unroll 1
     for (int k = 0, t = 0; ok; ++k) {
       const int r = k & 1;
       if (!mbar_wait_soon(&s.item_full[r], (k >> 1) & 1, 211)) break;
       const int n = s.item[r].n, len = s.item[r].len;
       if (!n || !mbar_wait_soon(&s.q_full[r], (k >> 1) & 1, 204)) break;
+#pragma unroll 1
       for (int i = 0; i < n; ++i, ++t) {  // S(t) = q k^T into buffer t & 1
         const int st = t % kFwdStages, bf = t & 1;
         ok = mbar_wait_soon(&s.k_full[st], (t / kFwdStages) & 1, 203) &&
@@ -316,14 +346,18 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
         __syncwarp();
       }
     }
-  } else if (warp == 6) {
+  } else if (warp == 10) {
+    regs_dec<40>();
     const uint32_t id = (DT == ATLAS_BF16 ? idesc_bf16_f32(BM, 64) : idesc_f16_f32(BM, 64)) | kMnB;
     const uint32_t vd = desc_lo(smem_u32(s.v[0]));
     bool ok = true;
+#pragma unroll 1
     for (int k = 0, t = 0; ok; ++k) {
       if (!mbar_wait_soon(&s.item_full[k & 1], (k >> 1) & 1, 213)) break;
       const int n = s.item[k & 1].n, len = s.item[k & 1].len;
-      if (!n) break;
+      // the last item's output has been read out of where this one's goes
+      if (!n || (k && !mbar_wait_soon(&s.o_free, (k - 1) & 1, 214))) break;
+#pragma unroll 1
       for (int i = 0; i < n; ++i, ++t) {
         const int st = t % kFwdStages, bf = t & 1;
         int lo, hi;
@@ -331,7 +365,6 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
         ok = mbar_wait_soon(&s.v_full[st], (t / kFwdStages) & 1, 205);
         if (!ok) break;
         if (hi & 15) zero_tile_rows(s.v[st], hi, up16(hi), lane);  // a sequence of one short tile: rows behind its end
-        // P(t) of an item's first tile comes after its warps have read the last item's output
         ok = mbar_wait_soon(&s.p_full[bf], (t >> 1) & 1, 206);
         if (!ok) break;
         tc_fence_after();
@@ -350,10 +383,14 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
         __syncwarp();
       }
     }
+  } else if (warp == 11) {
+    regs_dec<40>();
   } else if (warp < 4) {
+    regs_inc<152>();
     const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
     const float c = a.scale * kLog2e, limit = DT == ATLAS_BF16 ? 0x1p64f : 0x1p15f;
     bool ok = true;
+#pragma unroll 1
     for (int k = 0, t = 0; ok; ++k) {
       const int r = k & 1;
       ok = mbar_wait_soon(&s.item_full[r], (k >> 1) & 1, 212);
@@ -362,6 +399,7 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
       if (!it.n) break;
       const bool live = it.first + warp * 32 < it.len;
       float ref = kNegInf, l = 0.f;  // ref: in base 2, -inf while there is none
+#pragma unroll 1
       for (int i = 0; i < it.n; ++i, ++t) {
         const int bf = t & 1;
         const uint32_t buf = lanes + bf * KT;
@@ -371,33 +409,37 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
         if (!ok) break;
         tc_fence_after();
         if (live) {
-          if (i == 0) ref = fwd_max(buf, lo, hi) * c;
+          // one copy of the tile's code: instruction fetch is what many copies of it run out of first
+          if (lo > 0 || hi < KT) fwd_mask(buf, lo, hi);
+          if (i == 0) ref = fwd_max(buf, 32) * c;
           uint32_t p[KT / 2];
-          float sum = fwd_tile<DT>(buf, c, ref == kNegInf ? 0.f : -ref, lo, hi, p);
-          if (i > 0) {
+          float sum;
+          for (int again = 0;; ++again) {
+            sum = fwd_tile<DT>(buf, c, ref == kNegInf ? 0.f : -ref, lo, hi, p);
             const bool bad = ref == kNegInf || !(sum <= limit);
-            if (__any_sync(0xFFFFFFFFu, bad)) {
-              const float mx = fwd_max(buf, lo, hi) * c;
-              const float to = bad ? fmaxf(ref, mx) : ref;
+            if (again || !__any_sync(0xFFFFFFFFu, bad)) break;
+            const float mx = fwd_max(buf, KT) * c;
+            const float to = bad ? fmaxf(ref, mx) : ref;
+            if (i > 0) {
               const float f = ref == to || ref == kNegInf ? 1.f : ex2(ref - to);
               // the products up to here are complete, and P(t) has not been handed over
               ok = mbar_wait_soon(&s.o_done[bf ^ 1], ((t - 1) >> 1) & 1, 208);
               if (!ok) break;
               tc_fence_after();
-#pragma unroll
-              for (int h = 0; h < 4; ++h) {
+#pragma unroll 1
+              for (int h = 0; h < 64; h += 16) {
                 uint32_t o[16];
-                tmem_ld16(lanes + 192 + h * 16, o);
+                tmem_ld16(lanes + 192 + h, o);
                 tmem_ld_wait();
 #pragma unroll
                 for (int d = 0; d < 16; ++d) o[d] = __float_as_uint(__uint_as_float(o[d]) * f);
-                tmem_st16(lanes + 192 + h * 16, o);
+                tmem_st16(lanes + 192 + h, o);
               }
-              ref = to;
               l *= f;
-              sum = fwd_tile<DT>(buf, c, ref == kNegInf ? 0.f : -ref, lo, hi, p);
             }
+            ref = to;
           }
+          if (!ok) break;
           l += sum;
 #pragma unroll
           for (int h = 0; h < 3; ++h)
@@ -414,51 +456,76 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
         if (lane == 0) mbar_arrive(&s.p_full[bf]);
       }
       if (!ok) break;
-      if (live) {
-        ok = mbar_wait_soon(&s.o_done[(t - 1) & 1], ((t - 1) >> 1) & 1, 210);
-        if (!ok) break;
-        tc_fence_after();
-        const int row0 = it.first + warp * 32;  // the warp's first row
-        const float inv = 1.f / l;
-        const int64_t to = (int64_t)it.row0 + row0;
-        uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + it.outer * a.so.outer + it.head * a.so.head + to * a.so.row;
-        if (row0 + lane < it.len)
-          a.lse[((int64_t)it.outer * a.H + it.head) * a.rows + to + lane] = ((ref == kNegInf ? 0.f : ref) + log2f(l)) * kLn2;
+      s.stat[r][warp * 32 + lane] = make_float2(l, ref);
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&s.stat_full[r]);
+        mbar_arrive(&s.item_empty[r]);
+      }
+    }
+  } else {
+    regs_dec<48>();
+    const int quarter = warp & 3;
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+#pragma unroll 1
+    for (int k = 0, t = 0;; ++k) {
+      const int r = k & 1;
+      if (!mbar_wait(&s.item_full[r], (k >> 1) & 1, 215)) break;
+      const int n = s.item[r].n, len = s.item[r].len, row0 = s.item[r].first + quarter * 32;  // the warp's first row
+      if (!n) break;
+      t += n;
+      // the sums; with them the scores of the last tile are done, so that its product's barrier is at its phase
+      if (!mbar_wait(&s.stat_full[r], (k >> 1) & 1, 216) || !mbar_wait(&s.o_done[(t - 1) & 1], ((t - 1) >> 1) & 1, 210)) break;
+      tc_fence_after();
+      if (row0 < len) {
+        const float2 st = s.stat[r][quarter * 32 + lane];
+        const float inv = 1.f / st.x;
+        const int head = s.item[r].head;
+        const int64_t outer = s.item[r].outer, to = (int64_t)s.item[r].row0 + row0;
+        uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + outer * a.so.outer + head * a.so.head + to * a.so.row;
+        if (row0 + lane < len)
+          a.lse[(outer * a.H + head) * a.rows + to + lane] = ((st.y == kNegInf ? 0.f : st.y) + log2f(st.x)) * kLn2;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t o[32], w[16];
-          tmem_ld32(lanes + 192 + h * 32, o);
+        for (int h = 0; h < 4; ++h) {
+          uint32_t o[16];
+          uint4 w[2];
+          tmem_ld16(lanes + 192 + h * 16, o);
           tmem_ld_wait();
 #pragma unroll
-          for (int d = 0; d < 16; ++d) w[d] = pack2<DT>(__uint_as_float(o[2 * d]) * inv, __uint_as_float(o[2 * d + 1]) * inv);
+          for (int d = 0; d < 8; ++d)
+            reinterpret_cast<uint32_t*>(w)[d] = pack2<DT>(__uint_as_float(o[2 * d]) * inv, __uint_as_float(o[2 * d + 1]) * inv);
           if (vec) {
-            // through shared memory (16-byte pieces of row x swapped by x / 2, free of bank conflicts both ways), so
-            // that four lanes write 64 contiguous bytes of a row and an instruction covers 8 rows and not 32
-            uint4* st = s.stage[warp];
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              st[lane * 4 + (q ^ ((lane >> 1) & 3))] = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+            // through shared memory (16-byte pieces of row x swapped by x / 4, free of bank conflicts both ways), so
+            // that two lanes write 32 contiguous bytes of a row and an instruction covers 16 rows and not 32
+            uint4* b = s.stage[quarter];
+            b[lane * 2 + ((lane >> 2) & 1)] = w[0];
+            b[lane * 2 + (((lane >> 2) & 1) ^ 1)] = w[1];
             __syncwarp();
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const int x = q * 8 + (lane >> 2), d = (lane & 3) * 8 + h * 32;
-              const uint4 y = st[x * 4 + ((lane & 3) ^ ((x >> 1) & 3))];
-              if (row0 + x < it.len && d < a.D) *reinterpret_cast<uint4*>(dst + x * a.so.row + d) = y;
+            for (int q = 0; q < 2; ++q) {
+              const int x = q * 16 + (lane >> 1), d = (lane & 1) * 8 + h * 16;
+              const uint4 y = b[x * 2 + ((lane & 1) ^ ((x >> 2) & 1))];
+              if (row0 + x < len && d < a.D) *reinterpret_cast<uint4*>(dst + x * a.so.row + d) = y;
             }
             __syncwarp();
-          } else if (row0 + lane < it.len) {
-            store32(dst + lane * a.so.row + h * 32, w, a.D - h * 32, false);
+          } else if (row0 + lane < len) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (h * 16 + e < a.D) dst[lane * a.so.row + h * 16 + e] = (uint16_t)(reinterpret_cast<uint32_t*>(w)[e / 2] >> (16 * (e & 1)));
           }
         }
-        tc_fence_before();
       }
+      tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&s.item_empty[r]);
+      if (lane == 0) {
+        mbar_arrive(&s.o_free);
+        mbar_arrive(&s.item_empty[r]);
+      }
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 5) {
+  if (warp == 9) {
     tc_fence_after();
     tmem_dealloc(tmem, 256);
   }
@@ -587,12 +654,14 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
   BwdSmem& s = *reinterpret_cast<BwdSmem*>(raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.H / a.Hk;
   if (threadIdx.x == 0) {
+#pragma unroll 1
     for (int i = 0; i < kRing; ++i) {
       mbar_init(&s.item_full[i], 1);
       mbar_init(&s.item_empty[i], 4 * kGroups + 7);
       mbar_init(&s.a_full[i], 1);
       mbar_init(&s.acc_full[i], 1);
     }
+#pragma unroll 1
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&s.b_full[i], 1);
       mbar_init(&s.b_empty[i], 1);
@@ -647,6 +716,7 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
         }
         int row = 0, h = keys ? it.head * group : kh;
         bool ok = true;
+#pragma unroll 1
         for (int i = 0; i < it.n; ++i, ++t) {
           const int st = t % kStages;
           ok = t < kStages || mbar_wait_soon(&s.b_empty[st], ((t / kStages) & 1) ^ 1, 212);
@@ -674,12 +744,14 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
     const bool dp = warp == 18;
     const uint32_t base = DT == ATLAS_BF16 ? idesc_bf16_f32(BM, 0) : idesc_f16_f32(BM, 0);
     bool ok = true;
+#pragma unroll 1
     for (int k = 0, t = 0; ok; ++k) {
       const int r = k % kRing;
       if (!mbar_wait_soon(&s.item_full[r], (k / kRing) & 1, 213)) break;
       const int n = s.item[r].n, len = s.item[r].len, keys = s.item[r].keys;
       if (!n || !mbar_wait_soon(&s.a_full[r], (k / kRing) & 1, 214)) break;
       const uint32_t ar = desc_lo(smem_u32(dp ? s.a1[r] : s.a0[r]));
+#pragma unroll 1
       for (int i = 0, row = 0; i < n; ++i, ++t) {
         const int x = t % 3, st = t % kStages, cols = min(BN, len - row), c16 = up16(cols);
         uint8_t* tile = dp ? s.b1[st] : s.b0[st];
@@ -708,11 +780,13 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
   } else if (warp == 19) {
     const uint32_t base = DT == ATLAS_BF16 ? idesc_bf16_f32(BM, 64) : idesc_f16_f32(BM, 64), id = base | kMnB;
     bool ok = true;
+#pragma unroll 1
     for (int k = 0, t = 0; ok; ++k) {
       const int r = k % kRing;
       if (!mbar_wait_soon(&s.item_full[r], (k / kRing) & 1, 224)) break;
       const int n = s.item[r].n, len = s.item[r].len, keys = s.item[r].keys;
       if (!n || (k && !mbar_wait_soon(&s.acc_free, (k - 1) & 1, 217))) break;
+#pragma unroll 1
       for (int i = 0, row = 0; i < n; ++i, ++t) {
         const int x = t % 3, st = t % kStages, cols = min(BN, len - row);
         ok = mbar_wait_soon(&s.p_full[x], (t / 3) & 1, 218);
@@ -741,6 +815,7 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
   } else if (warp >= 4 * kGroups) {
     const int quarter = warp & 3;
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+#pragma unroll 1
     for (int k = 0;; ++k) {
       const int r = k % kRing;
       if (!mbar_wait_soon(&s.item_full[r], (k / kRing) & 1, 225)) break;
@@ -782,6 +857,7 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
     const float c = a.scale * kLog2e;
     bool ok = true;
+#pragma unroll 1
     for (int k = 0, t = 0; ok; ++k) {
       const int r = k % kRing;
       ok = mbar_wait_soon(&s.item_full[r], (k / kRing) & 1, 219);
@@ -798,6 +874,7 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
         delta = s.a_delta[r][own];
       }
       int left = it.len;  // columns from here to the end of the head
+#pragma unroll 1
       for (int i = 0; i < it.n; ++i, ++t, left -= BN) {
         if (left <= 0) left = it.len;
         if (t % kGroups != g) continue;

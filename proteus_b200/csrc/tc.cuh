@@ -51,6 +51,7 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 
 // Bounded wait on a phase parity: false (and the status word set to `code`) if it never completes.
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int code) {
+#pragma unroll 1
   for (uint32_t i = 0; i < kWaitLimit; ++i)
     if (mbar_try_wait(bar, parity)) return true;
   atomicCAS(&g_device_status, 0, code);
@@ -76,6 +77,7 @@ __device__ __forceinline__ bool mbar_wait_soon(uint64_t* bar, uint32_t parity, i
   return mbar_test(bar, parity) || mbar_wait(bar, parity, code);
 }
 __device__ __forceinline__ bool mbar_spin(uint64_t* bar, uint32_t parity, int code) {
+#pragma unroll 1
   for (uint32_t i = 0; i < kWaitLimit; ++i)
     if (mbar_test(bar, parity)) return true;
   atomicCAS(&g_device_status, 0, code);
