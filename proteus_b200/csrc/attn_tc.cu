@@ -81,18 +81,14 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return r;
 }
 
-// Up to 32 packed 16-bit elements of a row, of which `n` (or more, or none) exist; `vec`: 16-byte stores
-// are aligned and n a multiple of 8.
-__device__ __forceinline__ void store32(uint16_t* dst, const uint32_t (&w)[16], int n, bool vec) {
-  if (vec) {
+// Packed 16-bit elements of a row, of which `n` (or more, or none) exist, where 16-byte stores do not fit.
+struct Packed16 {
+  uint32_t w[8];
+};
+__device__ __noinline__ void store16_single(uint16_t* dst, Packed16 v, int n) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if (q * 8 < n) *reinterpret_cast<uint4*>(dst + q * 8) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 32; ++e)
-      if (e < n) dst[e] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
-  }
+  for (int e = 0; e < 16; ++e)
+    if (e < n) dst[e] = (uint16_t)(v.w[e / 2] >> (16 * (e & 1)));
 }
 
 // Zero the rows [from, to) of a tile of 128-byte rows, by the 32 lanes of a warp, and make the tensor
@@ -485,21 +481,20 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
         uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + outer * a.so.outer + head * a.so.head + to * a.so.row;
         if (row0 + lane < len)
           a.lse[(outer * a.H + head) * a.rows + to + lane] = ((st.y == kNegInf ? 0.f : st.y) + log2f(st.x)) * kLn2;
-#pragma unroll
+#pragma unroll 1
         for (int h = 0; h < 4; ++h) {
           uint32_t o[16];
-          uint4 w[2];
+          Packed16 w;
           tmem_ld16(lanes + 192 + h * 16, o);
           tmem_ld_wait();
 #pragma unroll
-          for (int d = 0; d < 8; ++d)
-            reinterpret_cast<uint32_t*>(w)[d] = pack2<DT>(__uint_as_float(o[2 * d]) * inv, __uint_as_float(o[2 * d + 1]) * inv);
+          for (int d = 0; d < 8; ++d) w.w[d] = pack2<DT>(__uint_as_float(o[2 * d]) * inv, __uint_as_float(o[2 * d + 1]) * inv);
           if (vec) {
             // through shared memory (16-byte pieces of row x swapped by x / 4, free of bank conflicts both ways), so
             // that two lanes write 32 contiguous bytes of a row and an instruction covers 16 rows and not 32
             uint4* b = s.stage[quarter];
-            b[lane * 2 + ((lane >> 2) & 1)] = w[0];
-            b[lane * 2 + (((lane >> 2) & 1) ^ 1)] = w[1];
+            b[lane * 2 + ((lane >> 2) & 1)] = make_uint4(w.w[0], w.w[1], w.w[2], w.w[3]);
+            b[lane * 2 + (((lane >> 2) & 1) ^ 1)] = make_uint4(w.w[4], w.w[5], w.w[6], w.w[7]);
             __syncwarp();
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
@@ -509,9 +504,7 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
             }
             __syncwarp();
           } else if (row0 + lane < len) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if (h * 16 + e < a.D) dst[lane * a.so.row + h * 16 + e] = (uint16_t)(reinterpret_cast<uint32_t*>(w)[e / 2] >> (16 * (e & 1)));
+            store16_single(dst + lane * a.so.row + h * 16, w, a.D - h * 16);
           }
         }
       }
@@ -827,22 +820,32 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
         const bool keys = it.keys;
         float mul = a.scale;
         if (DT == ATLAS_F16) mul /= gain_of(__ldg(a.amax + (int64_t)it.seq * a.Hk + (keys ? it.head : it.head / group)));
+#pragma unroll 1
+        for (int h = keys ? 0 : 2; h < 4; ++h) {  // dv (keys), then dk or dq, 32 columns at a time
+          uint32_t v[32];
+          tmem_ld32(lanes + 384 + h * 32, v);
+          tmem_ld_wait();
+          const float f = h < 2 ? 1.f : mul;
+          const Strides& so = h < 2 ? a.sdv : keys ? a.sdk : a.sdq;
+          uint16_t* dst = reinterpret_cast<uint16_t*>(h < 2 ? a.dv : keys ? a.dk : a.dq) + it.outer * so.outer +
+                          it.head * so.head + ((int64_t)it.row0 + row) * so.row;
 #pragma unroll
-        for (int h = 0; h < 4; ++h)
-          if (keys || h >= 2) {  // dv (keys), then dk or dq
-            uint32_t v[32], w[16];
-            tmem_ld32(lanes + 384 + h * 32, v);
-            tmem_ld_wait();
-            const float f = h < 2 ? 1.f : mul;
+          for (int e = 0; e < 2; ++e) {
+            Packed16 w;
+            const int col = (h & 1) * 32 + e * 16;
 #pragma unroll
-            for (int d = 0; d < 16; ++d) w[d] = pack2<DT>(__uint_as_float(v[2 * d]) * f, __uint_as_float(v[2 * d + 1]) * f);
-            if (row < it.len) {
-              const Strides& so = h < 2 ? a.sdv : keys ? a.sdk : a.sdq;
-              uint16_t* dst = reinterpret_cast<uint16_t*>(h < 2 ? a.dv : keys ? a.dk : a.dq) + it.outer * so.outer +
-                              it.head * so.head + ((int64_t)it.row0 + row) * so.row + (h & 1) * 32;
-              store32(dst, w, a.D - (h & 1) * 32, vec);
+            for (int d = 0; d < 8; ++d)
+              w.w[d] = pack2<DT>(__uint_as_float(v[e * 16 + 2 * d]) * f, __uint_as_float(v[e * 16 + 2 * d + 1]) * f);
+            if (row < it.len && col < a.D) {
+              if (vec) {
+                *reinterpret_cast<uint4*>(dst + col) = make_uint4(w.w[0], w.w[1], w.w[2], w.w[3]);
+                if (col + 8 < a.D) *reinterpret_cast<uint4*>(dst + col + 8) = make_uint4(w.w[4], w.w[5], w.w[6], w.w[7]);
+              } else {
+                store16_single(dst + col, w, a.D - col);
+              }
             }
           }
+        }
       }
       tc_fence_before();
       __syncwarp();

@@ -49,13 +49,18 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
   return ok != 0;
 }
 
+// Out of line: a wait is in many places of a kernel, and none of them should carry this along.
+static __device__ __noinline__ bool gave_up(int code) {
+  atomicCAS(&g_device_status, 0, code);
+  return false;
+}
+
 // Bounded wait on a phase parity: false (and the status word set to `code`) if it never completes.
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int code) {
 #pragma unroll 1
   for (uint32_t i = 0; i < kWaitLimit; ++i)
     if (mbar_try_wait(bar, parity)) return true;
-  atomicCAS(&g_device_status, 0, code);
-  return false;
+  return gave_up(code);
 }
 
 __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
@@ -80,8 +85,7 @@ __device__ __forceinline__ bool mbar_spin(uint64_t* bar, uint32_t parity, int co
 #pragma unroll 1
   for (uint32_t i = 0; i < kWaitLimit; ++i)
     if (mbar_test(bar, parity)) return true;
-  atomicCAS(&g_device_status, 0, code);
-  return false;
+  return gave_up(code);
 }
 
 // 2-D TMA tile load into shared memory, completion counted on `bar`; each CTA loads its own copy.
