@@ -367,36 +367,49 @@ __global__ void __launch_bounds__(kThreads) attn_delta_kernel(const AttnArgs a) 
   const T* o = reinterpret_cast<const T*>(a.o) + s.outer * a.so.outer + head * a.so.head + s.row0 * a.so.row;
   const T* g = reinterpret_cast<const T*>(a.dout) + s.outer * a.sdo.outer + head * a.sdo.head + s.row0 * a.sdo.row;
   float amax = 0.f;
-#pragma unroll 4
-  for (int k = 0; k < kAttnBlock / PER; ++k) {
-    const int r = s.first + k * PER + (int)threadIdx.x / G;
-    float v = 0.f;
-    if (r < s.len)
-      for (int d = sub * E; d < a.D; d += G * E) {
-        T x[E], y[E];
-        if (VEC) {
-          *reinterpret_cast<uint4*>(x) = __ldg(reinterpret_cast<const uint4*>(o + (int64_t)r * a.so.row + d));
-          *reinterpret_cast<uint4*>(y) = __ldg(reinterpret_cast<const uint4*>(g + (int64_t)r * a.sdo.row + d));
-        } else {
-          x[0] = o[(int64_t)r * a.so.row + d];
-          y[0] = g[(int64_t)r * a.sdo.row + d];
-        }
+  auto product = [&](T x, T y, float v) {
+    const float w = Elem<DT>::f(y);
+    if (DT == ATLAS_F16) amax = fabsf(w) > amax || w != w ? fabsf(w) : amax;
+    return fmaf(Elem<DT>::f(x), w, v);
+  };
+  constexpr int U = VEC ? 4 : 1;  // rows of a thread whose loads are under way at once
+#pragma unroll 1
+  for (int k0 = 0; k0 < kAttnBlock / PER; k0 += U) {
+    const int r0 = s.first + k0 * PER + (int)threadIdx.x / G;
+    float v[U], lse[U];
+    uint4 x[U], y[U];
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const float w = Elem<DT>::f(y[e]);
-          v = fmaf(Elem<DT>::f(x[e]), w, v);
-          if (DT == ATLAS_F16) amax = fabsf(w) > amax || w != w ? fabsf(w) : amax;
+    for (int u = 0; u < U; ++u) {
+      const int r = r0 + u * PER;
+      const bool on = r < s.len;
+      v[u] = lse[u] = 0.f;
+      if (VEC) {
+        x[u] = y[u] = make_uint4(0, 0, 0, 0);
+        if (on && sub * E < a.D) {
+          x[u] = __ldg(reinterpret_cast<const uint4*>(o + (int64_t)r * a.so.row + sub * E));
+          y[u] = __ldg(reinterpret_cast<const uint4*>(g + (int64_t)r * a.sdo.row + sub * E));
         }
+      } else if (on) {
+        for (int d = sub; d < a.D; d += G) v[u] = product(o[(int64_t)r * a.so.row + d], g[(int64_t)r * a.sdo.row + d], v[u]);
+      }
+      if (a.lse2 && sub == 0 && on) lse[u] = a.lse[(s.outer * a.H + head) * a.rows + s.row0 + r];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = r0 + u * PER;
+      if (VEC) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[u] = product(reinterpret_cast<const T*>(&x[u])[e], reinterpret_cast<const T*>(&y[u])[e], v[u]);
       }
 #pragma unroll
-    for (int m = G / 2; m; m >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, m);
-    if (sub == 0 && r < s.len) {
-      const int64_t at = (s.outer * a.H + head) * a.rows + s.row0 + r;
-      if (a.lse2) {
-        a.lse2[head * a.vec_ld + s.off + r] = a.lse[at] * -1.4426950408889634f;
-        a.delta2[head * a.vec_ld + s.off + r] = -v;
-      } else {
-        a.delta[at] = v;
+      for (int m = G / 2; m; m >>= 1) v[u] += __shfl_xor_sync(0xFFFFFFFFu, v[u], m);
+      if (sub == 0 && r < s.len) {
+        if (a.lse2) {
+          a.lse2[head * a.vec_ld + s.off + r] = lse[u] * -1.4426950408889634f;
+          a.delta2[head * a.vec_ld + s.off + r] = -v[u];
+        } else {
+          a.delta[(s.outer * a.H + head) * a.rows + s.row0 + r] = v[u];
+        }
       }
     }
   }
