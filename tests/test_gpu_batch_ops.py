@@ -213,6 +213,25 @@ def test_attention_and_gradient(lens, packed, dtype, D, H, Hk):
     assert (lse.transpose(1, 2)[off] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,H,Hk", [(8, 4, 2), (64, 2, 2), (13, 3, 1)])
+@pytest.mark.parametrize("L", [2, 3, 4, 9, 16])
+def test_attention_gradient_over_few_keys(L, D, H, Hk, dtype):
+    """Over few keys dP and delta nearly cancel, so that delta has to be better than the rounded output
+    makes it. What is left is the rounding of dS and that of the result, each off by at most half a step h
+    of every element, uniformly within it: h / sqrt(3) of the norm each at most, and sqrt(2 / 3) h together,
+    since they are independent. The limit is h; delta from the output passes it at 2, 3 and 4 keys (1.4 h,
+    1.2 h, 1.1 h in bf16)."""
+    KN = _kn()
+    q, k, v, do, plan, where, _ = _batch([L] * 150, True, H, Hk, D, dtype, seed=L)
+    ref, _ = _plain(q, k, v, do, where, D ** -0.5)
+    out, lse = KN.attention(q, k, v, plan)
+    h = torch.finfo(dtype).eps / 2
+    for name, t in zip(("dq", "dk", "dv"), KN.attention_grad(do, q, k, v, out, lse, plan)):
+        err = (t.double() - ref[name]).norm() / ref[name].norm()
+        assert err <= h, (name, (err / h).item())
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 def test_attention_scale_and_sharp_scores(dtype):
     """A given scale, and scores up to several hundred: one probability near 1, the others vanish."""
@@ -223,6 +242,45 @@ def test_attention_scale_and_sharp_scores(dtype):
         out, lse = KN.attention(q, k, v, plan, scale)
         dq, dk, dv = KN.attention_grad(do, q, k, v, out, lse, plan, scale)
         _check({"out": out, "lse": lse, "dq": dq, "dk": dk, "dv": dv}, ref, tol)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_attention_scores_rising_along_the_keys(dtype):
+    """Each 16 keys' scores stand 8 above the 16 before, from -200 to 190 over 800 keys: every reference that
+    the exponents had is left behind by more than any of the types has room for."""
+    KN = _kn()
+    q, k, v, do, plan, where, _ = _batch([800, 40, 161], True, 2, 1, 16, dtype, seed=5)
+    for o, r in where:
+        n = r.stop - r.start
+        q[o, :, r, 0] = 1.0
+        k[o, :, r, 0] = (torch.arange(n, device=DEV).div(16, rounding_mode="floor") * 8 - n / 4).to(dtype)
+    ref, tol = _plain(q, k, v, do, where, 1.0)
+    # Weights below fp32's normal range are taken as zero, off by up to 2^-126 each. With |dP - delta| < 2^6,
+    # |q| < 2^3, |k| < 2^8 and 1600 < 2^11 terms a sum is off by less than 2^-126 2^6 2^8 2^11 = 2^-101.
+    for name in ("out", "dq", "dk", "dv"):
+        tol[name] += 2.0 ** -101
+    out, lse = KN.attention(q, k, v, plan, 1.0)
+    dq, dk, dv = KN.attention_grad(do, q, k, v, out, lse, plan, 1.0)
+    _check({"out": out, "lse": lse, "dq": dq, "dk": dk, "dv": dv}, ref, tol)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("first", [1, 31, 32, 33, 64, 96, 130])
+def test_attention_first_scores_of_minus_infinity(first, dtype):
+    """Keys whose scores are -inf weigh nothing: the result is that of the other keys alone."""
+    KN = _kn()
+    q, k, v, do, plan, where, _ = _batch([200], True, 2, 2, 24, dtype, seed=6)
+    q[..., 0] = q[..., 0].abs() + 0.5
+    kk, vv = k[:, :, first:].contiguous(), v[:, :, first:].contiguous()
+    k[:, :, :first, 0] = float("-inf")
+    out, lse = KN.attention(q, k, v, plan)
+    s = q.double() @ kk.double().transpose(2, 3) * 24 ** -0.5
+    want = torch.softmax(s, -1) @ vv.double()
+    h = _half(dtype) if dtype != torch.float32 else U
+    # of P and of the result h each; scores off by some 30 roundings of fp32 at 10 or so
+    tol = 2 * h * (torch.softmax(s, -1) @ vv.double().abs()) + 2.0 ** -12 * h + 600 * U
+    assert ((out.double() - want).abs() <= tol).all()
+    assert (lse.double() - torch.logsumexp(s, -1)).abs().max() <= 600 * U
 
 
 @pytest.mark.parametrize("size", [2.0 ** -12, 1.0, 2.0 ** 5, 2.0 ** 9])
