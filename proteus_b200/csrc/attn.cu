@@ -18,7 +18,8 @@ int check(const AttnArgs& a, int dtype, const char* what) {
   ATLAS_REQUIRE(a.packed ? a.outer == 1 : a.outer == a.B, "%s: outer must be %s", what, a.packed ? "1" : "the batch");
   ATLAS_REQUIRE(a.H >= 1 && a.H <= 65535 && a.Hk >= 1 && a.H % a.Hk == 0, "%s: heads must be a multiple of the key heads", what);
   ATLAS_REQUIRE(a.D >= 1 && a.D <= kAttnMaxDim, "%s: head dimension must be in [1, %d]", what, kAttnMaxDim);
-  ATLAS_REQUIRE(a.cap >= 1 && a.cap <= (1LL << 29), "%s: bad block table", what);
+  ATLAS_REQUIRE(a.cap >= a.outer * a.rows / kAttnBlock + a.B + 1 && a.cap <= (1LL << 29),
+                "%s: the block table has too few or too many entries", what);
   ATLAS_REQUIRE(a.q && a.k && a.v && a.lse && a.cu && a.blocks && a.counts, "%s: null pointer", what);
   ATLAS_REQUIRE((uintptr_t)a.blocks % 8 == 0, "%s: the block table must be 8-byte aligned", what);
   return ATLAS_OK;

@@ -7,6 +7,7 @@ namespace atlas {
 
 constexpr int kAttnBlock = 128;  // rows of an entry of the block table
 constexpr int kAttnMaxDim = 64;
+constexpr int kAttnShort = 16;   // sequences whose gradient attn_delta_kernel makes whole
 
 struct Strides {
   int64_t outer, head, row;  // in elements; the last axis has unit stride
@@ -63,25 +64,56 @@ __device__ __forceinline__ SeqBlock seq_block(const AttnArgs& a, int64_t i) {
   return s;
 }
 
-// Rows of no sequence that this block's CTA sets to zero: behind a padded sequence's end (its last
-// block's), and behind the last sequence of a packed batch (shared out over the spare entries; the
-// table always has one).
-__device__ __forceinline__ bool idle_rows(const AttnArgs& a, const SeqBlock& s, int64_t i, int64_t* from, int64_t* to) {
-  if (a.packed) {
-    if (!s.spare) return false;
-    const int64_t n = a.counts[1], parts = a.cap - n, part = i - n;
-    int64_t end = a.cu[a.B];
-    if (end < 0) end = 0;
-    const int64_t left = a.rows - end;
-    if (left <= 0) return false;
-    *from = end + left * part / parts;
-    *to = end + left * (part + 1) / parts;
-    return *to > *from;
+// The rows of no sequence - behind a padded sequence's end, or behind the last sequence of a packed batch -
+// in order, shared out evenly over the spare entries of the table. The table has rows / 128 + B + 1 entries
+// and a sequence takes at most len / 128 + 1 of them, so that a share is 128 rows or less. (Given to a
+// sequence's own last entry, a batch of lengths 505 to 4040 spent 540 us in four CTAs that set thousands
+// of rows to zero.) Spare entry i, by warp `warp` of `warps`: each lane looks up a row of its own, lane(outer,
+// row) is called once for it by that lane, and row(outer, row, sub) by 8 lanes, sub 0-7.
+template <typename Lane, typename Row>
+__device__ __forceinline__ void idle_rows(const AttnArgs& a, int64_t i, int warp, int warps, int lane, Lane each, Row eight) {
+  const int64_t n = a.counts[1], parts = a.cap - n, part = i - n;
+  const int64_t all = a.packed ? a.rows : a.outer * a.rows, used = a.cu[a.B];
+  const int64_t left = all - (used < 0 ? 0 : used);
+  if (left <= 0 || n < 0) return;
+  const int64_t end = left * (part + 1) / parts;
+#pragma unroll 1
+  for (int64_t g0 = left * part / parts + 32 * warp; g0 < end; g0 += 32 * warps) {
+    const int64_t g = g0 + lane;
+    int64_t b = 0, r = all - left + g;
+    bool on = g < end;
+    if (!a.packed) {  // before sequence b lie b * rows - cu[b] of them
+#pragma unroll 1
+      for (int64_t hi = a.B; hi - b > 1;) {
+        const int64_t mid = (b + hi) >> 1;
+        if (mid * a.rows - a.cu[mid] <= g) b = mid;
+        else hi = mid;
+      }
+      r = g - b * a.rows + a.cu[b + 1];
+      on = on && r >= 0 && r < a.rows;
+    }
+    if (on) each(b, r);
+#pragma unroll 1
+    for (int j = lane >> 3; j < 32; j += 4) {
+      const int64_t bj = __shfl_sync(0xFFFFFFFFu, b, j), rj = __shfl_sync(0xFFFFFFFFu, r, j);
+      if (__shfl_sync(0xFFFFFFFFu, (int)on, j)) eight(bj, rj, lane & 7);
+    }
   }
-  if (!s.on || s.first + kAttnBlock < s.len) return false;
-  *from = s.len;
-  *to = a.rows;
-  return *to > *from;
+}
+
+// One row of a head set to zero by 8 lanes, 16 bytes at a time where it allows it.
+__device__ __forceinline__ void zero_row(void* dst, const Strides& st, int size, int64_t outer, int head, int64_t row, int D, int sub) {
+  char* p = reinterpret_cast<char*>(dst) + (outer * st.outer + head * st.head + row * st.row) * size;
+  const int bytes = D * size;
+  if ((((uintptr_t)p | (uintptr_t)bytes) & 15) == 0) {
+    for (int d = sub * 16; d < bytes; d += 128) *reinterpret_cast<uint4*>(p + d) = make_uint4(0, 0, 0, 0);
+  } else {
+#pragma unroll 1
+    for (int d = sub * size; d < bytes; d += 8 * size) {
+      if (size == 4) *reinterpret_cast<uint32_t*>(p + d) = 0;
+      else *reinterpret_cast<uint16_t*>(p + d) = 0;
+    }
+  }
 }
 
 // Sets a kernel's dynamic shared memory once per device (each launch of a short sequence would otherwise pay

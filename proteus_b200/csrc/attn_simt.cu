@@ -82,7 +82,7 @@ __device__ __forceinline__ void mm_rows(const float* a, const float* b, int ty, 
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) c[i][j] = 0.f;
-#pragma unroll 4
+#pragma unroll 2
   for (int d = 0; d < DP; d += 4) {
     float4 x[4], y[4];
 #pragma unroll
@@ -106,7 +106,7 @@ __device__ __forceinline__ void mm_rows(const float* a, const float* b, int ty, 
 template <int DP>
 __device__ __forceinline__ void mm_cols(const float* p, const float* v, int ty, int tx, float (&acc)[4][DP / 16]) {
   constexpr int C = DP / 16;
-#pragma unroll 4
+#pragma unroll 2
   for (int n = 0; n < BT; n += 4) {
     float4 x[4];
 #pragma unroll
@@ -137,14 +137,6 @@ __device__ __forceinline__ float row_sum(float v) {
   return v;
 }
 
-template <int DT>
-__device__ __forceinline__ void zero_rows(void* dst, const Strides& st, int64_t outer, int head, int64_t from, int64_t to, int D) {
-  using T = typename Elem<DT>::T;
-  T* p = reinterpret_cast<T*>(dst) + outer * st.outer + head * st.head;
-  for (int64_t r = from + threadIdx.x / 16; r < to; r += kThreads / 16)
-    for (int d = threadIdx.x % 16; d < D; d += 16) put<DT>(p + r * st.row + d, 0.f);
-}
-
 template <int DT, int DP>
 __device__ __forceinline__ void store_tile(void* dst, const Strides& st, int64_t outer, int head, int64_t row0, int first, int len,
                                            int D, int ty, int tx, const float (&acc)[4][DP / 16], const float (&mul)[4]) {
@@ -170,12 +162,10 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 2 : 3) attn_fwd_simt_kern
   const int head = blockIdx.y, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int64_t bi = blockIdx.x >> 1;
   const SeqBlock s = seq_block(a, bi);
-  int64_t z0, z1;
-  if (!(blockIdx.x & 1) && idle_rows(a, s, bi, &z0, &z1)) {
-    zero_rows<DT>(a.out, a.so, s.outer, head, z0, z1, a.D);
-    float* l = a.lse + (s.outer * a.H + head) * a.rows;
-    for (int64_t r = z0 + threadIdx.x; r < z1; r += kThreads) l[r] = 0.f;
-  }
+  if (s.spare && !(blockIdx.x & 1))
+    idle_rows(a, bi, threadIdx.x / 32, kThreads / 32, threadIdx.x % 32,
+              [&](int64_t o, int64_t r) { a.lse[(o * a.H + head) * a.rows + r] = 0.f; },
+              [&](int64_t o, int64_t r, int sub) { zero_row(a.out, a.so, sizeof(typename Elem<DT>::T), o, head, r, a.D, sub); });
   const int first = s.first + (blockIdx.x & 1) * BT;
   if (!s.on || first >= s.len) return;
   const int kh = head / (a.H / a.Hk);
@@ -270,17 +260,15 @@ __global__ void __launch_bounds__(kThreads, 2) attn_bwd_simt_kernel(const AttnAr
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, group = a.H / a.Hk;
   const int64_t bi = blockIdx.x >> 1;
   const SeqBlock s = seq_block(a, bi);
-  int64_t z0, z1;
-  if (!(blockIdx.x & 1) && idle_rows(a, s, bi, &z0, &z1)) {
-    if (KEYS) {
-      zero_rows<DT>(a.dk, a.sdk, s.outer, blockIdx.y, z0, z1, a.D);
-      zero_rows<DT>(a.dv, a.sdv, s.outer, blockIdx.y, z0, z1, a.D);
-    } else {
-      zero_rows<DT>(a.dq, a.sdq, s.outer, blockIdx.y, z0, z1, a.D);
-    }
-  }
+  if (s.spare && !(blockIdx.x & 1))
+    idle_rows(a, bi, threadIdx.x / 32, kThreads / 32, threadIdx.x % 32, [](int64_t, int64_t) {},
+              [&](int64_t o, int64_t r, int sub) {
+                constexpr int size = sizeof(typename Elem<DT>::T);
+                zero_row(KEYS ? a.dk : a.dq, KEYS ? a.sdk : a.sdq, size, o, blockIdx.y, r, a.D, sub);
+                if (KEYS) zero_row(a.dv, a.sdv, size, o, blockIdx.y, r, a.D, sub);
+              });
   const int first = s.first + (blockIdx.x & 1) * BT;
-  if (!s.on || first >= s.len) return;
+  if (!s.on || first >= s.len || s.len <= kAttnShort) return;
   const int kh = KEYS ? blockIdx.y : blockIdx.y / group;
   // the queries' scores in base 2: the factor goes to the tile of queries or keys that stays
   Tile<DT, DP> ta, tb;
@@ -341,37 +329,126 @@ __global__ void __launch_bounds__(kThreads, 2) attn_bwd_simt_kernel(const AttnAr
   }
 }
 
-// delta = sum_d dout out of the rows of a block and head, G lanes to a row: 8 lanes with 16-byte loads
-// where rows are aligned for them (VEC), else a warp. For the tensor-core kernels also what they need
-// beside it (see AttnArgs); the largest |dout| as bits, so that the order of the atomics does not matter.
-//
-// The rounding of a 16-bit out reaches dS = P (dP - delta) through delta. Over few keys dP and delta lie close
-// together, and it is the gradients' largest error: bf16, D = 8, relative norm of dq 5.4e-3 at 2 keys, 4.3e-3
-// at 4, 3.6e-3 from 10 to 24, where the roundings of dS and of the result alone make 2.5e-3. Sequences of up
-// to kExactKeys take delta = sum_j P_j (dout v_j) from the keys themselves; its work grows with len^2, and
-// past 16 keys the error that it saves no longer falls.
-constexpr int kExactKeys = 16;
+// The gradient of a sequence of up to kAttnShort rows and one key head: thread (r, c) makes the score of
+// query r and key c, then 4 columns of row r of dq, dk and dv. Tiles of 64 and 128 rows would be empty for the
+// most part: 288 pairs of rows with 10 heads took 90 us in the tensor-core kernel's items, 3 us each. Over few keys
+// dP and delta lie close together as well, and the rounding of a 16-bit out would be the gradients' largest
+// error (bf16, D = 8, relative norm of dq 5.4e-3 at 2 keys, 4.3e-3 at 4, 3.6e-3 at 16; the rounding of the
+// result alone is 1.7e-3): here delta is sum_j P_j dP_j, and dS stays in 32 bits.
+struct ShortSmem {
+  float k[kAttnShort][68], v[kAttnShort][68], q[kAttnShort][68], g[kAttnShort][68], p[kAttnShort][20], ds[kAttnShort][20];
+};
 
+template <int DT, bool VEC>
+__device__ __forceinline__ void short_grad(const AttnArgs& a, const SeqBlock& b, int kh, ShortSmem& s) {
+  using T = typename Elem<DT>::T;
+  static_assert(kThreads == kAttnShort * kAttnShort && kAttnMaxDim == 4 * kAttnShort, "a thread per pair of rows");
+  const int r = threadIdx.x / kAttnShort, c = threadIdx.x % kAttnShort, len = b.len, group = a.H / a.Hk;
+  auto load = [&](const void* src, const Strides& st, int head, float (&dst)[kAttnShort][68]) {
+    const T* p = reinterpret_cast<const T*>(src) + b.outer * st.outer + head * st.head + (b.row0 + r) * st.row + 4 * c;
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    if (r < len) {
+      if (VEC) {  // D is a multiple of 4
+        if (4 * c < a.D) {
+          T w[4];
+          if (sizeof(T) == 4) *reinterpret_cast<uint4*>(w) = __ldg(reinterpret_cast<const uint4*>(p));
+          else *reinterpret_cast<uint2*>(w) = __ldg(reinterpret_cast<const uint2*>(p));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = Elem<DT>::f(w[e]);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (4 * c + e < a.D) x[e] = Elem<DT>::f(p[e]);
+      }
+    }
+    *reinterpret_cast<float4*>(&dst[r][4 * c]) = make_float4(x[0], x[1], x[2], x[3]);
+  };
+  auto add = [](float4& acc, float w, const float4& x) {
+    acc.x = fmaf(w, x.x, acc.x);
+    acc.y = fmaf(w, x.y, acc.y);
+    acc.z = fmaf(w, x.z, acc.z);
+    acc.w = fmaf(w, x.w, acc.w);
+  };
+  auto store = [&](void* dst, const Strides& st, int head, const float4& x, float f) {
+    T* p = reinterpret_cast<T*>(dst) + b.outer * st.outer + head * st.head + (b.row0 + r) * st.row + 4 * c;
+    const float w[4] = {x.x * f, x.y * f, x.z * f, x.w * f};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (r < len && 4 * c + e < a.D) put<DT>(p + e, w[e]);
+  };
+  load(a.k, a.sk, kh, s.k);
+  load(a.v, a.sv, kh, s.v);
+  float4 dk = make_float4(0.f, 0.f, 0.f, 0.f), dv = dk;
+#pragma unroll 1
+  for (int h = kh * group; h < (kh + 1) * group; ++h) {
+    load(a.q, a.sq, h, s.q);
+    load(a.dout, a.sdo, h, s.g);
+    __syncthreads();
+    const bool on = r < len && c < len;
+    float p = 0.f, dp = 0.f;
+    if (on) {
+      const float lse = a.lse[(b.outer * a.H + h) * a.rows + b.row0 + r];
+      float sc = 0.f;
+#pragma unroll 1
+      for (int d = 0; d < a.D; d += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(&s.q[r][d]), y = *reinterpret_cast<const float4*>(&s.k[c][d]);
+        const float4 g = *reinterpret_cast<const float4*>(&s.g[r][d]), v = *reinterpret_cast<const float4*>(&s.v[c][d]);
+        sc = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, sc))));
+        dp = fmaf(g.x, v.x, fmaf(g.y, v.y, fmaf(g.z, v.z, fmaf(g.w, v.w, dp))));
+      }
+      p = ex2((sc * a.scale - lse) * kLog2e);
+    }
+    float delta = p * dp;
+#pragma unroll
+    for (int m = kAttnShort / 2; m; m >>= 1) delta += __shfl_xor_sync(0xFFFFFFFFu, delta, m);
+    s.p[r][c] = p;
+    s.ds[r][c] = on ? p * (dp - delta) : 0.f;
+    __syncthreads();
+    float4 dq = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (int j = 0; j < len; ++j) {
+      add(dq, s.ds[r][j], *reinterpret_cast<const float4*>(&s.k[j][4 * c]));
+      add(dk, s.ds[j][r], *reinterpret_cast<const float4*>(&s.q[j][4 * c]));
+      add(dv, s.p[j][r], *reinterpret_cast<const float4*>(&s.g[j][4 * c]));
+    }
+    store(a.dq, a.sdq, h, dq, a.scale);
+    __syncthreads();
+  }
+  store(a.dk, a.sdk, kh, dk, a.scale);
+  store(a.dv, a.sdv, kh, dv, 1.f);
+}
+
+// Before the gradient's kernels: delta = sum_d dout out of the rows of a block and head, G lanes to a row: 8
+// lanes with 16-byte loads where rows are aligned for them (VEC), else a warp; and the gradients of short
+// sequences. For the tensor-core kernel also what it needs beside it (see AttnArgs); the largest |dout| as
+// bits, so that the order of the atomics does not matter.
 template <int DT, bool VEC>
 __global__ void __launch_bounds__(kThreads) attn_delta_kernel(const AttnArgs a) {
   using T = typename Elem<DT>::T;
   constexpr int E = VEC ? 16 / sizeof(T) : 1;      // elements per load
   constexpr int G = VEC ? kAttnMaxDim / E : 32;    // lanes per row
   constexpr int PER = kThreads / G;                // rows at a time
+  __shared__ ShortSmem sm;
   const SeqBlock s = seq_block(a, blockIdx.x);
   const int head = blockIdx.y, sub = threadIdx.x % G;
   if (a.lse2) {  // before the tensor-core kernel: its counter, and the rows that it does not write
     if (blockIdx.x == 0 && head == 0 && threadIdx.x == 0) *a.counter = 0;
-    int64_t z0, z1;
-    if (idle_rows(a, s, blockIdx.x, &z0, &z1)) {
-      zero_rows<DT>(a.dq, a.sdq, s.outer, head, z0, z1, a.D);
-      if (head < a.Hk) {
-        zero_rows<DT>(a.dk, a.sdk, s.outer, head, z0, z1, a.D);
-        zero_rows<DT>(a.dv, a.sdv, s.outer, head, z0, z1, a.D);
-      }
-    }
+    if (s.spare)
+      idle_rows(a, blockIdx.x, threadIdx.x / 32, kThreads / 32, threadIdx.x % 32, [](int64_t, int64_t) {},
+                [&](int64_t o, int64_t r, int lane8) {
+                  zero_row(a.dq, a.sdq, sizeof(T), o, head, r, a.D, lane8);
+                  if (head < a.Hk) {
+                    zero_row(a.dk, a.sdk, sizeof(T), o, head, r, a.D, lane8);
+                    zero_row(a.dv, a.sdv, sizeof(T), o, head, r, a.D, lane8);
+                  }
+                });
   }
   if (!s.on) return;
+  if (s.len <= kAttnShort) {
+    if (s.first == 0 && head < a.Hk) short_grad<DT, VEC>(a, s, head, sm);
+    return;
+  }
   const T* o = reinterpret_cast<const T*>(a.o) + s.outer * a.so.outer + head * a.so.head + s.row0 * a.so.row;
   const T* g = reinterpret_cast<const T*>(a.dout) + s.outer * a.sdo.outer + head * a.sdo.head + s.row0 * a.sdo.row;
   float amax = 0.f;
@@ -382,66 +459,9 @@ __global__ void __launch_bounds__(kThreads) attn_delta_kernel(const AttnArgs a) 
   };
   const int64_t vec_at = head * a.vec_ld + s.off;
   const int64_t row_at = (s.outer * a.H + head) * a.rows + s.row0;
-  const bool exact = DT != ATLAS_F32 && s.len <= kExactKeys;
-  if (exact) {
-    constexpr int N = VEC ? E : kAttnMaxDim / G;  // a lane's elements: sub * E + e, or sub + G * e
-    const int kh = head / (a.H / a.Hk);
-    const T* q = reinterpret_cast<const T*>(a.q) + s.outer * a.sq.outer + head * a.sq.head + s.row0 * a.sq.row;
-    const T* k = reinterpret_cast<const T*>(a.k) + s.outer * a.sk.outer + kh * a.sk.head + s.row0 * a.sk.row;
-    const T* v = reinterpret_cast<const T*>(a.v) + s.outer * a.sv.outer + kh * a.sv.head + s.row0 * a.sv.row;
-    auto load = [&](const T* row, float (&x)[N]) {
-      if (VEC) {
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (sub * E < a.D) w = __ldg(reinterpret_cast<const uint4*>(row + sub * E));
-#pragma unroll
-        for (int e = 0; e < N; ++e) x[e] = Elem<DT>::f(reinterpret_cast<const T*>(&w)[e]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < N; ++e) x[e] = sub + G * e < a.D ? Elem<DT>::f(row[sub + G * e]) : 0.f;
-      }
-    };
-    const float c = a.scale * kLog2e;
-#pragma unroll 1
-    for (int r0 = 0; r0 < s.len; r0 += PER) {  // whole warps: the lanes of a row behind the end work on the last
-      const int r = r0 + (int)threadIdx.x / G, at = min(r, s.len - 1);
-      float x[N], y[N], sum = 0.f;
-      load(q + at * a.sq.row, x);
-      load(g + at * a.sdo.row, y);
-      if (DT == ATLAS_F16) {
-#pragma unroll
-        for (int e = 0; e < N; ++e) amax = fabsf(y[e]) > amax || y[e] != y[e] ? fabsf(y[e]) : amax;
-      }
-      const float nlse = a.lse[row_at + at] * -kLog2e;
-#pragma unroll 4
-      for (int j = 0; j < s.len; ++j) {
-        float kj[N], vj[N], sc = 0.f, dp = 0.f;
-        load(k + j * a.sk.row, kj);
-        load(v + j * a.sv.row, vj);
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-          sc = fmaf(x[e], kj[e], sc);
-          dp = fmaf(y[e], vj[e], dp);
-        }
-#pragma unroll
-        for (int m = G / 2; m; m >>= 1) {
-          sc += __shfl_xor_sync(0xFFFFFFFFu, sc, m);
-          dp += __shfl_xor_sync(0xFFFFFFFFu, dp, m);
-        }
-        sum = fmaf(ex2(fmaf(sc, c, nlse)), dp, sum);
-      }
-      if (sub == 0 && r < s.len) {
-        if (a.lse2) {
-          a.lse2[vec_at + r] = nlse;
-          a.delta2[vec_at + r] = -sum;
-        } else {
-          a.delta[row_at + r] = sum;
-        }
-      }
-    }
-  }
   constexpr int U = VEC ? 4 : 1;  // rows of a thread whose loads are under way at once
 #pragma unroll 1
-  for (int k0 = exact ? kAttnBlock / PER : 0; k0 < kAttnBlock / PER; k0 += U) {
+  for (int k0 = 0; k0 < kAttnBlock / PER; k0 += U) {
     const int r0 = s.first + k0 * PER + (int)threadIdx.x / G;
     float v[U], lse[U];
     uint4 x[U], y[U];

@@ -255,16 +255,9 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
       }
       __syncwarp();
       const SeqBlock b = more ? seq_block(a, x) : SeqBlock{};
-      int64_t z0, z1;
-      if (more && idle_rows(a, b, x, &z0, &z1)) {
-        uint16_t* o = reinterpret_cast<uint16_t*>(a.out) + b.outer * a.so.outer + head * a.so.head;
-        float* l = a.lse + (b.outer * a.H + head) * a.rows;
-#pragma unroll 1
-        for (int64_t r = z0; r < z1; ++r)
-          for (int d = lane; d < a.D; d += 32) o[r * a.so.row + d] = 0;
-#pragma unroll 1
-        for (int64_t r = z0 + lane; r < z1; r += 32) l[r] = 0.f;
-      }
+      if (more && b.spare)
+        idle_rows(a, x, 0, 1, lane, [&](int64_t o, int64_t r) { a.lse[(o * a.H + head) * a.rows + r] = 0.f; },
+                  [&](int64_t o, int64_t r, int sub) { zero_row(a.out, a.so, 2, o, head, r, a.D, sub); });
       if (!more || (b.on && b.first < b.len)) {
         const int r = k & 1, n = more ? (b.len + KT - 1) / KT : 0;
         ok = k < 2 || mbar_wait(&s.item_empty[r], ((k >> 1) & 1) ^ 1, 200);
@@ -674,60 +667,89 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
   const uint32_t tmem = s.tmem;
 
   if (warp == 16) {
-    if (elect_one()) {
-      const int total = (int)a.cap * (a.Hk + a.H);
-      int next = (int)atomicAdd(a.counter, 1u), k = 0, t = 0;
-      while (true) {
-        BwdItem it{};
-        while (next < total) {  // keys first: theirs are the longest items
-          const int y = next / (int)a.cap, x = next - y * (int)a.cap;
-          const SeqBlock b = seq_block(a, x);
-          next = (int)atomicAdd(a.counter, 1u);
-          if (!b.on || b.first >= b.len) continue;
-          it.keys = y < a.Hk;
-          it.head = it.keys ? y : y - a.Hk;
-          it.seq = b.seq; it.first = b.first; it.len = b.len; it.row0 = (int)b.row0; it.outer = (int)b.outer; it.off = b.off;
-          it.n = (b.len + BN - 1) / BN * (it.keys ? group : 1);
-          break;
-        }
-        const int r = k % kRing;
-        if (k >= kRing && !mbar_wait_soon(&s.item_empty[r], ((k / kRing) & 1) ^ 1, 211)) break;
-        s.item[r] = it;
-        mbar_arrive(&s.item_full[r]);
-        if (!it.n) break;
-        const bool keys = it.keys;
-        const int kh = it.head / group;
-        const float *lse2 = a.lse2 + it.off, *delta2 = a.delta2 + it.off;
-        mbar_arrive_expect_tx(&s.a_full[r], 2 * kTile + (keys ? 0 : 2 * BM * 4));
-        for (int half = 0; half < 2; ++half) {  // boxes of 64 rows
-          tma_load_4d(s.a0[r] + half * kHalf, keys ? &mk : &mq, 0, it.row0 + it.first + half * BN, it.head, it.outer, &s.a_full[r]);
-          tma_load_4d(s.a1[r] + half * kHalf, keys ? &mv : &mdo, 0, it.row0 + it.first + half * BN, it.head, it.outer, &s.a_full[r]);
-        }
-        if (!keys) {
-          bulk_load(s.a_lse[r], lse2 + it.head * a.vec_ld + it.first, BM * 4, &s.a_full[r]);
-          bulk_load(s.a_delta[r], delta2 + it.head * a.vec_ld + it.first, BM * 4, &s.a_full[r]);
-        }
-        int row = 0, h = keys ? it.head * group : kh;
-        bool ok = true;
+    const int64_t n = a.counts[1];
+    const int blocks = (int)(n < 0 ? 0 : n > a.cap ? a.cap : n), total = blocks * (a.Hk + a.H);
+    int k = 0, t = 0, ask = 1, at = 0;
+    if (lane == 0) at = (int)atomicAdd(a.counter, 1u);
+    bool ok = true;
 #pragma unroll 1
-        for (int i = 0; i < it.n; ++i, ++t) {
-          const int st = t % kStages;
-          ok = t < kStages || mbar_wait_soon(&s.b_empty[st], ((t / kStages) & 1) ^ 1, 212);
-          if (!ok) break;
-          mbar_arrive_expect_tx(&s.b_full[st], 2 * kHalf + (keys ? 2 * BN * 4 : 0));
-          tma_load_4d(s.b0[st], keys ? &mq : &mk, 0, it.row0 + row, h, it.outer, &s.b_full[st]);
-          tma_load_4d(s.b1[st], keys ? &mdo : &mv, 0, it.row0 + row, h, it.outer, &s.b_full[st]);
-          if (keys) {
-            bulk_load(s.b_lse[st], lse2 + h * a.vec_ld + row, BN * 4, &s.b_full[st]);
-            bulk_load(s.b_delta[st], delta2 + h * a.vec_ld + row, BN * 4, &s.b_full[st]);
+    while (ok) {
+      // Each lane looks up one of the items taken, one at first. While they are of short sequences, twice as
+      // many are taken the next time: a look-up costs a microsecond, which nothing hides if no item follows.
+      const int base = __shfl_sync(0xFFFFFFFFu, at, 0), mine = base + lane, y = blocks ? mine / blocks : 0;
+      BwdItem look{};
+      if (lane < ask && mine < total) {  // keys first: theirs are the longest items
+        const SeqBlock b = seq_block(a, mine - y * blocks);
+        if (b.on && b.first < b.len && b.len > kAttnShort) {
+          look.keys = y < a.Hk;
+          look.head = look.keys ? y : y - a.Hk;
+          look.seq = b.seq; look.first = b.first; look.len = b.len; look.row0 = (int)b.row0; look.outer = (int)b.outer; look.off = b.off;
+          look.n = (b.len + BN - 1) / BN * (look.keys ? group : 1);
+        }
+      }
+      const bool last = base + ask >= total;
+      uint32_t found = __ballot_sync(0xFFFFFFFFu, look.n > 0);
+      ask = found ? 1 : ask < 32 ? 2 * ask : 32;
+      if (lane == 0 && !last) at = (int)atomicAdd(a.counter, (uint32_t)ask);
+#pragma unroll 1
+      while (ok && (found || last)) {
+        const int r = k % kRing, from = __ffs(found) - 1;
+        const bool more = found != 0;
+        found &= found - 1;
+        BwdItem it{};
+        if (more) {
+          it.seq = __shfl_sync(0xFFFFFFFFu, look.seq, from);
+          it.first = __shfl_sync(0xFFFFFFFFu, look.first, from);
+          it.len = __shfl_sync(0xFFFFFFFFu, look.len, from);
+          it.head = __shfl_sync(0xFFFFFFFFu, look.head, from);
+          it.keys = __shfl_sync(0xFFFFFFFFu, look.keys, from);
+          it.n = __shfl_sync(0xFFFFFFFFu, look.n, from);
+          it.row0 = __shfl_sync(0xFFFFFFFFu, look.row0, from);
+          it.outer = __shfl_sync(0xFFFFFFFFu, look.outer, from);
+          it.off = __shfl_sync(0xFFFFFFFFu, look.off, from);
+        }
+        if (elect_one()) {
+          ok = k < kRing || mbar_wait_soon(&s.item_empty[r], ((k / kRing) & 1) ^ 1, 211);
+          if (ok) {
+            s.item[r] = it;
+            mbar_arrive(&s.item_full[r]);
           }
-          row += BN;
-          if (row >= it.len) {
-            row = 0;
-            ++h;
+          if (ok && more) {
+            const bool keys = it.keys;
+            const int kh = it.head / group;
+            const float *lse2 = a.lse2 + it.off, *delta2 = a.delta2 + it.off;
+            mbar_arrive_expect_tx(&s.a_full[r], 2 * kTile + (keys ? 0 : 2 * BM * 4));
+            for (int half = 0; half < 2; ++half) {  // boxes of 64 rows
+              tma_load_4d(s.a0[r] + half * kHalf, keys ? &mk : &mq, 0, it.row0 + it.first + half * BN, it.head, it.outer, &s.a_full[r]);
+              tma_load_4d(s.a1[r] + half * kHalf, keys ? &mv : &mdo, 0, it.row0 + it.first + half * BN, it.head, it.outer, &s.a_full[r]);
+            }
+            if (!keys) {
+              bulk_load(s.a_lse[r], lse2 + it.head * a.vec_ld + it.first, BM * 4, &s.a_full[r]);
+              bulk_load(s.a_delta[r], delta2 + it.head * a.vec_ld + it.first, BM * 4, &s.a_full[r]);
+            }
+            int row = 0, h = keys ? it.head * group : kh;
+#pragma unroll 1
+            for (int i = t; i < t + it.n; ++i) {
+              const int st = i % kStages;
+              ok = i < kStages || mbar_wait_soon(&s.b_empty[st], ((i / kStages) & 1) ^ 1, 212);
+              if (!ok) break;
+              mbar_arrive_expect_tx(&s.b_full[st], 2 * kHalf + (keys ? 2 * BN * 4 : 0));
+              tma_load_4d(s.b0[st], keys ? &mq : &mk, 0, it.row0 + row, h, it.outer, &s.b_full[st]);
+              tma_load_4d(s.b1[st], keys ? &mdo : &mv, 0, it.row0 + row, h, it.outer, &s.b_full[st]);
+              if (keys) {
+                bulk_load(s.b_lse[st], lse2 + h * a.vec_ld + row, BN * 4, &s.b_full[st]);
+                bulk_load(s.b_delta[st], delta2 + h * a.vec_ld + row, BN * 4, &s.b_full[st]);
+              }
+              row += BN;
+              if (row >= it.len) {
+                row = 0;
+                ++h;
+              }
+            }
           }
         }
-        if (!ok) break;
+        ok = __all_sync(0xFFFFFFFFu, ok) && more;  // the stream ends behind an item of no tiles
+        t += it.n;
         ++k;
       }
     }
@@ -980,7 +1002,7 @@ int bwd(const AttnArgs& a, cudaStream_t st) {
 // taken before the scale).
 bool attn_tc_takes(const AttnArgs& a, int dtype, bool grad) {
   if (dtype == ATLAS_F32 || !(a.scale > 0.f)) return false;
-  if (grad && (a.cap * (a.H + a.Hk) >= (1LL << 31) || !map_ok(a.dout, a.sdo, a.outer, a.H, a.rows))) return false;
+  if (grad && (a.cap * (a.H + a.Hk) >= (1LL << 30) || !map_ok(a.dout, a.sdo, a.outer, a.H, a.rows))) return false;
   return map_ok(a.q, a.sq, a.outer, a.H, a.rows) && map_ok(a.k, a.sk, a.outer, a.Hk, a.rows) &&
          map_ok(a.v, a.sv, a.outer, a.Hk, a.rows);
 }

@@ -192,6 +192,7 @@ def _check(got, ref, tol):
 
 
 LENS = [[1], [2], [37], [64], [65], [127, 128, 129], [1, 0, 300, 0], [257, 31, 1, 513], [0, 0, 5]]
+LENS += [[15, 16, 17, 18], [3, 140, 7, 0, 16, 2, 70]]  # the gradient's short sequences, among longer ones
 
 
 @pytest.mark.parametrize("lens", LENS, ids=str)
@@ -215,13 +216,13 @@ def test_attention_and_gradient(lens, packed, dtype, D, H, Hk):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("D,H,Hk", [(8, 4, 2), (64, 2, 2), (13, 3, 1)])
-@pytest.mark.parametrize("L", [2, 3, 4, 9, 16])
+@pytest.mark.parametrize("L", [2, 3, 4, 9, 16, 17])
 def test_attention_gradient_over_few_keys(L, D, H, Hk, dtype):
     """Over few keys dP and delta nearly cancel, so that delta has to be better than the rounded output
-    makes it. What is left is the rounding of dS and that of the result, each off by at most half a step h
-    of every element, uniformly within it: h / sqrt(3) of the norm each at most, and sqrt(2 / 3) h together,
-    since they are independent. The limit is h; delta from the output passes it at 2, 3 and 4 keys (1.4 h,
-    1.2 h, 1.1 h in bf16)."""
+    makes it. What may be left is the rounding of dS and that of the result, each off by at most half a step
+    h of every element, uniformly within it: h / sqrt(3) of the norm each at most, and sqrt(2 / 3) h
+    together, since they are independent. The limit is h; delta from the output passes it at 2, 3 and 4 keys
+    (1.4 h, 1.2 h, 1.1 h in bf16)."""
     KN = _kn()
     q, k, v, do, plan, where, _ = _batch([L] * 150, True, H, Hk, D, dtype, seed=L)
     ref, _ = _plain(q, k, v, do, where, D ** -0.5)
