@@ -18,7 +18,7 @@ int check(const AttnArgs& a, int dtype, const char* what) {
   ATLAS_REQUIRE(a.packed ? a.outer == 1 : a.outer == a.B, "%s: outer must be %s", what, a.packed ? "1" : "the batch");
   ATLAS_REQUIRE(a.H >= 1 && a.H <= 65535 && a.Hk >= 1 && a.H % a.Hk == 0, "%s: heads must be a multiple of the key heads", what);
   ATLAS_REQUIRE(a.D >= 1 && a.D <= kAttnMaxDim, "%s: head dimension must be in [1, %d]", what, kAttnMaxDim);
-  ATLAS_REQUIRE(a.cap >= a.outer * a.rows / kAttnBlock + a.B + 1 && a.cap <= (1LL << 29),
+  ATLAS_REQUIRE(a.cap >= attn_blocks(a.outer, a.rows, a.B) && a.cap <= (1LL << 29),
                 "%s: the block table has too few or too many entries", what);
   ATLAS_REQUIRE(a.q && a.k && a.v && a.lse && a.cu && a.blocks && a.counts, "%s: null pointer", what);
   ATLAS_REQUIRE((uintptr_t)a.blocks % 8 == 0, "%s: the block table must be 8-byte aligned", what);
@@ -48,7 +48,7 @@ extern "C" int atlas_attention(const void* q, const void* k, const void* v, int 
 }
 
 extern "C" int64_t atlas_attention_grad_ws_bytes(int64_t outer, int64_t rows, int64_t H, int64_t Hk, int64_t B) {
-  return 4 * (2 * H * attn_vec_ld(outer, rows, B) + B * Hk + 1);
+  return 16 * attn_blocks(outer, rows, B) + 4 * (2 * H * attn_vec_ld(outer, rows, B) + B * Hk + 2);
 }
 
 extern "C" int atlas_attention_grad(const void* dout, const void* q, const void* k, const void* v, const void* out,
@@ -75,9 +75,11 @@ extern "C" int atlas_attention_grad(const void* dout, const void* q, const void*
     return attn_simt(a, dtype, true, (cudaStream_t)stream);
   }
   a.vec_ld = attn_vec_ld(outer, rows, B);
-  a.lse2 = (float*)ws;
+  a.list = (int4*)ws;
+  a.lse2 = (float*)(a.list + attn_blocks(outer, rows, B));
   a.delta2 = a.lse2 + H * a.vec_ld;
   a.amax = (uint32_t*)(a.delta2 + H * a.vec_ld);
   a.counter = a.amax + B * Hk;
+  a.listed = a.counter + 1;
   return attn_tc(a, dtype, true, (cudaStream_t)stream);
 }

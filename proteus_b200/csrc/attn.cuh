@@ -21,11 +21,12 @@ struct AttnArgs {
   float* lse;    // [outer, H, rows]
   // Gradient only. CUDA cores: delta [outer, H, rows]. Tensor cores: for each head, negated, the
   // log-sum-exp in base 2 and delta of all sequences, each from a place that is a multiple of 16 bytes (seq_block's off;
-  // vec_ld values a head), the largest |dout| of a sequence and key head as bits (fp16), and the counter of
-  // work items.
+  // vec_ld values a head), the largest |dout| of a sequence and key head as bits (fp16), the counter of work items,
+  // and the blocks of more than kAttnShort rows, in no order: sequence, first row, length, prefix sum.
   float *delta, *lse2, *delta2;
   int64_t vec_ld;
-  uint32_t *amax, *counter;
+  uint32_t *amax, *counter, *listed;
+  int4* list;
   const int32_t *cu, *blocks;
   const int64_t* counts;
   int64_t outer, rows, B, cap;
@@ -43,6 +44,8 @@ struct SeqBlock {
   bool spare;  // an entry behind the last
 };
 
+__device__ __forceinline__ int64_t seq_off(int seq, int c0) { return (c0 + 4 * (int64_t)seq + 3) & ~(int64_t)3; }
+
 __device__ __forceinline__ SeqBlock seq_block(const AttnArgs& a, int64_t i) {
   SeqBlock s{};
   const int64_t n = a.counts[1];
@@ -59,45 +62,73 @@ __device__ __forceinline__ SeqBlock seq_block(const AttnArgs& a, int64_t i) {
   const int64_t len = c1 - c0, room = a.rows - s.row0;
   s.len = (int)(len < 0 ? 0 : len > room ? room : len);
   if (c0 < 0 || c0 + s.len > a.outer * a.rows) return s;
-  s.off = (c0 + 4 * (int64_t)e.x + 3) & ~(int64_t)3;
+  s.off = seq_off(e.x, (int)c0);
   s.on = true;
   return s;
+}
+
+// The last of sequences lo .. hi - 1 before which no more than g of a padded batch's idle rows lie, by a
+// warp: 32 of them at a time.
+__device__ __forceinline__ int64_t idle_seq(const AttnArgs& a, int64_t lo, int64_t hi, int64_t g, int lane) {
+#pragma unroll 1
+  while (hi - lo > 1) {
+    const int64_t step = (hi - lo + 31) / 32, mid = lo + lane * step;
+    const bool below = mid < hi && mid * a.rows - a.cu[mid] <= g;
+    const int64_t at = lo + (31 - __clz(__ballot_sync(0xFFFFFFFFu, below) | 1u)) * step;
+    lo = at;
+    hi = at + step < hi ? at + step : hi;
+  }
+  return lo;
 }
 
 // The rows of no sequence - behind a padded sequence's end, or behind the last sequence of a packed batch -
 // in order, shared out evenly over the spare entries of the table. The table has rows / 128 + B + 1 entries
 // and a sequence takes at most len / 128 + 1 of them, so that a share is 128 rows or less. (Given to a
 // sequence's own last entry, a batch of lengths 505 to 4040 spent 540 us in four CTAs that set thousands
-// of rows to zero.) Spare entry i, by warp `warp` of `warps`: each lane looks up a row of its own, lane(outer,
-// row) is called once for it by that lane, and row(outer, row, sub) by 8 lanes, sub 0-7.
-template <typename Lane, typename Row>
-__device__ __forceinline__ void idle_rows(const AttnArgs& a, int64_t i, int warp, int warps, int lane, Lane each, Row eight) {
-  const int64_t n = a.counts[1], parts = a.cap - n, part = i - n;
-  const int64_t all = a.packed ? a.rows : a.outer * a.rows, used = a.cu[a.B];
-  const int64_t left = all - (used < 0 ? 0 : used);
-  if (left <= 0 || n < 0) return;
-  const int64_t end = left * (part + 1) / parts;
+// of rows to zero.)
+struct IdleShare {
+  int64_t all, left, from, end;  // rows; of no sequence; this share's, numbered
+};
+__device__ __forceinline__ IdleShare idle_share(const AttnArgs& a, int64_t i) {
+  const int64_t n = a.counts[1], used = a.cu[a.B];
+  IdleShare s;
+  s.all = a.packed ? a.rows : a.outer * a.rows;
+  s.left = used < 0 ? s.all : used < s.all ? s.all - used : 0;
+  s.from = n < 0 || n > i ? s.left : s.left * (i - n) / (a.cap - n);
+  s.end = n < 0 || n > i ? s.left : s.left * (i - n + 1) / (a.cap - n);
+  return s;
+}
+
+// A lane's row of the share, number n0 + i of it (i < 32): false behind the share's end. For whole warps.
+__device__ __forceinline__ bool idle_row(const AttnArgs& a, const IdleShare& s, int64_t n0, int i, int64_t* outer, int64_t* row) {
+  const int lane = threadIdx.x % 32;
+  const int64_t g0 = s.from + n0, g = g0 + i;
+  if (g0 >= s.end) return false;
+  int64_t b = 0, r = s.all - s.left + g;
+  if (!a.packed) {  // before sequence b lie b * rows - cu[b] of them
+    int64_t hi = idle_seq(a, 0, a.B, g0 + 31, lane) + 1;
+    b = idle_seq(a, 0, hi, g0, lane);
 #pragma unroll 1
-  for (int64_t g0 = left * part / parts + 32 * warp; g0 < end; g0 += 32 * warps) {
-    const int64_t g = g0 + lane;
-    int64_t b = 0, r = all - left + g;
-    bool on = g < end;
-    if (!a.packed) {  // before sequence b lie b * rows - cu[b] of them
-#pragma unroll 1
-      for (int64_t hi = a.B; hi - b > 1;) {
-        const int64_t mid = (b + hi) >> 1;
-        if (mid * a.rows - a.cu[mid] <= g) b = mid;
-        else hi = mid;
-      }
-      r = g - b * a.rows + a.cu[b + 1];
-      on = on && r >= 0 && r < a.rows;
+    while (hi - b > 1) {
+      const int64_t mid = (b + hi) >> 1;
+      if (mid * a.rows - a.cu[mid] <= g) b = mid;
+      else hi = mid;
     }
-    if (on) each(b, r);
+    r = g - b * a.rows + a.cu[b + 1];
+  }
+  *outer = b;
+  *row = r;
+  return g < s.end && r >= 0 && r < a.rows;
+}
+
+// The rows of spare entry i by a CTA of n threads: f(outer, row, sub) by 8 threads for each.
+template <typename F>
+__device__ __forceinline__ void idle_rows(const AttnArgs& a, int64_t i, int n, F f) {
+  const IdleShare s = idle_share(a, i);
 #pragma unroll 1
-    for (int j = lane >> 3; j < 32; j += 4) {
-      const int64_t bj = __shfl_sync(0xFFFFFFFFu, b, j), rj = __shfl_sync(0xFFFFFFFFu, r, j);
-      if (__shfl_sync(0xFFFFFFFFu, (int)on, j)) eight(bj, rj, lane & 7);
-    }
+  for (int64_t at = threadIdx.x / 32 * 4; s.from + at < s.end; at += n / 8) {
+    int64_t o = 0, r = 0;
+    if (idle_row(a, s, at, threadIdx.x % 32 / 8, &o, &r)) f(o, r, threadIdx.x % 8);
   }
 }
 
@@ -128,6 +159,9 @@ inline int attn_smem_once(K kernel, int bytes, bool (&done)[64]) {
   if (dev >= 0 && dev < 64) done[dev] = true;
   return ATLAS_OK;
 }
+
+// Entries of the block table that a batch needs.
+__host__ __device__ inline int64_t attn_blocks(int64_t outer, int64_t rows, int64_t B) { return outer * rows / kAttnBlock + B + 1; }
 
 // Values a head of the padded vectors: every sequence's rows and up to 4 between two, and 128 that a
 // tile may read behind the last.

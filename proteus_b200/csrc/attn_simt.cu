@@ -21,6 +21,7 @@ namespace {
 constexpr int BT = 64;       // rows of a tile
 constexpr int PP = 80;       // row pitch of a tile of scores: the two ty of a warp in different bank halves
 constexpr int kThreads = 256;
+constexpr int kIdleHeads = 4;  // heads of a CTA that sets rows to zero: its time is the look-up's, 2.5 us
 constexpr float kNegInf = -__builtin_inff();
 
 template <int DT>
@@ -162,10 +163,16 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 2 : 3) attn_fwd_simt_kern
   const int head = blockIdx.y, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int64_t bi = blockIdx.x >> 1;
   const SeqBlock s = seq_block(a, bi);
-  if (s.spare && !(blockIdx.x & 1))
-    idle_rows(a, bi, threadIdx.x / 32, kThreads / 32, threadIdx.x % 32,
-              [&](int64_t o, int64_t r) { a.lse[(o * a.H + head) * a.rows + r] = 0.f; },
-              [&](int64_t o, int64_t r, int sub) { zero_row(a.out, a.so, sizeof(typename Elem<DT>::T), o, head, r, a.D, sub); });
+  if (s.spare) {
+    if (blockIdx.x & 1 || head % kIdleHeads) return;
+    idle_rows(a, bi, kThreads, [&](int64_t o, int64_t r, int sub) {
+      for (int h = head; h < min(head + kIdleHeads, a.H); ++h) {
+        zero_row(a.out, a.so, sizeof(typename Elem<DT>::T), o, h, r, a.D, sub);
+        if (sub == 0) a.lse[(o * a.H + h) * a.rows + r] = 0.f;
+      }
+    });
+    return;
+  }
   const int first = s.first + (blockIdx.x & 1) * BT;
   if (!s.on || first >= s.len) return;
   const int kh = head / (a.H / a.Hk);
@@ -260,13 +267,17 @@ __global__ void __launch_bounds__(kThreads, 2) attn_bwd_simt_kernel(const AttnAr
   const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, group = a.H / a.Hk;
   const int64_t bi = blockIdx.x >> 1;
   const SeqBlock s = seq_block(a, bi);
-  if (s.spare && !(blockIdx.x & 1))
-    idle_rows(a, bi, threadIdx.x / 32, kThreads / 32, threadIdx.x % 32, [](int64_t, int64_t) {},
-              [&](int64_t o, int64_t r, int sub) {
-                constexpr int size = sizeof(typename Elem<DT>::T);
-                zero_row(KEYS ? a.dk : a.dq, KEYS ? a.sdk : a.sdq, size, o, blockIdx.y, r, a.D, sub);
-                if (KEYS) zero_row(a.dv, a.sdv, size, o, blockIdx.y, r, a.D, sub);
-              });
+  if (s.spare) {
+    if (blockIdx.x & 1 || blockIdx.y % kIdleHeads) return;
+    idle_rows(a, bi, kThreads, [&](int64_t o, int64_t r, int sub) {
+      constexpr int size = sizeof(typename Elem<DT>::T);
+      for (int h = blockIdx.y; h < min((int)blockIdx.y + kIdleHeads, (int)gridDim.y); ++h) {
+        zero_row(KEYS ? a.dk : a.dq, KEYS ? a.sdk : a.sdq, size, o, h, r, a.D, sub);
+        if (KEYS) zero_row(a.dv, a.sdv, size, o, h, r, a.D, sub);
+      }
+    });
+    return;
+  }
   const int first = s.first + (blockIdx.x & 1) * BT;
   if (!s.on || first >= s.len || s.len <= kAttnShort) return;
   const int kh = KEYS ? blockIdx.y : blockIdx.y / group;
@@ -344,26 +355,27 @@ __device__ __forceinline__ void short_grad(const AttnArgs& a, const SeqBlock& b,
   using T = typename Elem<DT>::T;
   static_assert(kThreads == kAttnShort * kAttnShort && kAttnMaxDim == 4 * kAttnShort, "a thread per pair of rows");
   const int r = threadIdx.x / kAttnShort, c = threadIdx.x % kAttnShort, len = b.len, group = a.H / a.Hk;
-  auto load = [&](const void* src, const Strides& st, int head, float (&dst)[kAttnShort][68]) {
+  auto load = [&](const void* src, const Strides& st, int head) {
     const T* p = reinterpret_cast<const T*>(src) + b.outer * st.outer + head * st.head + (b.row0 + r) * st.row + 4 * c;
-    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
     if (r < len) {
       if (VEC) {  // D is a multiple of 4
         if (4 * c < a.D) {
-          T w[4];
+          alignas(16) T w[4];
           if (sizeof(T) == 4) *reinterpret_cast<uint4*>(w) = __ldg(reinterpret_cast<const uint4*>(p));
           else *reinterpret_cast<uint2*>(w) = __ldg(reinterpret_cast<const uint2*>(p));
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[e] = Elem<DT>::f(w[e]);
+          x = make_float4(Elem<DT>::f(w[0]), Elem<DT>::f(w[1]), Elem<DT>::f(w[2]), Elem<DT>::f(w[3]));
         }
       } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (4 * c + e < a.D) x[e] = Elem<DT>::f(p[e]);
+        if (4 * c < a.D) x.x = Elem<DT>::f(p[0]);
+        if (4 * c + 1 < a.D) x.y = Elem<DT>::f(p[1]);
+        if (4 * c + 2 < a.D) x.z = Elem<DT>::f(p[2]);
+        if (4 * c + 3 < a.D) x.w = Elem<DT>::f(p[3]);
       }
     }
-    *reinterpret_cast<float4*>(&dst[r][4 * c]) = make_float4(x[0], x[1], x[2], x[3]);
+    return x;
   };
+  auto row_of = [](float (&tile)[kAttnShort][68], int row, int col) -> float4& { return *reinterpret_cast<float4*>(&tile[row][col]); };
   auto add = [](float4& acc, float w, const float4& x) {
     acc.x = fmaf(w, x.x, acc.x);
     acc.y = fmaf(w, x.y, acc.y);
@@ -377,27 +389,32 @@ __device__ __forceinline__ void short_grad(const AttnArgs& a, const SeqBlock& b,
     for (int e = 0; e < 4; ++e)
       if (r < len && 4 * c + e < a.D) put<DT>(p + e, w[e]);
   };
-  load(a.k, a.sk, kh, s.k);
-  load(a.v, a.sv, kh, s.v);
-  float4 dk = make_float4(0.f, 0.f, 0.f, 0.f), dv = dk;
+  const bool on = r < len && c < len;
+  const float* lses = a.lse + b.outer * a.H * a.rows + b.row0 + r;
+  int h = kh * group;
+  row_of(s.k, r, 4 * c) = load(a.k, a.sk, kh);
+  row_of(s.v, r, 4 * c) = load(a.v, a.sv, kh);
+  float4 q = load(a.q, a.sq, h), g = load(a.dout, a.sdo, h), dk = make_float4(0.f, 0.f, 0.f, 0.f), dv = dk;
+  float lse = on ? lses[h * a.rows] : 0.f;
 #pragma unroll 1
-  for (int h = kh * group; h < (kh + 1) * group; ++h) {
-    load(a.q, a.sq, h, s.q);
-    load(a.dout, a.sdo, h, s.g);
+  for (int left = group; left; --left, ++h) {
+    row_of(s.q, r, 4 * c) = q;
+    row_of(s.g, r, 4 * c) = g;
     __syncthreads();
-    const bool on = r < len && c < len;
-    float p = 0.f, dp = 0.f;
+    float p = 0.f, dp = 0.f, sc = 0.f;
     if (on) {
-      const float lse = a.lse[(b.outer * a.H + h) * a.rows + b.row0 + r];
-      float sc = 0.f;
-#pragma unroll 1
+#pragma unroll 4
       for (int d = 0; d < a.D; d += 4) {
-        const float4 x = *reinterpret_cast<const float4*>(&s.q[r][d]), y = *reinterpret_cast<const float4*>(&s.k[c][d]);
-        const float4 g = *reinterpret_cast<const float4*>(&s.g[r][d]), v = *reinterpret_cast<const float4*>(&s.v[c][d]);
+        const float4 x = row_of(s.q, r, d), y = row_of(s.k, c, d), w = row_of(s.g, r, d), z = row_of(s.v, c, d);
         sc = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, sc))));
-        dp = fmaf(g.x, v.x, fmaf(g.y, v.y, fmaf(g.z, v.z, fmaf(g.w, v.w, dp))));
+        dp = fmaf(w.x, z.x, fmaf(w.y, z.y, fmaf(w.z, z.z, fmaf(w.w, z.w, dp))));
       }
       p = ex2((sc * a.scale - lse) * kLog2e);
+    }
+    if (left > 1) {  // the next head's rows are on their way
+      q = load(a.q, a.sq, h + 1);
+      g = load(a.dout, a.sdo, h + 1);
+      lse = on ? lses[(h + 1) * a.rows] : 0.f;
     }
     float delta = p * dp;
 #pragma unroll
@@ -406,11 +423,11 @@ __device__ __forceinline__ void short_grad(const AttnArgs& a, const SeqBlock& b,
     s.ds[r][c] = on ? p * (dp - delta) : 0.f;
     __syncthreads();
     float4 dq = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 1
+#pragma unroll 4
     for (int j = 0; j < len; ++j) {
-      add(dq, s.ds[r][j], *reinterpret_cast<const float4*>(&s.k[j][4 * c]));
-      add(dk, s.ds[j][r], *reinterpret_cast<const float4*>(&s.q[j][4 * c]));
-      add(dv, s.p[j][r], *reinterpret_cast<const float4*>(&s.g[j][4 * c]));
+      add(dq, s.ds[r][j], row_of(s.k, j, 4 * c));
+      add(dk, s.ds[j][r], row_of(s.q, j, 4 * c));
+      add(dv, s.p[j][r], row_of(s.g, j, 4 * c));
     }
     store(a.dq, a.sdq, h, dq, a.scale);
     __syncthreads();
@@ -419,46 +436,25 @@ __device__ __forceinline__ void short_grad(const AttnArgs& a, const SeqBlock& b,
   store(a.dv, a.sdv, kh, dv, 1.f);
 }
 
-// Before the gradient's kernels: delta = sum_d dout out of the rows of a block and head, G lanes to a row: 8
-// lanes with 16-byte loads where rows are aligned for them (VEC), else a warp; and the gradients of short
-// sequences. For the tensor-core kernel also what it needs beside it (see AttnArgs); the largest |dout| as
-// bits, so that the order of the atomics does not matter.
+// delta = sum_d dout out of the rows of a block and head, G lanes to a row: 8 lanes with 16-byte loads where
+// rows are aligned for them (VEC), else a warp. The largest |dout| as bits, so that the order of the atomics
+// does not matter.
 template <int DT, bool VEC>
-__global__ void __launch_bounds__(kThreads) attn_delta_kernel(const AttnArgs a) {
+__device__ __forceinline__ void delta_rows(const AttnArgs& a, const SeqBlock& s, int head) {
   using T = typename Elem<DT>::T;
   constexpr int E = VEC ? 16 / sizeof(T) : 1;      // elements per load
   constexpr int G = VEC ? kAttnMaxDim / E : 32;    // lanes per row
   constexpr int PER = kThreads / G;                // rows at a time
-  __shared__ ShortSmem sm;
-  const SeqBlock s = seq_block(a, blockIdx.x);
-  const int head = blockIdx.y, sub = threadIdx.x % G;
-  if (a.lse2) {  // before the tensor-core kernel: its counter, and the rows that it does not write
-    if (blockIdx.x == 0 && head == 0 && threadIdx.x == 0) *a.counter = 0;
-    if (s.spare)
-      idle_rows(a, blockIdx.x, threadIdx.x / 32, kThreads / 32, threadIdx.x % 32, [](int64_t, int64_t) {},
-                [&](int64_t o, int64_t r, int lane8) {
-                  zero_row(a.dq, a.sdq, sizeof(T), o, head, r, a.D, lane8);
-                  if (head < a.Hk) {
-                    zero_row(a.dk, a.sdk, sizeof(T), o, head, r, a.D, lane8);
-                    zero_row(a.dv, a.sdv, sizeof(T), o, head, r, a.D, lane8);
-                  }
-                });
-  }
-  if (!s.on) return;
-  if (s.len <= kAttnShort) {
-    if (s.first == 0 && head < a.Hk) short_grad<DT, VEC>(a, s, head, sm);
-    return;
-  }
+  const int sub = threadIdx.x % G;
   const T* o = reinterpret_cast<const T*>(a.o) + s.outer * a.so.outer + head * a.so.head + s.row0 * a.so.row;
   const T* g = reinterpret_cast<const T*>(a.dout) + s.outer * a.sdo.outer + head * a.sdo.head + s.row0 * a.sdo.row;
+  const int64_t vec_at = head * a.vec_ld + s.off, row_at = (s.outer * a.H + head) * a.rows + s.row0;
   float amax = 0.f;
   auto product = [&](T x, T y, float v) {
     const float w = Elem<DT>::f(y);
     if (DT == ATLAS_F16) amax = fabsf(w) > amax || w != w ? fabsf(w) : amax;
     return fmaf(Elem<DT>::f(x), w, v);
   };
-  const int64_t vec_at = head * a.vec_ld + s.off;
-  const int64_t row_at = (s.outer * a.H + head) * a.rows + s.row0;
   constexpr int U = VEC ? 4 : 1;  // rows of a thread whose loads are under way at once
 #pragma unroll 1
   for (int k0 = 0; k0 < kAttnBlock / PER; k0 += U) {
@@ -506,6 +502,37 @@ __global__ void __launch_bounds__(kThreads) attn_delta_kernel(const AttnArgs a) 
   }
 }
 
+// Before the gradient's kernels: delta, and the gradients of short sequences; for the tensor-core kernel also
+// the list of its blocks, and zero to the rows that it does not write. 16-bit: 160 MB of out and dout in 44 us,
+// 3.6 TB/s; what bounds it is the latency of a CTA's loads, two for its entry, then four rows of a thread at once.
+template <int DT, bool VEC>
+__global__ void __launch_bounds__(kThreads, 4) attn_delta_kernel(const AttnArgs a) {
+  __shared__ ShortSmem sm;
+  const SeqBlock s = seq_block(a, blockIdx.x);
+  const int head = blockIdx.y;
+  if (!s.on) {
+    if (s.spare && a.lse2 && head % kIdleHeads == 0)
+      idle_rows(a, blockIdx.x, kThreads, [&](int64_t o, int64_t r, int sub) {
+        constexpr int size = sizeof(typename Elem<DT>::T);
+        for (int h = head; h < min(head + kIdleHeads, a.H); ++h) {
+          zero_row(a.dq, a.sdq, size, o, h, r, a.D, sub);
+          if (h < a.Hk) {
+            zero_row(a.dk, a.sdk, size, o, h, r, a.D, sub);
+            zero_row(a.dv, a.sdv, size, o, h, r, a.D, sub);
+          }
+        }
+      });
+  } else if (s.len > kAttnShort) {
+    if (a.lse2 && head == 0 && threadIdx.x == 0 && s.first < s.len) {
+      const uint32_t i = atomicAdd(a.listed, 1u);
+      if (i < attn_blocks(a.outer, a.rows, a.B)) a.list[i] = make_int4(s.seq, s.first, s.len, a.cu[s.seq]);
+    }
+    delta_rows<DT, VEC>(a, s, head);
+  } else if (s.first == 0 && head < a.Hk) {
+    short_grad<DT, VEC>(a, s, head, sm);
+  }
+}
+
 }  // namespace
 
 namespace {
@@ -520,8 +547,8 @@ int vec_rows(const AttnArgs& a, int dtype, bool grad) {
 }
 template <int DT>
 void launch_delta(const AttnArgs& a, cudaStream_t st) {
-  const dim3 grid((unsigned)a.cap, a.H);
   const int size = DT == ATLAS_F32 ? 4 : 2;
+  const dim3 grid((unsigned)a.cap, a.H);
   if (a.D * size % 16 == 0 && rows_of_16(a.o, a.so, size) && rows_of_16(a.dout, a.sdo, size) && rows_of_16(a.q, a.sq, size) &&
       rows_of_16(a.k, a.sk, size) && rows_of_16(a.v, a.sv, size))
     attn_delta_kernel<DT, true><<<grid, kThreads, 0, st>>>(a);

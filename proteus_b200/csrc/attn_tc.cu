@@ -138,7 +138,8 @@ struct FwdSmem {
   FwdItem item[2];
   uint4 answer;
   uint64_t stat_full[2], o_free, item_full[2], item_empty[2], q_full[2], k_full[kFwdStages], k_empty[kFwdStages], v_full[kFwdStages],
-      v_empty[kFwdStages], s_full[2], p_full[2], o_done[2], taken;
+      v_empty[kFwdStages], s_full[2], p_full[2], o_done[2], taken, spare_full, spare_empty;
+  int2 spare;  // entry and head whose rows of no sequence are next
   uint32_t tmem;
 };
 
@@ -234,6 +235,8 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
       mbar_init(&s.v_empty[i], 1);
     }
     mbar_init(&s.taken, 1);
+    mbar_init(&s.spare_full, 1);
+    mbar_init(&s.spare_empty, 1);
     mbar_init(&s.o_free, 4);
     fence_barrier_init();
   }
@@ -245,7 +248,7 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
 
   if (warp == 8) {
     regs_dec<40>();
-    int x = blockIdx.x, head = blockIdx.y, k = 0, t = 0;
+    int x = blockIdx.x, head = blockIdx.y, k = 0, t = 0, z = 0;
     uint32_t asked = 0;
     bool more = true, ok = true;
     while (ok) {
@@ -255,9 +258,16 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
       }
       __syncwarp();
       const SeqBlock b = more ? seq_block(a, x) : SeqBlock{};
-      if (more && b.spare)
-        idle_rows(a, x, 0, 1, lane, [&](int64_t o, int64_t r) { a.lse[(o * a.H + head) * a.rows + r] = 0.f; },
-                  [&](int64_t o, int64_t r, int sub) { zero_row(a.out, a.so, 2, o, head, r, a.D, sub); });
+      if (more && b.spare) {
+        ok = z == 0 || mbar_wait_soon(&s.spare_empty, (z - 1) & 1, 215);
+        if (!ok) break;
+        if (elect_one()) {
+          s.spare = make_int2(x, head);
+          mbar_arrive(&s.spare_full);
+        }
+        __syncwarp();
+        ++z;
+      }
       if (!more || (b.on && b.first < b.len)) {
         const int r = k & 1, n = more ? (b.len + KT - 1) / KT : 0;
         ok = k < 2 || mbar_wait(&s.item_empty[r], ((k >> 1) & 1) ^ 1, 200);
@@ -301,6 +311,11 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
     }
+    if ((z == 0 || mbar_wait_soon(&s.spare_empty, (z - 1) & 1, 215)) && elect_one()) {
+      s.spare = make_int2(-1, 0);
+      mbar_arrive(&s.spare_full);
+    }
+    __syncwarp();
   } else if (warp == 9) {
     regs_dec<40>();
     const uint32_t base = DT == ATLAS_BF16 ? idesc_bf16_f32(BM, 0) : idesc_f16_f32(BM, 0);
@@ -374,6 +389,35 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
     }
   } else if (warp == 11) {
     regs_dec<40>();
+    // Rows of no sequence: 6 us of 125 when the warp that loads the tiles did it in between (109 sequences of 271
+    // to 302 rows in a batch of 302, 20 heads). It posts the end whatever happens, and this wait may be as long as the
+    // kernel, so its limit is a thousand others.
+#pragma unroll 1
+    for (int z = 0, tries = 0; tries < 1000;) {
+      if (!mbar_poll(&s.spare_full, z & 1)) {
+        ++tries;
+        continue;
+      }
+      const int2 at = s.spare;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.spare_empty);
+      if (at.x < 0) break;
+      const int head = at.y;
+      const IdleShare share = idle_share(a, at.x);
+#pragma unroll 1
+      for (int64_t n = 0; share.from + n < share.end; n += 32) {  // a lane looks up a row, 8 write it
+        int64_t o = 0, r = 0;
+        const bool on = idle_row(a, share, n, lane, &o, &r);
+        if (on) a.lse[(o * a.H + head) * a.rows + r] = 0.f;
+#pragma unroll 1
+        for (int j = lane >> 3; j < 32; j += 4) {
+          const int64_t oj = __shfl_sync(0xFFFFFFFFu, o, j), rj = __shfl_sync(0xFFFFFFFFu, r, j);
+          if (__shfl_sync(0xFFFFFFFFu, (int)on, j)) zero_row(a.out, a.so, 2, oj, head, rj, a.D, lane & 7);
+        }
+      }
+      ++z;
+      tries = 0;
+    }
   } else if (warp < 4) {
     regs_inc<152>();
     const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
@@ -635,7 +679,8 @@ __device__ __forceinline__ void bwd_tile(uint32_t at, float c, float gain, float
 template <int DT>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk,
-                   const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mdo, const AttnArgs a, int vec) {
+                   const __grid_constant__ CUtensorMap mv, const __grid_constant__ CUtensorMap mdo,
+                   const __grid_constant__ AttnArgs a, int vec) {
   extern __shared__ __align__(1024) uint8_t raw[];
   BwdSmem& s = *reinterpret_cast<BwdSmem*>(raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.H / a.Hk;
@@ -667,89 +712,61 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
   const uint32_t tmem = s.tmem;
 
   if (warp == 16) {
-    const int64_t n = a.counts[1];
-    const int blocks = (int)(n < 0 ? 0 : n > a.cap ? a.cap : n), total = blocks * (a.Hk + a.H);
-    int k = 0, t = 0, ask = 1, at = 0;
-    if (lane == 0) at = (int)atomicAdd(a.counter, 1u);
-    bool ok = true;
-#pragma unroll 1
-    while (ok) {
-      // Each lane looks up one of the items taken, one at first. While they are of short sequences, twice as
-      // many are taken the next time: a look-up costs a microsecond, which nothing hides if no item follows.
-      const int base = __shfl_sync(0xFFFFFFFFu, at, 0), mine = base + lane, y = blocks ? mine / blocks : 0;
-      BwdItem look{};
-      if (lane < ask && mine < total) {  // keys first: theirs are the longest items
-        const SeqBlock b = seq_block(a, mine - y * blocks);
-        if (b.on && b.first < b.len && b.len > kAttnShort) {
-          look.keys = y < a.Hk;
-          look.head = look.keys ? y : y - a.Hk;
-          look.seq = b.seq; look.first = b.first; look.len = b.len; look.row0 = (int)b.row0; look.outer = (int)b.outer; look.off = b.off;
-          look.n = (b.len + BN - 1) / BN * (look.keys ? group : 1);
-        }
-      }
-      const bool last = base + ask >= total;
-      uint32_t found = __ballot_sync(0xFFFFFFFFu, look.n > 0);
-      ask = found ? 1 : ask < 32 ? 2 * ask : 32;
-      if (lane == 0 && !last) at = (int)atomicAdd(a.counter, (uint32_t)ask);
-#pragma unroll 1
-      while (ok && (found || last)) {
-        const int r = k % kRing, from = __ffs(found) - 1;
-        const bool more = found != 0;
-        found &= found - 1;
+    if (elect_one()) {
+      const int blocks = (int)min((int64_t)*a.listed, attn_blocks(a.outer, a.rows, a.B)), total = blocks * (a.Hk + a.H);
+      int next = (int)atomicAdd(a.counter, 1u), k = 0, t = 0;
+      while (true) {
         BwdItem it{};
-        if (more) {
-          it.seq = __shfl_sync(0xFFFFFFFFu, look.seq, from);
-          it.first = __shfl_sync(0xFFFFFFFFu, look.first, from);
-          it.len = __shfl_sync(0xFFFFFFFFu, look.len, from);
-          it.head = __shfl_sync(0xFFFFFFFFu, look.head, from);
-          it.keys = __shfl_sync(0xFFFFFFFFu, look.keys, from);
-          it.n = __shfl_sync(0xFFFFFFFFu, look.n, from);
-          it.row0 = __shfl_sync(0xFFFFFFFFu, look.row0, from);
-          it.outer = __shfl_sync(0xFFFFFFFFu, look.outer, from);
-          it.off = __shfl_sync(0xFFFFFFFFu, look.off, from);
+        if (next < total) {  // keys first: theirs are the longest items
+          const int y = next / blocks;
+          const int4 b = a.list[next - y * blocks];
+          next = (int)atomicAdd(a.counter, 1u);
+          it.keys = y < a.Hk;
+          it.head = it.keys ? y : y - a.Hk;
+          it.seq = b.x; it.first = b.y; it.len = b.z;
+          it.row0 = a.packed ? b.w : 0;
+          it.outer = a.packed ? 0 : b.x;
+          it.off = seq_off(b.x, b.w);
+          it.n = (b.z + BN - 1) / BN * (it.keys ? group : 1);
         }
-        if (elect_one()) {
-          ok = k < kRing || mbar_wait_soon(&s.item_empty[r], ((k / kRing) & 1) ^ 1, 211);
-          if (ok) {
-            s.item[r] = it;
-            mbar_arrive(&s.item_full[r]);
-          }
-          if (ok && more) {
-            const bool keys = it.keys;
-            const int kh = it.head / group;
-            const float *lse2 = a.lse2 + it.off, *delta2 = a.delta2 + it.off;
-            mbar_arrive_expect_tx(&s.a_full[r], 2 * kTile + (keys ? 0 : 2 * BM * 4));
-            for (int half = 0; half < 2; ++half) {  // boxes of 64 rows
-              tma_load_4d(s.a0[r] + half * kHalf, keys ? &mk : &mq, 0, it.row0 + it.first + half * BN, it.head, it.outer, &s.a_full[r]);
-              tma_load_4d(s.a1[r] + half * kHalf, keys ? &mv : &mdo, 0, it.row0 + it.first + half * BN, it.head, it.outer, &s.a_full[r]);
-            }
-            if (!keys) {
-              bulk_load(s.a_lse[r], lse2 + it.head * a.vec_ld + it.first, BM * 4, &s.a_full[r]);
-              bulk_load(s.a_delta[r], delta2 + it.head * a.vec_ld + it.first, BM * 4, &s.a_full[r]);
-            }
-            int row = 0, h = keys ? it.head * group : kh;
+        const int r = k % kRing;
+        if (k >= kRing && !mbar_wait_soon(&s.item_empty[r], ((k / kRing) & 1) ^ 1, 211)) break;
+        s.item[r] = it;
+        mbar_arrive(&s.item_full[r]);
+        if (!it.n) break;
+        const bool keys = it.keys;
+        const int kh = it.head / group;
+        const float *lse2 = a.lse2 + it.off, *delta2 = a.delta2 + it.off;
+        mbar_arrive_expect_tx(&s.a_full[r], 2 * kTile + (keys ? 0 : 2 * BM * 4));
+        for (int half = 0; half < 2; ++half) {  // boxes of 64 rows
+          tma_load_4d(s.a0[r] + half * kHalf, keys ? &mk : &mq, 0, it.row0 + it.first + half * BN, it.head, it.outer, &s.a_full[r]);
+          tma_load_4d(s.a1[r] + half * kHalf, keys ? &mv : &mdo, 0, it.row0 + it.first + half * BN, it.head, it.outer, &s.a_full[r]);
+        }
+        if (!keys) {
+          bulk_load(s.a_lse[r], lse2 + it.head * a.vec_ld + it.first, BM * 4, &s.a_full[r]);
+          bulk_load(s.a_delta[r], delta2 + it.head * a.vec_ld + it.first, BM * 4, &s.a_full[r]);
+        }
+        int row = 0, h = keys ? it.head * group : kh;
+        bool ok = true;
 #pragma unroll 1
-            for (int i = t; i < t + it.n; ++i) {
-              const int st = i % kStages;
-              ok = i < kStages || mbar_wait_soon(&s.b_empty[st], ((i / kStages) & 1) ^ 1, 212);
-              if (!ok) break;
-              mbar_arrive_expect_tx(&s.b_full[st], 2 * kHalf + (keys ? 2 * BN * 4 : 0));
-              tma_load_4d(s.b0[st], keys ? &mq : &mk, 0, it.row0 + row, h, it.outer, &s.b_full[st]);
-              tma_load_4d(s.b1[st], keys ? &mdo : &mv, 0, it.row0 + row, h, it.outer, &s.b_full[st]);
-              if (keys) {
-                bulk_load(s.b_lse[st], lse2 + h * a.vec_ld + row, BN * 4, &s.b_full[st]);
-                bulk_load(s.b_delta[st], delta2 + h * a.vec_ld + row, BN * 4, &s.b_full[st]);
-              }
-              row += BN;
-              if (row >= it.len) {
-                row = 0;
-                ++h;
-              }
-            }
+        for (int i = 0; i < it.n; ++i, ++t) {
+          const int st = t % kStages;
+          ok = t < kStages || mbar_wait_soon(&s.b_empty[st], ((t / kStages) & 1) ^ 1, 212);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&s.b_full[st], 2 * kHalf + (keys ? 2 * BN * 4 : 0));
+          tma_load_4d(s.b0[st], keys ? &mq : &mk, 0, it.row0 + row, h, it.outer, &s.b_full[st]);
+          tma_load_4d(s.b1[st], keys ? &mdo : &mv, 0, it.row0 + row, h, it.outer, &s.b_full[st]);
+          if (keys) {
+            bulk_load(s.b_lse[st], lse2 + h * a.vec_ld + row, BN * 4, &s.b_full[st]);
+            bulk_load(s.b_delta[st], delta2 + h * a.vec_ld + row, BN * 4, &s.b_full[st]);
+          }
+          row += BN;
+          if (row >= it.len) {
+            row = 0;
+            ++h;
           }
         }
-        ok = __all_sync(0xFFFFFFFFu, ok) && more;  // the stream ends behind an item of no tiles
-        t += it.n;
+        if (!ok) break;
         ++k;
       }
     }
@@ -987,7 +1004,7 @@ int bwd(const AttnArgs& a, cudaStream_t st) {
   if (int rc = attn_smem_once(attn_bwd_tc_kernel<DT>, bytes, done)) return rc;
   const int vec = a.D % 8 == 0 && map_ok(a.dq, a.sdq, a.outer, a.H, a.rows) && map_ok(a.dk, a.sdk, a.outer, a.Hk, a.rows) &&
                   map_ok(a.dv, a.sdv, a.outer, a.Hk, a.rows);
-  if (DT == ATLAS_F16 && cudaMemsetAsync(a.amax, 0, (size_t)(a.B * a.Hk) * 4, st) != cudaSuccess)
+  if (cudaMemsetAsync(DT == ATLAS_F16 ? a.amax : a.counter, 0, (size_t)(DT == ATLAS_F16 ? a.B * a.Hk + 2 : 2) * 4, st) != cudaSuccess)
     return fail(ATLAS_ERR_CUDA, "attention_grad: clearing the workspace failed");
   if (int rc = attn_delta(a, DT, st)) return rc;
   const int64_t items = a.cap * (a.Hk + a.H);

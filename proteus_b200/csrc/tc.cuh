@@ -55,12 +55,16 @@ static __device__ __noinline__ bool gave_up(int code) {
   return false;
 }
 
-// Bounded wait on a phase parity: false (and the status word set to `code`) if it never completes.
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int code) {
+// Bounded wait on a phase parity: false if it never completes.
+__device__ __forceinline__ bool mbar_poll(uint64_t* bar, uint32_t parity) {
 #pragma unroll 1
   for (uint32_t i = 0; i < kWaitLimit; ++i)
     if (mbar_try_wait(bar, parity)) return true;
-  return gave_up(code);
+  return false;
+}
+// The same; the status word is set to `code` then.
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int code) {
+  return mbar_poll(bar, parity) || gave_up(code);
 }
 
 __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
@@ -76,18 +80,10 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
 }
 
 // The same wait for chains of short steps. try_wait takes 140 clocks on a phase that has completed already,
-// test_wait 45 (measured): look once before settling down to wait, or, for the few warps that feed
-// the tensor core, do nothing else but look.
+// test_wait 45 (measured): look once before settling down to wait.
 __device__ __forceinline__ bool mbar_wait_soon(uint64_t* bar, uint32_t parity, int code) {
   return mbar_test(bar, parity) || mbar_wait(bar, parity, code);
 }
-__device__ __forceinline__ bool mbar_spin(uint64_t* bar, uint32_t parity, int code) {
-#pragma unroll 1
-  for (uint32_t i = 0; i < kWaitLimit; ++i)
-    if (mbar_test(bar, parity)) return true;
-  return gave_up(code);
-}
-
 // 2-D TMA tile load into shared memory, completion counted on `bar`; each CTA loads its own copy.
 __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, int32_t c0, int32_t c1, uint64_t* bar) {
   asm volatile(

@@ -214,6 +214,30 @@ def test_attention_and_gradient(lens, packed, dtype, D, H, Hk):
     assert (lse.transpose(1, 2)[off] == 0).all()
 
 
+@pytest.mark.parametrize("B,longest", [(7, 700), (33, 150), (1100, 4), (3, 4)])
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 64), (torch.float16, 24), (torch.float32, 20), (torch.bfloat16, 13)])
+def test_attention_padded_is_packed_with_zero_rows_between(B, longest, dtype, D):
+    """A sequence's results do not depend on where its rows lie, and every row of no sequence comes out
+    as zero, however unevenly they are spread (lengths of 0 to `longest`, the last one alone or not at all)."""
+    KN = _kn()
+    g = torch.Generator().manual_seed(B)
+    lens = torch.randint(0, longest + 1, (B,), generator=g).tolist()
+    lens[0], lens[B // 2] = longest, 0
+    got = {}
+    for packed in (False, True):
+        q, k, v, do, plan, where, on = _batch(lens, packed, 6, 2, D, dtype, extra=5)
+        gen = torch.Generator(device=DEV).manual_seed(9)
+        rows = [torch.randn(4, 6, sum(lens), D, generator=gen, device=DEV).to(dtype)[i][:h] for i, h in enumerate((6, 2, 2, 6))]
+        for t, x in zip((q, k, v, do), rows):
+            t.transpose(1, 2)[on] = x.transpose(0, 1)
+        out, lse = KN.attention(q, k, v, plan)
+        got[packed] = (out, lse[..., None], *KN.attention_grad(do, q, k, v, out, lse, plan)), on
+    for a, b in zip(got[False][0], got[True][0]):
+        assert torch.equal(a.transpose(1, 2)[got[False][1]], b.transpose(1, 2)[got[True][1]])
+        for t, on in ((a, got[False][1]), (b, got[True][1])):
+            assert (t.transpose(1, 2)[~on] == 0).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("D,H,Hk", [(8, 4, 2), (64, 2, 2), (13, 3, 1)])
 @pytest.mark.parametrize("L", [2, 3, 4, 9, 16, 17])
