@@ -10,7 +10,7 @@
 // 128 x 128 tile of scores costs 1024 clocks of exponentials and 256 to 512 of products. The products
 // therefore only have to stay out of the way: operands come by TMA as 128-byte-swizzled rows, scores and
 // probabilities live in TMEM (P is written over S as 16-bit and is the next product's A operand
-// from there), one thread per row of scores needs no shuffles, and two CTAs per SM alternate.
+// from there), and one thread per row of scores needs no shuffles.
 //
 // Rows behind a sequence's end: their columns of S are masked, products stop at the next multiple of
 // 16, and the rows up to there are set to zero in shared memory where they are summed over, since
@@ -107,10 +107,11 @@ __device__ __forceinline__ int up16(int n) { return (n + 15) & ~15; }
 // an item's look-up, first loads and first scores hide behind the item before.
 //   warps 0-3   softmax, one thread per query
 //   warps 4-7   read an item's output, divide and write it, while the softmax is at the next item
-//   warp 8      TMA, items, and zeros in rows of no sequence
+//   warp 8      TMA and items
 //   warp 9      scores; TMEM: two buffers of scores (columns 0-95, 96-191), P(t) over the first half of S(t), the
 //               output in 192-255, where an item's products accumulate
 //   warp 10     products with v
+//   warp 11     zero to rows of no sequence
 // Registers are moved from the other eight warps to the softmax's: 384 x 80 = 128 (152 + 48 + 40).
 //
 // The reference that exponents are taken from is the maximum of a row's FIRST 32 scores, not a running one: any
@@ -259,7 +260,7 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
       __syncwarp();
       const SeqBlock b = more ? seq_block(a, x) : SeqBlock{};
       if (more && b.spare) {
-        ok = z == 0 || mbar_wait_soon(&s.spare_empty, (z - 1) & 1, 215);
+        ok = z == 0 || mbar_wait_soon(&s.spare_empty, (z - 1) & 1, 217);
         if (!ok) break;
         if (elect_one()) {
           s.spare = make_int2(x, head);
@@ -311,7 +312,7 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
     }
-    if ((z == 0 || mbar_wait_soon(&s.spare_empty, (z - 1) & 1, 215)) && elect_one()) {
+    if ((z == 0 || mbar_wait_soon(&s.spare_empty, (z - 1) & 1, 217)) && elect_one()) {
       s.spare = make_int2(-1, 0);
       mbar_arrive(&s.spare_full);
     }
@@ -568,7 +569,7 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
 // tiles of 64 rows B0, B1 (q, dout or k, v) come in turn:
 //   S = A0 B0^T, dP = A1 B1^T, and with the 16-bit P and dS, written over them, as A operands
 //   keys: dv += P B1, dk += dS B0;  queries: dq += dS B0.
-// One persistent CTA per SM takes items from a counter and runs their tiles as one stream, so that an
+// One persistent CTA per SM takes items of the list (attn_delta_kernel's) from a counter and runs their tiles as one stream, so that an
 // item's start (look-up, first loads) and end (reading the sums) hide behind its neighbours:
 //   warps 0-11  three groups of four, each takes every third tile: one thread per row
 //   warps 12-15 read an item's sums and write them out, while the groups are at the next item
@@ -581,7 +582,7 @@ constexpr int kBwdThreads = 640;
 constexpr int kGroups = 3;
 constexpr int BN = 64;
 constexpr uint32_t kHalf = BN * 128;
-constexpr int kRing = 2;    // items in flight: tile t + 2 may be two items ahead
+constexpr int kRing = 2;    // items in flight
 constexpr int kStages = 9;  // B tiles in flight
 
 struct BwdItem {

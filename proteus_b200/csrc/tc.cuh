@@ -191,17 +191,6 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, i
 // Shared-memory writes of this thread become visible to the tensor core's and TMA's reads.
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// D[tmem] (+)= A[tmem] * B[smem desc]: A holds two 16-bit K elements per 32-bit column, row = lane.
-__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
-                                          uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-
 // 16 (8) registers per thread -> 32 lanes x 16 (8) consecutive 32-bit columns.
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
@@ -248,19 +237,6 @@ __device__ __forceinline__ uint64_t sdesc_k_sw128(uint32_t addr) {
   d |= (uint64_t)((addr >> 4) & 0x3FFF);       // start address
   d |= (uint64_t)1 << 16;                      // leading byte offset (unused for swizzled K-major)
   d |= (uint64_t)(1024 >> 4) << 32;            // stride byte offset: next 8-row group
-  d |= (uint64_t)1 << 46;                      // descriptor version (sm_100)
-  d |= (uint64_t)2 << 61;                      // layout: 128-byte swizzle
-  return d;
-}
-
-// The same tile read with its rows as K (an MN-major operand of 64 elements, 128-byte swizzle): eight
-// rows of 128 bytes are one swizzle atom, the next eight K elements lie 1024 bytes further. One MMA of
-// K = 16 takes 2048 bytes.
-__device__ __forceinline__ uint64_t sdesc_mn_sw128(uint32_t addr) {
-  uint64_t d = 0;
-  d |= (uint64_t)((addr >> 4) & 0x3FFF);       // start address
-  d |= (uint64_t)1 << 16;                      // leading byte offset: next 64 elements of MN (there are none)
-  d |= (uint64_t)(1024 >> 4) << 32;            // stride byte offset: next 8 of K
   d |= (uint64_t)1 << 46;                      // descriptor version (sm_100)
   d |= (uint64_t)2 << 61;                      // layout: 128-byte swizzle
   return d;
