@@ -85,11 +85,15 @@ _KERNELS = {"atlas_grouped_merge": 6, "atlas_last_error": 0, "atlas_abi_version"
 LAUNCHES = {"count": 0}
 
 
-_KERNELS.update({"atlas_ctx_rows": 4, "atlas_ctx_annotations": 2, "atlas_attention_grad": 3})
+_KERNELS.update({"atlas_ctx_rows": 4, "atlas_ctx_annotations": 2})
 
 
 def _count_admit(args):  # candidates, plus the bulk-row kernel when there are bulk rows
     return 2 if (args[6] and args[20]) else 1
+
+
+def _count_attention_grad(args):  # delta, then one kernel on the tensor cores or two on CUDA cores (fp32)
+    return 3 if args[6] == 0 else 2
 
 
 def _count_maps(args):  # more than 1024 sequences: totals, a scan, then the outputs
@@ -97,7 +101,7 @@ def _count_maps(args):  # more than 1024 sequences: totals, a scan, then the out
 
 
 _KERNELS.update({"atlas_dense_select": 3,  # row-major count (+ keys in key order), row-major emit, hard columns
-                 "atlas_admit": _count_admit, "atlas_seq_maps": _count_maps})
+                 "atlas_admit": _count_admit, "atlas_seq_maps": _count_maps, "atlas_attention_grad": _count_attention_grad})
 _KERNELS.update({n: 0 for n in SIGNATURES if n.endswith("_bytes") or n.endswith("_i32")})
 
 

@@ -135,7 +135,8 @@ def attach_attention(model, check: bool = True):
     the hook handle (model.set_attn_implementation puts another attention back). The batch's attention_mask
     has to be ones followed by zeros, as Batch's are; `check` looks at it, which waits for the device once a
     forward, so a loop that builds its masks so itself turns it off. Rows of padding come out of attention
-    as zeros."""
+    as zeros. The plan of a forward is the model's: one forward at a time, and no gradient checkpointing
+    (refused), whose second run of a layer may meet the next batch's."""
     from transformers import AttentionInterface, AttentionMaskInterface
     AttentionInterface.register("atlas_rows", _rows_attention)
     AttentionMaskInterface.register("atlas_rows", lambda *a, **k: None)  # the plan says which rows are valid
@@ -150,7 +151,11 @@ def attach_attention(model, check: bool = True):
         mask = args[1] if len(args) > 1 else kwargs.get("attention_mask")
         if mask is None:
             mask = torch.ones(x.shape[:2], dtype=torch.int64, device=x.device)
-        if check and bool((mask[:, 1:] > mask[:, :-1]).any()):
+        if getattr(_module, "is_gradient_checkpointing", False) and _module.training and torch.is_grad_enabled():
+            raise ValueError("attention over the valid rows: a checkpointed layer would run again with the plan of a later batch")
+        if mask.dim() != 2 or mask.shape != x.shape[:2]:
+            raise ValueError(f"attention over the valid rows: attention_mask must be {list(x.shape[:2])}, got {list(mask.shape)}")
+        if check and bool(((mask[:, 1:] > mask[:, :-1]) | (mask[:, 1:] * mask[:, 1:] != mask[:, 1:])).any()):
             raise ValueError("attention over the valid rows: attention_mask must be ones followed by zeros in every row")
         holder.plan = batch_plan(mask)
 

@@ -396,7 +396,9 @@ def attention(q, k, v, plan: SeqPlan, scale: float | None = None):
     plan.stride, a packed one outer = 1. scale: D ** -0.5 if not given. Returns out (q's shape, memory
     [outer, rows, H, D]) and the log-sum-exp of the scores, fp32 [outer, H, rows]; both zero in rows of
     no sequence, whose inputs are never read (they may hold NaN). Differentiable in q, k and v (not
-    through the log-sum-exp)."""
+    through the log-sum-exp), once. A query whose scores are all -inf has log-sum-exp -inf and an output of
+    NaN. A backward pass that goes into a CUDA graph calls attention_grad: autograd's own must not be captured
+    while an eager graph of the same leaves is alive."""
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _Attention.apply(q, k, v, plan.cu, plan.blocks, plan.counts, plan.stride, scale)

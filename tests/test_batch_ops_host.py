@@ -107,6 +107,17 @@ def test_model_side_on_the_cpu():
     mask[0, 2] = 0
     with pytest.raises(ValueError, match="ones followed by zeros"):
         model(input_ids=ids, attention_mask=mask)
+    mask[0] = 2
+    with pytest.raises(ValueError, match="ones followed by zeros"):
+        model(input_ids=ids, attention_mask=mask)
+    with pytest.raises(ValueError, match="attention_mask must be"):
+        model(input_ids=ids, attention_mask=torch.ones(2, 5, dtype=torch.int64))
+    model.train()
+    model.gradient_checkpointing_enable()
+    with pytest.raises(ValueError, match="checkpointed"):
+        model(input_ids=ids, attention_mask=torch.ones_like(ids))
+    model.gradient_checkpointing_disable()
+    model.eval()
     hook.remove()
     model.set_attn_implementation("sdpa")
     assert torch.equal(model(input_ids=ids, attention_mask=torch.ones_like(mask)).last_hidden_state, before)
