@@ -10,9 +10,10 @@
 // dimension (the 16 tx of a half warp hit distinct banks, the ty broadcast). The next tile's rows are in
 // registers on their way while this one is worked on. Scores are in base 2 (the queries carry scale log2 e). The
 // exponents' reference is the maximum of a row's first tile; fp32 has range for 2^64 above it, and only a sum
-// beyond that (or no reference yet: scores of -inf so far) raises it and rescales. The gradient is two kernels, one CTA per key tile (dk, dv; all query
-// heads of its key head, one after the other) and one per query tile (dq): scores are computed twice, but no
-// sum crosses CTAs, so every result is the same from run to run.
+// beyond that (or no reference yet: scores of -inf so far) raises it and rescales. The gradient is two kernels, one CTA per key
+// tile (dk, dv; all query heads of its key head, one after the other) and one per query tile (dq): scores are
+// computed twice, but no sum crosses CTAs, so every result is the same from run to run. 40 sequences of 32 to 402 rows, 20 heads of 16,
+// fp32: 196 us forward (3 GFLOP, 0.21 of the FMA rate: the tiles' shared-memory reads and the exponentials' issue).
 #include "attn.cuh"
 
 namespace atlas {
@@ -503,8 +504,8 @@ __device__ __forceinline__ void delta_rows(const AttnArgs& a, const SeqBlock& s,
 }
 
 // Before the gradient's kernels: delta, and the gradients of short sequences; for the tensor-core kernel also
-// the list of its blocks, and zero to the rows that it does not write. 16-bit: 160 MB of out and dout in 44 us,
-// 3.6 TB/s; what bounds it is the latency of a CTA's loads, two for its entry, then four rows of a thread at once.
+// the list of its blocks, and zero to the rows that it does not write. 16-bit: 160 MB of out and dout in 39 us,
+// 4.1 TB/s; what bounds it is the latency of a CTA's loads, two for its entry, then four rows of a thread at once.
 template <int DT, bool VEC>
 __global__ void __launch_bounds__(kThreads, 4) attn_delta_kernel(const AttnArgs a) {
   __shared__ ShortSmem sm;

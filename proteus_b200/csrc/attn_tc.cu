@@ -123,6 +123,10 @@ __device__ __forceinline__ int up16(int n) { return (n + 15) & ~15; }
 //
 // The last tile of a sequence of several ends at the sequence's end and starts inside the tile before: its
 // columns `lo` .. are new, the ones below count as -inf, and no row behind the end is read.
+//
+// Measured: 109 sequences of 271 to 302 rows, 20 heads of 64, bf16: 118 us (323 MB, 2.7 TB/s; 46 GFLOP, 390 TFLOP/s; the
+// exponentials alone 39 us at 16 a clock and SM); 4 of 1 to 4096, 16 heads over 4: 185 us (107 GFLOP, 578 TFLOP/s);
+// one of 37, 20 heads of 24: 6 us.
 constexpr int kFwdThreads = 384;
 constexpr int KT = 96;
 constexpr int kFwdStages = 3;
@@ -569,8 +573,8 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
 // tiles of 64 rows B0, B1 (q, dout or k, v) come in turn:
 //   S = A0 B0^T, dP = A1 B1^T, and with the 16-bit P and dS, written over them, as A operands
 //   keys: dv += P B1, dk += dS B0;  queries: dq += dS B0.
-// One persistent CTA per SM takes items of the list (attn_delta_kernel's) from a counter and runs their tiles as one stream, so that an
-// item's start (look-up, first loads) and end (reading the sums) hide behind its neighbours:
+// One persistent CTA per SM takes items of the list (attn_delta_kernel's) from a counter and runs their tiles as
+// one stream, so that an item's start (look-up, first loads) and end (reading the sums) hide behind its neighbours:
 //   warps 0-11  three groups of four, each takes every third tile: one thread per row
 //   warps 12-15 read an item's sums and write them out, while the groups are at the next item
 //   warp 16     TMA: items, A tiles (ring of 3), B tiles with the queries' log-sum-exp and delta (ring)
@@ -578,6 +582,9 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
 //   warp 18     dP
 //   warp 19     sums (products of two small kinds cost their issuing warp 500 clocks a tile each)
 // TMEM: three buffers of S and dP (columns 128 x, 128 x + 64), the sums in 384-447 (dv) and 448-511.
+//
+// Measured (as the forward): 320 us (115 GFLOP that the formulas need, 359 TFLOP/s) and 399 us (267 GFLOP, 670 TFLOP/s).
+// A tile of 128 x 64 scores takes 1370 clocks; its products 590 (keys) and 470 (queries), its exponentials 512.
 constexpr int kBwdThreads = 640;
 constexpr int kGroups = 3;
 constexpr int BN = 64;

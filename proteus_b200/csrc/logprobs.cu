@@ -131,7 +131,9 @@ __device__ __forceinline__ float logprob_of(float x, const Stat& s, float lz, fl
 
 // ------------------------------------------------------------------------------------ short rows
 // V <= 32 NE: a warp keeps a whole row in registers (v = lane + 32 e). The alternatives are n rounds
-// of two warp reductions (largest key, then lowest index among its holders).
+// of two warp reductions (largest key, then lowest index among its holders). 30973 x 33 bf16: 9 us without
+// alternatives, 16 with five (2 MB: the reductions, one after the other, are what it takes); 8191 x 33 fp32 with 20
+// tokens 5.5 us.
 template <int DT, int NE>
 __global__ void __launch_bounds__(256) logprobs_short_kernel(const LpArgs a) {
   using T = typename Elem<DT>::T;
@@ -582,7 +584,7 @@ __device__ __forceinline__ float grad_of(const RowGrad& r, float x) {
   return r.none ? 0.f : p * fmaf(-r.b, fmaxf(y, -1000.f), r.a);
 }
 
-// V <= 32 NE: one warp per row.
+// V <= 32 NE: one warp per row. 30973 x 33 bf16: 7.6 us.
 template <int DT, int NE>
 __global__ void __launch_bounds__(256) logprobs_grad_short_kernel(const GradArgs a) {
   using T = typename Elem<DT>::T;
@@ -637,6 +639,7 @@ __global__ void __launch_bounds__(256) logprobs_grad_short_kernel(const GradArgs
 
 // Longer rows: grid (parts, rows); a CTA writes its part of the row, then the threads that hold the
 // first occurrence of a token in that part write that column again with the sum of its tokens' terms.
+// 4095 x 50003 bf16: 147 us, 5.6 TB/s, 0.85 of a copy's rate.
 constexpr int kGradThreads = 256;
 
 template <int DT>
