@@ -275,11 +275,10 @@ def seq_maps(lengths, n_rows: int, *, stride: int = 0, lead: int = 0, trail: int
         none = torch.full((n_rows,), -1, dtype=torch.int64, device=dev)
         return SeqMaps(torch.zeros(1, dtype=torch.int32, device=dev), none, none.clone(),
                        torch.full((cap, 2), -1, dtype=torch.int32, device=dev), torch.zeros(3, dtype=torch.int64, device=dev))
+    # new_empty without a dtype is the cheapest allocation: 1.3 us of the host's instead of 2.3
     cu = torch.empty(B + 1, dtype=torch.int32, device=dev)
-    blocks = torch.empty((cap, 2), dtype=torch.int32, device=dev)
     slots = torch.empty(n_rows, dtype=torch.int64, device=dev)
-    tok = torch.empty(n_rows, dtype=torch.int64, device=dev)
-    counts = torch.empty(3, dtype=torch.int64, device=dev)
+    blocks, tok, counts = cu.new_empty((cap, 2)), slots.new_empty(n_rows), slots.new_empty(3)
     need = _lib.load().atlas_seq_maps_ws_bytes(B)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     launch(dev, "atlas_seq_maps", lengths.data_ptr(), int(dt == torch.int64), B, n_rows, stride, lead, trail, ptr(seq),
@@ -291,7 +290,7 @@ def _rows_like(t, heads: int):
     """An uninitialised [outer, heads, rows, D] tensor whose memory is [outer, rows, heads, D], the
     layout the next projection reads."""
     o, _, n, d = t.shape
-    return torch.empty(o, n, heads, d, dtype=t.dtype, device=t.device).transpose(1, 2)
+    return t.new_empty_strided((o, heads, n, d), (n * heads * d, d, heads * d, 1))
 
 
 def _unit(t):
@@ -335,7 +334,7 @@ def _check_attention(q, k, v, plan):
 def _attention_forward(q, k, v, plan, scale):
     o, h, n, d, hk, B = _check_attention(q, k, v, plan)
     dev = q.device
-    out, lse = _rows_like(q, h), torch.empty(o, h, n, dtype=torch.float32, device=dev)
+    out, lse = _rows_like(q, h), q.new_empty((o, h, n), dtype=torch.float32)
     if B == 0 or out.numel() == 0:
         return out.zero_(), lse.zero_()
     q, k, v = _unit(q), _unit(k), _unit(v)
@@ -446,10 +445,11 @@ def _token_logprobs_forward(logits, tokens, top):
     if not 0 <= top <= min(32, V):
         raise ValueError(f"top must be in [0, min(32, V)], got {top} for V = {V}")
     (logits, ld), tokens = _plain_rows(logits, N, V), tokens.contiguous()
-    rank = torch.empty(tokens.shape, dtype=torch.int32, device=dev)
-    top_id = torch.empty((N, top), dtype=torch.int64, device=dev)
-    logprob, entropy, lse, top_logprob = torch.empty(N * (J + 2 + top), dtype=torch.float32, device=dev).split((N * J, N, N, N * top))
-    logprob, top_logprob = logprob.view(tokens.shape), top_logprob.view(N, top)
+    # new_empty without a dtype is the cheapest allocation: 1.3 us of the host's instead of 2.3
+    shape = tokens.shape
+    rank, top_id = torch.empty(shape, dtype=torch.int32, device=dev), tokens.new_empty((N, top))
+    logprob = torch.empty(shape, dtype=torch.float32, device=dev)
+    entropy, lse, top_logprob = logprob.new_empty(N), logprob.new_empty(N), logprob.new_empty((N, top))
     if N:
         launch(dev, "atlas_token_logprobs", logits.data_ptr(), dt, N, V, ld, tokens.data_ptr(), J, top, logprob.data_ptr(),
                rank.data_ptr(), entropy.data_ptr(), lse.data_ptr(), top_id.data_ptr(), top_logprob.data_ptr())
@@ -476,7 +476,7 @@ def token_logprobs_grad(logits, tokens, lse, entropy, g_logprob=None, g_entropy=
     if g_entropy is not None:
         g_entropy = _row_vector(logits, "g_entropy", g_entropy, (N,))
     (logits, ld), tokens = _plain_rows(logits, N, V), tokens.contiguous()
-    dx = torch.empty((N, V), dtype=logits.dtype, device=dev)
+    dx = logits.new_empty((N, V))
     if N:
         launch(dev, "atlas_token_logprobs_grad", logits.data_ptr(), dt, N, V, ld, tokens.data_ptr(), J, lse.data_ptr(),
                entropy.data_ptr(), ptr(g_logprob), ptr(g_entropy), dx.data_ptr(), V)

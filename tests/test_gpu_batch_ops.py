@@ -667,3 +667,87 @@ def test_token_logprobs_empty_and_refusals():
                 lambda: KN.token_logprobs_grad(x, t, r.lse, r.entropy, torch.ones(4, 1, device=DEV))):
         with pytest.raises(TypeError):
             bad()
+
+
+def test_attention_offsets_past_32_bits():
+    """A packed batch whose queries have more than 2^31 elements: its last sequences, with all their
+    heads, come out as they do alone."""
+    KN = _kn()
+    H, Hk, D, tail = 34, 2, 64, [77, 16, 130]
+    lens = [100] * 9990 + tail
+    n = sum(lens)
+    g = torch.Generator(device=DEV).manual_seed(0)
+    mk = lambda h: torch.empty(1, h, n, D, dtype=torch.bfloat16, device=DEV).normal_(generator=g)  # noqa: E731
+    q, k, v, do = mk(H), mk(Hk), mk(Hk), mk(H)
+    assert q.numel() > 2 ** 31
+    plan = KN.seq_maps(torch.tensor(lens, device=DEV), n).plan(0)
+    out, lse = KN.attention(q, k, v, plan)
+    grads = KN.attention_grad(do, q, k, v, out, lse, plan)
+    m = sum(tail)
+    cut = [x[:, :, -m:].contiguous() for x in (q, k, v, do)]
+    few = KN.seq_maps(torch.tensor(tail, device=DEV), m).plan(0)
+    o2, l2 = KN.attention(*cut[:3], few)
+    want = (o2, l2, *KN.attention_grad(cut[3], *cut[:3], o2, l2, few))
+    for a, b in zip((out, lse, *grads), want):
+        assert torch.equal(a[:, :, -m:], b)
+
+
+def test_token_logprobs_offsets_past_32_bits():
+    """More than 2^31 logits: the last rows come out as they do alone."""
+    KN = _kn()
+    N, V, last = 31000, 70001, 500
+    g = torch.Generator(device=DEV).manual_seed(0)
+    x = torch.empty(N, V, dtype=torch.bfloat16, device=DEV).normal_(generator=g)
+    assert x.numel() > 2 ** 31
+    tokens = torch.randint(0, V, (N, 2), generator=g, device=DEV)
+    gl = torch.randn(N, 2, generator=g, device=DEV)
+    r, w = KN.token_logprobs(x, tokens, top=3), KN.token_logprobs(x[-last:], tokens[-last:], top=3)
+    for a, b in zip(r, w):
+        assert torch.equal(a[-last:], b)
+    dx = KN.token_logprobs_grad(x, tokens, r.lse, r.entropy, gl)
+    dw = KN.token_logprobs_grad(x[-last:], tokens[-last:], w.lse, w.entropy, gl[-last:])
+    assert torch.equal(dx[-last:], dw)
+
+
+def test_two_streams_at_once():
+    """Calls under way together share nothing: the results are those of calls one after the other."""
+    KN = _kn()
+    sets = [_batch([300, 5, 170], True, 4, 2, 64, dt, seed=s)[:5] for s, dt in ((1, torch.bfloat16), (2, torch.float16))]
+    logits = [torch.randn(50, v, device=DEV) for v in (33, 20000)]
+    tokens = torch.arange(50, device=DEV)
+
+    def work(i):
+        q, k, v, do, plan = sets[i]
+        out, lse = KN.attention(q, k, v, plan)
+        return [out, lse, *KN.attention_grad(do, q, k, v, out, lse, plan), *KN.token_logprobs(logits[i], tokens % 33, top=4)]
+
+    want = [work(0), work(1)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(work(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for r in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(r, want[i]))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_expanded_and_scaled_inputs(dtype):
+    """Keys and values of one head expanded over the batch's key heads, a gradient that is one row
+    expanded, and a scale of zero: the same as with the copies."""
+    KN = _kn()
+    q, k, v, do, plan, where, on = _batch([40, 129], True, 4, 1, 32, dtype, seed=8)
+    ke, ve = k.expand(1, 2, -1, -1), v.expand(1, 2, -1, -1)
+    de = do[:, :1, :1].expand_as(q)
+    ref, tol = _plain(q, ke, ve, de, where, 32 ** -0.5)
+    out, lse = KN.attention(q, ke, ve, plan)
+    dq, dk, dv = KN.attention_grad(de, q, ke, ve, out, lse, plan)
+    _check({"out": out, "lse": lse, "dq": dq, "dk": dk, "dv": dv}, ref, tol)
+    ref, tol = _plain(q, k, v, do, where, 0.0)
+    out, lse = KN.attention(q, k, v, plan, 0.0)
+    dq, dk, dv = KN.attention_grad(do, q, k, v, out, lse, plan, 0.0)
+    _check({"out": out, "lse": lse, "dq": dq, "dk": dk, "dv": dv}, ref, tol)
