@@ -155,9 +155,91 @@ __device__ __forceinline__ void store_tile(void* dst, const Strides& st, int64_t
   }
 }
 
+// Short sequences: thread (r, c) makes the score of query r and key c, then 4 columns of a row r of a result.
+struct ShortSmem {
+  float k[kAttnShort][68], v[kAttnShort][68], q[kAttnShort][68], g[kAttnShort][68], p[kAttnShort][20], ds[kAttnShort][20];
+};
+
+__device__ __forceinline__ float4& row_of(float (&tile)[kAttnShort][68], int row, int col) {
+  return *reinterpret_cast<float4*>(&tile[row][col]);
+}
+__device__ __forceinline__ void add4(float4& acc, float w, const float4& x) {
+  acc.x = fmaf(w, x.x, acc.x);
+  acc.y = fmaf(w, x.y, acc.y);
+  acc.z = fmaf(w, x.z, acc.z);
+  acc.w = fmaf(w, x.w, acc.w);
+}
+// Columns 4 c .. of row r of a head; vec: rows of whole 16-byte pieces, so that D is a multiple of 4.
+template <int DT>
+__device__ __forceinline__ float4 short_load(const void* src, const Strides& st, const SeqBlock& b, int head, int r, int c, int D, bool vec) {
+  using T = typename Elem<DT>::T;
+  const T* p = reinterpret_cast<const T*>(src) + b.outer * st.outer + head * st.head + (b.row0 + r) * st.row + 4 * c;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (r >= b.len) return x;
+  if (vec) {
+    if (4 * c < D) {
+      alignas(16) T w[4];
+      if (sizeof(T) == 4) *reinterpret_cast<uint4*>(w) = __ldg(reinterpret_cast<const uint4*>(p));
+      else *reinterpret_cast<uint2*>(w) = __ldg(reinterpret_cast<const uint2*>(p));
+      x = make_float4(Elem<DT>::f(w[0]), Elem<DT>::f(w[1]), Elem<DT>::f(w[2]), Elem<DT>::f(w[3]));
+    }
+  } else {
+    if (4 * c < D) x.x = Elem<DT>::f(p[0]);
+    if (4 * c + 1 < D) x.y = Elem<DT>::f(p[1]);
+    if (4 * c + 2 < D) x.z = Elem<DT>::f(p[2]);
+    if (4 * c + 3 < D) x.w = Elem<DT>::f(p[3]);
+  }
+  return x;
+}
+template <int DT>
+__device__ __forceinline__ void short_store(void* dst, const Strides& st, const SeqBlock& b, int head, int r, int c, int D, const float4& x,
+                                            float f) {
+  using T = typename Elem<DT>::T;
+  T* p = reinterpret_cast<T*>(dst) + b.outer * st.outer + head * st.head + (b.row0 + r) * st.row + 4 * c;
+  const float w[4] = {x.x * f, x.y * f, x.z * f, x.w * f};
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (r < b.len && 4 * c + e < D) put<DT>(p + e, w[e]);
+}
+
 // ---------------------------------------------------------------------------------------- forward
+// A short sequence and head: 64 x 64 tiles would be empty for the most part (140 fp32 sequences of 1 to 3 rows, 40 heads
+// of 64: 204 us by those, 62 by this).
+template <int DT>
+__device__ __noinline__ void short_out(const AttnArgs& a, SeqBlock b, int head, ShortSmem& s, bool vec) {
+  const int r = threadIdx.x / kAttnShort, c = threadIdx.x % kAttnShort, len = b.len, kh = head / (a.H / a.Hk);
+  row_of(s.q, r, 4 * c) = short_load<DT>(a.q, a.sq, b, head, r, c, a.D, vec);
+  row_of(s.k, r, 4 * c) = short_load<DT>(a.k, a.sk, b, kh, r, c, a.D, vec);
+  row_of(s.v, r, 4 * c) = short_load<DT>(a.v, a.sv, b, kh, r, c, a.D, vec);
+  __syncthreads();
+  float x = kNegInf;
+  if (r < len && c < len) {
+    float sc = 0.f;
+#pragma unroll 4
+    for (int d = 0; d < a.D; d += 4) {
+      const float4 u = row_of(s.q, r, d), w = row_of(s.k, c, d);
+      sc = fmaf(u.x, w.x, fmaf(u.y, w.y, fmaf(u.z, w.z, fmaf(u.w, w.w, sc))));
+    }
+    x = sc * (a.scale * kLog2e);
+  }
+  float m = x;
+#pragma unroll
+  for (int o = kAttnShort / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+  const float ref = m == kNegInf ? 0.f : m, p = ex2(x - ref);
+  float sum = p;
+#pragma unroll
+  for (int o = kAttnShort / 2; o; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+  s.p[r][c] = p;
+  __syncwarp();  // a row's scores are of one half of a warp
+  float4 out = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int j = 0; j < len; ++j) add4(out, s.p[r][j], row_of(s.v, j, 4 * c));
+  short_store<DT>(a.out, a.so, b, head, r, c, a.D, out, 1.f / sum);
+  if (c == 0 && r < len) a.lse[(b.outer * a.H + head) * a.rows + b.row0 + r] = (ref + log2f(sum)) * kLn2;
+}
+
 template <int DT, int DP>
-__global__ void __launch_bounds__(kThreads, DP == 64 ? 2 : 3) attn_fwd_simt_kernel(const AttnArgs a, int vec) {
+__global__ void __launch_bounds__(kThreads, DP == 64 ? 2 : 3) attn_fwd_simt_kernel(const __grid_constant__ AttnArgs a, int vec) {
   extern __shared__ float sm[];
   constexpr int TILE = BT * (DP + 4);
   float *sq = sm, *sk = sm + TILE, *sv = sm + 2 * TILE, *sp = sm + 3 * TILE;
@@ -176,6 +258,10 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 2 : 3) attn_fwd_simt_kern
   }
   const int first = s.first + (blockIdx.x & 1) * BT;
   if (!s.on || first >= s.len) return;
+  if (s.len <= kAttnShort) {
+    short_out<DT>(a, s, head, *reinterpret_cast<ShortSmem*>(sm), vec);
+    return;
+  }
   const int kh = head / (a.H / a.Hk);
   Tile<DT, DP> tk, tv;
   tk.fetch(a.q, a.sq, s.outer, head, s.row0, first, s.len, a.D, vec);
@@ -347,49 +433,13 @@ __global__ void __launch_bounds__(kThreads, 2) attn_bwd_simt_kernel(const AttnAr
 // dP and delta lie close together as well, and the rounding of a 16-bit out would be the gradients' largest
 // error (bf16, D = 8, relative norm of dq 5.4e-3 at 2 keys, 4.3e-3 at 4, 3.6e-3 at 16; the rounding of the
 // result alone is 1.7e-3): here delta is sum_j P_j dP_j, and dS stays in 32 bits.
-struct ShortSmem {
-  float k[kAttnShort][68], v[kAttnShort][68], q[kAttnShort][68], g[kAttnShort][68], p[kAttnShort][20], ds[kAttnShort][20];
-};
-
 template <int DT, bool VEC>
 __device__ __forceinline__ void short_grad(const AttnArgs& a, const SeqBlock& b, int kh, ShortSmem& s) {
   using T = typename Elem<DT>::T;
   static_assert(kThreads == kAttnShort * kAttnShort && kAttnMaxDim == 4 * kAttnShort, "a thread per pair of rows");
   const int r = threadIdx.x / kAttnShort, c = threadIdx.x % kAttnShort, len = b.len, group = a.H / a.Hk;
-  auto load = [&](const void* src, const Strides& st, int head) {
-    const T* p = reinterpret_cast<const T*>(src) + b.outer * st.outer + head * st.head + (b.row0 + r) * st.row + 4 * c;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (r < len) {
-      if (VEC) {  // D is a multiple of 4
-        if (4 * c < a.D) {
-          alignas(16) T w[4];
-          if (sizeof(T) == 4) *reinterpret_cast<uint4*>(w) = __ldg(reinterpret_cast<const uint4*>(p));
-          else *reinterpret_cast<uint2*>(w) = __ldg(reinterpret_cast<const uint2*>(p));
-          x = make_float4(Elem<DT>::f(w[0]), Elem<DT>::f(w[1]), Elem<DT>::f(w[2]), Elem<DT>::f(w[3]));
-        }
-      } else {
-        if (4 * c < a.D) x.x = Elem<DT>::f(p[0]);
-        if (4 * c + 1 < a.D) x.y = Elem<DT>::f(p[1]);
-        if (4 * c + 2 < a.D) x.z = Elem<DT>::f(p[2]);
-        if (4 * c + 3 < a.D) x.w = Elem<DT>::f(p[3]);
-      }
-    }
-    return x;
-  };
-  auto row_of = [](float (&tile)[kAttnShort][68], int row, int col) -> float4& { return *reinterpret_cast<float4*>(&tile[row][col]); };
-  auto add = [](float4& acc, float w, const float4& x) {
-    acc.x = fmaf(w, x.x, acc.x);
-    acc.y = fmaf(w, x.y, acc.y);
-    acc.z = fmaf(w, x.z, acc.z);
-    acc.w = fmaf(w, x.w, acc.w);
-  };
-  auto store = [&](void* dst, const Strides& st, int head, const float4& x, float f) {
-    T* p = reinterpret_cast<T*>(dst) + b.outer * st.outer + head * st.head + (b.row0 + r) * st.row + 4 * c;
-    const float w[4] = {x.x * f, x.y * f, x.z * f, x.w * f};
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (r < len && 4 * c + e < a.D) put<DT>(p + e, w[e]);
-  };
+  auto load = [&](const void* src, const Strides& st, int head) { return short_load<DT>(src, st, b, head, r, c, a.D, VEC); };
+  auto store = [&](void* dst, const Strides& st, int head, const float4& x, float f) { short_store<DT>(dst, st, b, head, r, c, a.D, x, f); };
   const bool on = r < len && c < len;
   const float* lses = a.lse + b.outer * a.H * a.rows + b.row0 + r;
   int h = kh * group;
@@ -426,9 +476,9 @@ __device__ __forceinline__ void short_grad(const AttnArgs& a, const SeqBlock& b,
     float4 dq = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
     for (int j = 0; j < len; ++j) {
-      add(dq, s.ds[r][j], row_of(s.k, j, 4 * c));
-      add(dk, s.ds[j][r], row_of(s.q, j, 4 * c));
-      add(dv, s.p[j][r], row_of(s.g, j, 4 * c));
+      add4(dq, s.ds[r][j], row_of(s.k, j, 4 * c));
+      add4(dk, s.ds[j][r], row_of(s.q, j, 4 * c));
+      add4(dv, s.p[j][r], row_of(s.g, j, 4 * c));
     }
     store(a.dq, a.sdq, h, dq, a.scale);
     __syncthreads();
@@ -570,6 +620,7 @@ namespace {
 template <int DT, int DP>
 int fwd(const AttnArgs& a, cudaStream_t st) {
   const int bytes = (3 * BT * (DP + 4) + BT * PP) * 4;
+  static_assert((3 * BT * (DP + 4) + BT * PP) * 4 >= sizeof(ShortSmem), "short sequences use the same memory");
   static bool done[64] = {};
   if (int rc = attn_smem_once(attn_fwd_simt_kernel<DT, DP>, bytes, done)) return rc;
   attn_fwd_simt_kernel<DT, DP><<<dim3((unsigned)(2 * a.cap), a.H), kThreads, bytes, st>>>(a, vec_rows(a, DT, false));

@@ -222,8 +222,11 @@ __global__ void __launch_bounds__(256) logprobs_short_kernel(const LpArgs a) {
 // keys (order << 32 | ~index), sorted over the lanes; what beats the n-th of them is collected in
 // shared memory, and every 32 of those are sorted (bitonic) and merged into the list.
 // Threads of a CTA: 128 where rows fill the GPU (4095 x 50003 bf16: 98 us, 256 threads 104, 512 144: a row's
-// start and end overlap with other rows), 512 where a cluster shares one row (65537 bf16: 14 us, 128 20).
+// start and end overlap with other rows), 512 where a cluster shares one row (65537 bf16: 14 us, 128 20). With
+// alternatives registers are kept to 64, so that 8 CTAs or 2 fit an SM: with 20 of them 950 x 74074 bf16 took 197 us without that, 145
+// with it (25 rows: 35 and 27; one row of 65537: 17 and 19).
 constexpr int long_threads(int CL) { return CL == 1 ? 128 : 512; }
+constexpr int long_ctas(int CL, bool top) { return !top ? 0 : CL == 1 ? 8 : 2; }
 constexpr int kLongUnroll = 2;
 
 __device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int o) { return __shfl_xor_sync(kFull, v, o); }
@@ -237,12 +240,13 @@ __device__ __forceinline__ uint64_t bitonic_merge(uint64_t v, int lane) {
   }
   return v;
 }
-__device__ __forceinline__ uint64_t warp_sort_desc(uint64_t v, int lane) {
+template <typename K>
+__device__ __forceinline__ K warp_sort_desc(K v, int lane) {
 #pragma unroll
   for (int k = 2; k <= 32; k <<= 1)
 #pragma unroll
     for (int o = k >> 1; o; o >>= 1) {
-      const uint64_t w = shfl_xor64(v, o);
+      const K w = __shfl_xor_sync(kFull, v, o);
       const bool first = ((lane & o) == 0) == ((lane & k) == 0);
       v = first == (v > w) ? v : w;
     }
@@ -254,50 +258,13 @@ __device__ __forceinline__ uint64_t merge_lists(uint64_t a, uint64_t b, int lane
   return bitonic_merge(a > r ? a : r, lane);
 }
 
-struct TopList {
-  uint64_t list;   // this lane's entry
-  uint64_t bar;    // the n-th entry: what must be beaten
-  uint32_t bar_hi; // its order key
-  int held;        // entries waiting in buf
-  uint64_t* buf;   // shared, 64 per warp
-  int n;
-
-  __device__ void init(uint64_t* b, int n_) {
-    list = bar = 0;
-    bar_hi = 0;
-    held = 0;
-    buf = b;
-    n = n_;
-  }
-  // The n-th largest of the lanes' own largest values: n entries at least are as large.
-  __device__ __forceinline__ void seed(float mx, int lane) {
-    const uint64_t v = warp_sort_desc((uint64_t)order_key(mx) << 32, lane);
-    bar = __shfl_sync(kFull, v, n - 1) - 1;
-    bar_hi = (uint32_t)((bar + 1) >> 32);
-  }
-  __device__ __noinline__ void flush(int lane) {
-    __syncwarp();
-    const uint64_t v = lane < held ? buf[lane] : 0;
-    const uint64_t rest = lane + 32 < held ? buf[lane + 32] : 0;
-    __syncwarp();
-    buf[lane] = rest;
-    held = max(0, held - 32);
-    list = merge_lists(list, warp_sort_desc(v, lane), lane);
-    const uint64_t nth = __shfl_sync(kFull, list, n - 1);
-    if (nth > bar) {
-      bar = nth;
-      bar_hi = (uint32_t)(bar >> 32);
-    }
-    __syncwarp();
-  }
-  __device__ __forceinline__ void offer(uint64_t key, int lane) {
-    const bool in = key > bar;
-    const uint32_t m = __ballot_sync(kFull, in);
-    if (!m) return;
-    if (in) buf[held + __popc(m & ((1u << lane) - 1))] = key;
-    held += __popc(m);
-    if (held >= 32) flush(lane);
-  }
+// A warp's alternatives, in shared memory, and their code out of line: few values of a row get there, and in
+// registers, with a copy in every vector's code, they made kernels of 95 to 130 KB.
+struct TopState {
+  uint64_t list[32];  // largest first, one a lane
+  uint64_t buf[64];   // waiting
+  uint64_t bar;       // the n-th entry: what must be beaten
+  int held;           // entries waiting
 };
 
 __device__ __forceinline__ uint64_t full_key(uint32_t k, uint32_t id) { return ((uint64_t)k << 32) | (uint32_t)~id; }
@@ -345,6 +312,88 @@ struct Vec {
   }
 };
 
+// Sorts 32 of the waiting entries and merges them into the list.
+__device__ __noinline__ void top_flush(TopState& s, int n, int lane) {
+  const int held = s.held;
+  const uint64_t v = lane < held ? s.buf[lane] : 0;
+  const uint64_t rest = lane + 32 < held ? s.buf[lane + 32] : 0;
+  const uint64_t list = merge_lists(s.list[lane], warp_sort_desc(v, lane), lane);
+  const uint64_t nth = __shfl_sync(kFull, list, n - 1), bar = s.bar;
+  __syncwarp();
+  s.list[lane] = list;
+  s.buf[lane] = rest;
+  if (lane == 0) {
+    s.held = max(0, held - 32);
+    if (nth > bar) s.bar = nth;
+  }
+  __syncwarp();
+}
+
+// Offers the first `count` values of each lane's vector, columns v .. (`on`: there are any), and returns the
+// order key that a value has to reach from now on. mx is the largest value that the lane has met: the n-th
+// largest of those is a bar too, since n entries are as large. It starts the bar, and raises it at every call
+// where few are wanted and a sort of 32 costs less than the values that would come without it (950 x 74074
+// bf16: 5 alternatives 103 us, 115 with the start alone; 20: 167 and 145).
+constexpr int kRaiseTop = 8;
+template <int DT>
+__device__ __noinline__ uint32_t top_offer(TopState& s, uint4 raw, int count, bool on, uint32_t v, float mx, int n, int lane) {
+  using T = typename Elem<DT>::T;
+  uint64_t bar = s.bar;
+  int held = s.held;
+  if (bar == 0 || n <= kRaiseTop) {
+    const uint32_t largest = order_key(mx);
+    const uint32_t nth = n == 1 ? __reduce_max_sync(kFull, largest) : __shfl_sync(kFull, warp_sort_desc(largest, lane), n - 1);
+    const uint64_t below = ((uint64_t)nth << 32) - 1;
+    if (below > bar) {
+      bar = below;
+      __syncwarp();
+      if (lane == 0) s.bar = bar;
+    }
+  }
+  uint32_t mine = 0;  // which of the lane's values reach the bar
+#pragma unroll
+  for (int i = 0; i < 16 / (int)sizeof(T); ++i) {
+    const float x = Elem<DT>::f(reinterpret_cast<const T*>(&raw)[i]);
+    mine |= (uint32_t)(on && i < count && order_key(x) >= (uint32_t)(bar >> 32)) << i;
+  }
+#pragma unroll 1
+  for (uint32_t left = __reduce_or_sync(kFull, mine); left; left &= left - 1) {
+    const int i = __ffs(left) - 1;
+    constexpr int per = 4 / sizeof(T);
+    const int w = i / per;
+    const uint32_t word = w < 2 ? (w == 0 ? raw.x : raw.y) : w == 2 ? raw.z : raw.w;
+    float x;
+    if constexpr (DT == ATLAS_F32) x = __uint_as_float(word);
+    else if constexpr (DT == ATLAS_BF16) x = __uint_as_float(i & 1 ? word & 0xFFFF0000u : word << 16);
+    else x = __half2float(__ushort_as_half((unsigned short)(i & 1 ? word >> 16 : word & 0xFFFFu)));
+    const uint64_t key = on ? full_key(order_key(x), v + i) : 0;
+    const bool in = key > bar;
+    const uint32_t m = __ballot_sync(kFull, in);
+    if (!m) continue;
+    if (in) s.buf[held + __popc(m & ((1u << lane) - 1))] = key;
+    held += __popc(m);
+    __syncwarp();
+    if (held >= 32) {
+      if (lane == 0) s.held = held;
+      __syncwarp();
+      top_flush(s, n, lane);
+      held -= 32;
+      bar = s.bar;
+    }
+  }
+  __syncwarp();
+  if (lane == 0) s.held = held;
+  __syncwarp();
+  return (uint32_t)(bar >> 32);
+}
+
+// A warp's view of them while it streams its part of a row.
+struct Top {
+  TopState* s;
+  uint32_t bar;  // order key
+  int n;
+};
+
 template <int G>
 struct Given {
   float x[G];
@@ -353,21 +402,17 @@ struct Given {
 
 // The columns v .. of one vector of this lane (`on`: there is one; the others are all -inf).
 template <int DT, int G, bool STATS, bool TOP>
-__device__ __forceinline__ void take(const Vec<DT>& q, bool on, uint32_t v, int lane, Stat& s, Given<G>& g, TopList& top) {
+__device__ __forceinline__ void take(const Vec<DT>& q, bool on, uint32_t v, int lane, Stat& s, Given<G>& g, Top& top) {
   constexpr int N = Vec<DT>::N;
   if (STATS) {
     const float mx = q.top();
     if (TOP) {
-      if (top.bar == 0) top.seed(on ? mx : kNegInf, lane);
       // NaN sorts first: the maximum passes over it, so it is looked for apart
       bool any = false;
 #pragma unroll
       for (int i = 0; i < N; ++i) any |= q.at(i) != q.at(i);
-      any |= on && order_key(mx) >= top.bar_hi;
-      if (__any_sync(kFull, any)) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) top.offer(on ? full_key(order_key(q.at(i)), v + i) : 0, lane);
-      }
+      any |= order_key(mx) >= top.bar;
+      if (__any_sync(kFull, on && any)) top.bar = top_offer<DT>(*top.s, q.raw, N, on, v, fmaxf(s.M, mx), top.n, lane);
     }
     if (mx > s.M) raise_to(s, mx);
     const float ref = ref_of(s.M);
@@ -394,10 +439,15 @@ __device__ __forceinline__ void take(const Vec<DT>& q, bool on, uint32_t v, int 
 }
 
 // One single column for each lane of a warp.
-template <int G, bool STATS, bool TOP>
-__device__ __forceinline__ void take_one(float x, bool on, uint32_t v, int lane, Stat& s, Given<G>& g, TopList& top) {
+template <int DT, int G, bool STATS, bool TOP>
+__device__ __forceinline__ void take_one(float x, bool on, uint32_t v, int lane, Stat& s, Given<G>& g, Top& top) {
   if (STATS) {
-    if (TOP) top.offer(on ? full_key(order_key(x), v) : 0, lane);
+    if (TOP) {
+      uint4 raw = make_uint4(__float_as_uint(x), 0, 0, 0);
+      if (DT == ATLAS_BF16) raw.x >>= 16;
+      if (DT == ATLAS_F16) raw.x = __half_as_ushort(__float2half_rn(x));  // exact: x is one
+      top.bar = top_offer<DT>(*top.s, raw, 1, on, v, fmaxf(s.M, x), top.n, lane);
+    }
     if (x > s.M) raise_to(s, x);
     add_term(s, x, ref_of(s.M));
   }
@@ -406,7 +456,7 @@ __device__ __forceinline__ void take_one(float x, bool on, uint32_t v, int lane,
 }
 
 template <int DT, int G, int NT, bool STATS, bool TOP>
-__device__ __forceinline__ void stream_row(const typename Elem<DT>::T* xr, int c0, int c1, Stat& s, Given<G>& g, TopList& top) {
+__device__ __forceinline__ void stream_row(const typename Elem<DT>::T* xr, int c0, int c1, Stat& s, Given<G>& g, Top& top) {
   using T = typename Elem<DT>::T;
   constexpr int VEC = 16 / sizeof(T), U = kLongUnroll;
   const int lane = threadIdx.x & 31;
@@ -418,7 +468,7 @@ __device__ __forceinline__ void stream_row(const typename Elem<DT>::T* xr, int c
   if (threadIdx.x < 32) {
     const int v = lane < head ? c0 + lane : t0 + lane - head;
     const bool on = v < c1;
-    take_one<G, STATS, TOP>(on ? Elem<DT>::f(xr[v]) : kNegInf, on, v, lane, s, g, top);
+    take_one<DT, G, STATS, TOP>(on ? Elem<DT>::f(xr[v]) : kNegInf, on, v, lane, s, g, top);
   }
   // U vectors of a thread are under way while the U before them are worked on
   const uint4* xv = reinterpret_cast<const uint4*>(xr + b0);
@@ -450,14 +500,14 @@ __device__ __forceinline__ void stream_row(const typename Elem<DT>::T* xr, int c
 
 template <int NT>
 struct LongSmem {
-  uint64_t buf[NT / 32][64];
+  TopState top[NT / 32];
   uint64_t list[32];
   Stat warp[NT / 32], cta;
   int cnt[kMaxGiven];
 };
 
 template <int DT, int G, int CL, bool TOP>
-__global__ void __launch_bounds__(long_threads(CL)) logprobs_long_kernel(const LpArgs a) {
+__global__ void __launch_bounds__(long_threads(CL), long_ctas(CL, TOP)) logprobs_long_kernel(const LpArgs a) {
   using T = typename Elem<DT>::T;
   constexpr int NT = long_threads(CL), NW = NT / 32;
   __shared__ LongSmem<NT> sm;
@@ -468,8 +518,11 @@ __global__ void __launch_bounds__(long_threads(CL)) logprobs_long_kernel(const L
   const T* xr = reinterpret_cast<const T*>(a.x) + row * a.ld;
   const int c0 = (int)((int64_t)V * part / CL), c1 = (int)((int64_t)V * (part + 1) / CL);
   Stat s{kNegInf, 0.f, 0.f};
-  TopList top;
-  top.init(sm.buf[w], max(a.top, 1));
+  Top top{&sm.top[w], 0, max(a.top, 1)};
+  if (TOP) {
+    sm.top[w].list[lane] = 0;
+    if (lane == 0) sm.top[w].bar = sm.top[w].held = 0;
+  }
   if (threadIdx.x < kMaxGiven) sm.cnt[threadIdx.x] = 0;
   __syncthreads();
   for (int j0 = 0; j0 == 0 || j0 < a.J; j0 += G) {
@@ -491,32 +544,31 @@ __global__ void __launch_bounds__(long_threads(CL)) logprobs_long_kernel(const L
   s = warp_join(s);
   if (lane == 0) sm.warp[w] = s;
   if (TOP) {
-    while (top.held > 0) top.flush(lane);
-    sm.buf[w][lane] = top.list;
+    while (sm.top[w].held > 0) top_flush(sm.top[w], top.n, lane);
   }
   __syncthreads();
   for (int o = NW / 2; TOP && o; o >>= 1) {
-    if (w < o) sm.buf[w][lane] = merge_lists(sm.buf[w][lane], sm.buf[w + o][lane], lane);
+    if (w < o) sm.top[w].list[lane] = merge_lists(sm.top[w].list[lane], sm.top[w + o].list[lane], lane);
     __syncthreads();
   }
   if (w == 0) {
     s = lane < NW ? sm.warp[lane] : Stat{kNegInf, 0.f, 0.f};
     s = warp_join(s);
     if (lane == 0) sm.cta = s;
-    sm.list[lane] = TOP ? sm.buf[0][lane] : 0;
+    sm.list[lane] = TOP ? sm.top[0].list[lane] : 0;
   }
   cg::cluster_group cl = cg::this_cluster();
   if (CL > 1) cl.sync();
   if (CL > 1 && TOP && part == 0) {  // the parts' lists, merged by a tree of warps
-    if (w < CL) sm.buf[w][lane] = cl.map_shared_rank(&sm, w < CL ? w : 0)->list[lane];
+    if (w < CL) sm.top[w].list[lane] = cl.map_shared_rank(&sm, w < CL ? w : 0)->list[lane];
     __syncthreads();
     for (int o = CL / 2; o; o >>= 1) {
-      if (w < o) sm.buf[w][lane] = merge_lists(sm.buf[w][lane], sm.buf[w + o][lane], lane);
+      if (w < o) sm.top[w].list[lane] = merge_lists(sm.top[w].list[lane], sm.top[w + o].list[lane], lane);
       __syncthreads();
     }
   }
   if (part == 0 && w == 0) {
-    const uint64_t list = CL > 1 ? sm.buf[0][lane] : sm.list[lane];
+    const uint64_t list = CL > 1 ? sm.top[0].list[lane] : sm.list[lane];
     if (CL > 1) {
       s = lane < CL ? cl.map_shared_rank(&sm, lane < CL ? lane : 0)->cta : Stat{kNegInf, 0.f, 0.f};
       s = warp_join(s);
