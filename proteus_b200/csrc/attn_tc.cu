@@ -316,7 +316,9 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
     }
-    if ((z == 0 || mbar_wait_soon(&s.spare_empty, (z - 1) & 1, 217)) && elect_one()) {
+    if (z) mbar_wait_soon(&s.spare_empty, (z - 1) & 1, 217);
+    __syncwarp();
+    if (elect_one()) {  // the end, whatever happened
       s.spare = make_int2(-1, 0);
       mbar_arrive(&s.spare_full);
     }
@@ -395,8 +397,8 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
   } else if (warp == 11) {
     regs_dec<40>();
     // Rows of no sequence: 6 us of 125 when the warp that loads the tiles did it in between (109 sequences of 271
-    // to 302 rows in a batch of 302, 20 heads). It posts the end whatever happens, and this wait may be as long as the
-    // kernel, so its limit is a thousand others.
+    // to 302 rows in a batch of 302, 20 heads). The end is posted whatever happens there, and a wait for the next may be
+    // as long as the kernel, so that its limit is a thousand others.
 #pragma unroll 1
     for (int z = 0, tries = 0; tries < 1000;) {
       if (!mbar_poll(&s.spare_full, z & 1)) {
