@@ -48,6 +48,8 @@ def test_attention_refusals():
         a = args(**kw)
         assert lib.atlas_attention_grad(p, p, p, p, p, p, *a, p, p, p, p, 1 << 20, None) == 1
         assert word in lib.atlas_last_error(), kw
+    # 2 x 200 rows: the row maps' table has 400 / 128 + 2 + 1 entries, and with fewer some rows would be left out
+    assert lib.atlas_attention(p, p, p, *args(rows=200, cap=5), p, p, None) == 1 and b"too few" in lib.atlas_last_error()
     assert lib.atlas_attention(None, p, p, *args(), p, p, None) == 1 and b"null pointer" in lib.atlas_last_error()
     assert lib.atlas_attention(p, p, p, 1, None, 2, 8, 4, 2, 16, p, p, p, 2, 3, 0, 1.0, p, p, None) == 1
     need = lib.atlas_attention_grad_ws_bytes(2, 8, 4, 2, 2)

@@ -751,3 +751,17 @@ def test_expanded_and_scaled_inputs(dtype):
     out, lse = KN.attention(q, k, v, plan, 0.0)
     dq, dk, dv = KN.attention_grad(do, q, k, v, out, lse, plan, 0.0)
     _check({"out": out, "lse": lse, "dq": dq, "dk": dk, "dv": dv}, ref, tol)
+
+
+@pytest.mark.parametrize("packed", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("B", [1, 40])
+def test_attention_of_empty_sequences_only(B, dtype, packed):
+    """Nothing to attend to: zeros, from inputs that are NaN throughout."""
+    KN = _kn()
+    q, k, v, do, plan, _, on = _batch([0] * B, packed, 4, 2, 32, dtype, extra=7)
+    assert not on.any() and q.isnan().all()
+    out, lse = KN.attention(q, k, v, plan)
+    for t in (out, lse, *KN.attention_grad(do, q, k, v, out, lse, plan)):
+        assert (t == 0).all()
+
