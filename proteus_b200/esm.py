@@ -155,7 +155,7 @@ def attach_attention(model, check: bool = True):
             raise ValueError("attention over the valid rows: a checkpointed layer would run again with the plan of a later batch")
         if mask.dim() != 2 or mask.shape != x.shape[:2]:
             raise ValueError(f"attention over the valid rows: attention_mask must be {list(x.shape[:2])}, got {list(mask.shape)}")
-        if check and bool(((mask[:, 1:] > mask[:, :-1]) | (mask[:, 1:] * mask[:, 1:] != mask[:, 1:])).any()):
+        if check and bool((mask * mask != mask).any() | (mask[:, 1:] > mask[:, :-1]).any()):
             raise ValueError("attention over the valid rows: attention_mask must be ones followed by zeros in every row")
         holder.plan = batch_plan(mask)
 
