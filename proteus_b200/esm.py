@@ -112,7 +112,7 @@ def attach(model, sink):
 
 
 class _RowsPlan:
-    """The plan of the forward that is under way, shared by a model's attention modules."""
+    """The plan of the forward that is under way, shared by a model's attention modules; None between forwards."""
     plan = None
 
 
@@ -120,7 +120,11 @@ def _rows_attention(module, query, key, value, attention_mask, scaling=None, dro
     """transformers' attention interface over kernels.attention: [B, H, L, D] in, [B, L, H, D] out."""
     if dropout or kw.get("is_causal"):
         raise ValueError("attention over the valid rows has neither dropout nor a causal mask")
-    out, _ = KN.attention(query, key, value, module.atlas_plan.plan, scaling)
+    plan = module.atlas_plan.plan
+    if plan is None:
+        raise RuntimeError("attention over the valid rows outside a forward of the model that attach_attention was given: "
+                           "no batch's rows are known here (a layer called alone, run again by a checkpoint, or after the handle's remove)")
+    out, _ = KN.attention(query, key, value, plan, scaling)
     return out.transpose(1, 2), None
 
 
@@ -130,37 +134,67 @@ def batch_plan(attention_mask: torch.Tensor) -> "KN.SeqPlan":
     return KN.seq_maps(attention_mask.sum(1, dtype=torch.int64), B * L, stride=L).plan(L)
 
 
-def attach_attention(model, check: bool = True):
+def _plan_of(model) -> _RowsPlan:
+    """The plan that the layers of `model` read: found through the model, so that a copy of it has its own."""
+    return model.encoder.layer[0].attention.self.atlas_plan
+
+
+def _set_plan(check, model, args, kwargs):
+    x = args[0] if args else kwargs.get("input_ids")
+    if x is None:
+        x = kwargs["inputs_embeds"]
+    mask = args[1] if len(args) > 1 else kwargs.get("attention_mask")
+    if mask is None:
+        mask = torch.ones(x.shape[:2], dtype=torch.int64, device=x.device)
+    if getattr(model, "is_gradient_checkpointing", False) and model.training and torch.is_grad_enabled():
+        raise ValueError("attention over the valid rows: a checkpointed layer would run again after the batch's plan is gone")
+    if mask.dim() != 2 or mask.shape != x.shape[:2]:
+        raise ValueError(f"attention over the valid rows: attention_mask must be {list(x.shape[:2])}, got {list(mask.shape)}")
+    if check and bool((mask * mask != mask).any() | (mask[:, 1:] > mask[:, :-1]).any()):
+        raise ValueError("attention over the valid rows: attention_mask must be ones followed by zeros in every row")
+    _plan_of(model).plan = batch_plan(mask)
+
+
+def _clear_plan(model, args, output):
+    _plan_of(model).plan = None
+
+
+class AttentionHandle:
+    """The hooks of attach_attention. remove() takes them off; until model.set_attn_implementation puts another
+    attention back, a forward then raises."""
+
+    def __init__(self, *handles):
+        self._handles = handles
+
+    def remove(self):
+        for h in self._handles:
+            h.remove()
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.remove()
+
+
+def attach_attention(model, check: bool = True) -> AttentionHandle:
     """Let every attention layer of `model` run kernels.attention over the valid rows of its batch; returns
-    the hook handle (model.set_attn_implementation puts another attention back). The batch's attention_mask
+    the hooks' handle (model.set_attn_implementation puts another attention back). The batch's attention_mask
     has to be ones followed by zeros, as Batch's are; `check` looks at it, which waits for the device once a
     forward, so a loop that builds its masks so itself turns it off. Rows of padding come out of attention
-    as zeros. The plan of a forward is the model's: one forward at a time, and no gradient checkpointing
-    (refused), whose second run of a layer may meet the next batch's."""
+    as zeros. The plan of a batch is the model's, from the start of its forward to the end: one forward at a
+    time, and a layer that runs outside one raises (called alone, or again by a checkpoint in the backward pass;
+    gradient checkpointing of the model is refused at once). A copy of the model has a plan of its own."""
+    from functools import partial
     from transformers import AttentionInterface, AttentionMaskInterface
     AttentionInterface.register("atlas_rows", _rows_attention)
     AttentionMaskInterface.register("atlas_rows", lambda *a, **k: None)  # the plan says which rows are valid
     holder = _RowsPlan()
     for layer in model.encoder.layer:
         layer.attention.self.atlas_plan = holder
-
-    def hook(_module, args, kwargs):
-        x = args[0] if args else kwargs.get("input_ids")
-        if x is None:
-            x = kwargs["inputs_embeds"]
-        mask = args[1] if len(args) > 1 else kwargs.get("attention_mask")
-        if mask is None:
-            mask = torch.ones(x.shape[:2], dtype=torch.int64, device=x.device)
-        if getattr(_module, "is_gradient_checkpointing", False) and _module.training and torch.is_grad_enabled():
-            raise ValueError("attention over the valid rows: a checkpointed layer would run again with the plan of a later batch")
-        if mask.dim() != 2 or mask.shape != x.shape[:2]:
-            raise ValueError(f"attention over the valid rows: attention_mask must be {list(x.shape[:2])}, got {list(mask.shape)}")
-        if check and bool((mask * mask != mask).any() | (mask[:, 1:] > mask[:, :-1]).any()):
-            raise ValueError("attention over the valid rows: attention_mask must be ones followed by zeros in every row")
-        holder.plan = batch_plan(mask)
-
     model.set_attn_implementation("atlas_rows")
-    return model.register_forward_pre_hook(hook, with_kwargs=True)
+    return AttentionHandle(model.register_forward_pre_hook(partial(_set_plan, check), with_kwargs=True),
+                           model.register_forward_hook(_clear_plan, always_call=True))
 
 
 def lm_head(model, name: str | None = None, seed: int = 0):

@@ -40,3 +40,102 @@ def test_masks_of_one_column_and_good_ones():
         mask = torch.tensor(mask)
         with pytest.raises(AtlasKernelError):
             model(input_ids=torch.full((1, 3), 5), attention_mask=mask)
+
+
+@pytest.fixture
+def plans(monkeypatch):
+    """Attention and row maps replaced by stand-ins that run on the CPU: the list gets the lengths that each layer's
+    attention was given."""
+    seen = []
+
+    class Maps:
+        def __init__(self, lengths):
+            self.lengths = lengths.tolist()
+
+        def plan(self, stride):
+            return self.lengths
+
+    def attention(q, k, v, plan, scale=None):
+        seen.append(plan)
+        return torch.zeros_like(q), None
+
+    monkeypatch.setattr(esm.KN, "seq_maps", lambda lengths, rows, stride: Maps(lengths))
+    monkeypatch.setattr(esm.KN, "attention", attention)
+    return seen
+
+
+def _mask(*lens, width=6):
+    return (torch.arange(width) < torch.tensor(lens)[:, None]).long()
+
+
+IDS = torch.full((2, 6), 5)
+
+
+def test_a_copy_of_the_model_has_its_own_plan(plans):
+    """Made after a forward, the copy's attention follows the copy's batches, and the other way round."""
+    import copy
+    import io
+    model = _tiny()
+    esm.attach_attention(model)
+    model(input_ids=IDS, attention_mask=_mask(6, 6))
+    other = copy.deepcopy(model)
+    plans.clear()
+    other(input_ids=IDS, attention_mask=_mask(3, 3))
+    model(input_ids=IDS, attention_mask=_mask(2, 5))
+    other(input_ids=IDS, attention_mask=_mask(1, 4))
+    assert plans == [[3, 3]] * 2 + [[2, 5]] * 2 + [[1, 4]] * 2
+    f = io.BytesIO()
+    torch.save(other, f)
+    f.seek(0)
+    plans.clear()
+    torch.load(f, weights_only=False)(input_ids=IDS, attention_mask=_mask(5, 1))
+    assert plans == [[5, 1]] * 2
+
+
+def test_the_plan_ends_with_the_forward(plans):
+    """What runs a layer outside the model's forward has no batch's plan, least of all the last batch's."""
+    model = _tiny()
+    hook = esm.attach_attention(model)
+    model(input_ids=IDS, attention_mask=_mask(6, 2))
+    plans.clear()
+    states = torch.zeros(2, 6, 16)
+    for call in (lambda: model.encoder(states), lambda: model.encoder.layer[1](states)):
+        with pytest.raises(RuntimeError, match="outside a forward"):
+            call()
+    hook.remove()
+    with pytest.raises(RuntimeError, match="outside a forward"):
+        model(input_ids=IDS, attention_mask=_mask(3, 3))
+    model.set_attn_implementation("sdpa")
+    model(input_ids=IDS, attention_mask=_mask(3, 3))
+    assert not plans
+    with esm.attach_attention(model):
+        model(input_ids=IDS, attention_mask=_mask(3, 3))
+    assert plans == [[3, 3]] * 2
+
+
+def test_a_failed_forward_leaves_no_plan(plans, monkeypatch):
+    model = _tiny()
+    esm.attach_attention(model)
+    with monkeypatch.context() as m:
+        m.setattr(model.encoder.layer[1].output, "forward", lambda *a: 1 / 0)
+        with pytest.raises(ZeroDivisionError):
+            model(input_ids=IDS, attention_mask=_mask(6, 6))
+    with pytest.raises(RuntimeError, match="outside a forward"):
+        model.encoder(torch.zeros(2, 6, 16))
+    with pytest.raises(ValueError):
+        model(input_ids=IDS, attention_mask=_mask(6, 6, width=7))
+    with pytest.raises(RuntimeError, match="outside a forward"):
+        model.encoder(torch.zeros(2, 6, 16))
+
+
+def test_a_checkpoint_that_runs_a_layer_again_raises(plans):
+    """torch.utils.checkpoint around a layer: its second run comes in the backward pass, after the forward."""
+    from torch.utils.checkpoint import checkpoint
+    model = _tiny()
+    esm.attach_attention(model)
+    layer = model.encoder.layer[0]
+    first = layer.forward
+    layer.forward = lambda *a, **k: checkpoint(first, *a, use_reentrant=False, **k)
+    out = model(input_ids=IDS, attention_mask=_mask(6, 6)).last_hidden_state
+    with pytest.raises(RuntimeError, match="outside a forward"):
+        out.sum().backward()
