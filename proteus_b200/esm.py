@@ -118,7 +118,7 @@ class _RowsPlan:
 
 def _rows_attention(module, query, key, value, attention_mask, scaling=None, dropout=0.0, **kw):
     """transformers' attention interface over kernels.attention: [B, H, L, D] in, [B, L, H, D] out."""
-    if dropout or kw.get("is_causal"):
+    if dropout or kw.get("is_causal") or getattr(module, "is_causal", False):
         raise ValueError("attention over the valid rows has neither dropout nor a causal mask")
     plan = module.atlas_plan.plan
     if plan is None:
@@ -184,9 +184,12 @@ def attach_attention(model, check: bool = True) -> AttentionHandle:
     forward, so a loop that builds its masks so itself turns it off. Rows of padding come out of attention
     as zeros. The plan of a batch is the model's, from the start of its forward to the end: one forward at a
     time, and a layer that runs outside one raises (called alone, or again by a checkpoint in the backward pass;
-    gradient checkpointing of the model is refused at once). A copy of the model has a plan of its own."""
+    gradient checkpointing of the model is refused at once). A copy of the model has a plan of its own. A decoder
+    (causal scores, or cross-attention) is refused."""
     from functools import partial
     from transformers import AttentionInterface, AttentionMaskInterface
+    if model.config.is_decoder or model.config.add_cross_attention:
+        raise ValueError("attention over the valid rows: every row attends to every row of its sequence, and this model is a decoder")
     AttentionInterface.register("atlas_rows", _rows_attention)
     AttentionMaskInterface.register("atlas_rows", lambda *a, **k: None)  # the plan says which rows are valid
     holder = _RowsPlan()

@@ -9,12 +9,12 @@ from proteus_b200 import esm
 from proteus_b200._lib import AtlasKernelError
 
 
-def _tiny(seed=0):
+def _tiny(seed=0, **kw):
     from transformers import EsmConfig, EsmModel
     torch.manual_seed(seed)
     cfg = EsmConfig(vocab_size=33, hidden_size=16, num_hidden_layers=2, num_attention_heads=2, intermediate_size=32,
                     max_position_embeddings=64, position_embedding_type="rotary", pad_token_id=1, mask_token_id=32,
-                    token_dropout=True, hidden_dropout_prob=0.0, attention_probs_dropout_prob=0.0)
+                    token_dropout=True, hidden_dropout_prob=0.0, attention_probs_dropout_prob=0.0, **kw)
     return EsmModel(cfg, add_pooling_layer=False).eval()
 
 
@@ -139,3 +139,20 @@ def test_a_checkpoint_that_runs_a_layer_again_raises(plans):
     out = model(input_ids=IDS, attention_mask=_mask(6, 6)).last_hidden_state
     with pytest.raises(RuntimeError, match="outside a forward"):
         out.sum().backward()
+
+
+@pytest.mark.parametrize("kw", [{"is_decoder": True}, {"is_decoder": True, "add_cross_attention": True}], ids=str)
+def test_decoders_are_refused(kw):
+    """Their scores are causal, which attention over all rows of a sequence is not."""
+    model = _tiny(**kw)
+    with pytest.raises(ValueError, match="decoder"):
+        esm.attach_attention(model)
+    assert model.config._attn_implementation != "atlas_rows"
+
+
+def test_a_layer_made_causal_afterwards(plans):
+    model = _tiny()
+    esm.attach_attention(model)
+    model.encoder.layer[1].attention.self.is_causal = True
+    with pytest.raises(ValueError, match="causal"):
+        model(input_ids=IDS, attention_mask=_mask(6, 6))
