@@ -9,6 +9,7 @@ import struct
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import call, dtype_code, launch, ptr, require_cuda, stream_ptr
@@ -218,6 +219,14 @@ def _same_device(first, **others):
             raise ValueError(f"{name} is on {t.device}, the first argument on {first.device}")
 
 
+def _refuse_tangents(**tensors):
+    """Forward-mode derivatives: a dual tensor has no requires_grad, and its result would come without a tangent."""
+    if getattr(forward_ad, "_current_level", 0) >= 0:  # a dual level is open; unpack_dual alone takes 0.8 us a tensor
+        for name, t in tensors.items():
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{name} carries a forward-mode tangent: only reverse-mode gradients are supported")
+
+
 class SeqPlan(NamedTuple):
     """Which rows of a batch's tensors belong to which sequence, as attention reads it: `cu` int32
     [B + 1] prefix sums of the lengths, `blocks` int32 [n, 2] and `counts` int64 [3] of seq_maps, and
@@ -348,7 +357,8 @@ def _attention_forward(q, k, v, plan, scale):
 def attention_grad(dout, q, k, v, out, lse, plan: SeqPlan, scale: float | None = None):
     """(dq, dk, dv) of attention(q, k, v, plan, scale) for the gradient `dout` of its output: the
     probabilities are computed again from `lse`, the keys' gradients summed over the query heads that
-    share them. No atomics: the same call gives the same bits. Rows of no sequence come out as zero."""
+    share them. No atomics on them: the same call gives the same bits. Rows of no sequence come out as zero."""
+    _refuse_tangents(dout=dout, q=q, k=k, v=v, out=out, lse=lse)
     o, h, n, d, hk, B = _check_attention(q, k, v, plan)
     dev = q.device
     if not (dout.device == dev and out.device == dev and lse.device == dev):
@@ -397,7 +407,8 @@ def attention(q, k, v, plan: SeqPlan, scale: float | None = None):
     no sequence, whose inputs are never read (they may hold NaN). Differentiable in q, k and v (not
     through the log-sum-exp), once. A query whose scores are all -inf has log-sum-exp -inf and an output of
     NaN. A backward pass that goes into a CUDA graph calls attention_grad: autograd's own must not be captured
-    while an eager graph of the same leaves is alive."""
+    while an eager graph of the same leaves is alive. Tensors with a forward-mode tangent are refused."""
+    _refuse_tangents(q=q, k=k, v=v)
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _Attention.apply(q, k, v, plan.cu, plan.blocks, plan.counts, plan.stride, scale)
@@ -468,6 +479,7 @@ def token_logprobs_grad(logits, tokens, lse, entropy, g_logprob=None, g_entropy=
     """Gradient by the logits, [N, V] in their dtype, of sum(g_logprob * logprob) + sum(g_entropy *
     entropy), from token_logprobs' lse and entropy. Either gradient may be None. A token given twice
     in a row counts twice; one outside [0, V) not at all."""
+    _refuse_tangents(logits=logits, lse=lse, entropy=entropy, g_logprob=g_logprob, g_entropy=g_entropy)
     N, V, J = _check_logits(logits, tokens)
     dt, dev = dtype_code(logits.dtype), logits.device
     lse, entropy = _row_vector(logits, "lse", lse, (N,)), _row_vector(logits, "entropy", entropy, (N,))
@@ -504,7 +516,9 @@ def token_logprobs(logits, tokens, top: int = 0) -> TokenLogprobs:
     logits are larger), the row's entropy and log-sum-exp (fp32 [N]), and the `top` (<= 32) most likely
     tokens (top_id int64, top_logprob fp32 [N, top]; ties to the lowest id). A token outside [0, V)
     means none: log probability 0, rank 0. A row of -inf only has log probabilities -inf and entropy 0.
-    logprob and entropy are differentiable in the logits."""
+    logprob and entropy are differentiable in the logits, once; a backward pass that goes into a CUDA graph calls
+    token_logprobs_grad, as with attention. Logits with a forward-mode tangent are refused."""
+    _refuse_tangents(logits=logits)
     if torch.is_grad_enabled() and logits.requires_grad:
         return TokenLogprobs(*_TokenLogprobs.apply(logits, tokens, top))
     return _token_logprobs_forward(logits, tokens, top)
