@@ -82,10 +82,13 @@ class CheckpointWriter:
     afterwards) and hands the disk write (tmp + fsync + rename), the pruning to the newest `keep`
     files and an optional follow-up (the run summary) to a background thread, so a multi-GB
     checkpoint no longer stalls the batch loop. One write is in flight at a time: a new checkpoint
-    first waits for the previous one. `wait` joins the write and re-raises its error, if any."""
+    first waits for the previous one. `wait` joins the write and re-raises its error, if any.
 
-    def __init__(self, ck_dir: Path, keep: int = 2):
-        self.ck_dir, self.keep = ck_dir, keep
+    A run resumed from a checkpoint does not repeat the batches before it, so what else was made of them
+    (`answers`, a ReadoutWriter) is on disk before the checkpoint's write begins."""
+
+    def __init__(self, ck_dir: Path, keep: int = 2, answers: "ReadoutWriter | None" = None):
+        self.ck_dir, self.keep, self.answers = ck_dir, keep, answers
         self._t = None
         self._err = None
 
@@ -100,6 +103,8 @@ class CheckpointWriter:
             self._err = e
 
     def save(self, obj, path: Path, after=None):
+        if self.answers is not None:
+            self.answers.drain(0)
         self.wait()
         self._t = threading.Thread(target=self._write, args=(obj, path, after), name="ckpt-writer")
         self._t.start()
@@ -116,8 +121,8 @@ class CheckpointWriter:
 class ReadoutWriter:
     """What the model answered, one file per batch of the plan. `put` starts the copies to pinned host memory;
     `drain(keep)` writes the batches whose copies are done, all but the newest `keep` at the latest, so that
-    the loop does not wait for the device. Written again, a batch's file has the same contents (a resumed run
-    repeats the batches after its checkpoint)."""
+    the loop does not wait for the device; a checkpoint waits for all (CheckpointWriter). Written again, a batch's
+    file has the same contents (a resumed run repeats the batches after its checkpoint)."""
 
     def __init__(self, d: Path):
         self.d = d
@@ -417,8 +422,8 @@ def main(argv=None):
     logf = open(out / ("batches.jsonl" if world == 1 else f"batches.rank{rank}.jsonl"), "a")
     ckpt_s, batch_s, last_ckpt_s = 0.0, 0.0, None
 
-    writer = CheckpointWriter(ck_dir, keep=2)
     answers = ReadoutWriter(out / "readout") if head is not None else None
+    writer = CheckpointWriter(ck_dir, keep=2, answers=answers)
 
     def save_ckpt(next_batch):
         """Snapshot now, write in the background; the time on the batch loop's path is the host copy
