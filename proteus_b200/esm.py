@@ -203,19 +203,21 @@ def attach_attention(model, check: bool = True) -> AttentionHandle:
 def lm_head(model, name: str | None = None, seed: int = 0):
     """The language-model head of an EsmModel (hidden states -> logits over its alphabet), in its dtype and on
     its device: of a local HuggingFace checkpoint directory `name`, else of the architecture with a seeded
-    random init; its projection is the model's own embedding matrix."""
+    random init. Its projection is the model's own embedding matrix (unless the checkpoint's two are not tied)."""
     import copy
     from transformers import EsmForMaskedLM
     w = model.get_input_embeddings().weight
     if name is not None and os.path.isdir(str(name)):
-        head = EsmForMaskedLM.from_pretrained(name).lm_head
+        whole = EsmForMaskedLM.from_pretrained(name)
+        head, tied = whole.lm_head, whole.config.tie_word_embeddings
     else:
         cfg = copy.deepcopy(model.config)
         cfg.num_hidden_layers = 1
         cfg._attn_implementation = "eager"
         torch.manual_seed(seed)
         with torch.device(w.device):
-            head = EsmForMaskedLM(cfg).lm_head
+            head, tied = EsmForMaskedLM(cfg).lm_head, True
+    if tied:  # as the checkpoint's own projection is; the model's embeddings may be a control's
         head.decoder.weight = w
     return head.to(device=w.device, dtype=w.dtype).eval()
 

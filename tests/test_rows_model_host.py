@@ -156,3 +156,27 @@ def test_a_layer_made_causal_afterwards(plans):
     model.encoder.layer[1].attention.self.is_causal = True
     with pytest.raises(ValueError, match="causal"):
         model(input_ids=IDS, attention_mask=_mask(6, 6))
+
+
+@pytest.mark.parametrize("tied", [True, False])
+def test_the_head_of_a_checkpoint_projects_with_the_models_embeddings(tmp_path, tied):
+    """Of a control too, whose embeddings are not the checkpoint's any more; a checkpoint with a projection of its own keeps it."""
+    from transformers import EsmForMaskedLM
+    torch.manual_seed(3)
+    cfg = _tiny().config
+    cfg.tie_word_embeddings = tied
+    whole = EsmForMaskedLM(cfg).eval()
+    with torch.no_grad():
+        whole.lm_head.bias.normal_()
+    whole.save_pretrained(tmp_path / "m")
+    own = whole.lm_head.decoder.weight
+    for control in ("none", "shuffled"):
+        model, _, _ = esm.load(str(tmp_path / "m"), control, dtype=torch.float32)
+        head = esm.lm_head(model, str(tmp_path / "m"))
+        w = model.get_input_embeddings().weight
+        assert (head.decoder.weight is w) == tied
+        assert torch.equal(head.decoder.weight, w if tied else own)
+        assert torch.equal(head.dense.weight, whole.lm_head.dense.weight) and torch.equal(head.bias, whole.lm_head.bias)
+    x = torch.randn(4, 16)
+    model, _, _ = esm.load(str(tmp_path / "m"), dtype=torch.float32)
+    assert torch.equal(esm.lm_head(model, str(tmp_path / "m"))(x), whole.lm_head(x))
