@@ -342,7 +342,8 @@ int atlas_seq_maps(const void* lengths, int lengths_i64, int64_t B, int64_t rows
  * q, k, v, out (attention) or dout, q, k, v, out, dq, dk, dv (attention_grad); unit stride along D.
  * lse: f32 [outer, H, rows] contiguous. ws: device bytes >= atlas_attention_grad_ws_bytes(...), 16-byte
  * aligned, of one call at a time. cu, blocks [cap, 2], counts: as written by atlas_seq_maps, cap at least
- * outer*rows/128 + B + 1; padded (packed = 0): outer = B, sequence b in the first cu[b+1]-cu[b] rows of outer
+ * outer*rows/128 + B + 1 (an entry that names no sequence, or a first position that is not a multiple of 128, is
+ * passed over); padded (packed = 0): outer = B, sequence b in the first cu[b+1]-cu[b] rows of outer
  * index b; packed: outer = 1, its rows are cu[b] .. cu[b+1]-1. Rows of no sequence are not read and come
  * out as zero. S, the softmax and all sums are fp32; for 16-bit tensors the probabilities and dS are rounded to
  * that type before they meet v, q, k or dout (not in the gradient of a sequence of up to 16 rows, which also

@@ -36,7 +36,8 @@ struct AttnArgs {
 
 // One entry of the block table: rows first .. first + 127 of sequence `seq`, whose rows are
 // row0 .. row0 + len - 1 of outer index `outer`. Everything is cut to the tensors' extents, so that a
-// table or prefix sums that do not belong to these tensors cannot lead outside them.
+// table or prefix sums that do not belong to these tensors cannot lead outside them; a first row that is not a
+// multiple of 128 is no entry (the gradient's bulk copies start there, which needs 16 bytes of alignment).
 struct SeqBlock {
   int seq, first, len;
   int64_t row0, outer, off;
@@ -52,7 +53,7 @@ __device__ __forceinline__ SeqBlock seq_block(const AttnArgs& a, int64_t i) {
   const int2 e = reinterpret_cast<const int2*>(a.blocks)[i];  // i < cap: both loads are under way at once
   s.spare = i >= n;
   if (s.spare) return s;
-  if (e.x < 0 || e.x >= a.B || e.y < 0) return s;
+  if (e.x < 0 || e.x >= a.B || e.y < 0 || e.y % kAttnBlock) return s;
   const int64_t c0 = a.cu[e.x], c1 = a.cu[e.x + 1];
   s.seq = e.x;
   s.first = e.y;

@@ -230,7 +230,9 @@ def _refuse_tangents(**tensors):
 class SeqPlan(NamedTuple):
     """Which rows of a batch's tensors belong to which sequence, as attention reads it: `cu` int32
     [B + 1] prefix sums of the lengths, `blocks` int32 [n, 2] and `counts` int64 [3] of seq_maps, and
-    `stride`, the rows of each sequence in a padded batch (0: packed end to end)."""
+    `stride`, the rows of each sequence in a padded batch (0: packed end to end). Attention passes over
+    entries of another table that name no sequence of the batch or a first position that is not a multiple
+    of 128, and leaves the rows of an entry that is missing as they were."""
     cu: torch.Tensor
     blocks: torch.Tensor
     counts: torch.Tensor
