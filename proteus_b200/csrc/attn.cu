@@ -48,7 +48,7 @@ extern "C" int atlas_attention(const void* q, const void* k, const void* v, int 
 }
 
 extern "C" int64_t atlas_attention_grad_ws_bytes(int64_t outer, int64_t rows, int64_t H, int64_t Hk, int64_t B) {
-  return 16 * attn_blocks(outer, rows, B) + 4 * (2 * H * attn_vec_ld(outer, rows, B) + B * Hk + 2);
+  return 16 * attn_blocks(outer, rows, B) + 4 * (3 * H * attn_vec_ld(outer, rows, B) + 2 * B * Hk + 2);
 }
 
 extern "C" int atlas_attention_grad(const void* dout, const void* q, const void* k, const void* v, const void* out,
@@ -78,8 +78,10 @@ extern "C" int atlas_attention_grad(const void* dout, const void* q, const void*
   a.list = (int4*)ws;
   a.lse2 = (float*)(a.list + attn_blocks(outer, rows, B));
   a.delta2 = a.lse2 + H * a.vec_ld;
-  a.amax = (uint32_t*)(a.delta2 + H * a.vec_ld);
-  a.counter = a.amax + B * Hk;
+  a.norm2 = a.delta2 + H * a.vec_ld;
+  a.top_dout = (uint32_t*)(a.norm2 + H * a.vec_ld);
+  a.top_v = a.top_dout + B * Hk;
+  a.counter = a.top_v + B * Hk;
   a.listed = a.counter + 1;
   return attn_tc(a, dtype, true, (cudaStream_t)stream);
 }

@@ -8,6 +8,7 @@ namespace atlas {
 constexpr int kAttnBlock = 128;  // rows of an entry of the block table
 constexpr int kAttnMaxDim = 64;
 constexpr int kAttnShort = 16;   // sequences whose gradient attn_delta_kernel makes whole
+constexpr int kProbBits = 15;    // the fp16 gradient holds a probability times 2^15
 
 struct Strides {
   int64_t outer, head, row;  // in elements; the last axis has unit stride
@@ -21,11 +22,12 @@ struct AttnArgs {
   float* lse;    // [outer, H, rows]
   // Gradient only. CUDA cores: delta [outer, H, rows]. Tensor cores: for each head, negated, the
   // log-sum-exp in base 2 and delta of all sequences, each from a place that is a multiple of 16 bytes (seq_block's off;
-  // vec_ld values a head), the largest |dout| of a sequence and key head as bits (fp16), the counter of work items,
-  // and the blocks of more than kAttnShort rows, in no order: sequence, first row, length, prefix sum.
-  float *delta, *lse2, *delta2;
+  // vec_ld values a head), the counter of work items, and the blocks of more than kAttnShort rows, in no order:
+  // sequence, first row, length, prefix sum. fp16 also: the squared norms of dout's rows (norm2, as lse2), and the
+  // largest of a sequence and key head as bits, of its query heads' rows of dout (top_dout) and of its rows of v (top_v).
+  float *delta, *lse2, *delta2, *norm2;
   int64_t vec_ld;
-  uint32_t *amax, *counter, *listed;
+  uint32_t *top_dout, *top_v, *counter, *listed;
   int4* list;
   const int32_t *cu, *blocks;
   const int64_t* counts;

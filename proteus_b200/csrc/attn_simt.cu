@@ -487,36 +487,52 @@ __device__ __forceinline__ void short_grad(const AttnArgs& a, const SeqBlock& b,
   store(a.dv, a.sdv, kh, dv, 1.f);
 }
 
+// 16 bytes, or one element, of a row: what a lane of the functions below reads of it.
+template <int DT, bool VEC>
+struct RowPart {
+  using T = typename Elem<DT>::T;
+  static constexpr int E = VEC ? 16 / sizeof(T) : 1;    // elements per load
+  static constexpr int G = VEC ? kAttnMaxDim / E : 32;  // lanes per row
+  static constexpr int PER = kThreads / G;              // rows at a time
+};
+
+__device__ __forceinline__ float sum_lanes(float v, int n) {
+  for (int m = n / 2; m; m >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, m);
+  return v;
+}
+// The largest of a warp's values (none negative; NaN is the largest) into *to, as bits, so that the order does not matter.
+__device__ __forceinline__ void raise_top(uint32_t* to, float v) {
+  const uint32_t u = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(fabsf(v)));
+  if ((threadIdx.x & 31) == 0) atomicMax(to, u);
+}
+
 // delta = sum_d dout out of the rows of a block and head, G lanes to a row: 8 lanes with 16-byte loads where
-// rows are aligned for them (VEC), else a warp. The largest |dout| as bits, so that the order of the atomics
-// does not matter.
+// rows are aligned for them (VEC), else a warp. fp16: the squared norms of dout's rows as well.
 template <int DT, bool VEC>
 __device__ __forceinline__ void delta_rows(const AttnArgs& a, const SeqBlock& s, int head) {
   using T = typename Elem<DT>::T;
-  constexpr int E = VEC ? 16 / sizeof(T) : 1;      // elements per load
-  constexpr int G = VEC ? kAttnMaxDim / E : 32;    // lanes per row
-  constexpr int PER = kThreads / G;                // rows at a time
+  constexpr int E = RowPart<DT, VEC>::E, G = RowPart<DT, VEC>::G, PER = RowPart<DT, VEC>::PER;
+  constexpr bool NORM = DT == ATLAS_F16;
   const int sub = threadIdx.x % G;
   const T* o = reinterpret_cast<const T*>(a.o) + s.outer * a.so.outer + head * a.so.head + s.row0 * a.so.row;
   const T* g = reinterpret_cast<const T*>(a.dout) + s.outer * a.sdo.outer + head * a.sdo.head + s.row0 * a.sdo.row;
   const int64_t vec_at = head * a.vec_ld + s.off, row_at = (s.outer * a.H + head) * a.rows + s.row0;
-  float amax = 0.f;
-  auto product = [&](T x, T y, float v) {
-    const float w = Elem<DT>::f(y);
-    if (DT == ATLAS_F16) amax = fabsf(w) > amax || w != w ? fabsf(w) : amax;
-    return fmaf(Elem<DT>::f(x), w, v);
-  };
+  float top = 0.f;
   constexpr int U = VEC ? 4 : 1;  // rows of a thread whose loads are under way at once
 #pragma unroll 1
   for (int k0 = 0; k0 < kAttnBlock / PER; k0 += U) {
     const int r0 = s.first + k0 * PER + (int)threadIdx.x / G;
-    float v[U], lse[U];
+    float v[U] = {}, n2[U] = {}, lse[U] = {};
     uint4 x[U], y[U];
+    auto product = [&](int u, T a0, T b0) {
+      const float w = Elem<DT>::f(b0);
+      v[u] = fmaf(Elem<DT>::f(a0), w, v[u]);
+      if (NORM) n2[u] = fmaf(w, w, n2[u]);
+    };
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int r = r0 + u * PER;
       const bool on = r < s.len;
-      v[u] = lse[u] = 0.f;
       if (VEC) {
         x[u] = y[u] = make_uint4(0, 0, 0, 0);
         if (on && sub * E < a.D) {
@@ -524,7 +540,7 @@ __device__ __forceinline__ void delta_rows(const AttnArgs& a, const SeqBlock& s,
           y[u] = __ldg(reinterpret_cast<const uint4*>(g + (int64_t)r * a.sdo.row + sub * E));
         }
       } else if (on) {
-        for (int d = sub; d < a.D; d += G) v[u] = product(o[(int64_t)r * a.so.row + d], g[(int64_t)r * a.sdo.row + d], v[u]);
+        for (int d = sub; d < a.D; d += G) product(u, o[(int64_t)r * a.so.row + d], g[(int64_t)r * a.sdo.row + d]);
       }
       if (a.lse2 && sub == 0 && on) lse[u] = a.lse[row_at + r];
     }
@@ -533,24 +549,58 @@ __device__ __forceinline__ void delta_rows(const AttnArgs& a, const SeqBlock& s,
       const int r = r0 + u * PER;
       if (VEC) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) v[u] = product(reinterpret_cast<const T*>(&x[u])[e], reinterpret_cast<const T*>(&y[u])[e], v[u]);
+        for (int e = 0; e < E; ++e) product(u, reinterpret_cast<const T*>(&x[u])[e], reinterpret_cast<const T*>(&y[u])[e]);
       }
-#pragma unroll
-      for (int m = G / 2; m; m >>= 1) v[u] += __shfl_xor_sync(0xFFFFFFFFu, v[u], m);
+      v[u] = sum_lanes(v[u], G);
+      if (NORM) n2[u] = sum_lanes(n2[u], G);
       if (sub == 0 && r < s.len) {
         if (a.lse2) {
-          a.lse2[vec_at + r] = lse[u] * -kLog2e;
+          a.lse2[vec_at + r] = fmaf(lse[u], -kLog2e, NORM ? (float)kProbBits : 0.f);
           a.delta2[vec_at + r] = -v[u];
+          if (NORM) a.norm2[vec_at + r] = n2[u];
         } else {
           a.delta[row_at + r] = v[u];
         }
       }
+      if (NORM) top = n2[u] > top || n2[u] != n2[u] ? n2[u] : top;
     }
   }
-  if (DT == ATLAS_F16 && a.lse2) {
-    const uint32_t u = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(amax));
-    if ((threadIdx.x & 31) == 0) atomicMax(a.amax + (int64_t)s.seq * a.Hk + head / (a.H / a.Hk), u);
+  if (NORM && a.lse2) raise_top(a.top_dout + (int64_t)s.seq * a.Hk + head / (a.H / a.Hk), top);
+}
+
+// The largest squared norm of rows first .. of a key head's v (fp16; see dS_scale in attn_tc.cu). Out of line: it takes
+// only what it needs, so that the kernel's arguments stay where they are.
+template <int DT, bool VEC>
+__device__ __noinline__ void value_norms(const typename Elem<DT>::T* v, int64_t stride, int first, int len, int D, uint32_t* to) {
+  using T = typename Elem<DT>::T;
+  constexpr int E = RowPart<DT, VEC>::E, G = RowPart<DT, VEC>::G, PER = RowPart<DT, VEC>::PER;
+  const int sub = threadIdx.x % G;
+  float top = 0.f;
+#pragma unroll 4
+  for (int k = 0; k < kAttnBlock / PER; ++k) {
+    const int r = first + k * PER + (int)threadIdx.x / G;
+    float n2 = 0.f;
+    if (r < len) {
+      if (VEC) {
+        if (sub * E < D) {
+          const uint4 x = __ldg(reinterpret_cast<const uint4*>(v + (int64_t)r * stride + sub * E));
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const float w = Elem<DT>::f(reinterpret_cast<const T*>(&x)[e]);
+            n2 = fmaf(w, w, n2);
+          }
+        }
+      } else {
+        for (int d = sub; d < D; d += G) {
+          const float w = Elem<DT>::f(v[(int64_t)r * stride + d]);
+          n2 = fmaf(w, w, n2);
+        }
+      }
+    }
+    n2 = sum_lanes(n2, G);
+    top = n2 > top || n2 != n2 ? n2 : top;
   }
+  raise_top(to, top);
 }
 
 // Before the gradient's kernels: delta, and the gradients of short sequences; for the tensor-core kernel also
@@ -579,6 +629,9 @@ __global__ void __launch_bounds__(kThreads, 4) attn_delta_kernel(const AttnArgs 
       if (i < attn_blocks(a.outer, a.rows, a.B)) a.list[i] = make_int4(s.seq, s.first, s.len, a.cu[s.seq]);
     }
     delta_rows<DT, VEC>(a, s, head);
+    if (DT == ATLAS_F16 && a.lse2 && head < a.Hk)
+      value_norms<DT, VEC>(reinterpret_cast<const typename Elem<DT>::T*>(a.v) + s.outer * a.sv.outer + head * a.sv.head + s.row0 * a.sv.row,
+                           a.sv.row, s.first, s.len, a.D, a.top_v + (int64_t)s.seq * a.Hk + head);
   } else if (s.first == 0 && head < a.Hk) {
     short_grad<DT, VEC>(a, s, head, sm);
   }

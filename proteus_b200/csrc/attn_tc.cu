@@ -609,12 +609,25 @@ struct BwdSmem {
   uint32_t tmem;
 };
 
-// dS of fp16 gradients is held in fp16, whose range ends at 6e-8: it is scaled by the power of two that
-// brings the largest |dout| of its sequence and key head to 2^-4, which leaves room for |v| summed over
-// the head dimension up to 2^19, and dk, dq are scaled back in fp32.
-__device__ __forceinline__ float gain_of(uint32_t amax_bits) {
-  const int e = (int)(amax_bits >> 23);
-  return e == 0 || e >= 250 ? 1.f : __uint_as_float((uint32_t)(250 - e) << 23);
+// fp16's range: 65504 down to steps of 2^-24, full precision down to 2^-14. A probability is held times 2^15 (the
+// exponent's reference is 15 lower), full down to 2^-29. dS = P (dP - delta) is held times the power of two that
+// brings its bound to 2^15: with |dP| <= |dout_i| |v_j|, and delta a mean of the dP, |dS| <= 2 |dout_i| max_j |v_j|,
+// full precision down to 2^-29 of the bound. The maximum over v's rows is the sequence's and key head's; |dout_i| is
+// the row's own for dq, and the largest of the key head's queries for dk, whose sums mix them. dv, dk and dq are
+// scaled back in fp32. (Norms of fp16 rows are 2^-24 to 2^19: the squares' product is 2^-96 to 2^76.)
+__device__ __forceinline__ float dS_scale(float dout2, float v2) {
+  const uint32_t u = __float_as_uint(dout2 * v2);
+  const int e = (int)(u >> 23) - 127;  // the norms' product is below 2^((e + 2) / 2), rounded down
+  return e <= -127 || e >= 128 ? 1.f : __uint_as_float((uint32_t)(14 - ((e + 2) >> 1) + 127) << 23);
+}
+constexpr float kProbScale = 1 << kProbBits;
+
+// The scale of dS of an item's row (queries), or of all its rows (keys). Rows behind the sequence's end have some
+// scale or other: the padded vectors reach 128 values further (AttnArgs), and such a row is not written.
+__device__ __forceinline__ float row_scale(const AttnArgs& a, const BwdItem& it, int row) {
+  const int64_t kh = (int64_t)it.seq * a.Hk + (it.keys ? it.head : it.head / (a.H / a.Hk));
+  const float dout2 = it.keys ? __uint_as_float(__ldg(a.top_dout + kh)) : __ldg(a.norm2 + it.head * a.vec_ld + it.off + row);
+  return dS_scale(dout2, __uint_as_float(__ldg(a.top_v + kh)));
 }
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -867,14 +880,14 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
       const int row = it.first + quarter * 32 + lane;
       if (it.first + quarter * 32 < it.len) {
         const bool keys = it.keys;
-        float mul = a.scale;
-        if (DT == ATLAS_F16) mul /= gain_of(__ldg(a.amax + (int64_t)it.seq * a.Hk + (keys ? it.head : it.head / group)));
+        const float mul = DT == ATLAS_F16 ? a.scale / row_scale(a, it, row) : a.scale;
+        const float mul_dv = DT == ATLAS_F16 ? 1.f / kProbScale : 1.f;
 #pragma unroll 1
         for (int h = keys ? 0 : 2; h < 4; ++h) {  // dv (keys), then dk or dq, 32 columns at a time
           uint32_t v[32];
           tmem_ld32(lanes + 384 + h * 32, v);
           tmem_ld_wait();
-          const float f = h < 2 ? 1.f : mul;
+          const float f = h < 2 ? mul_dv : mul;
           const Strides& so = h < 2 ? a.sdv : keys ? a.sdk : a.sdq;
           uint16_t* dst = reinterpret_cast<uint16_t*>(h < 2 ? a.dv : keys ? a.dk : a.dq) + it.outer * so.outer +
                           it.head * so.head + ((int64_t)it.row0 + row) * so.row;
@@ -918,7 +931,7 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
       if (!it.n) break;
       const bool live = it.first + quarter * 32 < it.len, keys = it.keys;
       float lse = 0.f, delta = 0.f, gain = 1.f;
-      if (DT == ATLAS_F16) gain = gain_of(__ldg(a.amax + (int64_t)it.seq * a.Hk + (keys ? it.head : it.head / group)));
+      if (DT == ATLAS_F16) gain = row_scale(a, it, it.first + own) / kProbScale;
       if (!keys) {
         ok = mbar_wait_soon(&s.a_full[r], (k / kRing) & 1, 220);
         if (!ok) break;
@@ -1014,7 +1027,7 @@ int bwd(const AttnArgs& a, cudaStream_t st) {
   if (int rc = attn_smem_once(attn_bwd_tc_kernel<DT>, bytes, done)) return rc;
   const int vec = a.D % 8 == 0 && map_ok(a.dq, a.sdq, a.outer, a.H, a.rows) && map_ok(a.dk, a.sdk, a.outer, a.Hk, a.rows) &&
                   map_ok(a.dv, a.sdv, a.outer, a.Hk, a.rows);
-  if (cudaMemsetAsync(DT == ATLAS_F16 ? a.amax : a.counter, 0, (size_t)(DT == ATLAS_F16 ? a.B * a.Hk + 2 : 2) * 4, st) != cudaSuccess)
+  if (cudaMemsetAsync(DT == ATLAS_F16 ? a.top_dout : a.counter, 0, (size_t)(DT == ATLAS_F16 ? 2 * a.B * a.Hk + 2 : 2) * 4, st) != cudaSuccess)
     return fail(ATLAS_ERR_CUDA, "attention_grad: clearing the workspace failed");
   if (int rc = attn_delta(a, DT, st)) return rc;
   const int64_t items = a.cap * (a.Hk + a.H);
