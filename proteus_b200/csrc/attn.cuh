@@ -135,6 +135,15 @@ __device__ __forceinline__ void idle_rows(const AttnArgs& a, int64_t i, int n, F
   }
 }
 
+// The exponents of a row's probabilities are taken from a reference R, and any R gives the same quotient: R is an
+// integer `shift` above the largest score known when it was chosen, rounded up to an integer (in base 2, so that R and
+// the log-sum-exp R - shift + log2(l 2^shift) lose nothing to it). A tile's sum above 2^-b, b = ceil log2 of how many
+// such sums a row has, moves R. So all weights together stay below 1 and a sum of weighted values below the largest
+// |v|: it is finite whenever the quotient is, which a reference left behind by scores that rise, or one that is the
+// running maximum (n |v|), does not give. Small values pay: what the largest weight adds is held to 2^(shift - 149).
+__device__ __forceinline__ int ceil_log2(int n) { return 32 - __clz(n - 1); }  // n >= 1
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
 // One row of a head set to zero by 8 lanes, 16 bytes at a time where it allows it.
 __device__ __forceinline__ void zero_row(void* dst, const Strides& st, int size, int64_t outer, int head, int64_t row, int D, int sub) {
   char* p = reinterpret_cast<char*>(dst) + (outer * st.outer + head * st.head + row * st.row) * size;

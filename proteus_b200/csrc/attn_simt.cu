@@ -9,8 +9,8 @@
 // scores; operands lie in shared memory as fp32 rows of DP + 4 words, read as float4 along the head
 // dimension (the 16 tx of a half warp hit distinct banks, the ty broadcast). The next tile's rows are in
 // registers on their way while this one is worked on. Scores are in base 2 (the queries carry scale log2 e). The
-// exponents' reference is the maximum of a row's first tile; fp32 has range for 2^64 above it, and only a sum
-// beyond that (or no reference yet: scores of -inf so far) raises it and rescales. The gradient is two kernels, one CTA per key
+// exponents' reference comes from the maximum of a row's first tile, with room for 2^8 above it (attn.cuh), and only a
+// sum beyond that (or no reference yet: scores of -inf so far) raises it and rescales. The gradient is two kernels, one CTA per key
 // tile (dk, dv; all query heads of its key head, one after the other) and one per query tile (dq): scores are
 // computed twice, but no sum crosses CTAs, so every result is the same from run to run. 40 sequences of 32 to 402 rows, 20 heads of 16,
 // fp32: 194 us forward (3 GFLOP, 0.21 of the FMA rate: the tiles' shared-memory reads and the exponentials' issue).
@@ -22,6 +22,7 @@ namespace {
 constexpr int BT = 64;       // rows of a tile
 constexpr int PP = 80;       // row pitch of a tile of scores: the two ty of a warp in different bank halves
 constexpr int kThreads = 256;
+constexpr int kRoom = 8;       // bits that scores may rise above the first tile's before its reference is raised
 constexpr int kIdleHeads = 4;  // heads of a CTA that sets rows to zero: its time is the look-up's, 2.5 us
 constexpr float kNegInf = -__builtin_inff();
 
@@ -229,12 +230,12 @@ __device__ __noinline__ void short_out(const AttnArgs& a, SeqBlock b, int head, 
   float sum = p;
 #pragma unroll
   for (int o = kAttnShort / 2; o; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-  s.p[r][c] = p;
+  s.p[r][c] = p / sum;  // before the values are summed: no sum above the largest of them
   __syncwarp();  // a row's scores are of one half of a warp
   float4 out = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
   for (int j = 0; j < len; ++j) add4(out, s.p[r][j], row_of(s.v, j, 4 * c));
-  short_store<DT>(a.out, a.so, b, head, r, c, a.D, out, 1.f / sum);
+  short_store<DT>(a.out, a.so, b, head, r, c, a.D, out, 1.f);
   if (c == 0 && r < len) a.lse[(b.outer * a.H + head) * a.rows + b.row0 + r] = (ref + log2f(sum)) * kLn2;
 }
 
@@ -263,6 +264,9 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 2 : 3) attn_fwd_simt_kern
     return;
   }
   const int kh = head / (a.H / a.Hk);
+  // a thread's sum is that of 4 of a tile's 64 columns
+  const int bits = ceil_log2((s.len + BT - 1) / BT) + 4, shift = bits + kRoom;
+  const float limit = pow2(-bits);
   Tile<DT, DP> tk, tv;
   tk.fetch(a.q, a.sq, s.outer, head, s.row0, first, s.len, a.D, vec);
   tk.put(sq, a.scale * kLog2e);
@@ -292,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 2 : 3) attn_fwd_simt_kern
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         if (n0 + tx + 16 * j >= s.len) c[i][j] = kNegInf;
-    auto highest = [&](int i) { return row_max(fmaxf(fmaxf(c[i][0], c[i][1]), fmaxf(c[i][2], c[i][3]))); };
+    auto highest = [&](int i) { return ceilf(row_max(fmaxf(fmaxf(c[i][0], c[i][1]), fmaxf(c[i][2], c[i][3])))) + shift; };
     if (n0 == 0) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) m[i] = highest(i);
@@ -306,7 +310,7 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 2 : 3) attn_fwd_simt_kern
 #pragma unroll
         for (int j = 0; j < 4; ++j) e[i][j] = ex2(c[i][j] - ref);
         sum[i] = (e[i][0] + e[i][1]) + (e[i][2] + e[i][3]);
-        bad |= m[i] == kNegInf || !(sum[i] <= 0x1p64f);
+        bad |= m[i] == kNegInf || !(sum[i] <= limit);
       }
     };
     powers();
@@ -336,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 2 : 3) attn_fwd_simt_kern
     l[i] = row_sum(l[i]);
     inv[i] = 1.f / l[i];
     const int r = first + ty + 16 * i;
-    if (tx == 0 && r < s.len) a.lse[(s.outer * a.H + head) * a.rows + s.row0 + r] = ((m[i] == kNegInf ? 0.f : m[i]) + log2f(l[i])) * kLn2;
+    if (tx == 0 && r < s.len) a.lse[(s.outer * a.H + head) * a.rows + s.row0 + r] = ((m[i] == kNegInf ? 0.f : m[i] - shift) + log2f(l[i] * pow2(shift))) * kLn2;
   }
   store_tile<DT, DP>(a.out, a.so, s.outer, head, s.row0, first, s.len, a.D, ty, tx, acc, inv);
 }

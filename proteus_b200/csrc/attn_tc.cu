@@ -114,12 +114,15 @@ __device__ __forceinline__ int up16(int n) { return (n + 15) & ~15; }
 //   warp 11     zero to rows of no sequence
 // Registers are moved from the other eight warps to the softmax's: 384 x 80 = 128 (152 + 48 + 40).
 //
-// The reference that exponents are taken from is the maximum of a row's FIRST 32 scores, not a running one: any
-// reference gives the same quotient, and fp32 sums and bf16 probabilities have range for 2^64 above it. So a
-// tile costs one pass (no maximum, no rescaling): a packed multiply-add, an exponential, a packed sum and half a
-// conversion a score. The tile's sum tells when the reference was too low (2^64; fp16 P: 2^15), or when there is
-// none yet (those scores all -inf); the warp then takes the tile's maximum, rescales the output in TMEM and
-// does the tile again, whose scores are still there, since P is held in registers until it is accepted.
+// The reference that exponents are taken from comes from the maximum of a row's FIRST 32 scores, not a running one: any
+// reference gives the same quotient. So a tile costs one pass (no maximum, no rescaling): a packed multiply-add, an
+// exponential, a packed sum and half a conversion a score. The tile's sum tells when the reference was too low, or when
+// there is none yet (those scores all -inf); the warp then takes the tile's maximum, rescales the output in TMEM and
+// does the tile again, whose scores are still there, since P is held in registers until it is accepted. bf16 has room
+// for 2^32 above those scores (attn.cuh says what that costs: here values below 2^-80 lose bits, since what falls below
+// 2^-126 in the tensor cores' sums is lost). Scores of a standard deviation of 12 over 4096 keys, 190 us if they never
+// pass it, take 262 with room for 2^32, 221 with 2^40, 201 with 2^48; those of 2, 190 with any.
+// fp16 P has room for 2^15, and a reference that is the maximum itself: its values end at 65504, its steps at 2^-24.
 //
 // The last tile of a sequence of several ends at the sequence's end and starts inside the tile before: its
 // columns `lo` .. are new, the ones below count as -inf, and no row behind the end is read.
@@ -155,6 +158,15 @@ __device__ __forceinline__ int key_tile(int i, int n, int len, int& lo, int& hi)
   hi = min(KT, len - from);
   return from;
 }
+
+// How far the reference of an item of n key tiles is above its row's scores, and the largest sum of a tile.
+constexpr int kRoom = 32;
+template <int DT>
+__device__ __forceinline__ int fwd_shift(int n) { return DT == ATLAS_BF16 ? ceil_log2(n) + kRoom : 0; }
+template <int DT>
+__device__ __forceinline__ float fwd_limit(int n) { return DT == ATLAS_BF16 ? pow2(-ceil_log2(n)) : 0x1p15f; }
+template <int DT>
+__device__ __forceinline__ float fwd_ref(float highest, int shift) { return DT == ATLAS_BF16 ? ceilf(highest) + shift : highest; }
 
 // Probabilities of a row's tile against `ref` (negated) into p, their sum returned.
 template <int DT>
@@ -428,7 +440,7 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
   } else if (warp < 4) {
     regs_inc<152>();
     const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
-    const float c = a.scale * kLog2e, limit = DT == ATLAS_BF16 ? 0x1p64f : 0x1p15f;
+    const float c = a.scale * kLog2e;
     bool ok = true;
 #pragma unroll 1
     for (int k = 0, t = 0; ok; ++k) {
@@ -439,6 +451,8 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
       if (!it.n) break;
       const bool live = it.first + warp * 32 < it.len;
       float ref = kNegInf, l = 0.f;  // ref: in base 2, -inf while there is none
+      const int shift = fwd_shift<DT>(it.n);
+      const float limit = fwd_limit<DT>(it.n);
 #pragma unroll 1
       for (int i = 0; i < it.n; ++i, ++t) {
         const int bf = t & 1;
@@ -451,14 +465,14 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
         if (live) {
           // one copy of the tile's code: instruction fetch is what many copies of it run out of first
           if (lo > 0 || hi < KT) fwd_mask(buf, lo, hi);
-          if (i == 0) ref = fwd_max(buf, 32) * c;
+          if (i == 0) ref = fwd_ref<DT>(fwd_max(buf, 32) * c, shift);
           uint32_t p[KT / 2];
           float sum;
           for (int again = 0;; ++again) {
             sum = fwd_tile<DT>(buf, c, ref == kNegInf ? 0.f : -ref, lo, hi, p);
             const bool bad = ref == kNegInf || !(sum <= limit);
             if (again || !__any_sync(0xFFFFFFFFu, bad)) break;
-            const float mx = fwd_max(buf, KT) * c;
+            const float mx = fwd_ref<DT>(fwd_max(buf, KT) * c, shift);
             const float to = bad ? fmaxf(ref, mx) : ref;
             if (i > 0) {
               const float f = ref == to || ref == kNegInf ? 1.f : ex2(ref - to);
@@ -520,11 +534,12 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
       if (row0 < len) {
         const float2 st = s.stat[r][quarter * 32 + lane];
         const float inv = 1.f / st.x;
+        const int shift = fwd_shift<DT>(n);
         const int head = s.item[r].head;
         const int64_t outer = s.item[r].outer, to = (int64_t)s.item[r].row0 + row0;
         uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + outer * a.so.outer + head * a.so.head + to * a.so.row;
         if (row0 + lane < len)
-          a.lse[(outer * a.H + head) * a.rows + to + lane] = ((st.y == kNegInf ? 0.f : st.y) + log2f(st.x)) * kLn2;
+          a.lse[(outer * a.H + head) * a.rows + to + lane] = ((st.y == kNegInf ? 0.f : st.y - shift) + log2f(st.x * pow2(shift))) * kLn2;
 #pragma unroll 1
         for (int h = 0; h < 4; ++h) {
           uint32_t o[16];
