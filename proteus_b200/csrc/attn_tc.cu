@@ -16,7 +16,8 @@
 // 16, and the rows up to there are set to zero in shared memory where they are summed over, since
 // 0 x NaN is NaN.
 //
-// Every wait is bounded (see tc.cuh); a wait that gives up records its code and the CTA leaves.
+// Every wait is bounded (see tc.cuh); a wait that gives up records its code and the CTA leaves, behind what it
+// still has under way (last_phases).
 #include "attn.cuh"
 #include "tc.cuh"
 
@@ -97,6 +98,13 @@ __device__ __forceinline__ void zero_tile_rows(uint8_t* tile, int from, int to, 
   for (int i = from * 8 + lane; i < to * 8; i += 32) reinterpret_cast<uint4*>(tile)[i] = make_uint4(0, 0, 0, 0);
   fence_async_smem();
   __syncwarp();
+}
+
+// Waits, with a limit, for the phases that `n` arrivals in turn on a ring of barriers end: a CTA's memory is
+// not another's before its copies have landed in it and its products have reported there.
+__device__ __forceinline__ void last_phases(uint64_t* ring, int size, int n) {
+#pragma unroll 1
+  for (int i = 0; i < size && i < n; ++i) mbar_poll(ring + i, ((n - 1 - i) / size) & 1);
 }
 
 __device__ __forceinline__ int up16(int n) { return (n + 15) & ~15; }
@@ -265,10 +273,11 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
 
   if (warp == 8) {
     regs_dec<40>();
-    int x = blockIdx.x, head = blockIdx.y, k = 0, t = 0, z = 0;
+    int x = blockIdx.x, head = blockIdx.y, k = 0, t = 0, z = 0, queries = 0;
     uint32_t asked = 0;
-    bool more = true, ok = true;
+    bool more = true, ok = true, answer_due = false;
     while (ok) {
+      answer_due = more;
       if (more && elect_one()) {  // the next item is on its way while this one is loaded
         mbar_arrive_expect_tx(&s.taken, 16);
         take_cta_async(&s.answer, &s.taken);
@@ -301,6 +310,7 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
           tma_load_4d(s.q[r], &mq, 0, r0 + b.first, head, o, &s.q_full[r]);
         }
         __syncwarp();
+        ++queries;
 #pragma unroll 1
         for (int i = 0; i < n; ++i, ++t) {
           const int st = t % kFwdStages;
@@ -321,8 +331,9 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
         ++k;
       }
       ok = mbar_wait_soon(&s.taken, asked & 1, 199);
-      ++asked;
       if (!ok) break;
+      ++asked;
+      answer_due = false;
       more = taken_cta(&s.answer, x, head);
       // the answer is read before the next one may overwrite it (generic reads, asynchronous write)
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -335,13 +346,19 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
       mbar_arrive(&s.spare_full);
     }
     __syncwarp();
+    // what this warp asked for lands before the CTA leaves; all has, unless a wait gave up
+    if (answer_due) mbar_poll(&s.taken, asked & 1);
+    last_phases(s.q_full, 2, queries);
+    last_phases(s.k_full, kFwdStages, t);
+    last_phases(s.v_full, kFwdStages, t);
   } else if (warp == 9) {
     regs_dec<40>();
     const uint32_t base = DT == ATLAS_BF16 ? idesc_bf16_f32(BM, 0) : idesc_f16_f32(BM, 0);
     const uint32_t qd = desc_lo(smem_u32(s.q[0])), kd = desc_lo(smem_u32(s.k[0]));
     bool ok = true;
+    int t = 0;
 #pragma unroll 1
-    for (int k = 0, t = 0; ok; ++k) {
+    for (int k = 0; ok; ++k) {
       const int r = k & 1;
       if (!mbar_wait_soon(&s.item_full[r], (k >> 1) & 1, 211)) break;
       const int n = s.item[r].n, len = s.item[r].len;
@@ -369,13 +386,16 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
         __syncwarp();
       }
     }
+    last_phases(s.k_empty, kFwdStages, t);  // the products are done, and have said so
+    last_phases(s.s_full, 2, t);
   } else if (warp == 10) {
     regs_dec<40>();
     const uint32_t id = (DT == ATLAS_BF16 ? idesc_bf16_f32(BM, 64) : idesc_f16_f32(BM, 64)) | kMnB;
     const uint32_t vd = desc_lo(smem_u32(s.v[0]));
     bool ok = true;
+    int t = 0;
 #pragma unroll 1
-    for (int k = 0, t = 0; ok; ++k) {
+    for (int k = 0; ok; ++k) {
       if (!mbar_wait_soon(&s.item_full[k & 1], (k >> 1) & 1, 213)) break;
       const int n = s.item[k & 1].n, len = s.item[k & 1].len;
       // the last item's output has been read out of where this one's goes
@@ -406,6 +426,8 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
         __syncwarp();
       }
     }
+    last_phases(s.o_done, 2, t);
+    last_phases(s.v_empty, kFwdStages, t);
   } else if (warp == 11) {
     regs_dec<40>();
     // Rows of no sequence: 6 us of 125 when the warp that loads the tiles did it in between (109 sequences of 271
@@ -752,7 +774,7 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
   if (warp == 16) {
     if (elect_one()) {
       const int blocks = (int)min((int64_t)*a.listed, attn_blocks(a.outer, a.rows, a.B)), total = blocks * (a.Hk + a.H);
-      int next = (int)atomicAdd(a.counter, 1u), k = 0, t = 0;
+      int next = (int)atomicAdd(a.counter, 1u), k = 0, t = 0, rows = 0;
       while (true) {
         BwdItem it{};
         if (next < total) {  // keys first: theirs are the longest items
@@ -784,6 +806,7 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
           bulk_load(s.a_lse[r], lse2 + it.head * a.vec_ld + it.first, BM * 4, &s.a_full[r]);
           bulk_load(s.a_delta[r], delta2 + it.head * a.vec_ld + it.first, BM * 4, &s.a_full[r]);
         }
+        ++rows;
         int row = 0, h = keys ? it.head * group : kh;
         bool ok = true;
 #pragma unroll 1
@@ -807,6 +830,9 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
         if (!ok) break;
         ++k;
       }
+      // the copies land before the CTA leaves; all have, unless a wait gave up
+      last_phases(s.a_full, kRing, rows);
+      last_phases(s.b_full, kStages, t);
     }
   } else if (warp == 17 || warp == 18) {
     // Warp 17: S, warp 18: dP. While the tensor core reads its operands, everything else that touches shared
@@ -814,8 +840,9 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
     const bool dp = warp == 18;
     const uint32_t base = DT == ATLAS_BF16 ? idesc_bf16_f32(BM, 0) : idesc_f16_f32(BM, 0);
     bool ok = true;
+    int t = 0;
 #pragma unroll 1
-    for (int k = 0, t = 0; ok; ++k) {
+    for (int k = 0; ok; ++k) {
       const int r = k % kRing;
       if (!mbar_wait_soon(&s.item_full[r], (k / kRing) & 1, 213)) break;
       const int n = s.item[r].n, len = s.item[r].len, keys = s.item[r].keys;
@@ -839,19 +866,21 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
           mma_f16_lo<true>(at, ar + 2, br + 2, id);
           mma_f16_lo<true>(at, ar + 4, br + 4, id);
           mma_f16_lo<true>(at, ar + 6, br + 6, id);
-          mma_commit(&s.s_full[x]);
           if (i == n - 1) mma_commit(&s.item_empty[r]);
+          mma_commit(&s.s_full[x]);
         }
         __syncwarp();
         row += BN;
         if (row >= len) row = 0;
       }
     }
+    last_phases(s.s_full, 3, t);  // the products are done, and have said so (with the other warp's of the same tiles)
   } else if (warp == 19) {
     const uint32_t base = DT == ATLAS_BF16 ? idesc_bf16_f32(BM, 64) : idesc_f16_f32(BM, 64), id = base | kMnB;
     bool ok = true;
+    int t = 0;
 #pragma unroll 1
-    for (int k = 0, t = 0; ok; ++k) {
+    for (int k = 0; ok; ++k) {
       const int r = k % kRing;
       if (!mbar_wait_soon(&s.item_full[r], (k / kRing) & 1, 224)) break;
       const int n = s.item[r].n, len = s.item[r].len, keys = s.item[r].keys;
@@ -870,18 +899,20 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
               if (keys) mma_f16_ts_lo(tmem + 384, at + kk * 8, br1 + kk * 128, id, i > 0 || kk > 0);
               mma_f16_ts_lo(tmem + 448, at + 64 + kk * 8, br0 + kk * 128, id, i > 0 || kk > 0);
             }
-          mma_commit(&s.x_done[x]);
-          mma_commit(&s.b_empty[st]);
           if (i == n - 1) {
             mma_commit(&s.acc_full[r]);
             mma_commit(&s.item_empty[r]);
           }
+          mma_commit(&s.x_done[x]);
+          mma_commit(&s.b_empty[st]);
         }
         __syncwarp();
         row += BN;
         if (row >= len) row = 0;
       }
     }
+    last_phases(s.x_done, 3, t);
+    last_phases(s.b_empty, kStages, t);
   } else if (warp >= 4 * kGroups) {
     const int quarter = warp & 3;
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
