@@ -358,6 +358,7 @@ int atlas_attention_grad(const void* dout, const void* q, const void* k, const v
                          int dtype, const int64_t* strides_host, int64_t outer, int64_t rows, int64_t H, int64_t Hk,
                          int64_t D, const int32_t* cu, const int32_t* blocks, const int64_t* counts, int64_t B,
                          int64_t cap, int packed, double scale, void* dq, void* dk, void* dv, void* ws, int64_t ws_bytes, void* stream);
+int atlas_attention_grad_kernels(void); /* kernels of the calling thread's last atlas_attention_grad that was launched */
 
 /* ------------------------------------------------------------------------------------------------
  * Log probabilities of given tokens, and their gradient. No counterpart in the reference.

@@ -81,7 +81,7 @@ def load(path: str | os.PathLike | None = None):
 
 # kernels launched per call (predicated kernels that exit early on the device still count)
 _KERNELS = {"atlas_grouped_merge": 6, "atlas_last_error": 0, "atlas_abi_version": 0, "atlas_device_status": 0,
-            "atlas_device_status_set": 0, "atlas_stats_enrich_supported": 0}
+            "atlas_device_status_set": 0, "atlas_stats_enrich_supported": 0, "atlas_attention_grad_kernels": 0}
 LAUNCHES = {"count": 0}
 
 
@@ -92,8 +92,8 @@ def _count_admit(args):  # candidates, plus the bulk-row kernel when there are b
     return 2 if (args[6] and args[20]) else 1
 
 
-def _count_attention_grad(args):  # delta, then one kernel on the tensor cores or two on CUDA cores (fp32)
-    return 3 if args[6] == 0 else 2
+def _count_attention_grad(args):  # by the kernels that its tensors' types and strides chose
+    return load().atlas_attention_grad_kernels()
 
 
 def _count_maps(args):  # more than 1024 sequences: totals, a scan, then the outputs
@@ -113,11 +113,11 @@ def _n_kernels(name: str, args) -> int:
 def call(name: str, *args):
     """Call an entry point and raise AtlasKernelError on a non-zero status."""
     lib = load()
-    LAUNCHES["count"] += _n_kernels(name, args)
     rc = getattr(lib, name)(*args)
     if rc != 0:
         msg = lib.atlas_last_error().decode(errors="replace")
         raise AtlasKernelError(f"{name} failed (status {rc}): {msg}")
+    LAUNCHES["count"] += _n_kernels(name, args)
     return rc
 
 

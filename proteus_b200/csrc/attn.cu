@@ -10,6 +10,8 @@ int attn_tc(const AttnArgs& a, int dtype, bool grad, cudaStream_t st);
 
 namespace {
 
+thread_local int grad_kernels = 0;  // of this thread's last atlas_attention_grad
+
 Strides at(const int64_t* s, int i) { return Strides{s[3 * i], s[3 * i + 1], s[3 * i + 2]}; }
 
 int check(const AttnArgs& a, int dtype, const char* what) {
@@ -47,6 +49,8 @@ extern "C" int atlas_attention(const void* q, const void* k, const void* v, int 
   return (attn_tc_takes(a, dtype, false) ? attn_tc : attn_simt)(a, dtype, false, (cudaStream_t)stream);
 }
 
+extern "C" int atlas_attention_grad_kernels(void) { return grad_kernels; }
+
 extern "C" int64_t atlas_attention_grad_ws_bytes(int64_t outer, int64_t rows, int64_t H, int64_t Hk, int64_t B) {
   return 16 * attn_blocks(outer, rows, B) + 4 * (3 * H * attn_vec_ld(outer, rows, B) + 2 * B * Hk + 2);
 }
@@ -70,7 +74,9 @@ extern "C" int atlas_attention_grad(const void* dout, const void* q, const void*
   ATLAS_REQUIRE(dout && out && dq && dk && dv && ws, "attention_grad: null pointer");
   ATLAS_REQUIRE(ws_bytes >= atlas_attention_grad_ws_bytes(outer, rows, H, Hk, B) && (uintptr_t)ws % 16 == 0,
                 "attention_grad: workspace too small, or not 16-byte aligned");
-  if (!attn_tc_takes(a, dtype, true)) {
+  const bool tc = attn_tc_takes(a, dtype, true);
+  grad_kernels = tc ? 2 : 3;  // delta, then one kernel, or on CUDA cores one for the keys and one for the queries
+  if (!tc) {
     a.delta = (float*)ws;
     return attn_simt(a, dtype, true, (cudaStream_t)stream);
   }
