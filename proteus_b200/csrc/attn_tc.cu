@@ -16,6 +16,15 @@
 // 16, and the rows up to there are set to zero in shared memory where they are summed over, since
 // 0 x NaN is NaN.
 //
+// What is rounded to 16 bits, and why: P before it meets v or dout, and dS before it meets k or q, since both are
+// operands of a 16-bit product; their sums (l, the outputs, dq, dk, dv), the scores, the log-sum-exp and delta are
+// fp32. A product's operand that is off by up to half a step, 2^-8 (bf16) or 2^-11 (fp16), independently for each key,
+// moves a result by as much of its norm as the result's own rounding does, so that the two together are 1.4 times
+// the one that no kernel avoids (bf16: 2.4e-3 of the norm for 1.7e-3). A second product with what the rounding left over would take that
+// away, for half as many tensor operations again and P written twice to TMEM; tensors whose neighbours in the model
+// are rounded as often do not show it, and fp32 tensors keep 24 bits. Exponentials are ex2 of a score in base 2: the
+// factor log2 e goes into the score's scale, which rounds it once, 2^-24 of the score.
+//
 // Every wait is bounded (see tc.cuh); a wait that gives up records its code and the CTA leaves, behind what it
 // still has under way (last_phases).
 #include "attn.cuh"

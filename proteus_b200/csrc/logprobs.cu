@@ -9,7 +9,9 @@
 // One read of the row: a larger maximum rescales Z and T (T <- e^(M-M') (T + Z (M - M'))). The
 // difference x - M is taken before the factor log2 e, so that logits at the type's lowest value stay
 // finite, and T holds the distances from the maximum, so that a sharp row's small entropy is no
-// difference of large numbers. Sums are fp32.
+// difference of large numbers. Sums are fp32. A term is ex2 of the rounded product d log2 e, off by |d| 2^-24 and 2 units
+// of the last place: of Z that is sum p |d| 2^-24, at most (entropy + log Z) 2^-24, the size of the rounding that lse itself
+// takes: the shorter form is enough.
 //
 // Rows: a row whose logits are all -inf has lse = -inf, log probability -inf, entropy 0 and a zero
 // gradient; a NaN or +inf makes the row's numbers NaN (NaN counts as the largest among the

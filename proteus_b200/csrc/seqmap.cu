@@ -10,7 +10,9 @@
 // sequences every CTA scans the lengths again for itself in shared memory (4 KB from L2) instead of
 // waiting for a scan kernel. Above that two launches of one CTA per 1024 sequences (totals, then prefix sums)
 // write to the workspace what the last one searches; its CTAs have long runs of outputs, so that the search
-// for a run's first and last sequence, 16 dependent reads for 65536, is paid twice a CTA and not a thread.
+// for a run's first and last sequence (a warp's, 4 dependent reads for 65536) is paid once a CTA and not a thread. The
+// kept positions' prefix sums of a run are then staged in shared memory; those of the blocks are not, and each entry of
+// the block table searches the run's part of them in global memory.
 #include "common.cuh"
 
 namespace atlas {
