@@ -16,14 +16,14 @@
 // 16, and the rows up to there are set to zero in shared memory where they are summed over, since
 // 0 x NaN is NaN.
 //
-// What is rounded to 16 bits, and why: P before it meets v or dout, and dS before it meets k or q, since both are
-// operands of a 16-bit product; their sums (l, the outputs, dq, dk, dv), the scores, the log-sum-exp and delta are
-// fp32. A product's operand that is off by up to half a step, 2^-8 (bf16) or 2^-11 (fp16), independently for each key,
-// moves a result by as much of its norm as the result's own rounding does, so that the two together are 1.4 times
-// the one that no kernel avoids (bf16: 2.4e-3 of the norm for 1.7e-3). A second product with what the rounding left over would take that
-// away, for half as many tensor operations again and P written twice to TMEM; tensors whose neighbours in the model
-// are rounded as often do not show it, and fp32 tensors keep 24 bits. Exponentials are ex2 of a score in base 2: the
-// factor log2 e goes into the score's scale, which rounds it once, 2^-24 of the score.
+// What is rounded to 16 bits, and why: P before it meets v or dout, and dS before it meets q, since both are operands
+// of a 16-bit product (dS before it meets k is held as two such values, see the gradient below). Their sums (l, the
+// outputs, dq, dk, dv), the scores, the log-sum-exp and delta are fp32. An operand that is off by up to half a step,
+// 2^-8 (bf16) or 2^-11 (fp16), independently for each key, moves a result by as much of its norm as the result's own
+// rounding does, so that the two together are 1.4 times the one that no kernel avoids (bf16: 2.4e-3 of the norm for
+// 1.7e-3). A second product with what the rounding left over takes that away, for half as many tensor operations again
+// and a second value written to TMEM; fp32 tensors keep 24 bits throughout. Exponentials are ex2 of a score in
+// base 2: the factor log2 e goes into the score's scale, which rounds it once, 2^-24 of the score.
 //
 // Every wait is bounded (see tc.cuh); a wait that gives up records its code and the CTA leaves, behind what it
 // still has under way (last_phases).
@@ -620,7 +620,11 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
 // both, but no sum crosses items. An item's two tiles A0, A1 (k, v or q, dout) stay in shared memory,
 // tiles of 64 rows B0, B1 (q, dout or k, v) come in turn:
 //   S = A0 B0^T, dP = A1 B1^T, and with the 16-bit P and dS, written over them, as A operands
-//   keys: dv += P B1, dk += dS B0;  queries: dq += dS B0.
+//   keys: dv += P B1, dk += dS B0;  queries: dq += dS B0, dS as two 16-bit values.
+// Queries have no use for P: its place holds what the rounding of dS left over, and a second product adds it. dq is
+// the result with the most errors otherwise (dS, delta's output, its own rounding: bf16 2.5e-3 of the norm on the batch
+// of 109 sequences below; 1.8e-3 so, 1.7e-3 being its own rounding), and the queries' items then take as long as the
+// keys', 15 us more of that batch's 372. The keys' would need a third place.
 // One persistent CTA per SM takes items of the list (attn_delta_kernel's) from a counter and runs their tiles as
 // one stream, so that an item's start (look-up, first loads) and end (reading the sums) hide behind its neighbours:
 //   warps 0-11  three groups of four, each takes every third tile: one thread per row
@@ -682,7 +686,22 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
-// P and dS of 16 columns of a row from their scores x and dP y, as packed pairs. lse and delta come
+// What packing (lo, hi) as `packed` has rounded away, packed.
+template <int DT>
+__device__ __forceinline__ uint32_t rest2(float lo, float hi, uint32_t packed) {
+  f32x2 had;
+  if (DT == ATLAS_BF16) {
+    had = pair(__uint_as_float((packed << 16) ^ 0x80000000u), __uint_as_float((packed & 0xFFFF0000u) ^ 0x80000000u));
+  } else {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&packed));
+    had = pair(-f.x, -f.y);
+  }
+  unpair(add2(pair(lo, hi), had), lo, hi);
+  return pack2<DT>(lo, hi);
+}
+
+// P and dS of 16 columns of a row from their scores x and dP y, as packed pairs (queries: in P's place what the
+// packing of dS has rounded away). lse and delta come
 // negated, in pairs (two fp32 operations an instruction); `left` columns are before the end.
 template <int DT, bool KEYS>
 __device__ __forceinline__ void bwd_part(const uint32_t (&x)[16], const uint32_t (&y)[16], f32x2 c2, f32x2 gain2, f32x2 nl, f32x2 nd,
@@ -705,8 +724,8 @@ __device__ __forceinline__ void bwd_part(const uint32_t (&x)[16], const uint32_t
       f32x2 g = add2(pair(__uint_as_float(y[o]), __uint_as_float(y[o + 1])), e[k]);
       if (DT == ATLAS_F16) g = mul2(g, gain2);
       unpair(mul2(g, pair(w0, w1)), g0, g1);
-      p[j / 2 + k] = pack2<DT>(w0, w1);
       d[j / 2 + k] = pack2<DT>(g0, g1);
+      p[j / 2 + k] = KEYS ? pack2<DT>(w0, w1) : rest2<DT>(g0, g1, d[j / 2 + k]);
     }
   }
   if (left < 16) {  // columns behind the end: whatever the scores were, nothing
@@ -717,7 +736,7 @@ __device__ __forceinline__ void bwd_part(const uint32_t (&x)[16], const uint32_t
       d[j] &= keep;
     }
   }
-  if (KEYS) tmem_st8(to_p, p);
+  tmem_st8(to_p, p);
   tmem_st8(to_d, d);
 }
 
@@ -907,6 +926,7 @@ attn_bwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
             if (kk * 16 < cols) {
               if (keys) mma_f16_ts_lo(tmem + 384, at + kk * 8, br1 + kk * 128, id, i > 0 || kk > 0);
               mma_f16_ts_lo(tmem + 448, at + 64 + kk * 8, br0 + kk * 128, id, i > 0 || kk > 0);
+              if (!keys) mma_f16_ts_lo(tmem + 448, at + kk * 8, br0 + kk * 128, id, 1);
             }
           if (i == n - 1) {
             mma_commit(&s.acc_full[r]);
