@@ -635,8 +635,8 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
 //   warp 19     sums (products of two small kinds cost their issuing warp 500 clocks a tile each)
 // TMEM: three buffers of S and dP (columns 128 x, 128 x + 64), the sums in 384-447 (dv) and 448-511.
 //
-// Measured (as the forward): 320 us (115 GFLOP that the formulas need, 359 TFLOP/s) and 399 us (267 GFLOP, 670 TFLOP/s).
-// A tile of 128 x 64 scores takes 1370 clocks; its products 590 (keys) and 470 (queries), its exponentials 512.
+// Measured (as the forward): 339 us (115 GFLOP that the formulas need, 339 TFLOP/s) and 433 us (267 GFLOP, 617 TFLOP/s).
+// A tile of 128 x 64 scores takes 1450 clocks; its products 590, its exponentials 512.
 constexpr int kBwdThreads = 640;
 constexpr int kGroups = 3;
 constexpr int BN = 64;
