@@ -346,7 +346,7 @@ int atlas_seq_maps(const void* lengths, int lengths_i64, int64_t B, int64_t rows
  * passed over); padded (packed = 0): outer = B, sequence b in the first cu[b+1]-cu[b] rows of outer
  * index b; packed: outer = 1, its rows are cu[b] .. cu[b+1]-1. Rows of no sequence are not read and come
  * out as zero. S, the softmax and all sums are fp32; for 16-bit tensors the probabilities and dS are rounded to
- * that type before they meet v, q, k or dout (not in the gradient of a sequence of up to 16 rows, which also
+ * that type before they meet v, dout or q, dS before it meets k to two of them (not in the gradient of a sequence of up to 16 rows, which also
  * takes delta from dout v instead of out). A query whose scores are all -inf has lse -inf and a NaN output.
  */
 int atlas_attention(const void* q, const void* k, const void* v, int dtype, const int64_t* strides_host, int64_t outer,
