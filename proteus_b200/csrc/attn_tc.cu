@@ -139,7 +139,9 @@ __device__ __forceinline__ int up16(int n) { return (n + 15) & ~15; }
 // for 2^32 above those scores (attn.cuh says what that costs: here values below 2^-80 lose bits, since what falls below
 // 2^-126 in the tensor cores' sums is lost). Scores of a standard deviation of 12 over 4096 keys, 190 us if they never
 // pass it, take 262 with room for 2^32, 221 with 2^40, 201 with 2^48; those of 2, 190 with any.
-// fp16 P has room for 2^15, and a reference that is the maximum itself: its values end at 65504, its steps at 2^-24.
+// fp16 values end at 65504 and have steps of 2^-24 below 2^-14: P's reference is 2^3 below those scores, so that n keys
+// of little weight are off by n 2^-28 of the largest at most (n = 2^17: half a step of the output), and it has room for
+// 2^13 above them. 2^8 below would take 260 us instead of 192 at scores of a standard deviation of 3, 2^3 takes 196.
 //
 // The last tile of a sequence of several ends at the sequence's end and starts inside the tile before: its
 // columns `lo` .. are new, the ones below count as -inf, and no row behind the end is read.
@@ -179,11 +181,10 @@ __device__ __forceinline__ int key_tile(int i, int n, int len, int& lo, int& hi)
 // How far the reference of an item of n key tiles is above its row's scores, and the largest sum of a tile.
 constexpr int kRoom = 32;
 template <int DT>
-__device__ __forceinline__ int fwd_shift(int n) { return DT == ATLAS_BF16 ? ceil_log2(n) + kRoom : 0; }
+__device__ __forceinline__ int fwd_shift(int n) { return DT == ATLAS_BF16 ? ceil_log2(n) + kRoom : -3; }  // fp16: 96 x 2^3, far below 65504
 template <int DT>
-__device__ __forceinline__ float fwd_limit(int n) { return DT == ATLAS_BF16 ? pow2(-ceil_log2(n)) : 0x1p15f; }
-template <int DT>
-__device__ __forceinline__ float fwd_ref(float highest, int shift) { return DT == ATLAS_BF16 ? ceilf(highest) + shift : highest; }
+__device__ __forceinline__ float fwd_limit(int n) { return DT == ATLAS_BF16 ? pow2(-ceil_log2(n)) : 65504.f; }
+__device__ __forceinline__ float fwd_ref(float highest, int shift) { return ceilf(highest) + shift; }
 
 // Probabilities of a row's tile against `ref` (negated) into p, their sum returned.
 template <int DT>
@@ -496,14 +497,14 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
         if (live) {
           // one copy of the tile's code: instruction fetch is what many copies of it run out of first
           if (lo > 0 || hi < KT) fwd_mask(buf, lo, hi);
-          if (i == 0) ref = fwd_ref<DT>(fwd_max(buf, 32) * c, shift);
+          if (i == 0) ref = fwd_ref(fwd_max(buf, 32) * c, shift);
           uint32_t p[KT / 2];
           float sum;
           for (int again = 0;; ++again) {
             sum = fwd_tile<DT>(buf, c, ref == kNegInf ? 0.f : -ref, lo, hi, p);
             const bool bad = ref == kNegInf || !(sum <= limit);
             if (again || !__any_sync(0xFFFFFFFFu, bad)) break;
-            const float mx = fwd_ref<DT>(fwd_max(buf, KT) * c, shift);
+            const float mx = fwd_ref(fwd_max(buf, KT) * c, shift);
             const float to = bad ? fmaxf(ref, mx) : ref;
             if (i > 0) {
               const float f = ref == to || ref == kNegInf ? 1.f : ex2(ref - to);

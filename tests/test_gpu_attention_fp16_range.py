@@ -133,3 +133,25 @@ def test_probabilities_below_the_normal_range():
     want = D ** -0.5 / n * (G @ (V.T @ K) - (G @ mean)[:, None] * K.sum(0))
     off = D ** -0.5 * H_STEP * (G.abs() @ mean.abs())[:, None] * K.mean(0).abs()
     assert ((dq[0, 0].double() - want).norm(dim=1) <= 3 * H_STEP * want.norm(dim=1) + off.norm(dim=1) + SUB * 8).all()
+
+
+@pytest.mark.parametrize("n", [3000, 17000])
+def test_output_of_many_small_weights(n):
+    """One key of weight near 1 and a value of zero, n others whose weights of e^-12 (2^-17.3) round alike: the output is their
+    share. h for each weight, h for the result, and a few roundings of fp32 at scores of 12."""
+    from proteus_b200 import kernels as KN
+    D = 16
+    g = torch.Generator(device=DEV).manual_seed(n)
+    k = torch.zeros(1, 1, n, D, dtype=torch.float16, device=DEV)
+    k[:, :, 0, 0] = 12.0
+    q = torch.zeros_like(k)
+    q[..., 0] = 1.0
+    v = (torch.rand(1, 1, n, D, generator=g, device=DEV) + 1).half()
+    v[:, :, 0] = 0.0
+    plan = KN.seq_maps(torch.tensor([n], device=DEV), n).plan(0)
+    out, lse = KN.attention(q, k, v, plan, 1.0)
+    w = torch.full((n,), -12.0, dtype=torch.float64, device=DEV).exp()
+    w[0] = 1.0
+    want = (w @ v[0, 0].double()) / w.sum()
+    assert ((out[0, 0].double() - want).abs() <= 2.1 * H_STEP * want + SUB).all()
+    assert (lse[0, 0].double() - (12 + w.sum().log())).abs().max() <= (n / 64 + 100) * 2.0 ** -24
