@@ -135,12 +135,13 @@ __device__ __forceinline__ void idle_rows(const AttnArgs& a, int64_t i, int n, F
   }
 }
 
-// The exponents of a row's probabilities are taken from a reference R, and any R gives the same quotient: R is an
-// integer `shift` above the largest score known when it was chosen, rounded up to an integer (in base 2, so that R and
-// the log-sum-exp R - shift + log2(l 2^shift) lose nothing to it). A tile's sum above 2^-b, b = ceil log2 of how many
-// such sums a row has, moves R. So all weights together stay below 1 and a sum of weighted values below the largest
-// |v|: it is finite whenever the quotient is, which a reference left behind by scores that rise, or one that is the
-// running maximum (n |v|), does not give. Small values pay: what the largest weight adds is held to 2^(shift - 149).
+// The exponents of a row's weights are taken from a reference, and any reference gives the same quotient: it is the
+// largest score known when it was chosen, so that a lone key's weight is 1 and nothing is lost to it. A tile's sum of
+// weights above 2^room moves it. Before they meet the values the weights (or the values) are scaled by
+// 2^-(room + b), b = ceil log2 of how many such sums a row has: all weights together are 1 at most then, and a sum of
+// weighted values stays below the largest |v|. It is finite whenever the quotient is, which neither a reference left
+// behind by rising scores nor a running maximum (n |v|) gives. Small values pay: what falls below the type's range by the
+// scale is lost.
 __device__ __forceinline__ int ceil_log2(int n) { return 32 - __clz(n - 1); }  // n >= 1
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 

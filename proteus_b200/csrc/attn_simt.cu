@@ -265,8 +265,7 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 2 : 3) attn_fwd_simt_kern
   }
   const int kh = head / (a.H / a.Hk);
   // a thread's sum is that of 4 of a tile's 64 columns
-  const int bits = ceil_log2((s.len + BT - 1) / BT) + 4, shift = bits + kRoom;
-  const float limit = pow2(-bits);
+  const float v_scale = pow2(-kRoom - 4 - ceil_log2((s.len + BT - 1) / BT));
   Tile<DT, DP> tk, tv;
   tk.fetch(a.q, a.sq, s.outer, head, s.row0, first, s.len, a.D, vec);
   tk.put(sq, a.scale * kLog2e);
@@ -283,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 2 : 3) attn_fwd_simt_kern
   for (int n0 = 0; n0 < s.len; n0 += BT) {
     __syncthreads();
     tk.put(sk, 1.f);
-    tv.put(sv, 1.f);
+    tv.put(sv, v_scale);
     __syncthreads();
     if (n0 + BT < s.len) {
       tk.fetch(a.k, a.sk, s.outer, kh, s.row0, n0 + BT, s.len, a.D, vec);
@@ -296,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 2 : 3) attn_fwd_simt_kern
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         if (n0 + tx + 16 * j >= s.len) c[i][j] = kNegInf;
-    auto highest = [&](int i) { return ceilf(row_max(fmaxf(fmaxf(c[i][0], c[i][1]), fmaxf(c[i][2], c[i][3])))) + shift; };
+    auto highest = [&](int i) { return row_max(fmaxf(fmaxf(c[i][0], c[i][1]), fmaxf(c[i][2], c[i][3]))); };
     if (n0 == 0) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) m[i] = highest(i);
@@ -310,7 +309,7 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 2 : 3) attn_fwd_simt_kern
 #pragma unroll
         for (int j = 0; j < 4; ++j) e[i][j] = ex2(c[i][j] - ref);
         sum[i] = (e[i][0] + e[i][1]) + (e[i][2] + e[i][3]);
-        bad |= m[i] == kNegInf || !(sum[i] <= limit);
+        bad |= m[i] == kNegInf || !(sum[i] <= (float)(1 << kRoom));
       }
     };
     powers();
@@ -338,9 +337,9 @@ __global__ void __launch_bounds__(kThreads, DP == 64 ? 2 : 3) attn_fwd_simt_kern
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     l[i] = row_sum(l[i]);
-    inv[i] = 1.f / l[i];
+    inv[i] = 1.f / (l[i] * v_scale);
     const int r = first + ty + 16 * i;
-    if (tx == 0 && r < s.len) a.lse[(s.outer * a.H + head) * a.rows + s.row0 + r] = ((m[i] == kNegInf ? 0.f : m[i] - shift) + log2f(l[i] * pow2(shift))) * kLn2;
+    if (tx == 0 && r < s.len) a.lse[(s.outer * a.H + head) * a.rows + s.row0 + r] = ((m[i] == kNegInf ? 0.f : m[i]) + log2f(l[i])) * kLn2;
   }
   store_tile<DT, DP>(a.out, a.so, s.outer, head, s.row0, first, s.len, a.D, ty, tx, acc, inv);
 }

@@ -139,9 +139,9 @@ __device__ __forceinline__ int up16(int n) { return (n + 15) & ~15; }
 // for 2^32 above those scores (attn.cuh says what that costs: here values below 2^-80 lose bits, since what falls below
 // 2^-126 in the tensor cores' sums is lost). Scores of a standard deviation of 12 over 4096 keys, 190 us if they never
 // pass it, take 262 with room for 2^32, 221 with 2^40, 201 with 2^48; those of 2, 190 with any.
-// fp16 values end at 65504 and have steps of 2^-24 below 2^-14: P's reference is 2^3 below those scores, so that n keys
-// of little weight are off by n 2^-28 of the largest at most (n = 2^17: half a step of the output), and it has room for
-// 2^13 above them. 2^8 below would take 260 us instead of 192 at scores of a standard deviation of 3, 2^3 takes 196.
+// fp16 values end at 65504 and have steps of 2^-24 below 2^-14: P is 2^3 times the weights, so that n keys of little
+// weight are off by n 2^-28 of the largest at most (n = 2^17: half a step of the output), and there is room for
+// 2^13. 2^8 times would take 260 us instead of 192 at scores of a standard deviation of 3, 2^3 takes 196.
 //
 // The last tile of a sequence of several ends at the sequence's end and starts inside the tile before: its
 // columns `lo` .. are new, the ones below count as -inf, and no row behind the end is read.
@@ -178,18 +178,17 @@ __device__ __forceinline__ int key_tile(int i, int n, int len, int& lo, int& hi)
   return from;
 }
 
-// How far the reference of an item of n key tiles is above its row's scores, and the largest sum of a tile.
+// What P is of the weights in an item of n key tiles, and the largest sum of a tile's weights.
 constexpr int kRoom = 32;
 template <int DT>
-__device__ __forceinline__ int fwd_shift(int n) { return DT == ATLAS_BF16 ? ceil_log2(n) + kRoom : -3; }  // fp16: 96 x 2^3, far below 65504
+__device__ __forceinline__ float fwd_scale(int n) { return DT == ATLAS_BF16 ? pow2(-kRoom - ceil_log2(n)) : 8.f; }
 template <int DT>
-__device__ __forceinline__ float fwd_limit(int n) { return DT == ATLAS_BF16 ? pow2(-ceil_log2(n)) : 65504.f; }
-__device__ __forceinline__ float fwd_ref(float highest, int shift) { return ceilf(highest) + shift; }
+constexpr float kLimit = DT == ATLAS_BF16 ? 0x1p32f : 65504.f / 8;
 
-// Probabilities of a row's tile against `ref` (negated) into p, their sum returned.
+// Weights of a row's tile against `ref` (negated), times `scale` into p, their sum returned.
 template <int DT>
-__device__ __forceinline__ float fwd_tile(uint32_t buf, float c, float nref, int lo, int hi, uint32_t (&p)[KT / 2]) {
-  const f32x2 c2 = pair(c, c), r2 = pair(nref, nref);
+__device__ __forceinline__ float fwd_tile(uint32_t buf, float c, float nref, float scale, int lo, int hi, uint32_t (&p)[KT / 2]) {
+  const f32x2 c2 = pair(c, c), r2 = pair(nref, nref), s2 = pair(scale, scale);
   uint32_t x[2][32];
   f32x2 sum[2] = {0, 0};
   tmem_ld32(buf, x[0]);
@@ -206,6 +205,7 @@ __device__ __forceinline__ float fwd_tile(uint32_t buf, float c, float nref, int
       a = ex2(a);
       b = ex2(b);
       sum[(j >> 1) & 1] = add2(sum[(j >> 1) & 1], pair(a, b));
+      unpair(mul2(pair(a, b), s2), a, b);
       p[h * 16 + j / 2] = pack2<DT>(a, b);
     }
   }
@@ -483,8 +483,7 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
       if (!it.n) break;
       const bool live = it.first + warp * 32 < it.len;
       float ref = kNegInf, l = 0.f;  // ref: in base 2, -inf while there is none
-      const int shift = fwd_shift<DT>(it.n);
-      const float limit = fwd_limit<DT>(it.n);
+      const float scale = fwd_scale<DT>(it.n);
 #pragma unroll 1
       for (int i = 0; i < it.n; ++i, ++t) {
         const int bf = t & 1;
@@ -497,14 +496,14 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
         if (live) {
           // one copy of the tile's code: instruction fetch is what many copies of it run out of first
           if (lo > 0 || hi < KT) fwd_mask(buf, lo, hi);
-          if (i == 0) ref = fwd_ref(fwd_max(buf, 32) * c, shift);
+          if (i == 0) ref = fwd_max(buf, 32) * c;
           uint32_t p[KT / 2];
           float sum;
           for (int again = 0;; ++again) {
-            sum = fwd_tile<DT>(buf, c, ref == kNegInf ? 0.f : -ref, lo, hi, p);
-            const bool bad = ref == kNegInf || !(sum <= limit);
+            sum = fwd_tile<DT>(buf, c, ref == kNegInf ? 0.f : -ref, scale, lo, hi, p);
+            const bool bad = ref == kNegInf || !(sum <= kLimit<DT>);
             if (again || !__any_sync(0xFFFFFFFFu, bad)) break;
-            const float mx = fwd_ref(fwd_max(buf, KT) * c, shift);
+            const float mx = fwd_max(buf, KT) * c;
             const float to = bad ? fmaxf(ref, mx) : ref;
             if (i > 0) {
               const float f = ref == to || ref == kNegInf ? 1.f : ex2(ref - to);
@@ -565,13 +564,12 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
       tc_fence_after();
       if (row0 < len) {
         const float2 st = s.stat[r][quarter * 32 + lane];
-        const float inv = 1.f / st.x;
-        const int shift = fwd_shift<DT>(n);
+        const float inv = 1.f / (st.x * fwd_scale<DT>(n));
         const int head = s.item[r].head;
         const int64_t outer = s.item[r].outer, to = (int64_t)s.item[r].row0 + row0;
         uint16_t* dst = reinterpret_cast<uint16_t*>(a.out) + outer * a.so.outer + head * a.so.head + to * a.so.row;
         if (row0 + lane < len)
-          a.lse[(outer * a.H + head) * a.rows + to + lane] = ((st.y == kNegInf ? 0.f : st.y - shift) + log2f(st.x * pow2(shift))) * kLn2;
+          a.lse[(outer * a.H + head) * a.rows + to + lane] = ((st.y == kNegInf ? 0.f : st.y) + log2f(st.x)) * kLn2;
 #pragma unroll 1
         for (int h = 0; h < 4; ++h) {
           uint32_t o[16];

@@ -27,3 +27,45 @@ def test_norms_of_the_errors(lens, H, Hk, D, dtype):
         for name, x, w, limit in zip(("dq", "dk", "dv"), got, _want(q, k, v, do, out, r, D ** -0.5), (1.03 / 3 ** 0.5, (2 / 3) ** 0.5, (2 / 3) ** 0.5)):
             err = (x[0, :, r].double() - w).norm()
             assert err <= limit * h * w.norm() + sub * w.numel() ** 0.5, (name, r, (err / w.norm() / h).item())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("D", [8, 13, 64])
+@pytest.mark.parametrize("packed", [True, False])
+def test_one_row_is_its_value(packed, D, dtype):
+    """A sequence of one row: its weight is 1, its output the value, bit for bit; so it is where every other key's weight
+    vanishes (scores 200 lower). Its log-sum-exp is the score: D products, the scale and two roundings of 2^-24 of it."""
+    from proteus_b200 import kernels as KN
+    q, k, v, _, plan, where, _ = _batch([1] * 40, packed, 4, 2, D, dtype, seed=D)
+    out, lse = KN.attention(q, k, v, plan)
+    for o, r in where:
+        assert torch.equal(out[o, :, r], v[o, :, r].repeat_interleave(2, 0))
+        s = (q[o, :, r].double() * k[o, :, r].double().repeat_interleave(2, 0)).sum(-1) * D ** -0.5
+        a = (q[o, :, r].double() * k[o, :, r].double().repeat_interleave(2, 0)).abs().sum(-1) * D ** -0.5
+        assert ((lse[o, :, r].double() - s).abs() <= 2.0 ** -24 * ((D + 4) * a + 4 * s.abs())).all()
+    q, k, v, _, plan, _, _ = _batch([150, 33], True, 4, 2, D, dtype, seed=D)
+    q.zero_()
+    k.zero_()
+    q[..., 0] = 1.0
+    k[:, :, 70, 0] = k[:, :, 150, 0] = 200.0
+    out, _ = KN.attention(q, k, v, plan, 1.0)
+    for r, at in ((slice(0, 150), 70), (slice(150, 183), 150)):
+        assert torch.equal(out[0, :, r], v[0, :, at].repeat_interleave(2, 0)[:, None].expand(4, r.stop - r.start, D))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("n", [2, 3, 10, 40, 300])
+def test_log_sum_exp_keeps_its_digits(n, dtype):
+    """Off by a score's roundings (D products and 3, of |q| |k| scale) and 2^-22 or so of a weight's exponential, on average over
+    its keys: an absolute error, however large or small the log-sum-exp is."""
+    from proteus_b200 import kernels as KN
+    D = 32
+    q, k, v, _, plan, where, _ = _batch([n] * 30, True, 2, 2, D, dtype, seed=n)
+    _, lse = KN.attention(q, k, v, plan)
+    for o, r in where:
+        s = q[o, :, r].double() @ k[o, :, r].double().transpose(1, 2) * D ** -0.5
+        a = (q[o, :, r].double().abs() @ k[o, :, r].double().abs().transpose(1, 2) * D ** -0.5).amax(-1)
+        w = torch.logsumexp(s, -1)
+        err = (lse[o, :, r].double() - w).abs()
+        assert (err <= 2.0 ** -24 * ((D + 3) * a + 2 * s.abs().amax(-1) + 8 + n / 8 + 2 * w.abs())).all()
+        assert err.norm() <= 2.0 ** -22 * (1 + w.norm())
