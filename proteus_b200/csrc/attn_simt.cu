@@ -157,7 +157,7 @@ __device__ __forceinline__ void store_tile(void* dst, const Strides& st, int64_t
 }
 
 // Short sequences: thread (r, c) makes the score of query r and key c, then 4 columns of a row r of a result.
-struct ShortSmem {
+struct alignas(16) ShortSmem {  // rows are read and written as float4
   float k[kAttnShort][68], v[kAttnShort][68], q[kAttnShort][68], g[kAttnShort][68], p[kAttnShort][20], ds[kAttnShort][20];
 };
 

@@ -11,7 +11,8 @@ pytestmark = pytest.mark.gpu
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("lens,H,Hk,D", [([290, 302, 271], 4, 4, 64), ([1366, 700], 4, 1, 64), ([90, 61, 40, 17], 4, 2, 32), ([513], 2, 2, 8)],
+@pytest.mark.parametrize("lens,H,Hk,D", [([290, 302, 271], 4, 4, 64), ([1366, 700], 4, 1, 64), ([90, 61, 40, 17], 4, 2, 32), ([513], 2, 2, 8),
+                                         ([255, 256, 257, 128, 129], 4, 2, 8), ([17, 30, 33, 63, 64, 65, 18] * 4, 2, 1, 16)],
                          ids=str)
 def test_norms_of_the_errors(lens, H, Hk, D, dtype):
     """The results are rounded to within half a step, h, uniformly: h / sqrt(3) of the norm at most. For dk and dv the
