@@ -146,8 +146,9 @@ __device__ __forceinline__ int up16(int n) { return (n + 15) & ~15; }
 // The last tile of a sequence of several ends at the sequence's end and starts inside the tile before: its
 // columns `lo` .. are new, the ones below count as -inf, and no row behind the end is read.
 //
-// Measured: 109 sequences of 271 to 302 rows, 20 heads of 64, bf16: 118 us (323 MB, 2.7 TB/s; 46 GFLOP, 390 TFLOP/s; the
-// exponentials alone 39 us at 16 a clock and SM); 4 of 1 to 4096, 16 heads over 4: 185 us (107 GFLOP, 578 TFLOP/s);
+// Measured: 109 sequences of 271 to 302 rows, 20 heads of 64, bf16: 121 us (323 MB, 2.7 TB/s; 46 GFLOP, 380 TFLOP/s; the
+// exponentials alone 39 us at 16 a clock and SM); 4 of 1 to 4096, 16 heads over 4: 193 us (107 GFLOP, 555 TFLOP/s; 8 of
+// them the weights' scale);
 // one of 37, 20 heads of 24: 6 us.
 constexpr int kFwdThreads = 384;
 constexpr int KT = 96;
@@ -634,7 +635,7 @@ attn_fwd_tc_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant
 //   warp 19     sums (products of two small kinds cost their issuing warp 500 clocks a tile each)
 // TMEM: three buffers of S and dP (columns 128 x, 128 x + 64), the sums in 384-447 (dv) and 448-511.
 //
-// Measured (as the forward): 339 us (115 GFLOP that the formulas need, 339 TFLOP/s) and 433 us (267 GFLOP, 617 TFLOP/s).
+// Measured (as the forward): 336 us (115 GFLOP that the formulas need, 342 TFLOP/s) and 429 us (267 GFLOP, 622 TFLOP/s).
 // A tile of 128 x 64 scores takes 1450 clocks; its products 590, its exponentials 512.
 constexpr int kBwdThreads = 640;
 constexpr int kGroups = 3;

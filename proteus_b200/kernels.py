@@ -220,11 +220,11 @@ def _same_device(first, **others):
 
 
 def _refuse_tangents(**tensors):
-    """Forward-mode derivatives: a dual tensor has no requires_grad, and its result would come without a tangent."""
-    if getattr(forward_ad, "_current_level", 0) >= 0:  # a dual level is open; unpack_dual alone takes 0.8 us a tensor
-        for name, t in tensors.items():
-            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
-                raise NotImplementedError(f"{name} carries a forward-mode tangent: only reverse-mode gradients are supported")
+    """Forward-mode derivatives: a dual tensor has no requires_grad, and its result would come without a tangent. Called
+    where a dual level is open (_current_level, 0.06 us to look at; unpack_dual takes 0.8 us a tensor)."""
+    for name, t in tensors.items():
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{name} carries a forward-mode tangent: only reverse-mode gradients are supported")
 
 
 class SeqPlan(NamedTuple):
@@ -360,7 +360,8 @@ def attention_grad(dout, q, k, v, out, lse, plan: SeqPlan, scale: float | None =
     """(dq, dk, dv) of attention(q, k, v, plan, scale) for the gradient `dout` of its output: the
     probabilities are computed again from `lse`, the keys' gradients summed over the query heads that
     share them. No atomics on them: the same call gives the same bits. Rows of no sequence come out as zero."""
-    _refuse_tangents(dout=dout, q=q, k=k, v=v, out=out, lse=lse)
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(dout=dout, q=q, k=k, v=v, out=out, lse=lse)
     o, h, n, d, hk, B = _check_attention(q, k, v, plan)
     dev = q.device
     if not (dout.device == dev and out.device == dev and lse.device == dev):
@@ -410,7 +411,8 @@ def attention(q, k, v, plan: SeqPlan, scale: float | None = None):
     through the log-sum-exp), once. A query whose scores are all -inf has log-sum-exp -inf and an output of
     NaN. A backward pass that goes into a CUDA graph calls attention_grad: autograd's own must not be captured
     while an eager graph of the same leaves is alive. Tensors with a forward-mode tangent are refused."""
-    _refuse_tangents(q=q, k=k, v=v)
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(q=q, k=k, v=v)
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _Attention.apply(q, k, v, plan.cu, plan.blocks, plan.counts, plan.stride, scale)
@@ -481,7 +483,8 @@ def token_logprobs_grad(logits, tokens, lse, entropy, g_logprob=None, g_entropy=
     """Gradient by the logits, [N, V] in their dtype, of sum(g_logprob * logprob) + sum(g_entropy *
     entropy), from token_logprobs' lse and entropy. Either gradient may be None. A token given twice
     in a row counts twice; one outside [0, V) not at all."""
-    _refuse_tangents(logits=logits, lse=lse, entropy=entropy, g_logprob=g_logprob, g_entropy=g_entropy)
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(logits=logits, lse=lse, entropy=entropy, g_logprob=g_logprob, g_entropy=g_entropy)
     N, V, J = _check_logits(logits, tokens)
     dt, dev = dtype_code(logits.dtype), logits.device
     lse, entropy = _row_vector(logits, "lse", lse, (N,)), _row_vector(logits, "entropy", entropy, (N,))
@@ -520,7 +523,8 @@ def token_logprobs(logits, tokens, top: int = 0) -> TokenLogprobs:
     means none: log probability 0, rank 0. A row of -inf only has log probabilities -inf and entropy 0.
     logprob and entropy are differentiable in the logits, once; a backward pass that goes into a CUDA graph calls
     token_logprobs_grad, as with attention. Logits with a forward-mode tangent are refused."""
-    _refuse_tangents(logits=logits)
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(logits=logits)
     if torch.is_grad_enabled() and logits.requires_grad:
         return TokenLogprobs(*_TokenLogprobs.apply(logits, tokens, top))
     return _token_logprobs_forward(logits, tokens, top)
